@@ -51,13 +51,15 @@ EXPORTED = (
     "gafime_allpairs_topk_host", "gafime_contiguous_bucket_upload_rows", "gafime_allpairs_rescored",
     "gafime_allpairs_topk_device", "gafime_topk_merge_device", "gafime_contiguous_bucket_upload_columns",
     "gafime_contiguous_bucket_device_columns", "gafime_contiguous_bucket_mark_updated",
+    "gafime_xent_forward", "gafime_xent_gradient", "gafime_xent_workspace", "gafime_grad_norm",
+    "gafime_grad_norm_workspace",
 )
 
 # kernel ids of the timing registry (GAFIME_KERNEL_* in the header)
 KERNEL_IDS = {"column_stats": 1, "pair_moments": 2, "epilogue_topk": 3, "merge": 4,
               "mi_pass1": 5, "mi_pass2": 6, "mi_finish": 7, "legacy_pair": 8,
               "finite_check": 9, "gram_tc": 10, "gram_prep": 11, "gram_reduce": 12,
-              "mi_class_copy": 13, "guard": 14}
+              "mi_class_copy": 13, "guard": 14, "xent": 15, "xent_tc": 16, "grad_norm": 17}
 
 
 class GafimeError(RuntimeError):
@@ -128,6 +130,14 @@ def _bind(lib: ctypes.CDLL) -> None:
         "gafime_pipeline_flush": ([_vp, _vp, _ip], _i),
         "gafime_pipeline_free": ([_vp], _i),
         "gafime_pearson_cuda": ([_vp, _vp, ctypes.c_int32, _vp], _i),
+        "gafime_xent_forward": ([_i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp,
+                                 ctypes.c_size_t, _vp], _i),
+        "gafime_xent_gradient": ([_i, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _f,
+                                  _i, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp], _i),
+        "gafime_xent_workspace": ([_i, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i,
+                                   ctypes.POINTER(ctypes.c_size_t)], _i),
+        "gafime_grad_norm": ([_vp, _vp, _vp, _i64, _vp, _f, _vp, _vp, ctypes.c_size_t, _vp], _i),
+        "gafime_grad_norm_workspace": ([_i64, ctypes.POINTER(ctypes.c_size_t)], _i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

@@ -1,0 +1,84 @@
+// xent.h -- softmax cross entropy of a linear head: what its two paths share.
+//   xent.cu      entry points, argument checks, the choice of path, the few-class path
+//   xent_tc.cu   many classes: logits, gradients of x and w as tcgen05 products
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/gafime_b200.h"
+
+namespace gafime {
+
+// One call: z = x w^T + bias over n rows, d features and c classes; strides in elements.
+struct XentCall {
+    int type;                    // GAFIME_TYPE_*
+    const void* x;
+    int64_t xr, xk;              // strides of a row and of a feature
+    const void* w;
+    int64_t wr, wk;              // strides of a class and of a feature
+    const float* bias;           // nullable, [c]
+    const int64_t* labels;       // [n]; negative: the row is left out
+    int64_t n, d, c;
+    const float* weight;         // nullable, row weights of the gradient
+    int64_t weight_stride;
+    float scale;                 // times the row weight
+    bool have_lse;               // loss and lse are inputs (a forward call wrote them)
+    float* loss;                 // [n]
+    float* lse;                  // [n]
+    void* dx;                    // nullable
+    int64_t dxr, dxk;
+    void* dw;                    // nullable, [c][d]
+    float* dbias;                // nullable, [c]
+    bool gradient;               // a gradient call (dx, dw and dbias may still all be null)
+    uint8_t* ws;
+    size_t ws_bytes;
+    cudaStream_t stream;
+};
+
+inline size_t xent_type_size(int type) { return type == GAFIME_TYPE_FP32 ? 4 : 2; }
+
+// Hands out 256-byte aligned pieces of the workspace; with a null base it only counts them.
+struct Carver {
+    uint8_t* base;
+    size_t used = 0;
+    explicit Carver(uint8_t* b) : base(b) {}
+    template <typename T>
+    T* take(size_t count) {
+        const size_t at = used;
+        used += (count * sizeof(T) + 255) / 256 * 256;
+        return base ? reinterpret_cast<T*>(base + at) : nullptr;
+    }
+};
+
+// Few classes (xent.cu): true when the class and feature counts fit its registers.
+bool xent_few_fits(const XentCall& a);
+size_t xent_few_workspace(const XentCall& a, int sms);
+cudaError_t xent_few(const XentCall& a, int sms);
+
+// Many classes (xent_tc.cu).
+size_t xent_tc_workspace(const XentCall& a, int sms);
+cudaError_t xent_tc(const XentCall& a, int sms);
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+    return (float)v;
+}
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) {
+    return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+}  // namespace gafime

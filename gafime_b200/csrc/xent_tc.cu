@@ -1,0 +1,1146 @@
+// xent_tc.cu -- softmax cross entropy of a linear head with many classes, on the tensor cores.
+//
+// The n x c logits never exist as a whole.  A forward call forms 128 x BN tiles of them in tensor
+// memory and keeps, per row, the running maximum and sum of exponentials.  A gradient call forms
+// them again piece by piece (kPieceBytes at a time), writes a piece's
+//   g_ij = r_i (exp(z_ij - lse_i) - [j = y(i)])
+// in 16 bits and multiplies it with both sides:
+//   lse   z = x w^T, online softmax in the epilogue              2 n d c FLOP
+//   g     z again, g in the epilogue                             2 n d c
+//   dx    g w        (classes summed; fp32 sums kept between class pieces)
+//   dw    g^T x      (rows summed; split over rows where the c x d tiles are few)
+//
+// Types.  16-bit x and w are multiplied as they are (TMA reads them in place where their
+// strides allow, else from a copy); g is rounded once to their type (half a step, 2^-8 or 2^-11
+// relative, independent from element to element, which is what rounding the result costs too).
+// fp32 is split into hi + lo fp16 (22 bits) after a power-of-two scale per feature, and every
+// product is hi hi + hi lo + lo hi, so its products hold about 2^-22:
+//   x'_ik = x_ik 2^s_k, |x'| < 2^14     w'_jk = w_jk 2^(t - s_k), |w'| < 2^14
+//   z = 2^-t sum x' w'      dw_jk = 2^(-u - s_k) sum g' x'      dx_ik = 2^(s_k - t - u) sum g' w'
+// with g' = g 2^u (u from the largest row weight, in fp16 too; u = 0 in bf16).
+//
+// Kernel (one CTA an SM, persistent, 12 warps): warp 0 queues the TMA loads of 128 x 64 and
+// BN x 64 operand tiles into a ring; warp 1 issues the MMAs into one of two tensor-memory
+// accumulators; warps 4-11 turn the other accumulator into sums, g, dx or partial dw.  Every
+// mbarrier wait is bounded; one that gives up records a code, and the call's losses and
+// gradients of w become NaN.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "engine.h"
+#include "tc.cuh"
+#include "xent.h"
+
+namespace gafime {
+
+namespace {
+
+constexpr int kThreads = 384;
+// Registers: 384 x 168 at launch = 128 x 40 (loads, MMAs) + 256 x 232 (epilogues, which keep a
+// tile's 128 sums a thread)
+constexpr int kControlRegs = 40, kEpiRegs = 232;
+static_assert(128 * kControlRegs + 256 * kEpiRegs <= kThreads * 168, "registers of the launch");
+constexpr int kEpiWarps = 8;
+constexpr int kBM = 128;
+constexpr int kBK = 64;                      // 16-bit values of K to a stage
+constexpr int kABytes = kBM * kBK * 2;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr size_t kPieceBytes = (size_t)128 << 20;   // of g: about what L2 keeps between its kernels
+
+enum { LSE = 0, G = 1, DX = 2, DW = 3 };
+
+constexpr int stage_bytes(int bn) { return kABytes + bn * kBK * 2; }
+constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
+constexpr size_t smem_of(int bn) { return (size_t)stages_of(bn) * stage_bytes(bn) + 1024 + 256; }
+
+// What the kernels of one call share on the device; cleared at its start.
+struct Meta {
+    int err;                 // code of a wait that gave up
+    uint32_t weight_bits;    // largest finite |row weight| as float bits
+    uint32_t w_exp;          // largest exponent of w_jk 2^-s_k, + kExpBias
+    uint32_t poison;         // some left-out row of x holds a value that is not finite
+};
+constexpr int kExpBias = 4096;
+
+// exponent that brings a largest magnitude below 2^14 (0 for nothing to bring)
+__device__ __forceinline__ int fit_exponent(uint32_t max_bits) {
+    if (max_bits == 0) return 0;
+    const int e = (int)(max_bits >> 23) - 127;
+    return min(126, max(-126, 13 - e));
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }   // -126 .. 127
+// v 2^e for any e that two factors reach
+__device__ __forceinline__ float scale2(float v, int e) {
+    e = min(252, max(-252, e));
+    const int h = e / 2;
+    return v * pow2i(h) * pow2i(e - h);
+}
+__device__ __forceinline__ int w_exponent(const Meta* m, int scaled) {
+    if (!scaled || m->w_exp == 0) return 0;
+    return min(126, max(-126, 13 - ((int)m->w_exp - kExpBias)));
+}
+__device__ __forceinline__ int g_exponent(const Meta* m, int half_g) { return half_g ? fit_exponent(m->weight_bits) : 0; }
+
+struct TcArgs {
+    CUtensorMap a[2], b[2];   // planes hi, lo
+    int scaled;               // fp32: power-of-two scales in force
+    int half_g;               // g in fp16 (scaled by 2^u), else bf16
+    int units, m_tiles, n_tiles, splits;
+    int per_split;            // LSE: class tiles of a split; DW: k blocks of a split
+    int k_blocks;
+    int chunk;                // k blocks summed in tensor memory at a time
+    int a_row0, b_row0;       // first row of the piece in the maps of x; of the class piece in that of w
+    int64_t rows;             // valid rows (LSE, G, DX: of x or the piece), DW: classes
+    int64_t row0;             // the piece's first row in labels, loss, dx
+    int64_t cols;             // valid columns: LSE, G: classes (of the piece); DX, DW: features
+    int64_t c_total;
+    int c0;                   // first class of the piece
+    Meta* meta;
+    const uint32_t* colmax;   // [d] largest |x_k| as float bits (fp32)
+    const float* bias2;       // bias in base 2, -inf past the classes
+    const int64_t* labels;
+    float2* part;             // LSE: [n][2 splits] maximum, sum
+    float* zy;                // LSE: label's logit, base 2
+    const float2* shift;      // G: [n] maximum and log2 of the sum
+    const float* loss;        // G
+    const float* weight;
+    int64_t weight_stride;
+    float scale;
+    void* g[2];               // G: planes [rows][ldg]
+    int64_t ldg;
+    float* bias_part;         // G: sums of 32 rows, [row tile x 4][ldg]; null: not wanted
+    void* dx;                 // DX
+    int64_t dxr, dxk;
+    int dx_vec;
+    float* dx_acc;            // DX: sums of earlier class pieces, [tile][BN][128]
+    int first, last;          // DX: first / last class piece; DW: first row piece
+    float* dw_part;           // DW: [split][class tile][feature tile][BN][128]
+    int64_t dw_split_stride;
+    int64_t dw_tile0;         // first tile of the class piece
+    int64_t n_total;          // DW: rows of x
+    const uint32_t* poison;   // DW: bit r of word r / 32: zero that row of x before it is multiplied
+};
+
+__device__ __forceinline__ uint32_t pack(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_dx(const TcArgs& a, int64_t row, int64_t col, int count, const float* v) {
+    T* p = (T*)a.dx + row * a.dxr + col * a.dxk;
+    if (a.dx_vec && count == 32) {
+        constexpr int V = 16 / sizeof(T);
+        #pragma unroll
+        for (int j = 0; j < 32; j += V) {
+            uint4 q;
+            if constexpr (sizeof(T) == 4) {
+                q = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]),
+                               __float_as_uint(v[j + 3]));
+            } else {
+                q = make_uint4(pack(v[j], v[j + 1], T{}), pack(v[j + 2], v[j + 3], T{}), pack(v[j + 4], v[j + 5], T{}),
+                               pack(v[j + 6], v[j + 7], T{}));
+            }
+            *reinterpret_cast<uint4*>(p + j) = q;
+        }
+    } else {
+        #pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < count) p[j * a.dxk] = from_float<T>(v[j]);
+    }
+}
+
+// A unit of work: `tiles` accumulator tiles (m, n), (m, n + 1), ... (more than one only in LSE),
+// each over the k blocks [kb, kb + kn), a.chunk of them at a time in tensor memory.
+struct Unit {
+    int m, n, split, tiles, kb, kn;
+};
+template <int MODE>
+__device__ __forceinline__ Unit unit_of(const TcArgs& a, int u) {
+    Unit t;
+    t.split = 0;
+    t.tiles = 1;
+    t.kb = 0;
+    t.kn = a.k_blocks;
+    if (MODE == LSE) {
+        t.m = u % a.m_tiles;
+        t.split = u / a.m_tiles;
+        t.n = t.split * a.per_split;
+        t.tiles = min(a.per_split, a.n_tiles - t.n);
+    } else if (MODE == G) {
+        t.m = u % a.m_tiles;
+        t.n = u / a.m_tiles;
+    } else if (MODE == DX) {
+        t.n = u % a.n_tiles;
+        t.m = u / a.n_tiles;
+    } else {
+        const int tiles = a.m_tiles * a.n_tiles, tile = u % tiles;
+        t.split = u / tiles;
+        t.n = tile % a.n_tiles;
+        t.m = tile / a.n_tiles;
+        t.kb = t.split * a.per_split;
+        t.kn = max(0, min(a.per_split, a.k_blocks - t.kb));
+    }
+    return t;
+}
+
+// Sums over the warp's lanes of 32 values each: lane j gets the sum of everyone's v[j].  Each
+// step halves what a lane holds: 31 shuffles in place of 32 x 5.
+__device__ __forceinline__ float column_sums(float* v, int lane) {
+    #pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const bool upper = lane & o;
+        #pragma unroll
+        for (int j = 0; j < o; ++j) {
+            const float send = upper ? v[j] : v[j + o], keep = upper ? v[j + o] : v[j];
+            v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    }
+    return v[0];
+}
+
+// v[i] for a run-time i in [0, 32): a select tree
+__device__ __forceinline__ float pick(const float* v, int i) {
+    float t[16];
+    #pragma unroll
+    for (int j = 0; j < 16; ++j) t[j] = i & 16 ? v[j + 16] : v[j];
+    #pragma unroll
+    for (int o = 8; o; o >>= 1)
+        #pragma unroll
+        for (int j = 0; j < o; ++j) t[j] = i & o ? t[j + o] : t[j];
+    return t[0];
+}
+
+// E: type of the operand planes; kPlanes: 1, or hi and lo of fp32
+template <int MODE, int BN, typename E, int kPlanes>
+__global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_constant__ TcArgs a) {
+    constexpr int S = stages_of(BN), kCols = BN / 2;   // ring stages; columns of an epilogue thread
+    constexpr bool kAMn = MODE == DW, kBMn = MODE == DX || MODE == DW;
+    constexpr bool kBf16 = sizeof(E) == 2 && !std::is_same<E, __half>::value;
+    constexpr uint32_t kId = tc::idesc(BN, kBf16, kAMn, kBMn);
+    extern __shared__ uint8_t raw[];
+    const uint32_t base = (tc::smem_addr(raw) + 1023) & ~1023u;
+    uint8_t* gbase = raw + (base - tc::smem_addr(raw));
+    const uint32_t bars = base + S * stage_bytes(BN);
+    const uint32_t full0 = bars, empty0 = bars + 8 * S, afull0 = bars + 16 * S, aempty0 = afull0 + 16,
+                   drain = afull0 + 32, slot = afull0 + 40;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int* err = &a.meta->err;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            tc::bar_init(full0 + 8 * s, 1);
+            tc::bar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            tc::bar_init(afull0 + 8 * s, 1);
+            tc::bar_init(aempty0 + 8 * s, kEpiWarps);
+        }
+        tc::bar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tc::tmem_alloc(slot, 2 * BN);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + (slot - base));
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
+        if (warp == 0) {
+            // ---- loads
+            if (lane == 0) {
+                uint32_t k = 0;   // stages handed out
+                bool ok = true;
+                for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+                    const Unit t = unit_of<MODE>(a, u);
+                    for (int r = 0; ok && r < t.tiles; ++r) {
+                        const int n = t.n + r;
+                        // two planes: a block of K takes two stages, (A hi, B lo) and (A lo, B hi)
+                        for (int i = 0; i < t.kn * kPlanes; ++i, ++k) {
+                            const int kb = t.kb + i / kPlanes;
+                            const CUtensorMap* ma = &a.a[i % kPlanes];
+                            const CUtensorMap* mb = &a.b[kPlanes - 1 - i % kPlanes];
+                            const uint32_t s = k % S, full = full0 + 8 * s;
+                            if (k >= S && !(ok = tc::bar_wait(empty0 + 8 * s, ((k / S) - 1) & 1, err, 1))) break;
+                            tc::bar_expect(full, stage_bytes(BN));
+                            const uint32_t sa = base + s * stage_bytes(BN), sb = sa + kABytes;
+                            if (kAMn) {
+                                tc::load_2d(sa, ma, full, t.m * kBM, kb * kBK);
+                                tc::load_2d(sa + kABytes / 2, ma, full, t.m * kBM + 64, kb * kBK);
+                            } else {
+                                tc::load_2d(sa, ma, full, kb * kBK, a.a_row0 + t.m * kBM);
+                            }
+                            if (kBMn) {
+                                #pragma unroll
+                                for (int q = 0; q < BN / 64; ++q)
+                                    tc::load_2d(sb + q * 8192, mb, full, n * BN + q * 64, a.b_row0 + kb * kBK);
+                            } else {
+                                tc::load_2d(sb, mb, full, kb * kBK, a.b_row0 + n * BN);
+                            }
+                        }
+                    }
+                }
+                if (!ok)   // copies in flight land before the CTA ends
+                    for (uint32_t j = k > S ? k - S : 0; j < k; ++j) tc::bar_wait(full0 + 8 * (j % S), (j / S) & 1, err, 2);
+            }
+        } else if (warp == 1) {
+            // ---- MMAs
+            uint32_t k = 0, acc = 0;
+            bool ok = true;
+            const bool scrub = MODE == DW && a.poison != nullptr && a.meta->poison != 0;
+            for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+                const Unit t = unit_of<MODE>(a, u);
+                const int end = t.tiles * t.kn;
+                for (int i = 0; ok && i < end;) {
+                    // one chunk: the blocks up to a multiple of a.chunk or the tile's end
+                    const int in_tile = i % t.kn, stop = i + min(a.chunk, t.kn - in_tile);
+                    const uint32_t d = tmem + (acc & 1) * BN;
+                    if (acc >= 2 && !(ok = tc::bar_wait_warp(aempty0 + 8 * (acc & 1), ((acc >> 1) - 1) & 1, err, 3))) break;
+                    tc::fence_after();
+                    bool more = false;
+                    for (; i < stop; ++i, k += kPlanes) {
+                        const uint32_t s = k % S;
+                        if (!(ok = tc::bar_wait_warp(full0 + 8 * s, (k / S) & 1, err, 4))) break;
+                        const uint32_t sa = base + s * stage_bytes(BN), sb = sa + kABytes;
+                        if (scrub) {
+                            // rows of x that are left out and not finite: 0 x them would be NaN
+                            const int64_t row = (int64_t)a.b_row0 + (int64_t)(t.kb + i) * kBK;
+                            for (int h = 0; h < 2; ++h) {
+                                uint32_t bits = row + 32 * h < a.n_total ? a.poison[row / 32 + h] : 0;
+                                while (bits) {
+                                    const int q = 32 * h + __ffs(bits) - 1;
+                                    bits &= bits - 1;
+                                    for (int o = lane; o < BN / 64 * 8; o += 32)
+                                        *reinterpret_cast<uint4*>(gbase + (sb - base) + (o >> 3) * 8192 + q * 128 +
+                                                                  (o & 7) * 16) = make_uint4(0, 0, 0, 0);
+                                }
+                            }
+                            tc::fence_async_smem();
+                            __syncwarp();
+                        }
+                        tc::fence_after();
+                        auto multiply = [&](uint32_t pa, uint32_t pb) {
+                            const uint64_t da = tc::desc(pa, kAMn), db = tc::desc(pb, kBMn);
+                            #pragma unroll
+                            for (int j = 0; j < kBK / 16; ++j) {
+                                tc::mma(d, da + j * (kAMn ? 2048 >> 4 : 32 >> 4), db + j * (kBMn ? 2048 >> 4 : 32 >> 4), kId,
+                                        more);
+                                more = true;
+                            }
+                        };
+                        if (lane == 0) multiply(sa, sb);
+                        if (kPlanes == 2) {
+                            // (hi, lo) is under way; (lo, hi), then (hi, hi) across the two stages
+                            const uint32_t s2 = (k + 1) % S, sa2 = base + s2 * stage_bytes(BN), sb2 = sa2 + kABytes;
+                            if (!(ok = tc::bar_wait_warp(full0 + 8 * s2, ((k + 1) / S) & 1, err, 4))) break;
+                            tc::fence_after();
+                            if (lane == 0) {
+                                multiply(sa2, sb2);
+                                multiply(sa, sb2);
+                                tc::commit(empty0 + 8 * s2);
+                            }
+                        }
+                        if (lane == 0) tc::commit(empty0 + 8 * s);
+                        __syncwarp();
+                    }
+                    if (ok && lane == 0) tc::commit(afull0 + 8 * (acc & 1));
+                    ++acc;
+                    __syncwarp();
+                }
+            }
+            // what was issued ends before the tensor memory is handed back
+            if (lane == 0) {
+                tc::commit(drain);
+                tc::bar_wait(drain, 0, err, 5);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ---- epilogues
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        uint32_t acc = 0;
+        bool ok = true;
+        const int te = w_exponent(a.meta, a.scaled), ue = g_exponent(a.meta, a.half_g);
+        const float f = pow2i(-te) * kLog2e;
+        for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+            const Unit t = unit_of<MODE>(a, u);
+            const int64_t row = (int64_t)t.m * kBM + quarter * 32 + lane;
+            const bool valid = row < a.rows;
+            int64_t y = -1;
+            float top = -INFINITY, sum = 0.f, zy = NAN;    // LSE
+            float2 sh = make_float2(0.f, 0.f);             // G
+            float wt = 0.f, gy = 0.f;
+            if (MODE != DW && valid) {
+                y = a.labels[a.row0 + row];
+                if (MODE == G && y >= 0) {
+                    sh = a.shift[a.row0 + row];
+                    wt = (a.weight ? a.weight[(a.row0 + row) * a.weight_stride] : 1.f) * a.scale;
+                    wt = scale2(wt, ue);
+                    // exp(z_y - lse) - 1 from the loss, without the cancellation
+                    gy = expm1f(-a.loss[a.row0 + row]) * wt;
+                    if (y >= a.c_total) wt = NAN;
+                }
+            }
+            for (int r = 0; ok && r < t.tiles && t.kn > 0; ++r) {
+                const int n = t.n + r;
+                // the tile's sums: chunks are added here, rounded to nearest (the tensor cores cut
+                // what falls below an accumulator's last bit, so a long sum there drifts)
+                float sums[kCols];
+                #pragma unroll
+                for (int j = 0; j < kCols; ++j) sums[j] = 0.f;
+                for (int kb = 0; ok && kb < t.kn; kb += a.chunk, ++acc) {
+                    if (!(ok = tc::bar_wait_warp(afull0 + 8 * (acc & 1), (acc >> 1) & 1, err, 6))) break;
+                    tc::fence_after();
+                    #pragma unroll
+                    for (int ch = 0; ch < kCols / 16; ++ch) {
+                        float v[16];
+                        tc::tmem_load16(tmem + (acc & 1) * BN + half * kCols + ch * 16 + lane_addr, v);
+                        #pragma unroll
+                        for (int j = 0; j < 16; ++j) sums[ch * 16 + j] += v[j];
+                    }
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::bar_arrive(aempty0 + 8 * (acc & 1));
+                }
+                if (!ok) break;
+                #pragma unroll
+                for (int ch = 0; ch < kCols / 32; ++ch) {
+                    const int col = half * kCols + ch * 32;
+                    const int64_t cb = (int64_t)n * BN + col;         // column of the piece
+                    if (cb >= a.cols) break;
+                    float* v = sums + ch * 32;
+                    if (MODE == LSE || MODE == G) {
+                        const float4* b4 = reinterpret_cast<const float4*>(a.bias2 + a.c0 + cb);
+                        #pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 b = __ldg(b4 + j);
+                            v[4 * j] = fmaf(v[4 * j], f, b.x);
+                            v[4 * j + 1] = fmaf(v[4 * j + 1], f, b.y);
+                            v[4 * j + 2] = fmaf(v[4 * j + 2], f, b.z);
+                            v[4 * j + 3] = fmaf(v[4 * j + 3], f, b.w);
+                        }
+                    }
+                    // the row's label among these columns
+                    const int64_t rel = y - a.c0 - cb;
+                    const bool here = (MODE == LSE || MODE == G) && rel >= 0 && rel < 32 && y < a.c_total;
+                    uint32_t hit = 0;
+                    if (MODE == LSE || MODE == G) hit = __ballot_sync(0xffffffffu, here);
+                    if (MODE == LSE) {
+                        float m = top;
+                        #pragma unroll
+                        for (int j = 0; j < 32; ++j) m = fmaxf(m, v[j]);
+                        const float shift = m == -INFINITY ? 0.f : m;   // nothing but excluded classes so far
+                        float s = 0.f;
+                        #pragma unroll
+                        for (int j = 0; j < 32; ++j) s += exp2f(v[j] - shift);
+                        sum = sum * exp2f(top - shift) + s;
+                        top = m;
+                        if (hit) {
+                            const float q = pick(v, (int)rel & 31);
+                            if (here) zy = q;
+                        }
+                    } else if (MODE == G) {
+                        #pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float p = exp2f((v[j] - sh.x) - sh.y) * wt;
+                            v[j] = y >= 0 ? p : 0.f;
+                        }
+                        if (valid) {
+                            E* hi = (E*)a.g[0] + row * a.ldg + cb;
+                            E* lo = kPlanes == 2 ? (E*)a.g[1] + row * a.ldg + cb : nullptr;
+                            #pragma unroll
+                            for (int j = 0; j < 32; j += 8) {
+                                if (cb + j >= a.ldg) break;
+                                uint32_t q[4];
+                                #pragma unroll
+                                for (int i = 0; i < 4; ++i) q[i] = pack(v[j + 2 * i], v[j + 2 * i + 1], E{});
+                                *reinterpret_cast<uint4*>(hi + j) = make_uint4(q[0], q[1], q[2], q[3]);
+                                if (kPlanes == 2) {
+                                    #pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        const float h0 = to_float(from_float<E>(v[j + 2 * i]));
+                                        const float h1 = to_float(from_float<E>(v[j + 2 * i + 1]));
+                                        q[i] = pack(v[j + 2 * i] - h0, v[j + 2 * i + 1] - h1, E{});
+                                    }
+                                    *reinterpret_cast<uint4*>(lo + j) = make_uint4(q[0], q[1], q[2], q[3]);
+                                }
+                            }
+                            if (here) {
+                                const E h = from_float<E>(gy);
+                                hi[rel] = h;
+                                if (kPlanes == 2) lo[rel] = from_float<E>(gy - to_float(h));
+                            }
+                        }
+                        if (a.bias_part) {
+                            // the bias's gradient from g before its rounding: 32 rows' sums a column
+                            float c = column_sums(v, lane);
+                            while (hit) {
+                                const int l = __ffs(hit) - 1;
+                                hit &= hit - 1;
+                                const int at = __shfl_sync(0xffffffffu, (int)rel, l);
+                                const float wl = __shfl_sync(0xffffffffu, wt, l);
+                                if (lane == at) c -= wl;
+                            }
+                            if (cb + lane < a.ldg) a.bias_part[((int64_t)t.m * 4 + quarter) * a.ldg + cb + lane] = c;
+                        }
+                    } else if (MODE == DX) {
+                        // unit index as the place of the sums: the same unit of every class piece
+                        float* keep = a.dx_acc + ((int64_t)u * BN + col) * kBM + quarter * 32 + lane;
+                        if (!a.first)
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] += keep[j * kBM];
+                        if (!a.last) {
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) keep[j * kBM] = v[j];
+                        } else if (valid) {
+                            const int count = (int)min((int64_t)32, a.cols - cb);
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                int e = -ue - te;
+                                if (kPlanes == 2 && j < count) e += fit_exponent(a.colmax[cb + j]);
+                                v[j] = y >= 0 ? scale2(v[j], e) : 0.f;
+                            }
+                            if (kPlanes == 2)
+                                store_dx<float>(a, a.row0 + row, cb, count, v);
+                            else
+                                store_dx<E>(a, a.row0 + row, cb, count, v);
+                        }
+                    } else {
+                        float* p = a.dw_part + t.split * a.dw_split_stride +
+                                   ((a.dw_tile0 + (int64_t)t.m * a.n_tiles + n) * BN + col) * kBM + quarter * 32 + lane;
+                        if (!a.first)
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] += p[j * kBM];
+                        #pragma unroll
+                        for (int j = 0; j < 32; ++j) p[j * kBM] = v[j];
+                    }
+                }
+            }
+            if (MODE == LSE && valid) {
+                a.part[row * (2 * a.splits) + 2 * t.split + half] = make_float2(top, sum);
+                if (!isnan(zy)) a.zy[row] = zy;   // one thread of all has the label's column
+            }
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 1) tc::tmem_free(tmem, 2 * BN);
+}
+
+// ---- before the products ---------------------------------------------------------------
+
+struct SetupArgs {
+    const int64_t* labels;
+    int64_t n;
+    const float* weight;      // nullable
+    int64_t weight_stride;
+    float scale;
+    int want_weight;          // largest row weight
+    const void* x;            // poison: 16-bit x read in place
+    int64_t xr, xk, d;
+    int bf16;
+    uint32_t* poison;         // nullable
+    const float* bias;
+    float* bias2;
+    int64_t c, c_pad;
+    float* zy;                // nullable: cleared to NaN
+    Meta* meta;
+};
+
+__global__ void __launch_bounds__(256) xent_setup_kernel(SetupArgs a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t gt = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = gt; i < a.c_pad; i += all)
+        a.bias2[i] = i < a.c ? (a.bias ? a.bias[i] * kLog2e : 0.f) : -INFINITY;
+    if (!a.want_weight && !a.poison && !a.zy) return;
+    float top = 0.f;
+    for (int64_t w = gt / 32; w < (a.n + 31) / 32; w += all / 32) {
+        const int64_t r = w * 32 + lane;
+        const bool in = r < a.n;
+        const bool kept = in && a.labels[r] >= 0;
+        if (a.zy && in) a.zy[r] = NAN;
+        if (a.want_weight && kept) {
+            const float v = fabsf((a.weight ? a.weight[r * a.weight_stride] : 1.f) * a.scale);
+            if (v <= 3.402823466e38f) top = fmaxf(top, v);
+        }
+        if (a.poison) {
+            uint32_t out = __ballot_sync(0xffffffffu, in && !kept), bad = 0;
+            while (out) {
+                const int q = __ffs(out) - 1;
+                out &= out - 1;
+                bool b = false;
+                const uint16_t* p = (const uint16_t*)a.x + (w * 32 + q) * a.xr;
+                const uint16_t inf = a.bf16 ? 0x7f80 : 0x7c00;
+                for (int64_t k = lane; k < a.d; k += 32) b |= (p[k * a.xk] & inf) == inf;
+                if (__any_sync(0xffffffffu, b)) bad |= 1u << q;
+            }
+            if (lane == 0) {
+                a.poison[w] = bad;
+                if (bad) a.meta->poison = 1;
+            }
+        }
+    }
+    if (a.want_weight) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (lane == 0 && m) atomicMax(&a.meta->weight_bits, m);
+    }
+}
+
+// lse and loss of a row from its partial maxima and sums; with the sums given (have_lse), only
+// the shift that g subtracts
+__global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part, int parts, const float* zy,
+                                                        const int64_t* labels, int64_t n, int have_lse, float* loss,
+                                                        float* lse, float2* shift, const Meta* meta) {
+    const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (r >= n) return;
+    if (have_lse) {
+        const double l2 = (double)lse[r] * 1.4426950408889634074;
+        const float hi = (float)l2;
+        shift[r] = make_float2(hi, isfinite(hi) ? (float)(l2 - hi) : 0.f);
+        return;
+    }
+    float m = -INFINITY;
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, part[r * parts + i].x);
+    const float sh = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+    for (int i = 0; i < parts; ++i) {
+        const float2 p = part[r * parts + i];
+        s += p.y * exp2f(p.x - sh);
+    }
+    const float l = log2f(s);
+    if (shift) shift[r] = make_float2(sh, l);
+    const bool kept = labels[r] >= 0;
+    const bool failed = meta->err != 0;
+    loss[r] = failed ? NAN : kept ? ((sh - zy[r]) + l) * kLn2 : 0.f;
+    if (lse) lse[r] = failed ? NAN : kept ? (float)(((double)sh + (double)l) * 0.69314718055994530942) : 0.f;
+}
+
+// largest finite |x_k| over the rows that count
+__global__ void __launch_bounds__(256) xent_colmax_kernel(const float* __restrict__ x, int64_t xr, int64_t xk,
+                                                          const int64_t* __restrict__ labels, int64_t n, int64_t d,
+                                                          int64_t rows, uint32_t* colmax) {
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t tiles_k = (d + 31) / 32;
+    const int64_t k0 = (blockIdx.x % tiles_k) * 32, r0 = (blockIdx.x / tiles_k) * rows;
+    const int64_t r1 = min(n, r0 + rows);
+    __shared__ uint32_t top[32];
+    if (threadIdx.x < 32) top[threadIdx.x] = 0;
+    __syncthreads();
+    if (xr == 1 && xk != 1) {
+        // a warp goes down one feature
+        for (int j = ty; j < 32 && k0 + j < d; j += 8) {
+            float m = 0.f;
+            for (int64_t r = r0 + tx; r < r1; r += 32) {
+                const float v = fabsf(x[r + (k0 + j) * xk]);
+                if (labels[r] >= 0 && v <= 3.402823466e38f) m = fmaxf(m, v);
+            }
+            const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+            if (tx == 0) top[j] = w;
+        }
+    } else {
+        float m = 0.f;
+        if (k0 + tx < d)
+            for (int64_t r = r0 + ty; r < r1; r += 8) {
+                const float v = fabsf(x[r * xr + (k0 + tx) * xk]);
+                if (labels[r] >= 0 && v <= 3.402823466e38f) m = fmaxf(m, v);
+            }
+        atomicMax(&top[tx], __float_as_uint(m));
+    }
+    __syncthreads();
+    if (threadIdx.x < 32 && k0 + threadIdx.x < d && top[threadIdx.x]) atomicMax(&colmax[k0 + threadIdx.x], top[threadIdx.x]);
+}
+
+// largest exponent of w_jk 2^-s_k
+__global__ void __launch_bounds__(256) xent_wmax_kernel(const float* __restrict__ w, int64_t wr, int64_t wk, int64_t c,
+                                                        int64_t d, const uint32_t* __restrict__ colmax, Meta* meta) {
+    int top = 0;
+    const int64_t all = c * d;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t j = wk == 1 ? i / d : i % c, k = wk == 1 ? i % d : i / c;
+        const uint32_t b = __float_as_uint(w[j * wr + k * wk]) & 0x7fffffffu;
+        if (b && b < 0x7f800000u) top = max(top, (int)(b >> 23) - 127 - fit_exponent(colmax[k]) + kExpBias);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0 && top) atomicMax(&meta->w_exp, (uint32_t)top);
+}
+
+// rows x d of any strides -> planes [rows][dp]; rows with a negative label become zeros.
+// fp32: hi and lo fp16 of the scaled value; 16 bits: a copy.
+template <typename T, typename E>
+__global__ void __launch_bounds__(256) xent_planes_kernel(const T* __restrict__ x, int64_t xr, int64_t xk,
+                                                          const int64_t* __restrict__ labels, int64_t n, int64_t d,
+                                                          int64_t dp, const uint32_t* __restrict__ colmax,
+                                                          const Meta* __restrict__ meta, int is_w, E* __restrict__ hi,
+                                                          E* __restrict__ lo) {
+    __shared__ float t[64][65];
+    const int64_t tiles_k = (dp + 63) / 64;
+    const int64_t k0 = (blockIdx.x % tiles_k) * 64, r0 = (blockIdx.x / tiles_k) * 64;
+    const bool down = xr == 1 && xk != 1;
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int r = down ? i & 63 : i >> 6, k = down ? i >> 6 : i & 63;
+        float v = 0.f;
+        if (r0 + r < n && k0 + k < d && (!labels || labels[r0 + r] >= 0)) v = to_float(x[(r0 + r) * xr + (k0 + k) * xk]);
+        t[r][k] = v;
+    }
+    __syncthreads();
+    const int k = (threadIdx.x & 31) * 2;
+    if (k0 + k >= dp) return;
+    int e0 = 0, e1 = 0;
+    if (sizeof(T) == 4) {
+        const int te = w_exponent(meta, 1);
+        const int s0 = k0 + k < d ? fit_exponent(colmax[k0 + k]) : 0, s1 = k0 + k + 1 < d ? fit_exponent(colmax[k0 + k + 1]) : 0;
+        e0 = is_w ? te - s0 : s0;
+        e1 = is_w ? te - s1 : s1;
+    }
+    for (int r = threadIdx.x >> 5; r < 64 && r0 + r < n; r += 8) {
+        float v0 = t[r][k], v1 = t[r][k + 1];
+        const int64_t at = (r0 + r) * dp + k0 + k;
+        if (sizeof(T) == 4) {
+            v0 = scale2(v0, e0);
+            v1 = scale2(v1, e1);
+            const float h0 = to_float(from_float<E>(v0)), h1 = to_float(from_float<E>(v1));
+            *reinterpret_cast<uint32_t*>(hi + at) = pack(v0, v1, E{});
+            // nothing below a value that is not finite
+            *reinterpret_cast<uint32_t*>(lo + at) = pack(isfinite(h0) ? v0 - h0 : 0.f, isfinite(h1) ? v1 - h1 : 0.f, E{});
+        } else {
+            *reinterpret_cast<uint32_t*>(hi + at) = pack(v0, v1, E{});
+        }
+    }
+}
+
+// ---- after the products ----------------------------------------------------------------
+
+// the bias's gradient from sums of 32 rows: 32 columns a block, one split of the lines
+__global__ void __launch_bounds__(256) xent_colsum_kernel(const float* __restrict__ sums, int64_t ldg, int64_t lines,
+                                                          int64_t cols, int64_t per_split, int first,
+                                                          double* __restrict__ part, int64_t c_total, int64_t c0) {
+    __shared__ double s[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + tx;
+    const int64_t r0 = blockIdx.y * per_split, r1 = min(lines, r0 + per_split);
+    double v = 0.0;
+    if (col < cols) {
+        #pragma unroll 4
+        for (int64_t r = r0 + ty; r < r1; r += 8) v += (double)sums[r * ldg + col];
+    }
+    s[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && col < cols) {
+        v = 0.0;
+        for (int i = 0; i < 8; ++i) v += s[i][tx];
+        double* p = part + blockIdx.y * c_total + c0 + col;
+        *p = first ? v : *p + v;
+    }
+}
+
+// dw from the splits' partial sums, and dbias
+template <typename T>
+__global__ void __launch_bounds__(256) xent_dw_kernel(const float* __restrict__ part, int splits, int64_t split_stride,
+                                                      int64_t n_tiles, int bn, int64_t c, int64_t d,
+                                                      const uint32_t* __restrict__ colmax, int scaled, int half_g,
+                                                      const Meta* __restrict__ meta, T* __restrict__ dw,
+                                                      const double* __restrict__ bias_part, int bias_splits,
+                                                      float* __restrict__ dbias) {
+    __shared__ float t[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const bool failed = meta->err != 0;
+    const int ue = g_exponent(meta, half_g);
+    const int64_t tiles_k = (d + 31) / 32;
+    const int64_t k0 = (blockIdx.x % tiles_k) * 32, c0 = (blockIdx.x / tiles_k) * 32;
+    if (dbias && k0 == 0 && ty == 0 && c0 + tx < c) {
+        double v = 0.0;
+        for (int s = 0; s < bias_splits; ++s) v += bias_part[s * c + c0 + tx];
+        dbias[c0 + tx] = failed ? NAN : (float)ldexp(v, -ue);
+    }
+    if (!dw) return;
+    for (int j = ty; j < 32; j += 8) {
+        double v = 0.0;
+        if (k0 + j < d && c0 + tx < c) {
+            const int64_t k = k0 + j;
+            const float* p = part + (((c0 / kBM) * n_tiles + k / bn) * bn + k % bn) * kBM + c0 % kBM + tx;
+            #pragma unroll 4
+            for (int s = 0; s < splits; ++s) v += (double)p[s * split_stride];
+            v = ldexp(v, -ue - (scaled ? fit_exponent(colmax[k]) : 0));
+        }
+        t[j][tx] = (float)v;
+    }
+    __syncthreads();
+    for (int j = ty; j < 32; j += 8)
+        if (c0 + j < c && k0 + tx < d) dw[(c0 + j) * d + k0 + tx] = from_float<T>(failed ? NAN : t[tx][j]);
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+    });
+    return fn;
+}
+
+// rows of `inner` 16-bit values, `ld` apart; boxes of 64 values x box_rows
+bool make_map(CUtensorMap* map, bool bf16, const void* base, int64_t inner, int64_t rows, int64_t ld, int box_rows) {
+    auto enc = encoder();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)base, dims,
+               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// columns of an accumulator tile: the smallest that holds the axis, 256 past that
+int tile_n(int64_t cols) { return cols <= 64 ? 64 : cols <= 128 ? 128 : 256; }
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// TMA reads 16-bit rows in place: contiguous rows, 16-byte aligned base and pitch
+bool in_place(int type, const void* p, int64_t row, int64_t col, int64_t len) {
+    return type != GAFIME_TYPE_FP32 && col == 1 && row >= len && (uintptr_t)p % 16 == 0 && row % 8 == 0;
+}
+
+struct Plan {
+    int planes, bn_c, bn_d;
+    bool x_in_place, w_in_place;
+    int64_t dp;
+    int64_t m_tiles, c_tiles;        // of the whole call
+    int splits, per_split;           // LSE
+    int64_t piece_rows, piece_classes, ldg;
+    int64_t dw_c_tiles, dw_d_tiles;  // 128 classes x bn_d features
+    int dw_splits, dw_per_split;
+    int bias_splits;
+    bool products;                   // dx or dw or dbias wanted
+    // workspace
+    Meta* meta;
+    uint32_t* colmax;
+    size_t meta_bytes;
+    float* bias2;
+    uint32_t* poison;
+    uint16_t *xh, *xl, *wh, *wl, *gh, *gl;
+    float2* part;
+    float* zy;
+    float2* shift;
+    float* dx_acc;
+    float* dw_part;
+    float* bias_sums;
+    double* bias_part;
+    size_t bytes;
+};
+
+Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
+    Plan p{};
+    p.planes = a.type == GAFIME_TYPE_FP32 ? 2 : 1;
+    p.bn_c = tile_n(a.c);
+    p.bn_d = tile_n(a.d);
+    p.x_in_place = in_place(a.type, a.x, a.xr, a.xk, a.d);
+    p.w_in_place = in_place(a.type, a.w, a.wr, a.wk, a.d);
+    p.dp = up(a.d, 8);
+    p.m_tiles = std::max<int64_t>(1, cdiv(a.n, kBM));
+    p.c_tiles = cdiv(a.c, p.bn_c);
+    // LSE: enough units of (row tile, run of class tiles) for every SM
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(p.c_tiles, cdiv(2 * sms, p.m_tiles)));
+    p.per_split = (int)cdiv(p.c_tiles, p.m_tiles >= 2 * sms ? 1 : want);
+    p.splits = (int)cdiv(p.c_tiles, p.per_split);
+    p.products = a.gradient && (a.dx || a.dw || a.dbias) && a.n > 0;
+
+    Carver cv(ws);
+    p.meta = cv.take<Meta>(1);
+    p.colmax = cv.take<uint32_t>(p.planes == 2 ? a.d : 0);
+    p.meta_bytes = cv.used;
+    p.bias2 = cv.take<float>(p.c_tiles * p.bn_c + 256);
+    if (p.planes == 2 || !p.x_in_place) p.xh = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
+    if (p.planes == 2) p.xl = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
+    if (p.planes == 2 || !p.w_in_place) p.wh = cv.take<uint16_t>(a.c * p.dp);
+    if (p.planes == 2) p.wl = cv.take<uint16_t>(a.c * p.dp);
+    p.part = cv.take<float2>(a.n * 2 * p.splits);
+    p.zy = cv.take<float>(a.n);
+    if (p.products) {
+        p.shift = cv.take<float2>(a.n);
+        if (p.x_in_place && a.dw) p.poison = cv.take<uint32_t>(cdiv(a.n, 32) + 2);
+        // a piece of g: rows for one row tile an SM, then as many classes as kPieceBytes hold
+        const int64_t es = 2 * p.planes;
+        p.piece_rows = std::min<int64_t>(up(a.n, kBM), (int64_t)sms * kBM);
+        p.piece_classes = std::max<int64_t>(1024, (int64_t)(kPieceBytes / (p.piece_rows * es)) / 256 * 256);
+        if (p.piece_classes >= a.c) {
+            p.piece_classes = a.c;
+            // few classes: more rows at once, still whole rounds of the SMs
+            const int64_t more = (int64_t)(kPieceBytes / (p.piece_rows * es * up(a.c, 8)));
+            if (more > 1) p.piece_rows = std::min<int64_t>(up(a.n, kBM), p.piece_rows * more);
+        }
+        p.ldg = up(p.piece_classes, 8);
+        p.gh = cv.take<uint16_t>(p.piece_rows * p.ldg);
+        if (p.planes == 2) p.gl = cv.take<uint16_t>(p.piece_rows * p.ldg);
+        p.dw_d_tiles = cdiv(a.d, p.bn_d);
+        p.dw_c_tiles = cdiv(a.c, kBM);
+        if (a.dx && p.piece_classes < a.c)
+            p.dx_acc = cv.take<float>(cdiv(p.piece_rows, kBM) * p.dw_d_tiles * p.bn_d * kBM);
+        if (a.dw) {
+            const int64_t tiles = cdiv(p.piece_classes, kBM) * p.dw_d_tiles, blocks = cdiv(std::min(a.n, p.piece_rows), kBK);
+            const int64_t s = std::max<int64_t>(1, std::min<int64_t>(sms / tiles, blocks / 4));
+            p.dw_per_split = (int)cdiv(blocks, s);
+            p.dw_splits = (int)cdiv(blocks, p.dw_per_split);
+            p.dw_part = cv.take<float>(p.dw_splits * p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM);
+        }
+        if (a.dbias) {
+            const int64_t blocks = cdiv(p.piece_classes, 32);
+            p.bias_splits = (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(4 * sms, blocks), cdiv(p.piece_rows, 32 * 16)));
+            p.bias_sums = cv.take<float>(p.piece_rows / 32 * p.ldg);
+            p.bias_part = cv.take<double>(p.bias_splits * a.c);
+        }
+    }
+    p.bytes = cv.used;
+    return p;
+}
+
+template <int MODE, int BN, typename E, int kPlanes>
+cudaError_t launch_bn(const TcArgs& t, int sms, cudaStream_t stream) {
+    auto fn = xent_tc_kernel<MODE, BN, E, kPlanes>;
+    cudaError_t e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(BN));
+    if (e != cudaSuccess) return e;
+    // the epilogues take their registers from the launch's: one that has fewer would wait for good
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, (const void*)fn);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs * kThreads < 128 * kControlRegs + 256 * kEpiRegs) return cudaErrorLaunchOutOfResources;
+    KernelTimer kt(stream, GAFIME_KERNEL_XENT_TC);
+    fn<<<std::min(sms, t.units), kThreads, smem_of(BN), stream>>>(t);
+    return cudaGetLastError();
+}
+template <int MODE, typename E, int kPlanes>
+cudaError_t launch(const TcArgs& t, int bn, int sms, cudaStream_t stream) {
+    if (t.units <= 0) return cudaSuccess;
+    switch (bn) {
+        case 64: return launch_bn<MODE, 64, E, kPlanes>(t, sms, stream);
+        case 128: return launch_bn<MODE, 128, E, kPlanes>(t, sms, stream);
+        default: return launch_bn<MODE, 256, E, kPlanes>(t, sms, stream);
+    }
+}
+
+#define XENT_TRY(expr)                                \
+    do {                                              \
+        const cudaError_t e_ = (expr);                \
+        if (e_ != cudaSuccess) return e_;             \
+    } while (0)
+
+template <typename T, typename E>
+cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const int64_t* labels, int64_t rows, int64_t d,
+                   bool is_w, uint16_t* hi, uint16_t* lo, cudaStream_t stream) {
+    if (rows == 0) return cudaSuccess;
+    const int64_t blocks = cdiv(p.dp, 64) * cdiv(rows, 64);
+    KernelTimer kt(stream, GAFIME_KERNEL_XENT);
+    xent_planes_kernel<T, E><<<(unsigned)blocks, 256, 0, stream>>>(src, sr, sk, labels, rows, d, p.dp, p.colmax, p.meta,
+                                                                   is_w, (E*)hi, (E*)lo);
+    return cudaGetLastError();
+}
+
+template <typename T, typename E>
+cudaError_t run_tc(const XentCall& a, int sms) {
+    const Plan p = make_plan(a, sms, a.ws);
+    constexpr bool kBf16 = std::is_same<E, __nv_bfloat16>::value;
+    constexpr int kPlanes = std::is_same<T, float>::value ? 2 : 1;
+    const bool scaled = p.planes == 2;
+    cudaStream_t st = a.stream;
+    if (a.n == 0) {   // gradients of no rows
+        if (a.dw) XENT_TRY(cudaMemsetAsync(a.dw, 0, (size_t)(a.c * a.d) * sizeof(T), st));
+        if (a.dbias) XENT_TRY(cudaMemsetAsync(a.dbias, 0, a.c * 4, st));
+        return cudaSuccess;
+    }
+    XENT_TRY(cudaMemsetAsync(p.meta, 0, p.meta_bytes, st));
+    const bool forward = !a.have_lse;
+    {
+        SetupArgs s{};
+        s.labels = a.labels; s.n = a.n; s.weight = a.weight; s.weight_stride = a.weight_stride; s.scale = a.scale;
+        s.want_weight = p.products && !kBf16;
+        s.x = a.x; s.xr = a.xr; s.xk = a.xk; s.d = a.d; s.bf16 = kBf16;
+        s.poison = p.poison;
+        s.bias = a.bias; s.bias2 = p.bias2; s.c = a.c; s.c_pad = p.c_tiles * p.bn_c + 256;
+        s.zy = forward ? p.zy : nullptr;
+        s.meta = p.meta;
+        const int64_t threads = std::max<int64_t>(s.c_pad, p.poison ? a.n * 8 : a.n);
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_setup_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(8 * sms, cdiv(threads, 256))), 256, 0, st>>>(s);
+        XENT_TRY(cudaGetLastError());
+    }
+    if (scaled) {
+        {
+            const int64_t tiles_k = cdiv(a.d, 32);
+            const int64_t rows = std::max<int64_t>(64, cdiv(a.n * tiles_k, 8 * sms));
+            KernelTimer kt(st, GAFIME_KERNEL_XENT);
+            xent_colmax_kernel<<<(unsigned)(tiles_k * cdiv(a.n, rows)), 256, 0, st>>>((const float*)a.x, a.xr, a.xk, a.labels,
+                                                                                   a.n, a.d, rows, p.colmax);
+            XENT_TRY(cudaGetLastError());
+        }
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_wmax_kernel<<<(unsigned)std::min<int64_t>(8 * sms, cdiv(a.c * a.d, 1024)), 256, 0, st>>>(
+            (const float*)a.w, a.wr, a.wk, a.c, a.d, p.colmax, p.meta);
+        XENT_TRY(cudaGetLastError());
+    }
+    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, p.xh, p.xl, st)));
+    if (p.wh) XENT_TRY((planes<T, E>(p, (const T*)a.w, a.wr, a.wk, nullptr, a.c, a.d, true, p.wh, p.wl, st)));
+    // where the operands are read
+    const void *xs[2] = {p.xh ? (const void*)p.xh : a.x, p.xl}, *ws[2] = {p.wh ? (const void*)p.wh : a.w, p.wl};
+    const int64_t ldx = p.xh ? p.dp : a.xr, ldw = p.wh ? p.dp : a.wr;
+    auto map = [&](CUtensorMap (&m)[2], const void* const (&base)[2], int64_t inner, int64_t rows, int64_t ld, int box) {
+        for (int i = 0; i < p.planes; ++i)
+            if (!make_map(&m[i], kBf16, base[i], inner, rows, ld, box)) return cudaErrorInvalidValue;
+        return cudaSuccess;
+    };
+
+    TcArgs t{};
+    t.chunk = p.planes == 2 ? 1 : 4;
+    t.scaled = scaled;
+    t.half_g = !kBf16;
+    t.meta = p.meta;
+    t.colmax = p.colmax;
+    t.bias2 = p.bias2;
+    t.labels = a.labels;
+    t.weight = a.weight; t.weight_stride = a.weight_stride; t.scale = a.scale;
+    t.c_total = a.c;
+    t.splits = p.splits;
+    if (forward) {
+        TcArgs l = t;
+        XENT_TRY(map(l.a, xs, a.d, a.n, ldx, kBM));
+        XENT_TRY(map(l.b, ws, a.d, a.c, ldw, p.bn_c));
+        l.m_tiles = (int)p.m_tiles;
+        l.n_tiles = (int)p.c_tiles;
+        l.per_split = p.per_split;
+        l.units = l.m_tiles * p.splits;
+        l.k_blocks = (int)cdiv(a.d, kBK);
+        l.rows = a.n;
+        l.cols = a.c;
+        l.part = p.part;
+        l.zy = p.zy;
+        XENT_TRY((launch<LSE, E, kPlanes>(l, p.bn_c, sms, st)));
+    }
+    if (forward || p.products) {
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_join_kernel<<<(unsigned)cdiv(a.n, 256), 256, 0, st>>>(p.part, 2 * p.splits, p.zy, a.labels, a.n, !forward,
+                                                                   a.loss, a.lse, p.products ? p.shift : nullptr, p.meta);
+        XENT_TRY(cudaGetLastError());
+    }
+    if (!p.products) return cudaSuccess;
+
+    const void* gs[2] = {p.gh, p.gl};
+    for (int64_t r0 = 0; r0 < a.n; r0 += p.piece_rows) {
+        const int64_t rows = std::min(p.piece_rows, a.n - r0);
+        for (int64_t c0 = 0; c0 < a.c; c0 += p.piece_classes) {
+            const int64_t classes = std::min(p.piece_classes, a.c - c0);
+            TcArgs g = t;
+            XENT_TRY(map(g.a, xs, a.d, a.n, ldx, kBM));
+            XENT_TRY(map(g.b, ws, a.d, a.c, ldw, p.bn_c));
+            g.m_tiles = (int)cdiv(rows, kBM);
+            g.n_tiles = (int)cdiv(classes, p.bn_c);
+            g.units = g.m_tiles * g.n_tiles;
+            g.k_blocks = (int)cdiv(a.d, kBK);
+            g.a_row0 = (int)r0;
+            g.b_row0 = (int)c0;
+            g.rows = rows;
+            g.row0 = r0;
+            g.cols = classes;
+            g.c0 = (int)c0;
+            g.shift = p.shift;
+            g.loss = a.loss;
+            g.g[0] = p.gh;
+            g.g[1] = p.gl;
+            g.ldg = p.ldg;
+            g.bias_part = a.dbias ? p.bias_sums : nullptr;
+            XENT_TRY((launch<G, E, kPlanes>(g, p.bn_c, sms, st)));
+            if (a.dbias) {
+                const int64_t lines = g.m_tiles * 4;
+                KernelTimer kt(st, GAFIME_KERNEL_XENT);
+                xent_colsum_kernel<<<dim3((unsigned)cdiv(classes, 32), (unsigned)p.bias_splits), 256, 0, st>>>(
+                    p.bias_sums, p.ldg, lines, classes, cdiv(p.piece_rows / 32, p.bias_splits), r0 == 0, p.bias_part,
+                    a.c, c0);
+                XENT_TRY(cudaGetLastError());
+            }
+            if (a.dx) {
+                TcArgs x = t;
+                XENT_TRY(map(x.a, gs, classes, rows, p.ldg, kBM));
+                // the piece's classes of w
+                const void* wp[2] = {(const uint16_t*)ws[0] + c0 * ldw, ws[1] ? (const uint16_t*)ws[1] + c0 * ldw : nullptr};
+                XENT_TRY(map(x.b, wp, a.d, classes, ldw, kBK));
+                x.m_tiles = (int)cdiv(rows, kBM);
+                x.n_tiles = (int)p.dw_d_tiles;
+                x.units = x.m_tiles * x.n_tiles;
+                x.k_blocks = (int)cdiv(classes, kBK);
+                x.rows = rows;
+                x.row0 = r0;
+                x.cols = a.d;
+                x.dx = a.dx; x.dxr = a.dxr; x.dxk = a.dxk;
+                x.dx_vec = a.dxk == 1 && (uintptr_t)a.dx % 16 == 0 && a.dxr * (int64_t)sizeof(T) % 16 == 0;
+                x.dx_acc = p.dx_acc;
+                x.first = c0 == 0;
+                x.last = c0 + classes == a.c;
+                XENT_TRY((launch<DX, E, kPlanes>(x, p.bn_d, sms, st)));
+            }
+            if (a.dw) {
+                TcArgs w = t;
+                XENT_TRY(map(w.a, gs, classes, rows, p.ldg, kBK));
+                XENT_TRY(map(w.b, xs, a.d, a.n, ldx, kBK));
+                w.m_tiles = (int)cdiv(classes, kBM);
+                w.n_tiles = (int)p.dw_d_tiles;
+                w.units = w.m_tiles * w.n_tiles * p.dw_splits;
+                w.per_split = p.dw_per_split;
+                w.k_blocks = (int)cdiv(rows, kBK);
+                w.b_row0 = (int)r0;
+                w.row0 = r0;
+                w.n_total = a.n;
+                w.rows = classes;
+                w.cols = a.d;
+                w.first = r0 == 0;
+                w.dw_part = p.dw_part;
+                w.dw_split_stride = p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM;
+                w.dw_tile0 = c0 / kBM * p.dw_d_tiles;
+                w.poison = p.poison;
+                XENT_TRY((launch<DW, E, kPlanes>(w, p.bn_d, sms, st)));
+            }
+        }
+    }
+    if (a.dw || a.dbias) {
+        const int64_t blocks = cdiv(a.c, 32) * (a.dw ? cdiv(a.d, 32) : 1);
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_dw_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(
+            p.dw_part, p.dw_splits, p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM, p.dw_d_tiles, p.bn_d, a.c,
+            a.dw ? a.d : 1, p.colmax, scaled, !kBf16, p.meta, (T*)a.dw, p.bias_part, p.bias_splits, a.dbias);
+        XENT_TRY(cudaGetLastError());
+    }
+    return cudaSuccess;
+}
+
+}  // namespace
+
+size_t xent_tc_workspace(const XentCall& a, int sms) { return make_plan(a, sms, nullptr).bytes; }
+
+cudaError_t xent_tc(const XentCall& a, int sms) {
+    switch (a.type) {
+        case GAFIME_TYPE_FP32: return run_tc<float, __half>(a, sms);
+        case GAFIME_TYPE_FP16: return run_tc<__half, __half>(a, sms);
+        default: return run_tc<__nv_bfloat16, __nv_bfloat16>(a, sms);
+    }
+}
+
+}  // namespace gafime

@@ -1,0 +1,247 @@
+"""Operators of a linear softmax head on torch CUDA tensors: cross entropy over many classes
+without keeping the logits, with its gradients, and the gradients' global norm with clipping.
+
+They are what ``GafimeEngine``'s joint fit runs on, and the step of any head trained on the
+features and interactions a selector leaves.  Everything is queued on torch's current stream of
+the tensors' device; nothing waits, and calls can be captured into a CUDA graph.  Scratch memory
+comes from torch's allocator.  The kernels are those of ``gafime_xent_*`` and
+``gafime_grad_norm`` in libgafime_cuda.so; there is no other path.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from . import _native
+
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_DX, _DW, _DBIAS, _GRADIENT = 1, 2, 4, 8
+
+
+class XentGrad(NamedTuple):
+    """Result of softmax_xent_grad."""
+
+    loss: torch.Tensor                  # (n,) float32
+    lse: torch.Tensor                   # (n,) float32
+    dx: Optional[torch.Tensor]          # (n, d), x's type and order
+    dw: Optional[torch.Tensor]          # (c, d), w's type
+    dbias: Optional[torch.Tensor]       # (c,) float32
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(device: int, type_id: int, x_off: int, xr: int, xk: int, w_off: int, wr: int, wk: int,
+                     n: int, d: int, c: int, want: int) -> int:
+    """Of sizes, strides and alignments alone (x_off, w_off: addresses modulo 16)."""
+    out = ctypes.c_size_t(0)
+    lib = _native.load(require_gpu=False)
+    _native.check("gafime_xent_workspace", lib.gafime_xent_workspace(
+        type_id, 256 + x_off, xr, xk, 256 + w_off, wr, wk, n, d, c, want, ctypes.byref(out)))
+    return out.value
+
+
+def _check(x, w, labels, bias, row_weight):
+    if not isinstance(x, torch.Tensor) or not isinstance(w, torch.Tensor) or not isinstance(labels, torch.Tensor):
+        raise TypeError("x, w and labels must be torch tensors")
+    if x.dim() != 2 or w.dim() != 2 or labels.dim() != 1:
+        raise ValueError("x must be (n, d), w (c, d) and labels (n,)")
+    n, d = x.shape
+    c = w.shape[0]
+    if w.shape[1] != d or labels.shape[0] != n:
+        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, w {tuple(w.shape)}, labels {tuple(labels.shape)}")
+    if d < 1 or c < 1:
+        raise ValueError("at least one feature and one class are needed")
+    if x.dtype not in TYPES or w.dtype != x.dtype:
+        raise TypeError(f"x and w must both be float32, float16 or bfloat16, got {x.dtype} and {w.dtype}")
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"labels must be int64 or int32, got {labels.dtype}")
+    if bias is not None and (bias.shape != (c,) or bias.dtype != torch.float32):
+        raise ValueError(f"bias must be a float32 ({c},) tensor")
+    if row_weight is not None and (row_weight.shape != (n,) or row_weight.dtype != torch.float32):
+        raise ValueError(f"row_weight must be a float32 ({n},) tensor")
+    device = x.device
+    for name, t in (("x", x), ("w", w), ("labels", labels), ("bias", bias), ("row_weight", row_weight)):
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise ValueError(f"{name} must be on the GPU that holds x, got {t.device}")
+    return n, d, c
+
+
+def _call(x, w, labels, bias, n, d, c, want, row_weight=None, scale=1.0, loss=None, lse=None, dx=None, dw=None,
+          dbias=None):
+    """One library call on the current stream of x's device; loss and lse given: read, not written."""
+    lib = _native.load()
+    type_id = TYPES[x.dtype]
+    xp, wp = x.data_ptr(), w.data_ptr()
+    xr, xk = x.stride()
+    wr, wk = w.stride()
+    index = x.device.index
+    have = loss is not None
+    if labels.dtype != torch.int64 or (n > 1 and labels.stride(0) != 1):
+        labels = labels.to(torch.int64).contiguous()
+    if bias is not None and c > 1 and bias.stride(0) != 1:
+        bias = bias.contiguous()
+    with torch.cuda.device(index):
+        size = _workspace_bytes(index, type_id, xp % 16, xr, xk, wp % 16, wr, wk, n, d, c, want)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        if not have:
+            loss = torch.empty(n, dtype=torch.float32, device=x.device)
+            lse = torch.empty(n, dtype=torch.float32, device=x.device)
+        stream = torch.cuda.current_stream(index).cuda_stream
+        bias_p = None if bias is None else bias.data_ptr()
+        ws_p = None if ws is None else ws.data_ptr()
+        if want == 0:
+            _native.check("gafime_xent_forward", lib.gafime_xent_forward(
+                type_id, xp, xr, xk, wp, wr, wk, bias_p, labels.data_ptr(), n, d, c, loss.data_ptr(),
+                lse.data_ptr(), ws_p, size, stream))
+        else:
+            _native.check("gafime_xent_gradient", lib.gafime_xent_gradient(
+                type_id, xp, xr, xk, wp, wr, wk, bias_p, labels.data_ptr(), n, d, c,
+                None if row_weight is None else row_weight.data_ptr(),
+                0 if row_weight is None else row_weight.stride(0), scale, int(have), loss.data_ptr(),
+                lse.data_ptr(), None if dx is None else dx.data_ptr(), 0 if dx is None else dx.stride(0),
+                0 if dx is None else dx.stride(1), None if dw is None else dw.data_ptr(),
+                None if dbias is None else dbias.data_ptr(), ws_p, size, stream))
+    return loss, lse
+
+
+def _gradients(x, w, labels, bias, n, d, c, row_weight, scale, need_dx, need_dw, need_dbias, loss=None, lse=None):
+    dx = dw = dbias = None
+    if need_dx:
+        # x's order: a table held column by column gets its gradient column by column
+        if x.stride(0) == 1 and x.stride(1) != 1:
+            dx = torch.empty((d, n), dtype=x.dtype, device=x.device).t()
+        else:
+            dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    if need_dw:
+        dw = torch.empty((c, d), dtype=w.dtype, device=w.device)
+    if need_dbias:
+        dbias = torch.empty(c, dtype=torch.float32, device=x.device)
+    want = _GRADIENT | (_DX if need_dx else 0) | (_DW if need_dw else 0) | (_DBIAS if need_dbias else 0)
+    loss, lse = _call(x, w, labels, bias, n, d, c, want, row_weight, scale, loss, lse, dx, dw, dbias)
+    return XentGrad(loss, lse, dx, dw, dbias)
+
+
+class _SoftmaxXent(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, labels, bias):
+        n, d, c = x.shape[0], x.shape[1], w.shape[0]
+        loss, lse = _call(x, w, labels, bias, n, d, c, 0)
+        # the values as computed here: the caller may write into the loss it gets
+        ctx.save_for_backward(x, w, labels, bias, loss.clone(), lse)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        x, w, labels, bias, loss, lse = ctx.saved_tensors
+        need_x, need_w, _, need_b = ctx.needs_input_grad
+        if grad_loss.dtype != torch.float32:
+            grad_loss = grad_loss.float()
+        g = _gradients(x, w, labels, bias, x.shape[0], x.shape[1], w.shape[0], grad_loss, 1.0, need_x, need_w,
+                       need_b and bias is not None, loss, lse)
+        return g.dx, g.dw, None, g.dbias
+
+
+def softmax_xent(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
+                 bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Per-row softmax cross entropy of ``x @ w.T + bias``, (n,) float32, without keeping the
+    logits; differentiable in x, w and bias.
+
+    x (n, d) and w (c, d): float32, float16 or bfloat16 alike, any strides (a bucket's columns
+    as they are); labels (n,) int64 or int32; bias (c,) float32, -inf excludes a class.  A row
+    with a negative label is left out: loss 0, no part in any gradient, whatever its features
+    hold.  A label >= c makes the row's loss, and the gradients it enters, NaN.
+
+    To capture a backward pass into a CUDA graph, let go of eager graphs of the same leaves
+    first (torch's autograd waits for the stream on which they were made), or capture
+    softmax_xent_grad, which needs no autograd."""
+    _check(x, w, labels, bias, None)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)):
+        return _SoftmaxXent.apply(x, w, labels, bias)
+    return _call(x, w, labels, bias, x.shape[0], x.shape[1], w.shape[0], 0)[0]
+
+
+def softmax_xent_grad(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                      row_weight: Optional[torch.Tensor] = None, scale: float = 1.0, need_dx: bool = True,
+                      need_dw: bool = True) -> XentGrad:
+    """Losses, and the gradients of ``sum_i scale * row_weight[i] * loss[i]``, in one call: the
+    step of a fit whose row weights are known beforehand (1 / n for the mean).  With few classes
+    and need_dx=False that is one pass over x.  The gradient of a bias that is None is None.
+    Arguments as softmax_xent; row_weight (n,) float32, None for ones."""
+    n, d, c = _check(x, w, labels, bias, row_weight)
+    with torch.no_grad():
+        return _gradients(x.detach(), w.detach(), labels, bias, n, d, c, row_weight, float(scale), need_dx, need_dw,
+                          bias is not None)
+
+
+def _grad_norm(tensors: Sequence[torch.Tensor], out, max_norm: float) -> torch.Tensor:
+    tensors = list(tensors)
+    count = len(tensors)
+    if count == 0:
+        raise ValueError("at least one tensor is needed")
+    lib = _native.load()
+    device = tensors[0].device
+    if device.type != "cuda":
+        raise ValueError(f"the tensors must be on one GPU, got {device}")
+    index = device.index
+    ptrs, sizes, types = [], [], []
+    for t in tensors:
+        type_id = TYPES.get(t.dtype)
+        if type_id is None:
+            raise TypeError(f"tensors must be float32, float16 or bfloat16, got {t.dtype}")
+        if t.get_device() != index or not t.is_contiguous():
+            raise ValueError("the tensors must be contiguous and on one GPU")
+        ptrs.append(t.data_ptr())
+        sizes.append(t.numel())
+        types.append(type_id)
+    outs = None
+    if out is not None:
+        out = list(out)
+        if len(out) != count:
+            raise ValueError(f"{count} tensors, but {len(out)} outs")
+        outs = []
+        for t, o in zip(tensors, out):
+            if o is not t and (o.dtype != t.dtype or o.shape != t.shape or o.get_device() != index
+                               or not o.is_contiguous()):
+                raise ValueError("every out must have its tensor's shape, type and device, and be contiguous")
+            outs.append(o.data_ptr())
+        outs = (ctypes.c_void_p * count)(*outs)
+    with torch.cuda.device(index):
+        size = _norm_workspace(count)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        _native.check("gafime_grad_norm", lib.gafime_grad_norm(
+            (ctypes.c_void_p * count)(*ptrs), (ctypes.c_int64 * count)(*sizes), (ctypes.c_int * count)(*types), count,
+            outs, max_norm, norm.data_ptr(), ws.data_ptr(), size, torch.cuda.current_stream(index).cuda_stream))
+    return norm
+
+
+@functools.lru_cache(maxsize=1024)
+def _norm_workspace(count: int) -> int:
+    out = ctypes.c_size_t(0)
+    _native.check("gafime_grad_norm_workspace",
+                  _native.load(require_gpu=False).gafime_grad_norm_workspace(count, ctypes.byref(out)))
+    return out.value
+
+
+@torch.no_grad()
+def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
+    """2-norm over all elements of the tensors together, a float32 scalar on their GPU.  The
+    tensors are contiguous, float32, float16 or bfloat16 in any mix; squares are summed in fp64."""
+    return _grad_norm(tensors, None, 0.0)
+
+
+@torch.no_grad()
+def clip_grad_norm(tensors: Sequence[torch.Tensor], max_norm: float,
+                   out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Scale the tensors by min(1, max_norm / norm) of their norm together, in place or into
+    ``out`` (one contiguous tensor each, alike in shape and type, apart from one another and
+    from the tensors), and return the norm before it.  A norm that is not finite leaves the
+    values as they are: the caller sees it in the result and skips the step."""
+    max_norm = float(max_norm)
+    if not 0.0 <= max_norm <= 3.4028234663852886e38:
+        raise ValueError(f"max_norm must be a finite number >= 0, got {max_norm}")
+    tensors = list(tensors)
+    return _grad_norm(tensors, tensors if out is None else out, max_norm)

@@ -22,6 +22,7 @@
 #ifndef GAFIME_B200_H
 #define GAFIME_B200_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -349,6 +350,9 @@ int gafime_topk_merge(const int32_t* cand_i, const int32_t* cand_j, const double
 #define GAFIME_KERNEL_GRAM_REDUCE 12
 #define GAFIME_KERNEL_MI_CLASS_COPY 13
 #define GAFIME_KERNEL_GUARD 14
+#define GAFIME_KERNEL_XENT 15      /* few classes, and what surrounds the products */
+#define GAFIME_KERNEL_XENT_TC 16   /* many classes: the tensor-core products */
+#define GAFIME_KERNEL_GRAD_NORM 17
 
 /* NEW.  enable = 1: drop any previous records, then bracket every engine kernel
  * launch with CUDA events on its stream.  enable = 0: stop recording (the records
@@ -425,6 +429,85 @@ int gafime_contiguous_bucket_device_columns(ContiguousBucket bucket, int64_t c0,
 /* NEW.  Declares that features were written through gafime_contiguous_bucket_device_columns:
  * the next scoring call checks the whole matrix for non-finite values again. */
 int gafime_contiguous_bucket_mark_updated(ContiguousBucket bucket);
+
+/* ------------------------------------------------ NEW: class targets ---- */
+/*
+ * NEW -- no counterpart in the reference, whose scores treat features one by one.  What a
+ * linear softmax head over selected features and interactions needs to be fitted on the
+ * device: its loss with the gradients, and the gradients' global norm with clipping.
+ *
+ * These calls take device buffers and queue their work on `stream` (NULL: the default stream)
+ * of the current device without waiting, and allocate nothing: scratch memory is the caller's
+ * workspace, which belongs to the call until the stream has passed it (two calls that may
+ * overlap need two).  They can be captured into a CUDA graph.  Bad arguments return
+ * GAFIME_ERROR_INVALID_ARGS before any work.
+ */
+#define GAFIME_TYPE_FP32 0
+#define GAFIME_TYPE_FP16 1
+#define GAFIME_TYPE_BF16 2
+
+/* gradients a call computes (gafime_xent_workspace) */
+#define GAFIME_XENT_DX 1
+#define GAFIME_XENT_DW 2
+#define GAFIME_XENT_DBIAS 4
+#define GAFIME_XENT_GRADIENT 8   /* a gradient call, whichever of the three it wants */
+
+/*
+ * NEW.  Softmax cross entropy of a linear head, without keeping the logits:
+ *   z_ij = sum_k x_ik w_jk + bias_j,  lse_i = log sum_j exp z_ij,  loss_i = lse_i - z_i,label(i)
+ *
+ *   type        of x and w (GAFIME_TYPE_*).  Products are summed in fp32.
+ *   d_x         n x d; row i, feature k at i * x_row + k * x_col elements.  A bucket's columns
+ *               (gafime_contiguous_bucket_device_columns) are x_row = 1, x_col = ld.
+ *   d_w         c x d, likewise.
+ *   d_bias      c floats, or NULL.  -inf excludes a class.
+ *   d_labels    n class ids.  Negative: the row is left out (loss and lse 0, no part in any
+ *               gradient, whatever its features hold).  >= c: the row's loss is NaN.
+ *   d_loss      n floats;  d_lse: n floats, or NULL (for a later gradient call).
+ *   workspace   256-byte aligned, at least gafime_xent_workspace(... want = 0) bytes.
+ *
+ * Results are bit-identical from run to run.  A kernel whose bounded waits gave up (a fault)
+ * leaves NaN in every loss.
+ */
+int gafime_xent_forward(int type, const void* d_x, int64_t x_row, int64_t x_col, const void* d_w, int64_t w_row,
+                        int64_t w_col, const float* d_bias, const int64_t* d_labels, int64_t n, int64_t d, int64_t c,
+                        float* d_loss, float* d_lse, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * NEW.  The loss with the gradients of sum_i r_i loss_i, r_i = scale * d_row_weight[i * row_weight_stride]
+ * (NULL: 1):  g_ij = r_i (exp(z_ij - lse_i) - [j == label(i)]),
+ *   dx = g w (type of x, strides dx_row, dx_col),  dw = g^T x (type of w, c x d contiguous),
+ *   dbias_j = sum_i g_ij (fp32).  Any of the three may be NULL.
+ * have_lse = 0: computes d_loss and (unless NULL) d_lse as gafime_xent_forward does; with few
+ * classes the loss, dw and dbias take one pass over x.  have_lse = 1: d_loss and d_lse are those
+ * of a forward call on the same inputs and are only read.
+ * The outputs may not overlap the inputs.
+ */
+int gafime_xent_gradient(int type, const void* d_x, int64_t x_row, int64_t x_col, const void* d_w, int64_t w_row,
+                         int64_t w_col, const float* d_bias, const int64_t* d_labels, int64_t n, int64_t d, int64_t c,
+                         const float* d_row_weight, int64_t row_weight_stride, float scale, int have_lse, float* d_loss,
+                         float* d_lse, void* d_dx, int64_t dx_row, int64_t dx_col, void* d_dw, float* d_dbias,
+                         void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* NEW.  Workspace bytes of the call with these arguments (of the pointers only their alignment
+ * matters).  want: 0 for gafime_xent_forward, else GAFIME_XENT_GRADIENT with the gradients
+ * wanted.  Host only. */
+int gafime_xent_workspace(int type, const void* d_x, int64_t x_row, int64_t x_col, const void* d_w, int64_t w_row,
+                          int64_t w_col, int64_t n, int64_t d, int64_t c, int want, size_t* bytes_out);
+
+/*
+ * NEW.  2-norm over all elements of n_tensors contiguous tensors together (device pointers,
+ * element counts and GAFIME_TYPE_* in host arrays), summed in fp64 in a fixed order, to the
+ * device float *d_norm.  With d_outs (host array of device pointers) the tensors are also
+ * scaled to a norm of at most max_norm: out = g * min(1, max_norm / norm), rounded once;
+ * d_outs[i] is d_tensors[i] (in place) or memory that overlaps none of the tensors and outs.
+ * A norm that is not finite leaves the values as they are.  d_outs NULL: the norm only.
+ * workspace: 256-byte aligned, gafime_grad_norm_workspace(n_tensors) bytes.
+ */
+int gafime_grad_norm(const void* const* d_tensors, const int64_t* sizes, const int* types, int64_t n_tensors,
+                     void* const* d_outs, float max_norm, float* d_norm, void* d_workspace, size_t workspace_bytes,
+                     void* stream);
+int gafime_grad_norm_workspace(int64_t n_tensors, size_t* bytes_out);
 
 /* ------------------------------------------- NEW: no device allocation ---- */
 
