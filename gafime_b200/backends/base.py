@@ -2,7 +2,7 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, Iterable, List, Optional, Tuple
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -43,6 +43,10 @@ class Backend:
 
     def score_combos(self, X: np.ndarray, y: np.ndarray, combos: Iterable[Tuple[int, ...]],
                      metric_suite: MetricSuite) -> Dict[Tuple[int, ...], Dict[str, float]]:
+        raise NotImplementedError
+
+    def fit_joint(self, X: np.ndarray, y: np.ndarray, labels: np.ndarray, n_classes: int,
+                  combos: Sequence[Tuple[int, ...]], steps: int, clip: float, tolerance: float) -> Dict[str, object]:
         raise NotImplementedError
 
     def sample_indices(self, n_samples: int, rng: np.random.Generator):

@@ -188,6 +188,84 @@ class NativeCudaBackend(Backend):
                       div_eps=self.div_eps, mi_bins=mi_bins)
 
 
+    # -- joint fit ----------------------------------------------------------------
+    def fit_joint(self, X, y, labels, n_classes: int, combos: Sequence[Tuple[int, ...]], steps: int, clip: float,
+                  tolerance: float) -> Dict[str, object]:
+        """A softmax head on the combos' interaction values, standardised: full-batch descent
+        with Nesterov's momentum, every step one softmax_xent_grad over the resident columns."""
+        import torch
+
+        from .. import ops
+
+        if any(len(c) > 2 for c in combos):
+            raise NotImplementedError("combos of more than two features are not on the GPU path")
+        X = np.asarray(X)
+        y = np.asarray(y)
+        n, k = X.shape[0], len(combos)
+        bucket = self._resident(X, y).full
+        ptr, ld = bucket.device_columns(0, bucket.f)
+
+        class _Columns:
+            __cuda_array_interface__ = {"shape": (bucket.f, ld), "typestr": "<f4", "data": (ptr, False), "version": 3,
+                                        "stream": None}
+
+        with torch.cuda.device(self.device_id), torch.no_grad():
+            columns = torch.as_tensor(_Columns(), device=f"cuda:{self.device_id}")[:, :n]
+            # the combos' values column by column, as the bucket holds its features
+            values = torch.empty((k, n), dtype=torch.float32, device=columns.device)
+            centers, scales = [], []
+            for row, combo in zip(values, combos):
+                v = self._interaction(columns, combo)
+                mean = v.mean()
+                sd = (v - mean).square().mean().sqrt()
+                sd = torch.where(sd > 0, sd, torch.ones_like(sd))   # a constant says nothing: zeros
+                row.copy_((v - mean) / sd)
+                centers.append(mean)
+                scales.append(sd)
+            x = values.t()
+            target = torch.from_numpy(np.ascontiguousarray(labels, dtype=np.int64)).to(columns.device)
+            w = torch.zeros((n_classes, k), device=columns.device)
+            b = torch.zeros(n_classes, device=columns.device)
+            # curvature of the mean loss in (w, b): at most 1/2 of the largest eigenvalue of the
+            # values' second moments, which their trace k + 1 bounds
+            rate = 2.0 / (k + 1)
+            wv, bv, taken = w.clone(), b.clone(), 0
+            for step in range(steps):
+                g = ops.softmax_xent_grad(x, wv, target, bv, scale=1.0 / n, need_dx=False)
+                norm = ops.clip_grad_norm([g.dw, g.dbias], clip)
+                w1, b1 = wv - rate * g.dw, bv - rate * g.dbias
+                pull = step / (step + 3.0)
+                wv, bv = w1 + pull * (w1 - w), b1 + pull * (b1 - b)
+                w, b, taken = w1, b1, step + 1
+                if step % 8 == 7 and float(norm) <= tolerance:   # a look at the device every 8 steps
+                    break
+            last = ops.softmax_xent_grad(x, w, target, b, scale=1.0 / n, need_dx=False)
+            norm = ops.grad_norm([last.dw, last.dbias])
+            return {"weights": w.cpu().tolist(), "biases": b.cpu().tolist(),
+                    "centers": torch.stack(centers).cpu().tolist(), "scales": torch.stack(scales).cpu().tolist(),
+                    "log_loss": float(last.loss.double().mean()), "gradient_norm": float(norm), "steps": taken}
+
+    def _interaction(self, columns, combo: Tuple[int, ...]):
+        """A combo's values in fp64 from the resident fp32 columns, as the scores define them:
+        the raw column, or a op b (of centred columns with center)."""
+        import torch
+
+        a = columns[combo[0]].double()
+        if len(combo) == 1:
+            return a
+        c = columns[combo[1]].double()
+        if self.center:
+            a, c = a - a.mean(), c - c.mean()
+        if self.operator == "multiply":
+            return a * c
+        if self.operator == "add":
+            return a + c
+        if self.operator == "subtract":
+            return a - c
+        safe = torch.where(c.abs() < self.div_eps, torch.copysign(torch.full_like(c, self.div_eps), c), c)
+        return a / safe
+
+
 _BASE = {"pearson": "pearson", "r2": "pearson", "mutual_info": "mutual_info", "spearman": "spearman"}
 
 

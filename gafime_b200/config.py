@@ -37,3 +37,10 @@ class EngineConfig:
     operator: str = "multiply"
     center: bool = True
     div_eps: float = 1e-8
+    # Joint fit (new; off by default): steps of a softmax head fitted on the strongest combos
+    # together, for a target of classes.  The gradient's norm over weights and biases is clipped
+    # to joint_clip; the fit ends early when it falls below joint_tolerance.
+    joint_steps: int = 0
+    joint_combos: int = 16
+    joint_clip: float = 1.0
+    joint_tolerance: float = 1e-5

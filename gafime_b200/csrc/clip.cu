@@ -318,6 +318,9 @@ extern "C" int gafime_grad_norm(const void* const* d_tensors, const int64_t* siz
                              (d_outs && (!d_outs[i] || (uintptr_t)d_outs[i] % es))))
             return GAFIME_ERROR_INVALID_ARGS;
     }
+    int64_t chunks = 0;
+    for (int64_t i = 0; i < n_tensors; ++i) chunks += (sizes[i] + kChunk - 1) / kChunk;
+    if (chunks > 0x7fffffffll) return GAFIME_ERROR_INVALID_ARGS;
     try {
         if (d_outs && !ranges_apart(d_tensors, sizes, types, n_tensors, d_outs)) return GAFIME_ERROR_INVALID_ARGS;
     } catch (...) {

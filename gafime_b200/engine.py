@@ -1,7 +1,8 @@
 """GafimeEngine.analyze (gafime/engine.py:16-171) on the GPU backend.
 
 Same stages and random-generator order as the reference: unary scores -> top features ->
-pair plan -> pair scores -> bootstrap stability -> permutation p-values -> decision."""
+pair plan -> pair scores -> bootstrap stability -> permutation p-values -> (with
+joint_steps, new) a softmax head on the strongest combos together -> decision."""
 from __future__ import annotations
 
 from typing import Dict, Iterable, List, Optional, Tuple
@@ -14,7 +15,7 @@ from .metrics import metric_strength
 from .planning import plan_higher_order, plan_unary, select_top_features
 from .reporting import Decision, DiagnosticReport, InteractionResult
 from .utils import coerce_inputs, validate_budget
-from .validation import PermutationTester, StabilityAnalyzer
+from .validation import JointFitter, PermutationTester, StabilityAnalyzer
 
 
 class GafimeEngine:
@@ -49,11 +50,15 @@ class GafimeEngine:
             X_dev, y_dev, all_combos, cfg.num_repeats, rng)
         permutations = PermutationTester(self.metric_suite, backend).test(
             X_dev, y_dev, all_combos, cfg.permutation_tests, rng, actual_scores=scores)
+        joint = None
+        if cfg.joint_steps > 0:
+            joint, w = JointFitter(backend).fit(X_dev, y_dev, scores, cfg)
+            warnings.extend(w)
         decision = _make_decision(scores, permutations, stability, cfg)
         return DiagnosticReport(config=cfg, feature_names=names,
                                 interactions=unary_results + higher_results, stability=stability,
                                 permutations=permutations, warnings=warnings, decision=decision,
-                                backend=backend.info())
+                                backend=backend.info(), joint=joint)
 
     def _score_combos(self, X, y, combos, names: List[str]):
         combos = list(combos)

@@ -181,7 +181,6 @@ def _grad_norm(tensors: Sequence[torch.Tensor], out, max_norm: float) -> torch.T
     count = len(tensors)
     if count == 0:
         raise ValueError("at least one tensor is needed")
-    lib = _native.load()
     device = tensors[0].device
     if device.type != "cuda":
         raise ValueError(f"the tensors must be on one GPU, got {device}")
@@ -196,6 +195,7 @@ def _grad_norm(tensors: Sequence[torch.Tensor], out, max_norm: float) -> torch.T
         ptrs.append(t.data_ptr())
         sizes.append(t.numel())
         types.append(type_id)
+    lib = _native.load()
     outs = None
     if out is not None:
         out = list(out)

@@ -29,6 +29,26 @@ class PermutationResult:
 
 
 @dataclass(frozen=True)
+class JointResult:
+    """A softmax head on the strongest combos together: what they say about the classes jointly.
+
+    Logits of a row are weights @ ((values - centers) / scales) + biases with the combos'
+    interaction values; classes are the target's distinct values in order.  null_log_loss is
+    that of the class frequencies alone."""
+
+    combos: List[Tuple[int, ...]]
+    classes: List[float]
+    weights: List[List[float]]      # [class][combo]
+    biases: List[float]
+    centers: List[float]
+    scales: List[float]
+    log_loss: float
+    null_log_loss: float
+    gradient_norm: float            # of the mean loss at these weights and biases
+    steps: int
+
+
+@dataclass(frozen=True)
 class Decision:
     signal_detected: bool
     message: str
@@ -44,9 +64,10 @@ class DiagnosticReport:
     warnings: List[str] = field(default_factory=list)
     decision: Optional[Decision] = None
     backend: Optional[BackendInfo] = None
+    joint: Optional[JointResult] = None
 
     def to_dict(self) -> Dict[str, object]:
-        return {
+        out = {
             "config": self.config,
             "feature_names": self.feature_names,
             "interactions": [vars(r) for r in self.interactions],
@@ -56,3 +77,6 @@ class DiagnosticReport:
             "decision": None if self.decision is None else vars(self.decision),
             "backend": None if self.backend is None else vars(self.backend),
         }
+        if self.joint is not None:
+            out["joint"] = vars(self.joint)
+        return out

@@ -1,15 +1,17 @@
 """Bootstrap stability and permutation p-values (gafime/validation/stability.py:17-50,
 gafime/validation/permutation.py:17-54).  Both re-score through the backend, so every
 repeat runs on the GPU: a bootstrap gathers its rows on the device and a permutation
-uploads only the permuted target."""
+uploads only the permuted target.  The joint fit (no counterpart in the reference, whose
+scores treat combos one by one) runs on the resident columns too."""
 from __future__ import annotations
 
 from typing import Dict, List, Optional, Tuple
 
 import numpy as np
 
-from .metrics import MetricSuite
-from .reporting import PermutationResult, StabilityResult
+from .config import EngineConfig
+from .metrics import MetricSuite, metric_strength
+from .reporting import JointResult, PermutationResult, StabilityResult
 
 
 class StabilityAnalyzer:
@@ -67,3 +69,29 @@ class PermutationTester:
                         hits[c][m] += 1
         return [PermutationResult(c, {m: float((k + 1) / (num_permutations + 1)) for m, k in d.items()})
                 for c, d in hits.items()]
+
+
+class JointFitter:
+    """Fits one softmax head on the strongest combos together (config.joint_*)."""
+
+    max_classes = 65536
+
+    def __init__(self, backend) -> None:
+        self.backend = backend
+
+    def fit(self, X, y, scores: Dict[Tuple[int, ...], Dict[str, float]], config: EngineConfig
+            ) -> Tuple[Optional[JointResult], List[str]]:
+        if config.joint_combos < 1:
+            raise ValueError("joint_combos must be >= 1.")
+        if not scores:
+            return None, []
+        classes, labels = np.unique(y, return_inverse=True)
+        if len(classes) < 2 or len(classes) > min(self.max_classes, max(2, len(y) // 2)):
+            return None, [f"Joint fit skipped: the target has {len(classes)} distinct values for {len(y)} rows."]
+        ranked = sorted(scores, key=lambda c: metric_strength(scores[c]), reverse=True)
+        combos = ranked[: config.joint_combos]
+        fit = self.backend.fit_joint(X, y, labels, len(classes), combos, config.joint_steps, config.joint_clip,
+                                     config.joint_tolerance)
+        share = np.bincount(labels, minlength=len(classes)) / len(labels)
+        return JointResult(combos=combos, classes=[float(c) for c in classes],
+                           null_log_loss=float(-(share * np.log(share)).sum()), **fit), []
