@@ -64,9 +64,9 @@ __global__ void __launch_bounds__(1024) xent_few_sum_kernel(const float* __restr
 
 FewPlan few_plan(const XentCall& a, int sms) {
     FewPlan p{};
-    const int d = (int)a.d, c = (int)a.c, es = (int)xent_type_size(a.type), V = 16 / es;
+    const int d = (int)a.d, c = (int)a.c, es = (int)xent_type_size(a.type);
     p.cp = c <= 4 ? std::max(2, c) : c <= 6 ? 6 : c <= 8 ? 8 : 16;
-    const int line = p.cp == 2 ? 2 : (p.cp + 3) / 4 * 4;   // floats of a row of w and g in shared memory
+    const int line = (p.cp + 1) / 2 * 2;   // classes of a line of w and g in shared memory
     p.cols = a.xr == 1 && a.xk != 1;
     p.grad = a.gradient && (a.dw || a.dbias || a.dx);
     FewArgs& k = p.k;
@@ -75,30 +75,30 @@ FewPlan few_plan(const XentCall& a, int sms) {
     k.weight = a.weight; k.weight_stride = a.weight_stride; k.scale = a.scale;
     k.have_lse = a.have_lse;
     k.loss = a.loss; k.lse = a.lse; k.dx = a.dx; k.dxr = a.dxr; k.dxk = a.dxk;
-    k.d_pad = (d + kFewFeatures - 1) / kFewFeatures * kFewFeatures;
+    p.features = few_narrow(p.cp, p.grad) && (!p.grad || d <= 512) ? 64 : 128;
+    k.d_pad = (d + p.features - 1) / p.features * p.features;
     const int64_t line_stride = p.cols ? a.xk : a.xr;
     k.vec_ok = (p.cols ? a.xr == 1 : a.xk == 1) && (uintptr_t)a.x % 16 == 0 && line_stride >= 0 &&
                line_stride * es % 16 == 0;
-    k.warps = p.grad ? k.d_pad / kFewFeatures : 1;
-    k.groups = std::max(1, 4 / k.warps);
+    k.warps = p.grad ? k.d_pad / p.features : 1;
+    k.groups = std::max(1, (p.features == 64 ? 8 : 4) / k.warps);
     const int warps = k.warps * k.groups;
     p.threads = 32 * warps;
     auto smem = [&](int rows) {
-        return (size_t)warps * rows * kFewFeatures * es +
-               sizeof(float) * ((size_t)k.d_pad * line + (p.grad ? (size_t)warps * kRowsMost * line : 0) +
+        return (size_t)warps * rows * p.features * es +
+               sizeof(float) * ((size_t)k.d_pad * line + (p.grad ? (size_t)warps * kRowsMost * line * (p.cols ? 1 : 2) : 0) +
                                 (p.grad && k.warps > 1 ? 2 * (size_t)warps * p.cp * 32 : 0)) +
                (p.grad ? sizeof(double) * k.groups * p.cp * 32 : 0);
     };
-    // CTAs an SM holds: registers allow 16 warps of up to 128
+    // CTAs an SM holds: registers allow 24 warps of 85 or 16 of 128
     auto resident = [&](int rows) {
-        return (int)std::min<size_t>(16 / warps, (227 * 1024) / (smem(rows) + 1024));
+        return (int)std::min<size_t>((p.features == 64 ? 24 : 16) / warps, (227 * 1024) / (smem(rows) + 1024));
     };
     // Rows of a tile: 32, half of that where fewer than ten warps an SM would be left, and fewer
     // still where SMs would be left without a tile
     int rows = kRowsMost;
     if (resident(rows) * warps < 10 && resident(16) * warps > resident(rows) * warps) rows = 16;
-    while (rows > 8 && (a.n + rows - 1) / rows < 4 * sms) rows /= 2;
-    while (rows > std::max(8, V) && resident(rows) < 1) rows /= 2;
+    while (rows > 8 && ((a.n + rows - 1) / rows < 4 * sms || resident(rows) < 1)) rows /= 2;
     k.rows = rows;
     k.log_rows = rows == 32 ? 5 : rows == 16 ? 4 : 3;
     k.n_tiles = (int)((a.n + rows - 1) / rows);

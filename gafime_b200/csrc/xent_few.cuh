@@ -5,15 +5,16 @@
 // multiply-adds a value and the shared-memory traffic around them keep up: about 5.5 cycles an
 // SM for 32 fp32 values at the measured copy rate.
 //
-// A warp owns a tile of kRowsMost (or fewer) rows x 128 features in shared memory, which it
-// fills with its own asynchronous copies; W warps side by side cover the features.  Tiles are
-// not double-buffered: a warp that waits for its copies leaves the SM to eleven others, which
-// costs no barrier and no second tile.
+// A warp owns a tile of 32 rows (fewer in small calls) x 64 or 128 features in shared memory,
+// which it fills with its own asynchronous copies; W warps side by side cover the features.
+// Tiles are not double-buffered: a warp that waits for its copies leaves the SM to up to 23
+// others, which costs no barrier and no second tile (measured against two buffers of half the
+// rows: 64-byte pieces of columns instead of 128 cost more than the overlap gained).
 //   1. a lane is a row: partial dot products with c accumulators, w broadcast from shared memory
 //      (fewer rows than lanes: the lanes of a row share the features)
 //   2. the W partial logits are added through shared memory (the only barrier); a lane computes
 //      its row's softmax, loss and g, and leaves g in shared memory
-//   3. a lane is four features: c x 4 sums of g x over the tile's rows
+//   3. a lane is two or four features: c sums each of g x over the tile's rows
 // Without gradients a warp walks over the features by itself, and there is no barrier at all.
 // The sums of step 3 move to a partial in global memory every kFlushRows rows: short fp32
 // chains, added in fp64 in a fixed order by xent_few_sum_kernel at the end.
@@ -30,7 +31,9 @@
 
 namespace gafime {
 
-constexpr int kFewFeatures = 128;     // of a warp's tile
+// Features of a warp's tile: 64 where its sums fit into 85 registers a thread with the rest (24
+// warps an SM) and few enough warps cover the features, else 128.
+constexpr bool few_narrow(int, bool grad) { return !grad; }
 constexpr int kRowsMost = 32;
 constexpr int kFlushRows = 256;
 
@@ -63,7 +66,7 @@ struct FewArgs {
 
 struct FewPlan {
     FewArgs k;
-    int cp, grid, threads;
+    int cp, grid, threads, features;
     bool cols, grad;
     size_t smem;
 };
@@ -82,91 +85,94 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) 
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// Geometry of a tile: bytes of a line, and the exchange of its 16-byte units.
-template <typename T, bool COLS>
+// Geometry of a tile of R rows: bytes of a line, and the exchange of its 16-byte units.  The
+// pattern repeats every 8 lines, so unrolled loops need a few precomputed offsets only.
+template <typename T, bool COLS, int R, int F>
 struct Tile {
-    int line_bytes, shift, mask;
-    __device__ explicit Tile(int rows) {
-        line_bytes = (COLS ? rows : kFewFeatures) * (int)sizeof(T);
-        const int units = line_bytes / 16;                    // of a line
-        mask = units >= 8 ? 7 : units - 1;
-        shift = units >= 8 ? 0 : units == 4 ? 1 : units == 2 ? 2 : 3;
-    }
+    static constexpr int kLine = (COLS ? R : F) * (int)sizeof(T);
+    static constexpr int kUnits = kLine / 16;                 // of a line
+    static constexpr int kMask = kUnits >= 8 ? 7 : kUnits - 1;
+    static constexpr int kShift = kUnits >= 8 ? 0 : kUnits == 4 ? 1 : kUnits == 2 ? 2 : 3;
+    // byte offset of unit q of line l
+    static __device__ __forceinline__ int unit(int l, int q) { return l * kLine + ((q ^ ((l >> kShift) & kMask)) << 4); }
     // byte offset of element e of line l
-    __device__ __forceinline__ int at(int l, int e) const {
+    static __device__ __forceinline__ int at(int l, int e) {
         const int b = e * (int)sizeof(T);
-        return l * line_bytes + (((b >> 4) ^ ((l >> shift) & mask)) << 4) + (b & 15);
+        return unit(l, b >> 4) + (b & 15);
     }
 };
 
 // Queue a warp's copies of rows [r0, r0 + R) x features [k0, k0 + 128).  Rows and features past
 // the table read zero in units that hold some of it; other units are never used.
-template <typename T, bool COLS>
-__device__ __forceinline__ void load_tile(const FewArgs& a, const Tile<T, COLS>& g, uint8_t* tile, int64_t r0, int k0,
-                                          int lane) {
-    constexpr int V = 16 / sizeof(T);
-    const int left = (int)min((int64_t)a.rows, a.n - r0), feats = min(kFewFeatures, a.d - k0);
+template <typename T, bool COLS, int R, int F>
+__device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64_t r0, int k0, int lane) {
+    using Geo = Tile<T, COLS, R, F>;
+    constexpr int V = 16 / sizeof(T), U = Geo::kUnits;
+    constexpr int LS = U >= 32 ? 1 : 32 / U;                  // lines a warp covers at a time
+    const int left = (int)min((int64_t)R, a.n - r0), feats = min(F, a.d - k0);
     const T* x = (const T*)a.x + r0 * a.xr + (int64_t)k0 * a.xk;
     const uint32_t dst = (uint32_t)__cvta_generic_to_shared(tile);
     const int lines = COLS ? feats : left, len = COLS ? left : feats;
     const int64_t ls = COLS ? a.xk : a.xr, es = COLS ? a.xr : a.xk;
     if (a.vec_ok) {
-        const int units = COLS ? a.rows / V : (feats + V - 1) / V;
-        if (COLS || units == kFewFeatures / V) {
-            // a power of two of units to a line
-            const int lu = COLS ? a.log_rows - (sizeof(T) == 4 ? 2 : 3) : (sizeof(T) == 4 ? 5 : 4);
-            for (int i = lane; i < (lines << lu); i += 32) {
-                const int l = i >> lu, q = i & ((1 << lu) - 1);
-                const int bytes = max(0, min(V, len - q * V)) * (int)sizeof(T);
-                copy16(dst + g.at(l, q * V), bytes ? x + l * ls + q * V : x, bytes);
+        const int l0 = lane / U, q = lane % U;
+        const int bytes = max(0, min(V, len - q * V)) * (int)sizeof(T);
+        const T* src = x + l0 * ls + (bytes ? q * V : 0);
+        const int64_t hop = LS * ls;
+        if (bytes || COLS) {
+            // l0 and j LS share no bit, so the exchange splits into a lane's part and j's
+            const int own = l0 * Geo::kLine + ((q ^ ((l0 >> Geo::kShift) & Geo::kMask)) << 4);
+            constexpr int kAll = (COLS ? F : R) / LS;
+            if (lines == (COLS ? F : R)) {
+                #pragma unroll 8
+                for (int j = 0; j < kAll; ++j, src += hop)
+                    copy16(dst + j * LS * Geo::kLine + (own ^ ((((j * LS) >> Geo::kShift) & Geo::kMask) << 4)), src, bytes);
+            } else {
+                for (int j = 0; l0 + j * LS < lines; ++j, src += hop)
+                    copy16(dst + j * LS * Geo::kLine + (own ^ ((((j * LS) >> Geo::kShift) & Geo::kMask) << 4)), src, bytes);
             }
-        } else {
-            for (int l = 0; l < lines; ++l)
-                for (int q = lane; q < units; q += 32) {
-                    const int bytes = min(V, len - q * V) * (int)sizeof(T);
-                    copy16(dst + g.at(l, q * V), x + l * ls + q * V, bytes);
-                }
         }
     } else {
         // any strides: element by element, neighbouring lanes on neighbouring elements
-        const int full = COLS ? a.rows : (feats + V - 1) / V * V;
+        const int full = COLS ? R : (feats + V - 1) / V * V;
         for (int l = 0; l < lines; ++l)
             for (int e = lane; e < full; e += 32) {
                 if constexpr (sizeof(T) == 4) {
-                    copy4(dst + g.at(l, e), e < len ? x + l * ls + e * es : x, e < len ? 4 : 0);
+                    copy4(dst + Geo::at(l, e), e < len ? x + l * ls + e * es : x, e < len ? 4 : 0);
                 } else {
-                    *reinterpret_cast<T*>(tile + g.at(l, e)) = e < len ? x[l * ls + e * es] : from_float<T>(0.f);
+                    *reinterpret_cast<T*>(tile + Geo::at(l, e)) = e < len ? x[l * ls + e * es] : from_float<T>(0.f);
                 }
             }
     }
-    if (!COLS && left < a.rows) {
+    if (!COLS && left < R) {
         // rows past the table: their lanes read them in step 1
-        for (int l = left; l < a.rows; ++l)
-            for (int q = lane; q < kFewFeatures / V; q += 32)
-                *reinterpret_cast<uint4*>(tile + g.at(l, q * V)) = make_uint4(0, 0, 0, 0);
+        for (int l = left; l < R; ++l)
+            for (int q = lane; q < U; q += 32) *reinterpret_cast<uint4*>(tile + Geo::unit(l, q)) = make_uint4(0, 0, 0, 0);
     }
 }
 
-// CP floats, of which the first C count, from a line of whole float4 (float2 for two)
+// Packed pairs of floats: one instruction multiplies and adds both (fma.rn.f32x2).
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ void unpair(float& lo, float& hi, Pair p) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ void fma2(Pair& d, Pair a, Pair b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b)); }
+
+// Classes of a line in shared memory, padded so that C pairs are whole 16-byte units.
 template <int C>
-struct Line {
-    static constexpr int kPitch = C <= 2 ? 2 : (C + 3) / 4 * 4;
-};
+constexpr int padded() { return (C + 1) / 2 * 2; }
+// C pairs from 16-byte units
 template <int C>
-__device__ __forceinline__ void load_line(float (&v)[C], const float* p) {
-    if constexpr (C == 2) {
-        const float2 t = *reinterpret_cast<const float2*>(p);
-        v[0] = t.x;
-        v[1] = t.y;
-    } else {
-        #pragma unroll
-        for (int c = 0; c < C; c += 4) {
-            const float4 t = *reinterpret_cast<const float4*>(p + c);
-            v[c] = t.x;
-            if (c + 1 < C) v[c + 1] = t.y;
-            if (c + 2 < C) v[c + 2] = t.z;
-            if (c + 3 < C) v[c + 3] = t.w;
-        }
+__device__ __forceinline__ void load_pairs(Pair (&v)[C], const float* p) {
+    const ulonglong2* q = reinterpret_cast<const ulonglong2*>(p);
+    #pragma unroll
+    for (int c = 0; c < C; c += 2) {
+        const ulonglong2 t = q[c / 2];
+        v[c] = t.x;
+        if (c + 1 < C) v[c + 1] = t.y;
     }
 }
 
@@ -195,27 +201,183 @@ __device__ __forceinline__ void load4(float (&v)[4], const uint8_t* p, __nv_bflo
     v[3] = __uint_as_float(t.y & 0xffff0000u);
 }
 
+__device__ __forceinline__ void load_some(float (&v)[2], const uint8_t* p, float) {
+    const float2 t = *reinterpret_cast<const float2*>(p);
+    v[0] = t.x;
+    v[1] = t.y;
+}
+__device__ __forceinline__ void load_some(float (&v)[2], const uint8_t* p, __half) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(p));
+    v[0] = t.x;
+    v[1] = t.y;
+}
+__device__ __forceinline__ void load_some(float (&v)[2], const uint8_t* p, __nv_bfloat16) {
+    const uint32_t t = *reinterpret_cast<const uint32_t*>(p);
+    v[0] = __uint_as_float(t << 16);
+    v[1] = __uint_as_float(t & 0xffff0000u);
+}
+template <typename T>
+__device__ __forceinline__ void load_some(float (&v)[4], const uint8_t* p, T t) {
+    load4(v, p, t);
+}
+
+// Step 1: this lane's share of its row's dot products with w, [64 feature pairs][classes][2].  Pairs
+// of neighbouring features are multiplied together; their two sums meet at the end.
+template <typename T, int C, bool COLS, int R, int F>
+__device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const float* w, int feats, int lane) {
+    using Geo = Tile<T, COLS, R, F>;
+    constexpr int P = 2 * padded<C>(), S = 32 / R;            // floats of a feature pair; lanes that share a row
+    const int row = lane & (R - 1), share = lane / R;
+    Pair sum[C], wv[C];
+    #pragma unroll
+    for (int c = 0; c < C; ++c) sum[c] = 0;
+    if (COLS) {
+        // four pairs of the share's at a time: lines 2 (share + j S) and the next one, whose
+        // exchange repeats with 8 S lines
+        int off[8];
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) off[j] = Geo::at(2 * (share + (j >> 1) * S) + (j & 1), row);
+        const float* wk = w + share * P;
+        int k = 0;
+        for (; k + 8 * S <= feats; k += 8 * S) {
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const Pair x = pair(to_float(*reinterpret_cast<const T*>(tile + off[2 * j])),
+                                    to_float(*reinterpret_cast<const T*>(tile + off[2 * j + 1])));
+                load_pairs<C>(wv, wk + j * S * P);
+                #pragma unroll
+                for (int c = 0; c < C; ++c) fma2(sum[c], x, wv[c]);
+            }
+            tile += 8 * S * Geo::kLine;
+            wk += 4 * S * P;
+        }
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = k + 2 * (share + j * S);
+            if (at < feats) {
+                // an odd last feature has no neighbour in the tile
+                const Pair x = pair(to_float(*reinterpret_cast<const T*>(tile + off[2 * j])),
+                                    at + 1 < feats ? to_float(*reinterpret_cast<const T*>(tile + off[2 * j + 1])) : 0.f);
+                load_pairs<C>(wv, wk + j * S * P);
+                #pragma unroll
+                for (int c = 0; c < C; ++c) fma2(sum[c], x, wv[c]);
+            }
+        }
+    } else {
+        constexpr int V = 16 / sizeof(T);
+        const int x0 = row & 7;
+        const uint8_t* line = tile + row * Geo::kLine;
+        // a unit of V features; w is zero past the features, and so is x up to a whole unit
+        #pragma unroll 4
+        for (int q = share; q * V < feats; q += S) {
+            #pragma unroll
+            for (int h = 0; h < V / 4; ++h) {
+                float xv[4];
+                load4(xv, line + ((q ^ x0) << 4) + 8 * h, T{});
+                #pragma unroll
+                for (int v = 0; v < 4; v += 2) {
+                    const Pair x = pair(xv[v], xv[v + 1]);
+                    load_pairs<C>(wv, w + (q * V + 4 * h + v) / 2 * P);
+                    #pragma unroll
+                    for (int c = 0; c < C; ++c) fma2(sum[c], x, wv[c]);
+                }
+            }
+        }
+    }
+    #pragma unroll
+    for (int c = 0; c < C; ++c) {
+        float lo, hi;
+        unpair(lo, hi, sum[c]);
+        z[c] += lo + hi;
+    }
+}
+
+// Step 3: the lane's features' sums of g x over the tile's rows; g is zero for rows that do not
+// count.  `bad`: rows left out that hold no numbers (0 x NaN is NaN), skipped.
+//   columns: pairs of rows, g as [row pairs][classes][2]; the two sums of a pair meet at a flush
+//   rows: pairs of features, g as [rows][classes][2 alike]
+template <typename T, int C, bool COLS, int R, int F>
+__device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], const uint8_t* tile, const float* g,
+                                     uint32_t bad, int feats, int lane) {
+    using Geo = Tile<T, COLS, R, F>;
+    constexpr int CL = padded<C>();
+    if (COLS) {
+        // lines lane + 32 f exchange alike; four rows of a line at a time
+        const uint8_t* line = tile + lane * Geo::kLine;
+        const int x0 = ((lane >> Geo::kShift) & Geo::kMask) << 4;
+        constexpr int B = C <= 8 ? C : 8;                     // classes at a time: g of four rows in registers
+        #pragma unroll
+        for (int c0 = 0; c0 < C; c0 += B) {
+            #pragma unroll 2
+            for (int r = 0; r < R; r += 4) {
+                Pair g0[B], g1[B];
+                load_pairs<B>(g0, g + (r / 2 * CL + c0) * 2);
+                load_pairs<B>(g1, g + ((r / 2 + 1) * CL + c0) * 2);
+                const int b = r * (int)sizeof(T);
+                const uint8_t* p = line + (((b >> 4 << 4) ^ x0) + (b & 15));
+                #pragma unroll
+                for (int f = 0; f < F / 32; ++f) {
+                    if (32 * f >= feats) break;
+                    float xv[4];
+                    load4(xv, p + 32 * f * Geo::kLine, T{});
+                    if (bad)
+                        #pragma unroll
+                        for (int v = 0; v < 4; ++v)
+                            if ((bad >> (r + v)) & 1) xv[v] = 0.f;
+                    const Pair a = pair(xv[0], xv[1]), b2 = pair(xv[2], xv[3]);
+                    #pragma unroll
+                    for (int c = 0; c < B; ++c) {
+                        fma2(acc[f][c0 + c], a, g0[c]);
+                        fma2(acc[f][c0 + c], b2, g1[c]);
+                    }
+                }
+            }
+        }
+    } else {
+        constexpr int N = F / 32;                             // neighbouring features of a lane
+        const int b = N * lane * (int)sizeof(T);
+        const int own = (b >> 4) << 4;
+        const uint8_t* p = tile + (b & 15);
+        #pragma unroll 8
+        for (int r = 0; r < R; ++r) {
+            if ((bad >> r) & 1) continue;
+            float xv[N];
+            Pair gv[C];
+            load_some(xv, p + r * Geo::kLine + (own ^ ((r & 7) << 4)), T{});
+            load_pairs<C>(gv, g + r * CL * 2);
+            #pragma unroll
+            for (int f = 0; f < N; f += 2) {
+                const Pair x = pair(xv[f], xv[f + 1]);
+                #pragma unroll
+                for (int c = 0; c < C; ++c) fma2(acc[f / 2][c], x, gv[c]);
+            }
+        }
+    }
+}
+
 // C: classes the code has room for (a.c of them exist); GRAD: dw and dbias wanted or dx
-template <typename T, int C, bool COLS, bool GRAD, bool DX>
-__global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
-    constexpr int CL = Line<C>::kPitch;
+template <typename T, int C, bool COLS, bool GRAD, bool DX, int F>
+__global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few_kernel(const FewArgs a) {
+    constexpr int CL = padded<C>(), NF = GRAD ? F / 32 : 1;   // NF: features a lane sums in step 3
+    constexpr int NP = !GRAD ? 1 : COLS ? NF : NF / 2;         // its sums: pairs over rows, or over features
+    constexpr int GL = COLS ? CL : 2 * CL;                     // floats of a row of g
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int W = a.warps, group = warp / W, wg = warp - group * W;   // warp wg of its group
     const int R = a.rows;
-    const Tile<T, COLS> geo(R);
     const int warps = W * a.groups;
-    const int tile_bytes = R * kFewFeatures * (int)sizeof(T);
+    const int tile_bytes = R * F * (int)sizeof(T);
     uint8_t* tile = smem + (size_t)warp * tile_bytes;
-    float* ws = reinterpret_cast<float*>(smem + (size_t)warps * tile_bytes);   // w: [d_pad][CL]
-    float* gs = ws + (size_t)a.d_pad * CL + (size_t)warp * (GRAD ? kRowsMost * CL : 0);   // g: [rows][CL], a warp's own
-    float* red = ws + (size_t)a.d_pad * CL + (size_t)warps * (GRAD ? kRowsMost * CL : 0);   // [2][groups][W][C][32]
+    float* ws = reinterpret_cast<float*>(smem + (size_t)warps * tile_bytes);   // w: [d_pad / 2][CL][2]
+    float* gs = ws + (size_t)a.d_pad * CL + (size_t)warp * (GRAD ? kRowsMost * GL : 0);   // g, a warp's own
+    float* red = ws + (size_t)a.d_pad * CL + (size_t)warps * (GRAD ? kRowsMost * GL : 0);   // [2][groups][W][C][32]
     double* bsum = reinterpret_cast<double*>(red + (W > 1 ? 2 * (size_t)warps * C * 32 : 0)) +
                    (size_t)group * C * 32;                                                  // bias: [C][32] a group
 
     for (int i = threadIdx.x; i < a.d_pad * CL; i += blockDim.x) {
         const int k = i / CL, c = i % CL;
-        ws[i] = c < a.c && k < a.d ? to_float(((const T*)a.w)[c * a.wr + k * a.wk]) : 0.f;
+        ws[(k / 2 * CL + c) * 2 + (k & 1)] =
+            c < a.c && k < a.d ? to_float(((const T*)a.w)[c * a.wr + k * a.wk]) : 0.f;
     }
     float bias[C];
     #pragma unroll
@@ -224,16 +386,17 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
         for (int c = 0; c < C; ++c) bsum[c * 32 + lane] = 0.0;
     __syncthreads();
 
-    float acc[GRAD ? 4 : 1][C], db[C];
+    Pair acc[NP][C];
+    float db[C];
     #pragma unroll
-    for (int f = 0; f < (GRAD ? 4 : 1); ++f)
+    for (int f = 0; f < NP; ++f)
         #pragma unroll
-        for (int c = 0; c < C; ++c) acc[f][c] = 0.f;
+        for (int c = 0; c < C; ++c) acc[f][c] = 0;
     #pragma unroll
     for (int c = 0; c < C; ++c) db[c] = 0.f;
 
     const int row = lane & (R - 1), share = lane >> a.log_rows, shares = 32 >> a.log_rows;
-    const int kw = wg * kFewFeatures;                      // GRAD: the warp's features
+    const int kw = wg * F;                      // GRAD: the warp's features
     // the groups of all CTAs take tiles in turn, one group of every CTA first
     const int64_t first = (int64_t)group * gridDim.x + blockIdx.x, step = (int64_t)a.groups * gridDim.x;
     const size_t part_at = (size_t)first * a.c * a.d_pad;
@@ -244,15 +407,22 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
     auto flush = [&]() {
         if (a.part) {
             #pragma unroll
-            for (int f = 0; f < (GRAD ? 4 : 1); ++f) {
-                const int k = kw + (COLS ? lane + 32 * f : 4 * lane + f);
+            for (int f = 0; f < NP; ++f) {
                 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    if (c < a.c) {
-                        float* p = a.part + part_at + (size_t)c * a.d_pad + k;
-                        *p = flushed ? *p + acc[f][c] : acc[f][c];
+                    float lo, hi;
+                    unpair(lo, hi, acc[f][c]);
+                    acc[f][c] = 0;
+                    if (c >= a.c) continue;
+                    float* p = a.part + part_at + (size_t)c * a.d_pad + kw;
+                    if (COLS) {
+                        p += lane + 32 * f;
+                        *p = flushed ? *p + (lo + hi) : lo + hi;
+                    } else {
+                        p += NF * lane + 2 * f;
+                        p[0] = flushed ? p[0] + lo : lo;
+                        p[1] = flushed ? p[1] + hi : hi;
                     }
-                    acc[f][c] = 0.f;
                 }
             }
         }
@@ -266,51 +436,58 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
         since = 0;
     };
 
+    // The warp's tiles in order: with gradients one of every tile of rows, else all features of a
+    // tile of rows in turn.
+    const int k_first = GRAD ? kw : 0, k_step = GRAD ? a.d_pad : F;
+    auto load = [&](int64_t t, int k0) {
+        if (R == 32)
+            load_tile<T, COLS, 32, F>(a, tile, t * R, k0, lane);
+        else if (R == 16)
+            load_tile<T, COLS, 16, F>(a, tile, t * R, k0, lane);
+        else
+            load_tile<T, COLS, 8, F>(a, tile, t * R, k0, lane);
+    };
+    struct Meta {
+        int64_t y;
+        float weight, lse;
+    };
+    auto meta_of = [&](int64_t t) {
+        Meta m = {-1, 0.f, 0.f};
+        const int64_t gr = t * R + row;
+        if (t < a.n_tiles && gr < a.n) {
+            m.y = a.labels[gr];
+            if (GRAD) m.weight = (a.weight ? a.weight[gr * a.weight_stride] : 1.f) * a.scale;
+            if (a.have_lse) m.lse = a.lse[gr];
+        }
+        return m;
+    };
+    Meta meta = meta_of(first);
     for (int64_t t = first; t < a.n_tiles; t += step) {
         const int64_t r0 = t * R, gr = r0 + row;
         float z[C];
         #pragma unroll
         for (int c = 0; c < C; ++c) z[c] = 0.f;
-        int64_t y64 = -1;
-        float rw = 0.f, shift_in = 0.f;
-        for (int k0 = GRAD ? kw : 0; k0 < a.d; k0 += GRAD ? a.d_pad : kFewFeatures) {
+        Meta next = meta;
+        for (int k0 = k_first; k0 < a.d; k0 += k_step) {
             __syncwarp();                                  // the tile's last readers are done
-            load_tile<T, COLS>(a, geo, tile, r0, k0, lane);
+            load(t, k0);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            if (k0 == (GRAD ? kw : 0) && gr < a.n) {       // meanwhile
-                y64 = a.labels[gr];
-                if (GRAD) rw = (a.weight ? a.weight[gr * a.weight_stride] : 1.f) * a.scale;
-                if (a.have_lse) shift_in = a.lse[gr];
-            }
+            if (k0 == k_first) next = meta_of(t + step);
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
             // 1. a lane is a row
-            const int feats = min(kFewFeatures, a.d - k0);
-            const float* wk = ws + (size_t)k0 * CL;
-            if (COLS) {
-                #pragma unroll 4
-                for (int k = share; k < feats; k += shares) {
-                    const float xv = to_float(*reinterpret_cast<const T*>(tile + geo.at(k, row)));
-                    float wv[C];
-                    load_line<C>(wv, wk + k * CL);
-                    #pragma unroll
-                    for (int c = 0; c < C; ++c) z[c] = fmaf(xv, wv[c], z[c]);
-                }
-            } else {
-                #pragma unroll 2
-                for (int k = share * 4; k < feats; k += shares * 4) {
-                    float xv[4];
-                    load4(xv, tile + geo.at(row, k), T{});
-                    #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        float wv[C];
-                        load_line<C>(wv, wk + (k + v) * CL);
-                        #pragma unroll
-                        for (int c = 0; c < C; ++c) z[c] = fmaf(xv[v], wv[c], z[c]);
-                    }
-                }
-            }
+            const int feats = min(F, a.d - k0);
+            const float* wk = ws + (size_t)k0 * CL;                // k0 / 2 pairs of 2 CL
+            if (R == 32)
+                dots<T, C, COLS, 32, F>(z, tile, wk, feats, lane);
+            else if (R == 16)
+                dots<T, C, COLS, 16, F>(z, tile, wk, feats, lane);
+            else
+                dots<T, C, COLS, 8, F>(z, tile, wk, feats, lane);
         }
+        const int64_t y64 = meta.y;
+        const float rw = meta.weight, shift_in = meta.lse;
+        meta = next;
         for (int o = R; o < 32; o <<= 1)
             #pragma unroll
             for (int c = 0; c < C; ++c) z[c] += __shfl_xor_sync(0xffffffffu, z[c], o);
@@ -322,6 +499,7 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
             asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(W * 32) : "memory");
             #pragma unroll
             for (int c = 0; c < C; ++c) z[c] = 0.f;
+            #pragma unroll 2
             for (int w = 0; w < W; ++w)
                 #pragma unroll
                 for (int c = 0; c < C; ++c) z[c] += mine[(w * C + c) * 32 + lane];
@@ -329,6 +507,7 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
         }
         const bool kept = y64 >= 0;
         const int y = kept && y64 < a.c ? (int)y64 : -1;   // kept with y < 0: no such class
+        const bool finite = fabsf(z[0]) <= 3.402823466e38f;   // any NaN or infinity in the row shows here
         float m = -INFINITY, zy = NAN, s = 0.f;
         #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -351,7 +530,8 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
         if (GRAD) {
             // with this call's own sum, e / s; else exp of the difference to the given lse
             const float inv = 1.f / s;
-            const uint32_t mask = __ballot_sync(0xffffffffu, kept);   // bit r (r + R, ...): row r counts
+            // bit r (and r + R, ...) for row r
+            const uint32_t mask = __ballot_sync(0xffffffffu, kept), bad = __ballot_sync(0xffffffffu, !kept && !finite);
             #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const float p = a.have_lse ? expf(z[c] - shift_in) : e[c] * inv;
@@ -360,81 +540,56 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
                 if (c >= a.c) g = 0.f;
                 e[c] = g;
                 if (share == 0) {
-                    gs[row * CL + c] = g;
+                    if (COLS)
+                        gs[(row / 2 * CL + c) * 2 + (row & 1)] = g;
+                    else
+                        *reinterpret_cast<Pair*>(gs + (row * CL + c) * 2) = pair(g, g);
                     db[c] += g;
                 }
             }
             __syncwarp();
             if (DX) {
-                const int left = (int)min((int64_t)R, a.n - r0), feats = min(kFewFeatures, a.d - kw);
+                const int left = (int)min((int64_t)R, a.n - r0), feats = min(F, a.d - kw);
                 T* dx = (T*)a.dx + r0 * a.dxr + (int64_t)kw * a.dxk;
                 const float* wk = ws + (size_t)kw * CL;
                 if (COLS) {
                     // neighbouring lanes are neighbouring rows
                     if (row < left)
-                        for (int k = share; k < feats; k += shares) {
-                            float wv[C], v = 0.f;
-                            load_line<C>(wv, wk + k * CL);
+                        for (int k = 2 * share; k < feats; k += 2 * shares) {
+                            Pair wv[C], v = 0;
+                            load_pairs<C>(wv, wk + k * CL);
                             #pragma unroll
-                            for (int c = 0; c < C; ++c) v = fmaf(e[c], wv[c], v);
-                            dx[row * a.dxr + k * a.dxk] = from_float<T>(kept ? v : 0.f);
+                            for (int c = 0; c < C; ++c) fma2(v, pair(e[c], e[c]), wv[c]);
+                            float lo, hi;
+                            unpair(lo, hi, v);
+                            dx[row * a.dxr + k * a.dxk] = from_float<T>(kept ? lo : 0.f);
+                            if (k + 1 < feats) dx[row * a.dxr + (k + 1) * a.dxk] = from_float<T>(kept ? hi : 0.f);
                         }
                 } else {
                     for (int k = lane; k < feats; k += 32) {
                         float wv[C];
-                        load_line<C>(wv, wk + k * CL);
+                        #pragma unroll
+                        for (int c = 0; c < C; ++c) wv[c] = wk[(k / 2 * CL + c) * 2 + (k & 1)];
                         #pragma unroll 4
                         for (int r = 0; r < left; ++r) {
-                            float g[C], v = 0.f;
-                            load_line<C>(g, gs + r * CL);
+                            float v = 0.f;
                             #pragma unroll
-                            for (int c = 0; c < C; ++c) v = fmaf(g[c], wv[c], v);
+                            for (int c = 0; c < C; ++c) v = fmaf(gs[(r * CL + c) * 2], wv[c], v);
                             dx[r * a.dxr + k * a.dxk] = from_float<T>((mask >> r) & 1 ? v : 0.f);
                         }
                     }
                 }
             }
-            // 3. a lane is four features
-            if (a.part && mask) {
-                const uint32_t all = R == 32 ? 0xffffffffu : (1u << R) - 1;
-                if (COLS) {
-                    const int feats = min(kFewFeatures, a.d - kw);
-                    auto sums = [&](bool whole) {
-                        #pragma unroll 2
-                        for (int r = 0; r < R; r += 4) {
-                            #pragma unroll
-                            for (int f = 0; f < 4; ++f) {
-                                if (32 * f >= feats) break;
-                                float xv[4];
-                                load4(xv, tile + geo.at(lane + 32 * f, r), T{});
-                                #pragma unroll
-                                for (int v = 0; v < 4; ++v) {
-                                    // what a left-out row holds may be no number
-                                    const float xk = whole || ((mask >> (r + v)) & 1) ? xv[v] : 0.f;
-                                    float g[C];
-                                    load_line<C>(g, gs + (r + v) * CL);
-                                    #pragma unroll
-                                    for (int c = 0; c < C; ++c) acc[f][c] = fmaf(g[c], xk, acc[f][c]);
-                                }
-                            }
-                        }
-                    };
-                    if ((mask & all) == all)
-                        sums(true);
+            // 3. a lane is two or four features
+            if constexpr (GRAD) {
+                if (a.part && mask) {
+                    const int feats = min(F, a.d - kw);
+                    if (R == 32)
+                        sums<T, C, COLS, 32, F>(acc, tile, gs, bad, feats, lane);
+                    else if (R == 16)
+                        sums<T, C, COLS, 16, F>(acc, tile, gs, bad, feats, lane);
                     else
-                        sums(false);
-                } else {
-                    #pragma unroll 4
-                    for (int r = 0; r < R; ++r) {
-                        if (!((mask >> r) & 1)) continue;
-                        float xv[4], g[C];
-                        load4(xv, tile + geo.at(r, 4 * lane), T{});
-                        load_line<C>(g, gs + r * CL);
-                        #pragma unroll
-                        for (int f = 0; f < 4; ++f)
-                            #pragma unroll
-                            for (int c = 0; c < C; ++c) acc[f][c] = fmaf(g[c], xv[f], acc[f][c]);
-                    }
+                        sums<T, C, COLS, 8, F>(acc, tile, gs, bad, feats, lane);
                 }
             }
             since += R;
@@ -454,15 +609,24 @@ __global__ void __launch_bounds__(512, 1) xent_few_kernel(const FewArgs a) {
     }
 }
 
-template <typename T, int C, bool COLS, bool GRAD, bool DX>
-cudaError_t launch(const FewPlan& p, cudaStream_t stream) {
-    auto fn = xent_few_kernel<T, C, COLS, GRAD, DX>;
+template <typename T, int C, bool COLS, bool GRAD, bool DX, int F>
+cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
+    auto fn = xent_few_kernel<T, C, COLS, GRAD, DX, F>;
     const cudaError_t e =
         cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
     if (e != cudaSuccess) return e;
     KernelTimer kt(stream, GAFIME_KERNEL_XENT);
     fn<<<p.grid, p.threads, p.smem, stream>>>(p.k);
     return cudaGetLastError();
+}
+
+template <typename T, int C, bool COLS, bool GRAD, bool DX>
+cudaError_t launch(const FewPlan& p, cudaStream_t s) {
+    if constexpr (few_narrow(C, GRAD))
+        if (p.features == 64) return launch_f<T, C, COLS, GRAD, DX, 64>(p, s);
+    if constexpr (GRAD)
+        if (p.features == 128) return launch_f<T, C, COLS, GRAD, DX, 128>(p, s);
+    return cudaErrorInvalidValue;
 }
 
 template <typename T, int C>
