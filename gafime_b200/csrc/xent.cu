@@ -23,7 +23,6 @@ namespace gafime {
 
 namespace {
 
-constexpr int kFewMaxC = 16;
 constexpr int kFewMaxD = 2048;
 constexpr size_t kFewMaxSmem = 226 * 1024;
 
@@ -75,13 +74,13 @@ FewPlan few_plan(const XentCall& a, int sms) {
     k.weight = a.weight; k.weight_stride = a.weight_stride; k.scale = a.scale;
     k.have_lse = a.have_lse;
     k.loss = a.loss; k.lse = a.lse; k.dx = a.dx; k.dxr = a.dxr; k.dxk = a.dxk;
-    p.features = few_narrow(p.cp, p.grad) && (!p.grad || d <= 512) ? 64 : 128;
+    p.features = few_features(p.grad);
     k.d_pad = (d + p.features - 1) / p.features * p.features;
     const int64_t line_stride = p.cols ? a.xk : a.xr;
     k.vec_ok = (p.cols ? a.xr == 1 : a.xk == 1) && (uintptr_t)a.x % 16 == 0 && line_stride >= 0 &&
                line_stride * es % 16 == 0;
     k.warps = p.grad ? k.d_pad / p.features : 1;
-    k.groups = std::max(1, (p.features == 64 ? 8 : 4) / k.warps);
+    k.groups = std::max(1, (p.grad ? 4 : 8) / k.warps);
     const int warps = k.warps * k.groups;
     p.threads = 32 * warps;
     auto smem = [&](int rows) {
@@ -92,7 +91,7 @@ FewPlan few_plan(const XentCall& a, int sms) {
     };
     // CTAs an SM holds: registers allow 24 warps of 85 or 16 of 128
     auto resident = [&](int rows) {
-        return (int)std::min<size_t>((p.features == 64 ? 24 : 16) / warps, (227 * 1024) / (smem(rows) + 1024));
+        return (int)std::min<size_t>((p.grad ? 16 : 24) / warps, (227 * 1024) / (smem(rows) + 1024));
     };
     // Rows of a tile: 32, half of that where fewer than ten warps an SM would be left, and fewer
     // still where SMs would be left without a tile
@@ -130,7 +129,9 @@ cudaError_t few_sum(const XentCall& a, const FewPlan& p) {
 
 bool xent_few_fits(const XentCall& a) {
     if (a.c > kFewMaxC || a.d > kFewMaxD) return false;
-    return few_plan(a, 148).smem <= kFewMaxSmem;
+    if (a.gradient && (a.dx || a.dw || a.dbias) && a.c > kFewMaxGrad) return false;
+    const FewPlan p = few_plan(a, 148);
+    return p.threads <= 512 && p.smem <= kFewMaxSmem;
 }
 
 size_t xent_few_workspace(const XentCall& a, int sms) {

@@ -31,9 +31,11 @@
 
 namespace gafime {
 
-// Features of a warp's tile: 64 where its sums fit into 85 registers a thread with the rest (24
-// warps an SM) and few enough warps cover the features, else 128.
-constexpr bool few_narrow(int, bool grad) { return !grad; }
+// Most classes of this path.  With gradients 8: at 16 their sums leave no registers (200000 x 1024
+// fp32: 1.5 to 3.1 ms a step, the tensor cores' path 1.5 ms); without, 16 (0.34 ms against 1.04 ms).
+constexpr int kFewMaxC = 16, kFewMaxGrad = 8;
+// Features of a warp's tile: 128 with gradients, 64 without (24 warps an SM in place of 12).
+constexpr int few_features(bool grad) { return grad ? 128 : 64; }
 constexpr int kRowsMost = 32;
 constexpr int kFlushRows = 256;
 
@@ -221,52 +223,93 @@ __device__ __forceinline__ void load_some(float (&v)[4], const uint8_t* p, T t) 
     load4(v, p, t);
 }
 
-// Step 1: this lane's share of its row's dot products with w, [64 feature pairs][classes][2].  Pairs
-// of neighbouring features are multiplied together; their two sums meet at the end.
+// The row of its tile that a lane finishes in step 2 (lanes past R share one).
+//   columns: lane = share G + group; it multiplies rows 4 group .. 4 group + 3 (16 bytes of a
+//            line) and keeps the one that its share names
+//   rows:    lane = share R + row; it multiplies that row alone (four rows a lane, the columns'
+//            way, measured the same at 2 classes and slower from 6 on)
+template <bool COLS, int R>
+struct Lanes {
+    static constexpr int kGroups = R / 4, kShares = COLS ? 32 / kGroups : 32 / R;
+    static __device__ __forceinline__ int row(int lane) {
+        return COLS ? 4 * (lane % kGroups) + ((lane / kGroups) & 3) : lane % R;
+    }
+};
+
+// Step 1: dot products of the tile's rows with w, all of row Lanes::row(lane) in z at the end.
+// w: columns [features][classes], pairs of rows multiplied together, a value of w for four rows;
+// rows [feature pairs][classes][2], pairs of features.
 template <typename T, int C, bool COLS, int R, int F>
 __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const float* w, int feats, int lane) {
     using Geo = Tile<T, COLS, R, F>;
-    constexpr int P = 2 * padded<C>(), S = 32 / R;            // floats of a feature pair; lanes that share a row
-    const int row = lane & (R - 1), share = lane / R;
-    Pair sum[C], wv[C];
-    #pragma unroll
-    for (int c = 0; c < C; ++c) sum[c] = 0;
-    if (COLS) {
-        // four pairs of the share's at a time: lines 2 (share + j S) and the next one, whose
-        // exchange repeats with 8 S lines
-        int off[8];
+    using L = Lanes<COLS, R>;
+    constexpr int CL = padded<C>(), S = L::kShares;
+    if constexpr (COLS) {
+        constexpr int G = L::kGroups, B = C <= 6 ? C : 4;     // B: classes at a time
+        const int group = lane % G, share = lane / G;
         #pragma unroll
-        for (int j = 0; j < 8; ++j) off[j] = Geo::at(2 * (share + (j >> 1) * S) + (j & 1), row);
-        const float* wk = w + share * P;
-        int k = 0;
-        for (; k + 8 * S <= feats; k += 8 * S) {
+        for (int c0 = 0; c0 < C; c0 += B) {
+            float part[4][B];
+            Pair sum[2][B];
             #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const Pair x = pair(to_float(*reinterpret_cast<const T*>(tile + off[2 * j])),
-                                    to_float(*reinterpret_cast<const T*>(tile + off[2 * j + 1])));
-                load_pairs<C>(wv, wk + j * S * P);
+            for (int c = 0; c < B; ++c) sum[0][c] = sum[1][c] = 0;
+            // lines share, share + S, ...: S a multiple of 4, so two exchanges in turn
+            const uint8_t* p0 = tile + Geo::at(share, 4 * group);
+            const uint8_t* p1 = tile + Geo::at(share + S, 4 * group);
+            const float* wk = w + share * CL + c0;
+            auto line = [&](const uint8_t* p, const float* wl) {
+                float xv[4], wv[B];
+                load4(xv, p, T{});
                 #pragma unroll
-                for (int c = 0; c < C; ++c) fma2(sum[c], x, wv[c]);
+                for (int c = 0; c < B; c += 2) {
+                    const float2 t = *reinterpret_cast<const float2*>(wl + c);
+                    wv[c] = t.x;
+                    if (c + 1 < B) wv[c + 1] = t.y;
+                }
+                const Pair a = pair(xv[0], xv[1]), b = pair(xv[2], xv[3]);
+                #pragma unroll
+                for (int c = 0; c < B; ++c) {
+                    const Pair ww = pair(wv[c], wv[c]);
+                    fma2(sum[0][c], a, ww);
+                    fma2(sum[1][c], b, ww);
+                }
+            };
+            int k = share;
+            #pragma unroll 2
+            for (; k + S < feats; k += 2 * S) {
+                line(p0, wk);
+                line(p1, wk + S * CL);
+                p0 += 2 * S * Geo::kLine;
+                p1 += 2 * S * Geo::kLine;
+                wk += 2 * S * CL;
             }
-            tile += 8 * S * Geo::kLine;
-            wk += 4 * S * P;
-        }
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int at = k + 2 * (share + j * S);
-            if (at < feats) {
-                // an odd last feature has no neighbour in the tile
-                const Pair x = pair(to_float(*reinterpret_cast<const T*>(tile + off[2 * j])),
-                                    at + 1 < feats ? to_float(*reinterpret_cast<const T*>(tile + off[2 * j + 1])) : 0.f);
-                load_pairs<C>(wv, wk + j * S * P);
+            if (k < feats) line(p0, wk);
+            #pragma unroll
+            for (int c = 0; c < B; ++c) {
+                unpair(part[0][c], part[1][c], sum[0][c]);
+                unpair(part[2][c], part[3][c], sum[1][c]);
+            }
+            // the lane keeps row i = share & 3 of its four: the first two steps of the sum over the
+            // lanes halve what is held, as in column_sums
+            #pragma unroll
+            for (int c = 0; c < B; ++c) {
+                const bool odd = share & 1, high = share & 2;
+                const float s0 = odd ? part[0][c] : part[1][c], k0 = odd ? part[1][c] : part[0][c];
+                const float s1 = odd ? part[2][c] : part[3][c], k1 = odd ? part[3][c] : part[2][c];
+                const float u0 = k0 + __shfl_xor_sync(0xffffffffu, s0, G), u1 = k1 + __shfl_xor_sync(0xffffffffu, s1, G);
+                float t = (high ? u1 : u0) + __shfl_xor_sync(0xffffffffu, high ? u0 : u1, 2 * G);
                 #pragma unroll
-                for (int c = 0; c < C; ++c) fma2(sum[c], x, wv[c]);
+                for (int o = 4 * G; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+                if (c0 + c < C) z[c0 + c] += t;
             }
         }
     } else {
         constexpr int V = 16 / sizeof(T);
-        const int x0 = row & 7;
+        const int row = lane % R, share = lane / R, x0 = row & 7;
         const uint8_t* line = tile + row * Geo::kLine;
+        Pair sum[C], wv[C];
+        #pragma unroll
+        for (int c = 0; c < C; ++c) sum[c] = 0;
         // a unit of V features; w is zero past the features, and so is x up to a whole unit
         #pragma unroll 4
         for (int q = share; q * V < feats; q += S) {
@@ -277,18 +320,21 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
                 #pragma unroll
                 for (int v = 0; v < 4; v += 2) {
                     const Pair x = pair(xv[v], xv[v + 1]);
-                    load_pairs<C>(wv, w + (q * V + 4 * h + v) / 2 * P);
+                    load_pairs<C>(wv, w + (q * V + 4 * h + v) * CL);
                     #pragma unroll
                     for (int c = 0; c < C; ++c) fma2(sum[c], x, wv[c]);
                 }
             }
         }
-    }
-    #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        float lo, hi;
-        unpair(lo, hi, sum[c]);
-        z[c] += lo + hi;
+        #pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float lo, hi;
+            unpair(lo, hi, sum[c]);
+            float t = lo + hi;
+            #pragma unroll
+            for (int o = R; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            z[c] += t;
+        }
     }
 }
 
@@ -357,7 +403,7 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
 
 // C: classes the code has room for (a.c of them exist); GRAD: dw and dbias wanted or dx
 template <typename T, int C, bool COLS, bool GRAD, bool DX, int F>
-__global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : 3) xent_few_kernel(const FewArgs a) {
     constexpr int CL = padded<C>(), NF = GRAD ? F / 32 : 1;   // NF: features a lane sums in step 3
     constexpr int NP = !GRAD ? 1 : COLS ? NF : NF / 2;         // its sums: pairs over rows, or over features
     constexpr int GL = COLS ? CL : 2 * CL;                     // floats of a row of g
@@ -368,7 +414,7 @@ __global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few
     const int warps = W * a.groups;
     const int tile_bytes = R * F * (int)sizeof(T);
     uint8_t* tile = smem + (size_t)warp * tile_bytes;
-    float* ws = reinterpret_cast<float*>(smem + (size_t)warps * tile_bytes);   // w: [d_pad / 2][CL][2]
+    float* ws = reinterpret_cast<float*>(smem + (size_t)warps * tile_bytes);   // w, [d_pad][CL] or [d_pad / 2][CL][2]
     float* gs = ws + (size_t)a.d_pad * CL + (size_t)warp * (GRAD ? kRowsMost * GL : 0);   // g, a warp's own
     float* red = ws + (size_t)a.d_pad * CL + (size_t)warps * (GRAD ? kRowsMost * GL : 0);   // [2][groups][W][C][32]
     double* bsum = reinterpret_cast<double*>(red + (W > 1 ? 2 * (size_t)warps * C * 32 : 0)) +
@@ -376,7 +422,7 @@ __global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few
 
     for (int i = threadIdx.x; i < a.d_pad * CL; i += blockDim.x) {
         const int k = i / CL, c = i % CL;
-        ws[(k / 2 * CL + c) * 2 + (k & 1)] =
+        ws[COLS ? i : (k / 2 * CL + c) * 2 + (k & 1)] =
             c < a.c && k < a.d ? to_float(((const T*)a.w)[c * a.wr + k * a.wk]) : 0.f;
     }
     float bias[C];
@@ -395,10 +441,15 @@ __global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few
     #pragma unroll
     for (int c = 0; c < C; ++c) db[c] = 0.f;
 
-    const int row = lane & (R - 1), share = lane >> a.log_rows, shares = 32 >> a.log_rows;
+    const int row = R == 32   ? Lanes<COLS, 32>::row(lane)
+                    : R == 16 ? Lanes<COLS, 16>::row(lane)
+                              : Lanes<COLS, 8>::row(lane);
+    const int share = lane >> a.log_rows, shares = 32 >> a.log_rows;   // among the lanes with this row
     const int kw = wg * F;                      // GRAD: the warp's features
-    // the groups of all CTAs take tiles in turn, one group of every CTA first
-    const int64_t first = (int64_t)group * gridDim.x + blockIdx.x, step = (int64_t)a.groups * gridDim.x;
+    // The groups of a CTA take neighbouring tiles (of a wide table's columns they then read the
+    // same pages); where there are few tiles, one group of every CTA comes first.
+    const int64_t step = (int64_t)a.groups * gridDim.x;
+    const int64_t first = a.n_tiles >= step ? (int64_t)blockIdx.x * a.groups + group : (int64_t)group * gridDim.x + blockIdx.x;
     const size_t part_at = (size_t)first * a.c * a.d_pad;
     int parity = 0, since = 0;
     bool flushed = false;
@@ -488,9 +539,6 @@ __global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few
         const int64_t y64 = meta.y;
         const float rw = meta.weight, shift_in = meta.lse;
         meta = next;
-        for (int o = R; o < 32; o <<= 1)
-            #pragma unroll
-            for (int c = 0; c < C; ++c) z[c] += __shfl_xor_sync(0xffffffffu, z[c], o);
         // 2. logits of all warps, softmax, loss, g
         if (GRAD && W > 1) {
             float* mine = red + ((size_t)(parity * a.groups + group) * W) * C * 32;
@@ -530,8 +578,9 @@ __global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few
         if (GRAD) {
             // with this call's own sum, e / s; else exp of the difference to the given lse
             const float inv = 1.f / s;
-            // bit r (and r + R, ...) for row r
-            const uint32_t mask = __ballot_sync(0xffffffffu, kept), bad = __ballot_sync(0xffffffffu, !kept && !finite);
+            // bit r: row r is left out and holds something that is no number
+            uint32_t bad = 0;
+            if (__any_sync(0xffffffffu, !kept && !finite)) bad = __reduce_or_sync(0xffffffffu, !kept && !finite ? 1u << row : 0u);
             #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const float p = a.have_lse ? expf(z[c] - shift_in) : e[c] * inv;
@@ -551,19 +600,17 @@ __global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few
             if (DX) {
                 const int left = (int)min((int64_t)R, a.n - r0), feats = min(F, a.d - kw);
                 T* dx = (T*)a.dx + r0 * a.dxr + (int64_t)kw * a.dxk;
+                const uint32_t rows_in = COLS ? 0 : __reduce_or_sync(0xffffffffu, kept ? 1u << row : 0u);   // rows that count
                 const float* wk = ws + (size_t)kw * CL;
                 if (COLS) {
                     // neighbouring lanes are neighbouring rows
                     if (row < left)
-                        for (int k = 2 * share; k < feats; k += 2 * shares) {
-                            Pair wv[C], v = 0;
-                            load_pairs<C>(wv, wk + k * CL);
+                        #pragma unroll 4
+                        for (int k = share; k < feats; k += shares) {
+                            float v = 0.f;
                             #pragma unroll
-                            for (int c = 0; c < C; ++c) fma2(v, pair(e[c], e[c]), wv[c]);
-                            float lo, hi;
-                            unpair(lo, hi, v);
-                            dx[row * a.dxr + k * a.dxk] = from_float<T>(kept ? lo : 0.f);
-                            if (k + 1 < feats) dx[row * a.dxr + (k + 1) * a.dxk] = from_float<T>(kept ? hi : 0.f);
+                            for (int c = 0; c < C; ++c) v = fmaf(e[c], wk[k * CL + c], v);
+                            dx[row * a.dxr + k * a.dxk] = from_float<T>(kept ? v : 0.f);
                         }
                 } else {
                     for (int k = lane; k < feats; k += 32) {
@@ -575,14 +622,14 @@ __global__ void __launch_bounds__(F == 64 ? 256 : 512, F == 64 ? 3 : 1) xent_few
                             float v = 0.f;
                             #pragma unroll
                             for (int c = 0; c < C; ++c) v = fmaf(gs[(r * CL + c) * 2], wv[c], v);
-                            dx[r * a.dxr + k * a.dxk] = from_float<T>((mask >> r) & 1 ? v : 0.f);
+                            dx[r * a.dxr + k * a.dxk] = from_float<T>((rows_in >> r) & 1 ? v : 0.f);
                         }
                     }
                 }
             }
             // 3. a lane is two or four features
             if constexpr (GRAD) {
-                if (a.part && mask) {
+                if (a.part && __any_sync(0xffffffffu, kept)) {
                     const int feats = min(F, a.d - kw);
                     if (R == 32)
                         sums<T, C, COLS, 32, F>(acc, tile, gs, bad, feats, lane);
@@ -622,18 +669,17 @@ cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
 
 template <typename T, int C, bool COLS, bool GRAD, bool DX>
 cudaError_t launch(const FewPlan& p, cudaStream_t s) {
-    if constexpr (few_narrow(C, GRAD))
-        if (p.features == 64) return launch_f<T, C, COLS, GRAD, DX, 64>(p, s);
-    if constexpr (GRAD)
-        if (p.features == 128) return launch_f<T, C, COLS, GRAD, DX, 128>(p, s);
-    return cudaErrorInvalidValue;
+    return launch_f<T, C, COLS, GRAD, DX, few_features(GRAD)>(p, s);
 }
 
 template <typename T, int C>
 cudaError_t launch_c(const FewPlan& p, cudaStream_t s) {
     if (!p.grad) return p.cols ? launch<T, C, true, false, false>(p, s) : launch<T, C, false, false, false>(p, s);
-    if (!p.k.dx) return p.cols ? launch<T, C, true, true, false>(p, s) : launch<T, C, false, true, false>(p, s);
-    return p.cols ? launch<T, C, true, true, true>(p, s) : launch<T, C, false, true, true>(p, s);
+    if constexpr (C <= kFewMaxGrad) {
+        if (!p.k.dx) return p.cols ? launch<T, C, true, true, false>(p, s) : launch<T, C, false, true, false>(p, s);
+        return p.cols ? launch<T, C, true, true, true>(p, s) : launch<T, C, false, true, true>(p, s);
+    }
+    return cudaErrorInvalidValue;
 }
 
 template <typename T>
