@@ -59,7 +59,10 @@ enum { LSE = 0, G = 1, DX = 2, DW = 3 };
 
 constexpr int stage_bytes(int bn) { return kABytes + bn * kBK * 2; }
 constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
-constexpr size_t smem_of(int bn) { return (size_t)stages_of(bn) * stage_bytes(bn) + 1024 + 256; }
+// an epilogue warp's outgoing 32 x 32 block: fp32, or hi and lo in 16 bits
+constexpr int kOutBytes = 4096;
+constexpr size_t smem_of(int bn) { return (size_t)stages_of(bn) * stage_bytes(bn) + kEpiWarps * kOutBytes + 1024 + 256; }
+static_assert(smem_of(256) <= 232448 && smem_of(128) <= 232448 && smem_of(64) <= 232448, "shared memory per CTA");
 
 // What the kernels of one call share on the device; cleared at its start.
 struct Meta {
@@ -91,6 +94,7 @@ __device__ __forceinline__ int g_exponent(const Meta* m, int half_g) { return ha
 
 struct TcArgs {
     CUtensorMap a[2], b[2];   // planes hi, lo
+    CUtensorMap out[2];       // G: planes of g; DX: dx
     int scaled;               // fp32: power-of-two scales in force
     int half_g;               // g in fp16 (scaled by 2^u), else bf16
     int units, m_tiles, n_tiles, splits;
@@ -114,12 +118,11 @@ struct TcArgs {
     const float* weight;
     int64_t weight_stride;
     float scale;
-    void* g[2];               // G: planes [rows][ldg]
-    int64_t ldg;
+    int64_t ldg;              // G: columns of its planes
     float* bias_part;         // G: sums of 32 rows, [row tile x 4][ldg]; null: not wanted
     void* dx;                 // DX
     int64_t dxr, dxk;
-    int dx_vec;
+    int dx_map;               // out[0] is valid; else element stores
     float* dx_acc;            // DX: sums of earlier class pieces, [tile][BN][128]
     int first, last;          // DX: first / last class piece; DW: first row piece
     float* dw_part;           // DW: [split][class tile][feature tile][BN][128]
@@ -138,28 +141,32 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Outgoing blocks of 32 rows (the lanes) x 32 columns in shared memory, as TMA stores read them:
+// 16-byte units of a row exchanged by the 64-byte (16 bits) or 128-byte (fp32) swizzle, which
+// also spreads the lanes' writes over the banks.
 template <typename T>
-__device__ __forceinline__ void store_dx(const TcArgs& a, int64_t row, int64_t col, int count, const float* v) {
-    T* p = (T*)a.dx + row * a.dxr + col * a.dxk;
-    if (a.dx_vec && count == 32) {
-        constexpr int V = 16 / sizeof(T);
-        #pragma unroll
-        for (int j = 0; j < 32; j += V) {
-            uint4 q;
-            if constexpr (sizeof(T) == 4) {
-                q = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]),
-                               __float_as_uint(v[j + 3]));
-            } else {
-                q = make_uint4(pack(v[j], v[j + 1], T{}), pack(v[j + 2], v[j + 3], T{}), pack(v[j + 4], v[j + 5], T{}),
-                               pack(v[j + 6], v[j + 7], T{}));
-            }
-            *reinterpret_cast<uint4*>(p + j) = q;
-        }
-    } else {
-        #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < count) p[j * a.dxk] = from_float<T>(v[j]);
+__device__ __forceinline__ int out_unit(int row, int q) {
+    return sizeof(T) == 4 ? row * 128 + ((q ^ (row & 7)) << 4) : row * 64 + ((q ^ ((row >> 1) & 3)) << 4);
+}
+template <typename T>
+__device__ __forceinline__ void out_write(uint8_t* block, int row, const float* v) {
+    constexpr int V = 16 / sizeof(T);
+    #pragma unroll
+    for (int q = 0; q < 32 / V; ++q) {
+        uint4 u;
+        if constexpr (sizeof(T) == 4)
+            u = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]),
+                           __float_as_uint(v[4 * q + 3]));
+        else
+            u = make_uint4(pack(v[8 * q], v[8 * q + 1], T{}), pack(v[8 * q + 2], v[8 * q + 3], T{}),
+                           pack(v[8 * q + 4], v[8 * q + 5], T{}), pack(v[8 * q + 6], v[8 * q + 7], T{}));
+        *reinterpret_cast<uint4*>(block + out_unit<T>(row, q)) = u;
     }
+}
+template <typename T>
+__device__ __forceinline__ T* out_at(uint8_t* block, int row, int col) {
+    constexpr int V = 16 / sizeof(T);
+    return reinterpret_cast<T*>(block + out_unit<T>(row, col / V)) + col % V;
 }
 
 // A unit of work: `tiles` accumulator tiles (m, n), (m, n + 1), ... (more than one only in LSE),
@@ -233,7 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
     extern __shared__ uint8_t raw[];
     const uint32_t base = (tc::smem_addr(raw) + 1023) & ~1023u;
     uint8_t* gbase = raw + (base - tc::smem_addr(raw));
-    const uint32_t bars = base + S * stage_bytes(BN);
+    const uint32_t outs = base + S * stage_bytes(BN);         // a multiple of 1024
+    const uint32_t bars = outs + kEpiWarps * kOutBytes;
     const uint32_t full0 = bars, empty0 = bars + 8 * S, afull0 = bars + 16 * S, aempty0 = afull0 + 16,
                    drain = afull0 + 32, slot = afull0 + 40;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -373,6 +381,8 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        const uint32_t out_addr = outs + (warp - 4) * kOutBytes;
+        uint8_t* out = gbase + (out_addr - base);
         uint32_t acc = 0;
         bool ok = true;
         const int te = w_exponent(a.meta, a.scaled), ue = g_exponent(a.meta, a.half_g);
@@ -460,31 +470,31 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                             const float p = exp2f((v[j] - sh.x) - sh.y) * wt;
                             v[j] = y >= 0 ? p : 0.f;
                         }
-                        if (valid) {
-                            E* hi = (E*)a.g[0] + row * a.ldg + cb;
-                            E* lo = kPlanes == 2 ? (E*)a.g[1] + row * a.ldg + cb : nullptr;
+                        tc::store_wait_read();       // the block's last store has read it
+                        out_write<E>(out, lane, v);
+                        if (here) *out_at<E>(out, lane, (int)rel) = from_float<E>(gy);
+                        if (kPlanes == 2) {
                             #pragma unroll
                             for (int j = 0; j < 32; j += 8) {
-                                if (cb + j >= a.ldg) break;
                                 uint32_t q[4];
                                 #pragma unroll
-                                for (int i = 0; i < 4; ++i) q[i] = pack(v[j + 2 * i], v[j + 2 * i + 1], E{});
-                                *reinterpret_cast<uint4*>(hi + j) = make_uint4(q[0], q[1], q[2], q[3]);
-                                if (kPlanes == 2) {
-                                    #pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const float h0 = to_float(from_float<E>(v[j + 2 * i]));
-                                        const float h1 = to_float(from_float<E>(v[j + 2 * i + 1]));
-                                        q[i] = pack(v[j + 2 * i] - h0, v[j + 2 * i + 1] - h1, E{});
-                                    }
-                                    *reinterpret_cast<uint4*>(lo + j) = make_uint4(q[0], q[1], q[2], q[3]);
+                                for (int i = 0; i < 4; ++i) {
+                                    const float h0 = to_float(from_float<E>(v[j + 2 * i]));
+                                    const float h1 = to_float(from_float<E>(v[j + 2 * i + 1]));
+                                    q[i] = pack(v[j + 2 * i] - h0, v[j + 2 * i + 1] - h1, E{});
                                 }
+                                *reinterpret_cast<uint4*>(out + 2048 + out_unit<E>(lane, j / 8)) =
+                                    make_uint4(q[0], q[1], q[2], q[3]);
                             }
-                            if (here) {
-                                const E h = from_float<E>(gy);
-                                hi[rel] = h;
-                                if (kPlanes == 2) lo[rel] = from_float<E>(gy - to_float(h));
-                            }
+                            if (here) *out_at<E>(out + 2048, lane, (int)rel) = from_float<E>(gy - to_float(from_float<E>(gy)));
+                        }
+                        tc::fence_async_smem();
+                        __syncwarp();
+                        const int64_t y0 = (int64_t)t.m * kBM + quarter * 32;
+                        if (lane == 0 && y0 < a.rows) {
+                            tc::store_2d(&a.out[0], out_addr, (int)cb, (int)y0);
+                            if (kPlanes == 2) tc::store_2d(&a.out[1], out_addr + 2048, (int)cb, (int)y0);
+                            tc::store_commit();
                         }
                         if (a.bias_part) {
                             // the bias's gradient from g before its rounding: 32 rows' sums a column
@@ -507,7 +517,8 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                         if (!a.last) {
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) keep[j * kBM] = v[j];
-                        } else if (valid) {
+                        } else {
+                            using D = typename std::conditional<kPlanes == 2, float, E>::type;
                             const int count = (int)min((int64_t)32, a.cols - cb);
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) {
@@ -515,10 +526,34 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                                 if (kPlanes == 2 && j < count) e += fit_exponent(a.colmax[cb + j]);
                                 v[j] = y >= 0 ? scale2(v[j], e) : 0.f;
                             }
-                            if (kPlanes == 2)
-                                store_dx<float>(a, a.row0 + row, cb, count, v);
-                            else
-                                store_dx<E>(a, a.row0 + row, cb, count, v);
+                            const int64_t y0 = (int64_t)t.m * kBM + quarter * 32;
+                            D* dx = (D*)a.dx + (a.row0 + y0) * a.dxr + cb * a.dxk;
+                            if (a.dxr == 1 && a.dxk != 1) {
+                                // column by column: neighbouring lanes are neighbouring rows
+                                if (valid)
+                                    #pragma unroll
+                                    for (int j = 0; j < 32; ++j)
+                                        if (j < count) dx[lane + j * a.dxk] = from_float<D>(v[j]);
+                            } else {
+                                tc::store_wait_read();
+                                out_write<D>(out, lane, v);
+                                if (a.dx_map) {
+                                    tc::fence_async_smem();
+                                    __syncwarp();
+                                    if (lane == 0 && y0 < a.rows) {
+                                        tc::store_2d(&a.out[0], out_addr, (int)cb, (int)(a.row0 + y0));
+                                        tc::store_commit();
+                                    }
+                                } else {
+                                    // rows that TMA cannot reach: one at a time, a lane a column
+                                    __syncwarp();
+                                    const int rows = (int)min((int64_t)32, a.rows - y0);
+                                    if (lane < count)
+                                        #pragma unroll 8
+                                        for (int i = 0; i < rows; ++i) dx[i * a.dxr + lane * a.dxk] = *out_at<D>(out, i, lane);
+                                    __syncwarp();
+                                }
+                            }
                         }
                     } else {
                         float* p = a.dw_part + t.split * a.dw_split_stride +
@@ -536,6 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                 if (!isnan(zy)) a.zy[row] = zy;   // one thread of all has the label's column
             }
         }
+        tc::store_wait_all();
     }
     tc::fence_before();
     __syncthreads();
@@ -631,39 +667,72 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     if (lse) lse[r] = failed ? NAN : kept ? (float)(((double)sh + (double)l) * 0.69314718055994530942) : 0.f;
 }
 
-// largest finite |x_k| over the rows that count
+// Rows read four features at a time: unit features, 16-byte aligned rows.
+__host__ __device__ inline bool rows_vector(const void* p, int64_t sr, int64_t sk) {
+    return sk == 1 && sr >= 0 && (uintptr_t)p % 16 == 0 && sr % 4 == 0;
+}
+__device__ __forceinline__ float4 load_quad(const float* row, int64_t k, int64_t d) {
+    if (k + 4 <= d) return *reinterpret_cast<const float4*>(row + k);
+    return make_float4(k < d ? row[k] : 0.f, k + 1 < d ? row[k + 1] : 0.f, k + 2 < d ? row[k + 2] : 0.f, 0.f);
+}
+__device__ __forceinline__ float finite_abs(float v) {
+    v = fabsf(v);
+    return v <= 3.402823466e38f ? v : 0.f;
+}
+
+// Largest finite |x_k| over the rows that count.  A block takes `rows` rows and, row by row, a
+// run of 4 x 256 features (a thread four of them, several rows at once where the features are
+// fewer), else 32 features with a warp going down one of them at a time.
 __global__ void __launch_bounds__(256) xent_colmax_kernel(const float* __restrict__ x, int64_t xr, int64_t xk,
                                                           const int64_t* __restrict__ labels, int64_t n, int64_t d,
-                                                          int64_t rows, uint32_t* colmax) {
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t tiles_k = (d + 31) / 32;
-    const int64_t k0 = (blockIdx.x % tiles_k) * 32, r0 = (blockIdx.x / tiles_k) * rows;
-    const int64_t r1 = min(n, r0 + rows);
-    __shared__ uint32_t top[32];
-    if (threadIdx.x < 32) top[threadIdx.x] = 0;
+                                                          int64_t rows, int vector, uint32_t* colmax) {
+    __shared__ uint32_t top[1024];
+    const int64_t width = vector ? 1024 : 32, blocks_k = (d + width - 1) / width;
+    const int64_t k0 = (blockIdx.x % blocks_k) * width, r0 = (blockIdx.x / blocks_k) * rows, r1 = min(n, r0 + rows);
+    for (int i = threadIdx.x; i < width; i += 256) top[i] = 0;
     __syncthreads();
-    if (xr == 1 && xk != 1) {
-        // a warp goes down one feature
+    if (vector) {
+        const int quads = (int)min((int64_t)256, (d - k0 + 3) / 4), at_once = 256 / quads;
+        const int quad = threadIdx.x % quads, ro = threadIdx.x / quads;
+        if (ro < at_once) {
+            float m[4] = {0.f, 0.f, 0.f, 0.f};
+            #pragma unroll 4
+            for (int64_t r = r0 + ro; r < r1; r += at_once) {
+                const float4 v = load_quad(x + r * xr, k0 + 4 * quad, d);
+                if (labels[r] < 0) continue;
+                m[0] = fmaxf(m[0], finite_abs(v.x));
+                m[1] = fmaxf(m[1], finite_abs(v.y));
+                m[2] = fmaxf(m[2], finite_abs(v.z));
+                m[3] = fmaxf(m[3], finite_abs(v.w));
+            }
+            for (int i = 0; i < 4; ++i) atomicMax(&top[4 * quad + i], __float_as_uint(m[i]));
+        }
+    } else if (xr == 1 && xk != 1) {
+        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
         for (int j = ty; j < 32 && k0 + j < d; j += 8) {
             float m = 0.f;
+            #pragma unroll 8
             for (int64_t r = r0 + tx; r < r1; r += 32) {
-                const float v = fabsf(x[r + (k0 + j) * xk]);
-                if (labels[r] >= 0 && v <= 3.402823466e38f) m = fmaxf(m, v);
+                const float v = finite_abs(x[r + (k0 + j) * xk]);
+                if (labels[r] >= 0) m = fmaxf(m, v);
             }
             const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
             if (tx == 0) top[j] = w;
         }
     } else {
+        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
         float m = 0.f;
         if (k0 + tx < d)
+            #pragma unroll 4
             for (int64_t r = r0 + ty; r < r1; r += 8) {
-                const float v = fabsf(x[r * xr + (k0 + tx) * xk]);
-                if (labels[r] >= 0 && v <= 3.402823466e38f) m = fmaxf(m, v);
+                const float v = finite_abs(x[r * xr + (k0 + tx) * xk]);
+                if (labels[r] >= 0) m = fmaxf(m, v);
             }
         atomicMax(&top[tx], __float_as_uint(m));
     }
     __syncthreads();
-    if (threadIdx.x < 32 && k0 + threadIdx.x < d && top[threadIdx.x]) atomicMax(&colmax[k0 + threadIdx.x], top[threadIdx.x]);
+    for (int i = threadIdx.x; i < width; i += 256)
+        if (k0 + i < d && top[i]) atomicMax(&colmax[k0 + i], top[i]);
 }
 
 // largest exponent of w_jk 2^-s_k
@@ -680,47 +749,101 @@ __global__ void __launch_bounds__(256) xent_wmax_kernel(const float* __restrict_
     if ((threadIdx.x & 31) == 0 && top) atomicMax(&meta->w_exp, (uint32_t)top);
 }
 
-// rows x d of any strides -> planes [rows][dp]; rows with a negative label become zeros.
-// fp32: hi and lo fp16 of the scaled value; 16 bits: a copy.
+// Exponent that a plane's values of feature k are scaled by.
+__device__ __forceinline__ int plane_exponent(const uint32_t* colmax, const Meta* meta, int64_t k, int64_t d, int is_w) {
+    const int e = k < d ? fit_exponent(colmax[k]) : 0;
+    return is_w ? w_exponent(meta, 1) - e : e;
+}
+// hi and lo of two scaled values; nothing below a value that is not finite
+__device__ __forceinline__ void split2(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(v0, v1);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack(isfinite(f.x) ? v0 - f.x : 0.f, isfinite(f.y) ? v1 - f.y : 0.f, __half{});
+}
+
+// fp32 rows in 16-byte units -> planes [rows][dp], hi and lo fp16 of the scaled values; rows with
+// a negative label become zeros.  A thread keeps four features and their scales over its rows.
+__global__ void __launch_bounds__(256) xent_planes_rows_kernel(const float* __restrict__ x, int64_t xr,
+                                                               const int64_t* __restrict__ labels, int64_t n, int64_t d,
+                                                               int64_t dp, int64_t rows, const uint32_t* __restrict__ colmax,
+                                                               const Meta* __restrict__ meta, int is_w,
+                                                               __half* __restrict__ hi, __half* __restrict__ lo) {
+    const int64_t blocks_k = (dp + 1023) / 1024;
+    const int64_t k0 = (blockIdx.x % blocks_k) * 1024, r0 = (blockIdx.x / blocks_k) * rows, r1 = min(n, r0 + rows);
+    const int quads = (int)min((int64_t)256, (dp - k0) / 4), at_once = 256 / quads;
+    const int quad = threadIdx.x % quads, ro = threadIdx.x / quads;
+    if (ro >= at_once) return;
+    const int64_t k = k0 + 4 * quad;
+    float f0[4], f1[4];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = plane_exponent(colmax, meta, k + i, d, is_w), h = e / 2;
+        f0[i] = pow2i(h);
+        f1[i] = pow2i(e - h);
+    }
+    #pragma unroll 4
+    for (int64_t r = r0 + ro; r < r1; r += at_once) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!labels || labels[r] >= 0) v = load_quad(x + r * xr, k, d);
+        uint2 h, l;
+        split2(v.x * f0[0] * f1[0], v.y * f0[1] * f1[1], h.x, l.x);
+        split2(v.z * f0[2] * f1[2], v.w * f0[3] * f1[3], h.y, l.y);
+        *reinterpret_cast<uint2*>(hi + r * dp + k) = h;
+        *reinterpret_cast<uint2*>(lo + r * dp + k) = l;
+    }
+}
+
+// rows x d of any strides -> planes [rows][dp], a 64 x 64 tile a block; rows with a negative label
+// become zeros.  fp32: hi and lo fp16 of the scaled value; 16 bits: a copy.
 template <typename T, typename E>
 __global__ void __launch_bounds__(256) xent_planes_kernel(const T* __restrict__ x, int64_t xr, int64_t xk,
                                                           const int64_t* __restrict__ labels, int64_t n, int64_t d,
                                                           int64_t dp, const uint32_t* __restrict__ colmax,
                                                           const Meta* __restrict__ meta, int is_w, E* __restrict__ hi,
                                                           E* __restrict__ lo) {
-    __shared__ float t[64][65];
+    __shared__ float t[64][65];      // [feature][row]
     const int64_t tiles_k = (dp + 63) / 64;
     const int64_t k0 = (blockIdx.x % tiles_k) * 64, r0 = (blockIdx.x / tiles_k) * 64;
     const bool down = xr == 1 && xk != 1;
+    #pragma unroll 4
     for (int i = threadIdx.x; i < 64 * 64; i += 256) {
         const int r = down ? i & 63 : i >> 6, k = down ? i >> 6 : i & 63;
         float v = 0.f;
         if (r0 + r < n && k0 + k < d && (!labels || labels[r0 + r] >= 0)) v = to_float(x[(r0 + r) * xr + (k0 + k) * xk]);
-        t[r][k] = v;
+        t[k][r] = v;
     }
     __syncthreads();
-    const int k = (threadIdx.x & 31) * 2;
+    // 8 features of a row to a thread, 16 bytes of a plane
+    const int k = (threadIdx.x & 7) * 8;
     if (k0 + k >= dp) return;
-    int e0 = 0, e1 = 0;
-    if (sizeof(T) == 4) {
-        const int te = w_exponent(meta, 1);
-        const int s0 = k0 + k < d ? fit_exponent(colmax[k0 + k]) : 0, s1 = k0 + k + 1 < d ? fit_exponent(colmax[k0 + k + 1]) : 0;
-        e0 = is_w ? te - s0 : s0;
-        e1 = is_w ? te - s1 : s1;
-    }
-    for (int r = threadIdx.x >> 5; r < 64 && r0 + r < n; r += 8) {
-        float v0 = t[r][k], v1 = t[r][k + 1];
-        const int64_t at = (r0 + r) * dp + k0 + k;
-        if (sizeof(T) == 4) {
-            v0 = scale2(v0, e0);
-            v1 = scale2(v1, e1);
-            const float h0 = to_float(from_float<E>(v0)), h1 = to_float(from_float<E>(v1));
-            *reinterpret_cast<uint32_t*>(hi + at) = pack(v0, v1, E{});
-            // nothing below a value that is not finite
-            *reinterpret_cast<uint32_t*>(lo + at) = pack(isfinite(h0) ? v0 - h0 : 0.f, isfinite(h1) ? v1 - h1 : 0.f, E{});
-        } else {
-            *reinterpret_cast<uint32_t*>(hi + at) = pack(v0, v1, E{});
+    float f0[8], f1[8];
+    if constexpr (sizeof(T) == 4) {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = plane_exponent(colmax, meta, k0 + k + i, d, is_w), h = e / 2;
+            f0[i] = pow2i(h);
+            f1[i] = pow2i(e - h);
         }
+    }
+    #pragma unroll
+    for (int r = threadIdx.x >> 3; r < 64; r += 32) {
+        if (r0 + r >= n) break;
+        const int64_t at = (r0 + r) * dp + k0 + k;
+        uint32_t h[4], l[4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v0 = t[k + 2 * i][r], v1 = t[k + 2 * i + 1][r];
+            if constexpr (sizeof(T) == 4) {
+                v0 = v0 * f0[2 * i] * f1[2 * i];
+                v1 = v1 * f0[2 * i + 1] * f1[2 * i + 1];
+                split2(v0, v1, h[i], l[i]);
+            } else {
+                h[i] = pack(v0, v1, E{});
+            }
+        }
+        *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
     }
 }
 
@@ -798,6 +921,24 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
             fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
     });
     return fn;
+}
+
+// rows of `inner` values, `ld` apart, written in blocks of 32 x 32
+bool make_out_map(CUtensorMap* map, int type, const void* base, int64_t inner, int64_t rows, int64_t ld) {
+    auto enc = encoder();
+    if (!enc) return false;
+    const bool wide = type == GAFIME_TYPE_FP32;
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * (wide ? 4 : 2)};
+    cuuint32_t box[2] = {32, 32};
+    cuuint32_t estr[2] = {1, 1};
+    return enc(map,
+               wide                          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+               : type == GAFIME_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+               2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // rows of `inner` 16-bit values, `ld` apart; boxes of 64 values x box_rows
@@ -948,8 +1089,17 @@ cudaError_t launch(const TcArgs& t, int bn, int sms, cudaStream_t stream) {
 
 template <typename T, typename E>
 cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const int64_t* labels, int64_t rows, int64_t d,
-                   bool is_w, uint16_t* hi, uint16_t* lo, cudaStream_t stream) {
-    if (rows == 0) return cudaSuccess;
+                   bool is_w, uint16_t* hi, uint16_t* lo, int sms, cudaStream_t stream) {
+    if constexpr (sizeof(T) == 4) {
+        if (rows_vector(src, sr, sk)) {
+            const int64_t blocks_k = cdiv(p.dp, 1024);
+            const int64_t per = std::max<int64_t>(16, cdiv(rows * blocks_k, 16 * sms));
+            KernelTimer kt(stream, GAFIME_KERNEL_XENT);
+            xent_planes_rows_kernel<<<(unsigned)(blocks_k * cdiv(rows, per)), 256, 0, stream>>>(
+                src, sr, labels, rows, d, p.dp, per, p.colmax, p.meta, is_w, (__half*)hi, (__half*)lo);
+            return cudaGetLastError();
+        }
+    }
     const int64_t blocks = cdiv(p.dp, 64) * cdiv(rows, 64);
     KernelTimer kt(stream, GAFIME_KERNEL_XENT);
     xent_planes_kernel<T, E><<<(unsigned)blocks, 256, 0, stream>>>(src, sr, sk, labels, rows, d, p.dp, p.colmax, p.meta,
@@ -987,11 +1137,12 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     }
     if (scaled) {
         {
-            const int64_t tiles_k = cdiv(a.d, 32);
-            const int64_t rows = std::max<int64_t>(64, cdiv(a.n * tiles_k, 8 * sms));
+            const int vector = rows_vector(a.x, a.xr, a.xk);
+            const int64_t blocks_k = cdiv(a.d, vector ? 1024 : 32);
+            const int64_t rows = std::max<int64_t>(64, cdiv(a.n * blocks_k, 8 * sms));
             KernelTimer kt(st, GAFIME_KERNEL_XENT);
-            xent_colmax_kernel<<<(unsigned)(tiles_k * cdiv(a.n, rows)), 256, 0, st>>>((const float*)a.x, a.xr, a.xk, a.labels,
-                                                                                   a.n, a.d, rows, p.colmax);
+            xent_colmax_kernel<<<(unsigned)(blocks_k * cdiv(a.n, rows)), 256, 0, st>>>(
+                (const float*)a.x, a.xr, a.xk, a.labels, a.n, a.d, rows, vector, p.colmax);
             XENT_TRY(cudaGetLastError());
         }
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
@@ -999,8 +1150,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             (const float*)a.w, a.wr, a.wk, a.c, a.d, p.colmax, p.meta);
         XENT_TRY(cudaGetLastError());
     }
-    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, p.xh, p.xl, st)));
-    if (p.wh) XENT_TRY((planes<T, E>(p, (const T*)a.w, a.wr, a.wk, nullptr, a.c, a.d, true, p.wh, p.wl, st)));
+    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, p.xh, p.xl, sms, st)));
+    if (p.wh) XENT_TRY((planes<T, E>(p, (const T*)a.w, a.wr, a.wk, nullptr, a.c, a.d, true, p.wh, p.wl, sms, st)));
     // where the operands are read
     const void *xs[2] = {p.xh ? (const void*)p.xh : a.x, p.xl}, *ws[2] = {p.wh ? (const void*)p.wh : a.w, p.wl};
     const int64_t ldx = p.xh ? p.dp : a.xr, ldw = p.wh ? p.dp : a.wr;
@@ -1064,8 +1215,9 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             g.c0 = (int)c0;
             g.shift = p.shift;
             g.loss = a.loss;
-            g.g[0] = p.gh;
-            g.g[1] = p.gl;
+            for (int i = 0; i < p.planes; ++i)
+                if (!make_out_map(&g.out[i], kBf16 ? GAFIME_TYPE_BF16 : GAFIME_TYPE_FP16, gs[i], p.ldg, rows, p.ldg))
+                    return cudaErrorInvalidValue;
             g.ldg = p.ldg;
             g.bias_part = a.dbias ? p.bias_sums : nullptr;
             XENT_TRY((launch<G, E, kPlanes>(g, p.bn_c, sms, st)));
@@ -1091,7 +1243,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 x.row0 = r0;
                 x.cols = a.d;
                 x.dx = a.dx; x.dxr = a.dxr; x.dxk = a.dxk;
-                x.dx_vec = a.dxk == 1 && (uintptr_t)a.dx % 16 == 0 && a.dxr * (int64_t)sizeof(T) % 16 == 0;
+                x.dx_map = a.dxk == 1 && (uintptr_t)a.dx % 16 == 0 && a.dxr >= a.d && a.dxr * (int64_t)sizeof(T) % 16 == 0;
+                if (x.dx_map && !make_out_map(&x.out[0], a.type, a.dx, a.d, a.n, a.dxr)) return cudaErrorInvalidValue;
                 x.dx_acc = p.dx_acc;
                 x.first = c0 == 0;
                 x.last = c0 + classes == a.c;
