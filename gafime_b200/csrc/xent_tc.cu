@@ -417,15 +417,25 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                     if (!(ok = tc::bar_wait_warp(afull0 + 8 * (acc & 1), (acc >> 1) & 1, err, 6))) break;
                     tc::fence_after();
                     #pragma unroll
-                    for (int ch = 0; ch < kCols / 16; ++ch) {
-                        float v[16];
-                        tc::tmem_load16(tmem + (acc & 1) * BN + half * kCols + ch * 16 + lane_addr, v);
+                    for (int ch = 0; ch < kCols / 32; ch += 2) {
+                        // two loads under way before the wait
+                        float v[32], w[32];
+                        const uint32_t at = tmem + (acc & 1) * BN + half * kCols + ch * 32 + lane_addr;
+                        tc::tmem_load32(at, v);
+                        if constexpr (kCols > 32) tc::tmem_load32(at + 32, w);
+                        tc::tmem_wait(v);
+                        if constexpr (kCols > 32) tc::tmem_settle(w);
+                        if (ch + 2 >= kCols / 32) {
+                            tc::fence_before();
+                            __syncwarp();
+                            if (lane == 0) tc::bar_arrive(aempty0 + 8 * (acc & 1));
+                        }
                         #pragma unroll
-                        for (int j = 0; j < 16; ++j) sums[ch * 16 + j] += v[j];
+                        for (int j = 0; j < 32; ++j) sums[ch * 32 + j] += v[j];
+                        if constexpr (kCols > 32)
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) sums[ch * 32 + 32 + j] += w[j];
                     }
-                    tc::fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::bar_arrive(aempty0 + 8 * (acc & 1));
                 }
                 if (!ok) break;
                 #pragma unroll
@@ -1032,7 +1042,7 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
             const int64_t more = (int64_t)(kPieceBytes / (p.piece_rows * es * up(a.c, 8)));
             if (more > 1) p.piece_rows = std::min<int64_t>(up(a.n, kBM), p.piece_rows * more);
         }
-        p.ldg = up(p.piece_classes, 8);
+        p.ldg = up(p.piece_classes, 64);   // whole 128-byte lines: TMA boxes meet no line twice
         p.gh = cv.take<uint16_t>(p.piece_rows * p.ldg);
         if (p.planes == 2) p.gl = cv.take<uint16_t>(p.piece_rows * p.ldg);
         p.dw_d_tiles = cdiv(a.d, p.bn_d);
