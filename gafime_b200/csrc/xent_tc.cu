@@ -53,7 +53,7 @@ constexpr int kBK = 64;                      // 16-bit values of K to a stage
 constexpr int kABytes = kBM * kBK * 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr size_t kPieceBytes = (size_t)128 << 20;   // of g: about what L2 keeps between its kernels
+constexpr size_t kPieceBytes = (size_t)256 << 20;   // of g
 
 enum { LSE = 0, G = 1, DX = 2, DW = 3 };
 
@@ -85,6 +85,12 @@ __device__ __forceinline__ float scale2(float v, int e) {
     e = min(252, max(-252, e));
     const int h = e / 2;
     return v * pow2i(h) * pow2i(e - h);
+}
+// 2^v; below 2^-126 zero, which is nothing beside the sums it enters (2^-22 relative otherwise)
+__device__ __forceinline__ float exp2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
 __device__ __forceinline__ int w_exponent(const Meta* m, int scaled) {
     if (!scaled || m->w_exp == 0) return 0;
@@ -123,6 +129,8 @@ struct TcArgs {
     void* dx;                 // DX
     int64_t dxr, dxk;
     int dx_map;               // out[0] is valid; else element stores
+    const float* undo;        // DX, fp32: two factors a feature, undo_pitch apart, 2^(s_k - t - u)
+    int64_t undo_pitch;
     float* dx_acc;            // DX: sums of earlier class pieces, [tile][BN][128]
     int first, last;          // DX: first / last class piece; DW: first row piece
     float* dw_part;           // DW: [split][class tile][feature tile][BN][128]
@@ -394,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
             int64_t y = -1;
             float top = -INFINITY, sum = 0.f, zy = NAN;    // LSE
             float2 sh = make_float2(0.f, 0.f);             // G
-            float wt = 0.f, gy = 0.f;
+            float wt = 0.f, ws = 0.f, gy = 0.f;            // ws: the weight over the row's sum
             if (MODE != DW && valid) {
                 y = a.labels[a.row0 + row];
                 if (MODE == G && y >= 0) {
@@ -404,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                     // exp(z_y - lse) - 1 from the loss, without the cancellation
                     gy = expm1f(-a.loss[a.row0 + row]) * wt;
                     if (y >= a.c_total) wt = NAN;
+                    ws = wt * exp2f(-sh.y);
                 }
             }
             for (int r = 0; ok && r < t.tiles && t.kn > 0; ++r) {
@@ -467,8 +476,8 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                         const float shift = m == -INFINITY ? 0.f : m;   // nothing but excluded classes so far
                         float s = 0.f;
                         #pragma unroll
-                        for (int j = 0; j < 32; ++j) s += exp2f(v[j] - shift);
-                        sum = sum * exp2f(top - shift) + s;
+                        for (int j = 0; j < 32; ++j) s += exp2_fast(v[j] - shift);
+                        sum = sum * exp2_fast(top - shift) + s;
                         top = m;
                         if (hit) {
                             const float q = pick(v, (int)rel & 31);
@@ -477,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                     } else if (MODE == G) {
                         #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float p = exp2f((v[j] - sh.x) - sh.y) * wt;
+                            const float p = exp2_fast(v[j] - sh.x) * ws;
                             v[j] = y >= 0 ? p : 0.f;
                         }
                         tc::store_wait_read();       // the block's last store has read it
@@ -530,12 +539,25 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                         } else {
                             using D = typename std::conditional<kPlanes == 2, float, E>::type;
                             const int count = (int)min((int64_t)32, a.cols - cb);
-                            #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                int e = -ue - te;
-                                if (kPlanes == 2 && j < count) e += fit_exponent(a.colmax[cb + j]);
-                                v[j] = y >= 0 ? scale2(v[j], e) : 0.f;
+                            if (kPlanes == 2) {
+                                const float4* f4 = reinterpret_cast<const float4*>(a.undo + cb);
+                                const float4* g4 = reinterpret_cast<const float4*>(a.undo + a.undo_pitch + cb);
+                                #pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const float4 p = __ldg(f4 + j), q = __ldg(g4 + j);
+                                    v[4 * j] = v[4 * j] * p.x * q.x;
+                                    v[4 * j + 1] = v[4 * j + 1] * p.y * q.y;
+                                    v[4 * j + 2] = v[4 * j + 2] * p.z * q.z;
+                                    v[4 * j + 3] = v[4 * j + 3] * p.w * q.w;
+                                }
+                            } else {
+                                const float q = pow2i(-ue);
+                                #pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] *= q;
                             }
+                            if (y < 0)
+                                #pragma unroll
+                                for (int j = 0; j < 32; ++j) v[j] = 0.f;
                             const int64_t y0 = (int64_t)t.m * kBM + quarter * 32;
                             D* dx = (D*)a.dx + (a.row0 + y0) * a.dxr + cb * a.dxk;
                             if (a.dxr == 1 && a.dxk != 1) {
@@ -804,6 +826,17 @@ __global__ void __launch_bounds__(256) xent_planes_rows_kernel(const float* __re
     }
 }
 
+// Factors that undo the scales of a gradient of x: 2^(s_k - t - u) as two that fp32 holds.
+__global__ void __launch_bounds__(256) xent_undo_kernel(const uint32_t* __restrict__ colmax, int64_t d, int64_t pitch,
+                                                        const Meta* __restrict__ meta, float* __restrict__ undo) {
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (k >= pitch) return;
+    const int e = (k < d ? fit_exponent(colmax[k]) : 0) - w_exponent(meta, 1) - g_exponent(meta, 1);
+    const int c = min(252, max(-252, e)), h = c / 2;
+    undo[k] = pow2i(h);
+    undo[pitch + k] = pow2i(c - h);
+}
+
 // rows x d of any strides -> planes [rows][dp], a 64 x 64 tile a block; rows with a negative label
 // become zeros.  fp32: hi and lo fp16 of the scaled value; 16 bits: a copy.
 template <typename T, typename E>
@@ -996,6 +1029,8 @@ struct Plan {
     float* zy;
     float2* shift;
     float* dx_acc;
+    float* undo;
+    int64_t undo_pitch;
     float* dw_part;
     float* bias_sums;
     double* bias_part;
@@ -1047,6 +1082,8 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
         if (p.planes == 2) p.gl = cv.take<uint16_t>(p.piece_rows * p.ldg);
         p.dw_d_tiles = cdiv(a.d, p.bn_d);
         p.dw_c_tiles = cdiv(a.c, kBM);
+        p.undo_pitch = p.dw_d_tiles * p.bn_d;
+        if (a.dx && p.planes == 2) p.undo = cv.take<float>(2 * p.undo_pitch);
         if (a.dx && p.piece_classes < a.c)
             p.dx_acc = cv.take<float>(cdiv(p.piece_rows, kBM) * p.dw_d_tiles * p.bn_d * kBM);
         if (a.dw) {
@@ -1172,7 +1209,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     };
 
     TcArgs t{};
-    t.chunk = p.planes == 2 ? 1 : 4;
+    t.chunk = p.planes == 2 ? 1 : 8;
     t.scaled = scaled;
     t.half_g = !kBf16;
     t.meta = p.meta;
@@ -1205,6 +1242,11 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     }
     if (!p.products) return cudaSuccess;
 
+    if (p.undo) {
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_undo_kernel<<<(unsigned)cdiv(p.undo_pitch, 256), 256, 0, st>>>(p.colmax, a.d, p.undo_pitch, p.meta, p.undo);
+        XENT_TRY(cudaGetLastError());
+    }
     const void* gs[2] = {p.gh, p.gl};
     for (int64_t r0 = 0; r0 < a.n; r0 += p.piece_rows) {
         const int64_t rows = std::min(p.piece_rows, a.n - r0);
@@ -1255,6 +1297,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 x.dx = a.dx; x.dxr = a.dxr; x.dxk = a.dxk;
                 x.dx_map = a.dxk == 1 && (uintptr_t)a.dx % 16 == 0 && a.dxr >= a.d && a.dxr * (int64_t)sizeof(T) % 16 == 0;
                 if (x.dx_map && !make_out_map(&x.out[0], a.type, a.dx, a.d, a.n, a.dxr)) return cudaErrorInvalidValue;
+                x.undo = p.undo;
+                x.undo_pitch = p.undo_pitch;
                 x.dx_acc = p.dx_acc;
                 x.first = c0 == 0;
                 x.last = c0 + classes == a.c;
