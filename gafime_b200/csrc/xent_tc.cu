@@ -620,10 +620,6 @@ struct SetupArgs {
     int64_t weight_stride;
     float scale;
     int want_weight;          // largest row weight
-    const void* x;            // poison: 16-bit x read in place
-    int64_t xr, xk, d;
-    int bf16;
-    uint32_t* poison;         // nullable
     const float* bias;
     float* bias2;
     int64_t c, c_pad;
@@ -636,7 +632,7 @@ __global__ void __launch_bounds__(256) xent_setup_kernel(SetupArgs a) {
     const int64_t gt = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
     for (int64_t i = gt; i < a.c_pad; i += all)
         a.bias2[i] = i < a.c ? (a.bias ? a.bias[i] * kLog2e : 0.f) : -INFINITY;
-    if (!a.want_weight && !a.poison && !a.zy) return;
+    if (!a.want_weight && !a.zy) return;
     float top = 0.f;
     for (int64_t w = gt / 32; w < (a.n + 31) / 32; w += all / 32) {
         const int64_t r = w * 32 + lane;
@@ -647,22 +643,6 @@ __global__ void __launch_bounds__(256) xent_setup_kernel(SetupArgs a) {
             const float v = fabsf((a.weight ? a.weight[r * a.weight_stride] : 1.f) * a.scale);
             if (v <= 3.402823466e38f) top = fmaxf(top, v);
         }
-        if (a.poison) {
-            uint32_t out = __ballot_sync(0xffffffffu, in && !kept), bad = 0;
-            while (out) {
-                const int q = __ffs(out) - 1;
-                out &= out - 1;
-                bool b = false;
-                const uint16_t* p = (const uint16_t*)a.x + (w * 32 + q) * a.xr;
-                const uint16_t inf = a.bf16 ? 0x7f80 : 0x7c00;
-                for (int64_t k = lane; k < a.d; k += 32) b |= (p[k * a.xk] & inf) == inf;
-                if (__any_sync(0xffffffffu, b)) bad |= 1u << q;
-            }
-            if (lane == 0) {
-                a.poison[w] = bad;
-                if (bad) a.meta->poison = 1;
-            }
-        }
     }
     if (a.want_weight) {
         const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
@@ -670,12 +650,39 @@ __global__ void __launch_bounds__(256) xent_setup_kernel(SetupArgs a) {
     }
 }
 
+// Marks left-out rows of a 16-bit x read in place that hold a value that is no number; a warp a row.
+__global__ void __launch_bounds__(256) xent_poison_kernel(const int64_t* __restrict__ labels, int64_t n,
+                                                          const uint16_t* __restrict__ x, int64_t xr, int64_t d, int bf16,
+                                                          uint32_t* poison, Meta* meta) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t inf = bf16 ? 0x7f80 : 0x7c00;
+    for (int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32; r < n; r += (int64_t)gridDim.x * blockDim.x / 32) {
+        if (labels[r] >= 0) continue;
+        bool b = false;
+        // rows read in place start on 16 bytes
+        const uint4* p = reinterpret_cast<const uint4*>(x + r * xr);
+        for (int64_t k = lane; k < d / 8; k += 32) {
+            const uint4 q = p[k];
+            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) b |= (u[i] & inf) == inf || (u[i] >> 16 & inf) == inf;
+        }
+        if (lane < d % 8) b |= (x[r * xr + d / 8 * 8 + lane] & inf) == inf;
+        if (__any_sync(0xffffffffu, b) && lane == 0) {
+            atomicOr(&poison[r / 32], 1u << (r % 32));
+            meta->poison = 1;
+        }
+    }
+}
+
 // lse and loss of a row from its partial maxima and sums; with the sums given (have_lse), only
 // the shift that g subtracts
-__global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part, int parts, const float* zy,
-                                                        const int64_t* labels, int64_t n, int have_lse, float* loss,
-                                                        float* lse, float2* shift, const Meta* meta) {
-    const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+__global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part, int parts, int lanes,
+                                                        const float* zy, const int64_t* labels, int64_t n, int have_lse,
+                                                        float* loss, float* lse, float2* shift, const Meta* meta) {
+    // `lanes` neighbouring threads to a row, 1 or 32
+    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, r = at / lanes;
+    const int lane = (int)(at % lanes);
     if (r >= n) return;
     if (have_lse) {
         const double l2 = (double)lse[r] * 1.4426950408889634074;
@@ -684,13 +691,20 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
         return;
     }
     float m = -INFINITY;
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, part[r * parts + i].x);
+    for (int i = lane; i < parts; i += lanes) m = fmaxf(m, part[r * parts + i].x);
+    if (lanes == 32)
+        #pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float sh = m == -INFINITY ? 0.f : m;
     float s = 0.f;
-    for (int i = 0; i < parts; ++i) {
+    for (int i = lane; i < parts; i += lanes) {
         const float2 p = part[r * parts + i];
         s += p.y * exp2f(p.x - sh);
     }
+    if (lanes == 32)
+        #pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane != 0) return;
     const float l = log2f(s);
     if (shift) shift[r] = make_float2(sh, l);
     const bool kept = labels[r] >= 0;
@@ -915,40 +929,50 @@ __global__ void __launch_bounds__(256) xent_colsum_kernel(const float* __restric
     }
 }
 
-// dw from the splits' partial sums, and dbias
-template <typename T>
+// dw from the splits' partial sums, and dbias.  A block makes 32 classes x F features, 8 warps
+// in turn a feature each: 32 where there are few splits, 8 where each output adds up many.
+template <typename T, int F>
 __global__ void __launch_bounds__(256) xent_dw_kernel(const float* __restrict__ part, int splits, int64_t split_stride,
                                                       int64_t n_tiles, int bn, int64_t c, int64_t d,
                                                       const uint32_t* __restrict__ colmax, int scaled, int half_g,
                                                       const Meta* __restrict__ meta, T* __restrict__ dw,
                                                       const double* __restrict__ bias_part, int bias_splits,
                                                       float* __restrict__ dbias) {
-    __shared__ float t[32][33];
+    __shared__ float t[F][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const bool failed = meta->err != 0;
     const int ue = g_exponent(meta, half_g);
-    const int64_t tiles_k = (d + 31) / 32;
-    const int64_t k0 = (blockIdx.x % tiles_k) * 32, c0 = (blockIdx.x / tiles_k) * 32;
+    const int64_t tiles_k = (d + F - 1) / F;
+    const int64_t k0 = (blockIdx.x % tiles_k) * F, c0 = (blockIdx.x / tiles_k) * 32;
     if (dbias && k0 == 0 && ty == 0 && c0 + tx < c) {
         double v = 0.0;
         for (int s = 0; s < bias_splits; ++s) v += bias_part[s * c + c0 + tx];
         dbias[c0 + tx] = failed ? NAN : (float)ldexp(v, -ue);
     }
     if (!dw) return;
-    for (int j = ty; j < 32; j += 8) {
-        double v = 0.0;
+    #pragma unroll
+    for (int j = ty; j < F; j += 8) {
+        float out = 0.f;
         if (k0 + j < d && c0 + tx < c) {
             const int64_t k = k0 + j;
             const float* p = part + (((c0 / kBM) * n_tiles + k / bn) * bn + k % bn) * kBM + c0 % kBM + tx;
-            #pragma unroll 4
-            for (int s = 0; s < splits; ++s) v += (double)p[s * split_stride];
-            v = ldexp(v, -ue - (scaled ? fit_exponent(colmax[k]) : 0));
+            if (splits == 1) {
+                out = *p;
+            } else {
+                double v = 0.0;
+                #pragma unroll 8
+                for (int s = 0; s < splits; ++s) v += (double)p[s * split_stride];
+                out = (float)v;
+            }
+            out = scale2(out, -ue - (scaled ? fit_exponent(colmax[k]) : 0));
         }
-        t[j][tx] = (float)v;
+        t[j][tx] = out;
     }
     __syncthreads();
-    for (int j = ty; j < 32; j += 8)
-        if (c0 + j < c && k0 + tx < d) dw[(c0 + j) * d + k0 + tx] = from_float<T>(failed ? NAN : t[tx][j]);
+    for (int i = threadIdx.x; i < 32 * F; i += 256) {
+        const int j = i / F, k = i % F;
+        if (c0 + j < c && k0 + k < d) dw[(c0 + j) * d + k0 + k] = from_float<T>(failed ? NAN : t[k][j]);
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -1056,6 +1080,7 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
     Carver cv(ws);
     p.meta = cv.take<Meta>(1);
     p.colmax = cv.take<uint32_t>(p.planes == 2 ? a.d : 0);
+    if (a.gradient && a.dw && p.x_in_place && a.n > 0) p.poison = cv.take<uint32_t>(cdiv(a.n, 32) + 2);
     p.meta_bytes = cv.used;
     p.bias2 = cv.take<float>(p.c_tiles * p.bn_c + 256);
     if (p.planes == 2 || !p.x_in_place) p.xh = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
@@ -1066,7 +1091,6 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
     p.zy = cv.take<float>(a.n);
     if (p.products) {
         p.shift = cv.take<float2>(a.n);
-        if (p.x_in_place && a.dw) p.poison = cv.take<uint32_t>(cdiv(a.n, 32) + 2);
         // a piece of g: rows for one row tile an SM, then as many classes as kPieceBytes hold
         const int64_t es = 2 * p.planes;
         p.piece_rows = std::min<int64_t>(up(a.n, kBM), (int64_t)sms * kBM);
@@ -1172,14 +1196,18 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         SetupArgs s{};
         s.labels = a.labels; s.n = a.n; s.weight = a.weight; s.weight_stride = a.weight_stride; s.scale = a.scale;
         s.want_weight = p.products && !kBf16;
-        s.x = a.x; s.xr = a.xr; s.xk = a.xk; s.d = a.d; s.bf16 = kBf16;
-        s.poison = p.poison;
         s.bias = a.bias; s.bias2 = p.bias2; s.c = a.c; s.c_pad = p.c_tiles * p.bn_c + 256;
         s.zy = forward ? p.zy : nullptr;
         s.meta = p.meta;
-        const int64_t threads = std::max<int64_t>(s.c_pad, p.poison ? a.n * 8 : a.n);
+        const int64_t threads = std::max<int64_t>(s.c_pad, a.n);
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
         xent_setup_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(8 * sms, cdiv(threads, 256))), 256, 0, st>>>(s);
+        XENT_TRY(cudaGetLastError());
+    }
+    if (p.poison) {
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_poison_kernel<<<(unsigned)std::min<int64_t>(8 * sms, cdiv(a.n, 8)), 256, 0, st>>>(
+            a.labels, a.n, (const uint16_t*)a.x, a.xr, a.d, kBf16, p.poison, p.meta);
         XENT_TRY(cudaGetLastError());
     }
     if (scaled) {
@@ -1236,8 +1264,10 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     }
     if (forward || p.products) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_join_kernel<<<(unsigned)cdiv(a.n, 256), 256, 0, st>>>(p.part, 2 * p.splits, p.zy, a.labels, a.n, !forward,
-                                                                   a.loss, a.lse, p.products ? p.shift : nullptr, p.meta);
+        const int lanes = forward && p.splits >= 16 ? 32 : 1;
+        xent_join_kernel<<<(unsigned)cdiv(a.n * lanes, 256), 256, 0, st>>>(p.part, 2 * p.splits, lanes, p.zy, a.labels, a.n,
+                                                                           !forward, a.loss, a.lse,
+                                                                           p.products ? p.shift : nullptr, p.meta);
         XENT_TRY(cudaGetLastError());
     }
     if (!p.products) return cudaSuccess;
@@ -1328,11 +1358,13 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         }
     }
     if (a.dw || a.dbias) {
-        const int64_t blocks = cdiv(a.c, 32) * (a.dw ? cdiv(a.d, 32) : 1);
+        const bool many = a.dw && p.dw_splits > 4;
+        const int64_t blocks = cdiv(a.c, 32) * (a.dw ? cdiv(a.d, many ? 8 : 32) : 1);
+        auto fn = many ? xent_dw_kernel<T, 8> : xent_dw_kernel<T, 32>;
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_dw_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(
-            p.dw_part, p.dw_splits, p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM, p.dw_d_tiles, p.bn_d, a.c,
-            a.dw ? a.d : 1, p.colmax, scaled, !kBf16, p.meta, (T*)a.dw, p.bias_part, p.bias_splits, a.dbias);
+        fn<<<(unsigned)blocks, 256, 0, st>>>(p.dw_part, p.dw_splits, p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM, p.dw_d_tiles,
+                                             p.bn_d, a.c, a.dw ? a.d : 1, p.colmax, scaled, !kBf16, p.meta, (T*)a.dw,
+                                             p.bias_part, p.bias_splits, a.dbias);
         XENT_TRY(cudaGetLastError());
     }
     return cudaSuccess;
