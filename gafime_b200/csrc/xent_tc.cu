@@ -19,11 +19,11 @@
 //   z = 2^-t sum x' w'      dw_jk = 2^(-u - s_k) sum g' x'      dx_ik = 2^(s_k - t - u) sum g' w'
 // with g' = g 2^u (u from the largest row weight, in fp16 too; u = 0 in bf16).
 //
-// Kernel (one CTA an SM, persistent, 12 warps): warp 0 queues the TMA loads of 128 x 64 and
-// BN x 64 operand tiles into a ring; warp 1 issues the MMAs into one of two tensor-memory
-// accumulators; warps 4-11 turn the other accumulator into sums, g, dx or partial dw.  Every
-// mbarrier wait is bounded; one that gives up records a code, and the call's losses and
-// gradients of w become NaN.
+// Kernel (pairs of CTAs, one CTA an SM, persistent, 12 warps; a pair makes 256 x BN tiles): warp 0
+// queues its CTA's TMA loads of 128 x 64 of A and BN / 2 x 64 of B into a ring; warp 1 of the
+// pair's first CTA issues the MMAs into one of two tensor-memory accumulators; warps 4-11 turn
+// the other accumulator's 128 rows of their CTA into sums, g, dx or dw.  Every mbarrier wait is
+// bounded; one that gives up records a code, and the call's losses and gradients of w become NaN.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -48,7 +48,8 @@ constexpr int kThreads = 384;
 constexpr int kControlRegs = 40, kEpiRegs = 232;
 static_assert(128 * kControlRegs + 256 * kEpiRegs <= kThreads * 168, "registers of the launch");
 constexpr int kEpiWarps = 8;
-constexpr int kBM = 128;
+constexpr int kBM = 128;                     // rows of a CTA's half of a tile
+constexpr int kPM = 256;                     // rows of a pair's tile
 constexpr int kBK = 64;                      // 16-bit values of K to a stage
 constexpr int kABytes = kBM * kBK * 2;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -57,8 +58,8 @@ constexpr size_t kPieceBytes = (size_t)256 << 20;   // of g
 
 enum { LSE = 0, G = 1, DX = 2, DW = 3 };
 
-constexpr int stage_bytes(int bn) { return kABytes + bn * kBK * 2; }
-constexpr int stages_of(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
+constexpr int stage_bytes(int bn) { return kABytes + bn / 2 * kBK * 2; }   // of one CTA
+constexpr int stages_of(int bn) { return bn == 256 ? 6 : 8; }
 // an epilogue warp's outgoing 32 x 32 block: fp32, or hi and lo in 16 bits
 constexpr int kOutBytes = 4096;
 constexpr size_t smem_of(int bn) { return (size_t)stages_of(bn) * stage_bytes(bn) + kEpiWarps * kOutBytes + 1024 + 256; }
@@ -69,7 +70,7 @@ struct Meta {
     int err;                 // code of a wait that gave up
     uint32_t weight_bits;    // largest finite |row weight| as float bits
     uint32_t w_exp;          // largest exponent of w_jk 2^-s_k, + kExpBias
-    uint32_t poison;         // some left-out row of x holds a value that is not finite
+    uint32_t poison;         // some left-out row of an x read in place holds a value that is not finite
 };
 constexpr int kExpBias = 4096;
 
@@ -126,18 +127,18 @@ struct TcArgs {
     float scale;
     int64_t ldg;              // G: columns of its planes
     float* bias_part;         // G: sums of 32 rows, [row tile x 4][ldg]; null: not wanted
-    void* dx;                 // DX
+    void* dx;                 // DX; DW: dw
     int64_t dxr, dxk;
     int dx_map;               // out[0] is valid; else element stores
-    const float* undo;        // DX, fp32: two factors a feature, undo_pitch apart, 2^(s_k - t - u)
+    const float* undo;        // DX, DW in fp32: two factors a feature, undo_pitch apart
     int64_t undo_pitch;
     float* dx_acc;            // DX: sums of earlier class pieces, [tile][BN][128]
-    int first, last;          // DX: first / last class piece; DW: first row piece
-    float* dw_part;           // DW: [split][class tile][feature tile][BN][128]
+    int first, last;          // DX: first / last class piece; DW: first / last row piece
+    float* dw_part;           // DW: [split][128-class tile][feature tile][BN][128]
+    int dw_direct;            // DW: one split, whose last piece goes to dx (dw) with out[0]
     int64_t dw_split_stride;
     int64_t dw_tile0;         // first tile of the class piece
-    int64_t n_total;          // DW: rows of x
-    const uint32_t* poison;   // DW: bit r of word r / 32: zero that row of x before it is multiplied
+    int cleaned;              // DW: b[1] is a copy of x without such rows, there when meta->poison is set
 };
 
 __device__ __forceinline__ uint32_t pack(float a, float b, __half) {
@@ -240,7 +241,7 @@ __device__ __forceinline__ float pick(const float* v, int i) {
 
 // E: type of the operand planes; kPlanes: 1, or hi and lo of fp32
 template <int MODE, int BN, typename E, int kPlanes>
-__global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_constant__ TcArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_constant__ TcArgs a) {
     constexpr int S = stages_of(BN), kCols = BN / 2;   // ring stages; columns of an epilogue thread
     constexpr bool kAMn = MODE == DW, kBMn = MODE == DX || MODE == DW;
     constexpr bool kBf16 = sizeof(E) == 2 && !std::is_same<E, __half>::value;
@@ -253,6 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
     const uint32_t full0 = bars, empty0 = bars + 8 * S, afull0 = bars + 16 * S, aempty0 = afull0 + 16,
                    drain = afull0 + 32, slot = afull0 + 40;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)tc::cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     int* err = &a.meta->err;
 
     if (threadIdx.x == 0) {
@@ -262,14 +265,14 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
         }
         for (int s = 0; s < 2; ++s) {
             tc::bar_init(afull0 + 8 * s, 1);
-            tc::bar_init(aempty0 + 8 * s, kEpiWarps);
+            tc::bar_init(aempty0 + 8 * s, 2 * kEpiWarps);   // of both CTAs, in the leader
         }
         tc::bar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tc::tmem_alloc(slot, 2 * BN);
     tc::fence_before();
-    __syncthreads();
+    tc::cluster_sync();
     tc::fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gbase + (slot - base));
 
@@ -280,44 +283,45 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
             if (lane == 0) {
                 uint32_t k = 0;   // stages handed out
                 bool ok = true;
-                for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+                const bool clean = MODE == DW && a.cleaned && a.meta->poison != 0;
+                const uint32_t full_l = tc::in_leader(full0);
+                for (int u = pair; ok && u < a.units; u += pairs) {
                     const Unit t = unit_of<MODE>(a, u);
+                    const int m0 = t.m * kPM + rank * kBM;
                     for (int r = 0; ok && r < t.tiles; ++r) {
-                        const int n = t.n + r;
+                        const int n0 = (t.n + r) * BN + rank * (BN / 2);
                         // two planes: a block of K takes two stages, (A hi, B lo) and (A lo, B hi)
                         for (int i = 0; i < t.kn * kPlanes; ++i, ++k) {
                             const int kb = t.kb + i / kPlanes;
                             const CUtensorMap* ma = &a.a[i % kPlanes];
-                            const CUtensorMap* mb = &a.b[kPlanes - 1 - i % kPlanes];
-                            const uint32_t s = k % S, full = full0 + 8 * s;
+                            const CUtensorMap* mb = &a.b[clean ? 1 : kPlanes - 1 - i % kPlanes];
+                            const uint32_t s = k % S, full = full_l + 8 * s;
+                            // (a wait of a second is over long after the copies before it)
                             if (k >= S && !(ok = tc::bar_wait(empty0 + 8 * s, ((k / S) - 1) & 1, err, 1))) break;
-                            tc::bar_expect(full, stage_bytes(BN));
+                            if (rank == 0) tc::bar_expect(full0 + 8 * s, 2 * stage_bytes(BN));
                             const uint32_t sa = base + s * stage_bytes(BN), sb = sa + kABytes;
                             if (kAMn) {
-                                tc::load_2d(sa, ma, full, t.m * kBM, kb * kBK);
-                                tc::load_2d(sa + kABytes / 2, ma, full, t.m * kBM + 64, kb * kBK);
+                                tc::load_2d(sa, ma, full, m0, kb * kBK);
+                                tc::load_2d(sa + kABytes / 2, ma, full, m0 + 64, kb * kBK);
                             } else {
-                                tc::load_2d(sa, ma, full, kb * kBK, a.a_row0 + t.m * kBM);
+                                tc::load_2d(sa, ma, full, kb * kBK, a.a_row0 + m0);
                             }
                             if (kBMn) {
                                 #pragma unroll
-                                for (int q = 0; q < BN / 64; ++q)
-                                    tc::load_2d(sb + q * 8192, mb, full, n * BN + q * 64, a.b_row0 + kb * kBK);
+                                for (int q = 0; q < BN / 128; ++q)
+                                    tc::load_2d(sb + q * 8192, mb, full, n0 + q * 64, a.b_row0 + kb * kBK);
                             } else {
-                                tc::load_2d(sb, mb, full, kb * kBK, a.b_row0 + n * BN);
+                                tc::load_2d(sb, mb, full, kb * kBK, a.b_row0 + n0);
                             }
                         }
                     }
                 }
-                if (!ok)   // copies in flight land before the CTA ends
-                    for (uint32_t j = k > S ? k - S : 0; j < k; ++j) tc::bar_wait(full0 + 8 * (j % S), (j / S) & 1, err, 2);
             }
-        } else if (warp == 1) {
-            // ---- MMAs
+        } else if (warp == 1 && rank == 0) {
+            // ---- MMAs, for both CTAs
             uint32_t k = 0, acc = 0;
             bool ok = true;
-            const bool scrub = MODE == DW && a.poison != nullptr && a.meta->poison != 0;
-            for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+            for (int u = pair; ok && u < a.units; u += pairs) {
                 const Unit t = unit_of<MODE>(a, u);
                 const int end = t.tiles * t.kn;
                 for (int i = 0; ok && i < end;) {
@@ -327,52 +331,50 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                     if (acc >= 2 && !(ok = tc::bar_wait_warp(aempty0 + 8 * (acc & 1), ((acc >> 1) - 1) & 1, err, 3))) break;
                     tc::fence_after();
                     bool more = false;
-                    for (; i < stop; ++i, k += kPlanes) {
-                        const uint32_t s = k % S;
-                        if (!(ok = tc::bar_wait_warp(full0 + 8 * s, (k / S) & 1, err, 4))) break;
-                        const uint32_t sa = base + s * stage_bytes(BN), sb = sa + kABytes;
-                        if (scrub) {
-                            // rows of x that are left out and not finite: 0 x them would be NaN
-                            const int64_t row = (int64_t)a.b_row0 + (int64_t)(t.kb + i) * kBK;
-                            for (int h = 0; h < 2; ++h) {
-                                uint32_t bits = row + 32 * h < a.n_total ? a.poison[row / 32 + h] : 0;
-                                while (bits) {
-                                    const int q = 32 * h + __ffs(bits) - 1;
-                                    bits &= bits - 1;
-                                    for (int o = lane; o < BN / 64 * 8; o += 32)
-                                        *reinterpret_cast<uint4*>(gbase + (sb - base) + (o >> 3) * 8192 + q * 128 +
-                                                                  (o & 7) * 16) = make_uint4(0, 0, 0, 0);
-                                }
-                            }
-                            tc::fence_async_smem();
-                            __syncwarp();
+                    auto multiply = [&](uint32_t sa, uint32_t sb) {   // stages of A and of B
+                        const uint64_t da = tc::desc(base + sa * stage_bytes(BN), kAMn);
+                        const uint64_t db = tc::desc(base + sb * stage_bytes(BN) + kABytes, kBMn);
+                        #pragma unroll
+                        for (int j = 0; j < kBK / 16; ++j) {
+                            tc::mma(d, da + j * (kAMn ? 2048 >> 4 : 32 >> 4), db + j * (kBMn ? 2048 >> 4 : 32 >> 4), kId, more);
+                            more = true;
                         }
-                        tc::fence_after();
-                        auto multiply = [&](uint32_t pa, uint32_t pb) {
-                            const uint64_t da = tc::desc(pa, kAMn), db = tc::desc(pb, kBMn);
-                            #pragma unroll
-                            for (int j = 0; j < kBK / 16; ++j) {
-                                tc::mma(d, da + j * (kAMn ? 2048 >> 4 : 32 >> 4), db + j * (kBMn ? 2048 >> 4 : 32 >> 4), kId,
-                                        more);
-                                more = true;
-                            }
-                        };
-                        if (lane == 0) multiply(sa, sb);
-                        if (kPlanes == 2) {
-                            // (hi, lo) is under way; (lo, hi), then (hi, hi) across the two stages
-                            const uint32_t s2 = (k + 1) % S, sa2 = base + s2 * stage_bytes(BN), sb2 = sa2 + kABytes;
-                            if (!(ok = tc::bar_wait_warp(full0 + 8 * s2, ((k + 1) / S) & 1, err, 4))) break;
+                    };
+                    if constexpr (kPlanes == 1) {
+                        for (; i < stop; ++i, ++k) {
+                            const uint32_t s = k % S;
+                            if (!(ok = tc::bar_wait_warp(full0 + 8 * s, (k / S) & 1, err, 4))) break;
                             tc::fence_after();
                             if (lane == 0) {
-                                multiply(sa2, sb2);
-                                multiply(sa, sb2);
-                                tc::commit(empty0 + 8 * s2);
+                                multiply(s, s);
+                                tc::commit_both(empty0 + 8 * s);
                             }
+                            __syncwarp();
                         }
-                        if (lane == 0) tc::commit(empty0 + 8 * s);
+                    } else {
+                        // the chunk's small products first, hi lo and lo hi, as its stages arrive
+                        // (A hi with B lo, A lo with B hi); then hi hi across each pair of stages:
+                        // what the tensor cores cut off is a part of the sum so far
+                        const uint32_t k0 = k;
+                        for (; i < stop; ++i) {
+                            for (int h = 0; ok && h < 2; ++h, ++k) {
+                                const uint32_t s = k % S;
+                                if (!(ok = tc::bar_wait_warp(full0 + 8 * s, (k / S) & 1, err, 4))) break;
+                                tc::fence_after();
+                                if (lane == 0) multiply(s, s);
+                                __syncwarp();
+                            }
+                            if (!ok) break;
+                        }
+                        if (ok && lane == 0)
+                            for (uint32_t q = k0; q < k; q += 2) {
+                                multiply(q % S, (q + 1) % S);
+                                tc::commit_both(empty0 + 8 * (q % S));
+                                tc::commit_both(empty0 + 8 * ((q + 1) % S));
+                            }
                         __syncwarp();
                     }
-                    if (ok && lane == 0) tc::commit(afull0 + 8 * (acc & 1));
+                    if (ok && lane == 0) tc::commit_both(afull0 + 8 * (acc & 1));
                     ++acc;
                     __syncwarp();
                 }
@@ -395,9 +397,11 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
         bool ok = true;
         const int te = w_exponent(a.meta, a.scaled), ue = g_exponent(a.meta, a.half_g);
         const float f = pow2i(-te) * kLog2e;
-        for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x) {
+        const uint32_t aempty_l = tc::in_leader(aempty0);
+        for (int u = pair; ok && u < a.units; u += pairs) {
             const Unit t = unit_of<MODE>(a, u);
-            const int64_t row = (int64_t)t.m * kBM + quarter * 32 + lane;
+            const int mt = 2 * t.m + rank;                 // this CTA's 128 rows
+            const int64_t y0 = (int64_t)mt * kBM + quarter * 32, row = y0 + lane;
             const bool valid = row < a.rows;
             int64_t y = -1;
             float top = -INFINITY, sum = 0.f, zy = NAN;    // LSE
@@ -437,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                         if (ch + 2 >= kCols / 32) {
                             tc::fence_before();
                             __syncwarp();
-                            if (lane == 0) tc::bar_arrive(aempty0 + 8 * (acc & 1));
+                            if (lane == 0) tc::bar_arrive_cluster(aempty_l + 8 * (acc & 1));
                         }
                         #pragma unroll
                         for (int j = 0; j < 32; ++j) sums[ch * 32 + j] += v[j];
@@ -509,7 +513,6 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                         }
                         tc::fence_async_smem();
                         __syncwarp();
-                        const int64_t y0 = (int64_t)t.m * kBM + quarter * 32;
                         if (lane == 0 && y0 < a.rows) {
                             tc::store_2d(&a.out[0], out_addr, (int)cb, (int)y0);
                             if (kPlanes == 2) tc::store_2d(&a.out[1], out_addr + 2048, (int)cb, (int)y0);
@@ -525,76 +528,70 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
                                 const float wl = __shfl_sync(0xffffffffu, wt, l);
                                 if (lane == at) c -= wl;
                             }
-                            if (cb + lane < a.ldg) a.bias_part[((int64_t)t.m * 4 + quarter) * a.ldg + cb + lane] = c;
+                            if (cb + lane < a.ldg) a.bias_part[((int64_t)mt * 4 + quarter) * a.ldg + cb + lane] = c;
                         }
-                    } else if (MODE == DX) {
-                        // unit index as the place of the sums: the same unit of every class piece
-                        float* keep = a.dx_acc + ((int64_t)u * BN + col) * kBM + quarter * 32 + lane;
+                    } else {
+                        // sums of earlier pieces: dx of class pieces, a place a unit; dw of row pieces
+                        float* keep = MODE == DX ? a.dx_acc + ((int64_t)(2 * u + rank) * BN + col) * kBM
+                                                 : a.dw_part + t.split * a.dw_split_stride +
+                                                       ((a.dw_tile0 + (int64_t)mt * a.n_tiles + n) * BN + col) * kBM;
+                        keep += quarter * 32 + lane;
                         if (!a.first)
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] += keep[j * kBM];
-                        if (!a.last) {
+                        if (!a.last || (MODE == DW && !a.dw_direct)) {
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) keep[j * kBM] = v[j];
-                        } else {
-                            using D = typename std::conditional<kPlanes == 2, float, E>::type;
-                            const int count = (int)min((int64_t)32, a.cols - cb);
-                            if (kPlanes == 2) {
-                                const float4* f4 = reinterpret_cast<const float4*>(a.undo + cb);
-                                const float4* g4 = reinterpret_cast<const float4*>(a.undo + a.undo_pitch + cb);
-                                #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const float4 p = __ldg(f4 + j), q = __ldg(g4 + j);
-                                    v[4 * j] = v[4 * j] * p.x * q.x;
-                                    v[4 * j + 1] = v[4 * j + 1] * p.y * q.y;
-                                    v[4 * j + 2] = v[4 * j + 2] * p.z * q.z;
-                                    v[4 * j + 3] = v[4 * j + 3] * p.w * q.w;
-                                }
-                            } else {
-                                const float q = pow2i(-ue);
-                                #pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] *= q;
+                            continue;
+                        }
+                        using D = typename std::conditional<kPlanes == 2, float, E>::type;
+                        const int count = (int)min((int64_t)32, a.cols - cb);
+                        if (kPlanes == 2) {
+                            const float4* f4 = reinterpret_cast<const float4*>(a.undo + cb);
+                            const float4* g4 = reinterpret_cast<const float4*>(a.undo + a.undo_pitch + cb);
+                            #pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float4 p = __ldg(f4 + j), q = __ldg(g4 + j);
+                                v[4 * j] = v[4 * j] * p.x * q.x;
+                                v[4 * j + 1] = v[4 * j + 1] * p.y * q.y;
+                                v[4 * j + 2] = v[4 * j + 2] * p.z * q.z;
+                                v[4 * j + 3] = v[4 * j + 3] * p.w * q.w;
                             }
-                            if (y < 0)
+                        } else {
+                            const float q = pow2i(-ue);
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] *= q;
+                        }
+                        if (MODE == DX && y < 0)
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                        D* dx = (D*)a.dx + (a.row0 + y0) * a.dxr + cb * a.dxk;
+                        if (a.dxr == 1 && a.dxk != 1) {
+                            // column by column: neighbouring lanes are neighbouring rows
+                            if (valid)
                                 #pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] = 0.f;
-                            const int64_t y0 = (int64_t)t.m * kBM + quarter * 32;
-                            D* dx = (D*)a.dx + (a.row0 + y0) * a.dxr + cb * a.dxk;
-                            if (a.dxr == 1 && a.dxk != 1) {
-                                // column by column: neighbouring lanes are neighbouring rows
-                                if (valid)
-                                    #pragma unroll
-                                    for (int j = 0; j < 32; ++j)
-                                        if (j < count) dx[lane + j * a.dxk] = from_float<D>(v[j]);
-                            } else {
-                                tc::store_wait_read();
-                                out_write<D>(out, lane, v);
-                                if (a.dx_map) {
-                                    tc::fence_async_smem();
-                                    __syncwarp();
-                                    if (lane == 0 && y0 < a.rows) {
-                                        tc::store_2d(&a.out[0], out_addr, (int)cb, (int)(a.row0 + y0));
-                                        tc::store_commit();
-                                    }
-                                } else {
-                                    // rows that TMA cannot reach: one at a time, a lane a column
-                                    __syncwarp();
-                                    const int rows = (int)min((int64_t)32, a.rows - y0);
-                                    if (lane < count)
-                                        #pragma unroll 8
-                                        for (int i = 0; i < rows; ++i) dx[i * a.dxr + lane * a.dxk] = *out_at<D>(out, i, lane);
-                                    __syncwarp();
+                                for (int j = 0; j < 32; ++j)
+                                    if (j < count) dx[lane + j * a.dxk] = from_float<D>(v[j]);
+                        } else {
+                            tc::store_wait_read();
+                            out_write<D>(out, lane, v);
+                            if (a.dx_map) {
+                                tc::fence_async_smem();
+                                __syncwarp();
+                                if (lane == 0 && y0 < a.rows) {
+                                    tc::store_2d(&a.out[0], out_addr, (int)cb, (int)(a.row0 + y0));
+                                    tc::store_commit();
                                 }
+                            } else {
+                                // rows that TMA cannot reach: one at a time, a lane a column
+                                __syncwarp();
+                                const int rows = (int)min((int64_t)32, a.rows - y0);
+                                if (lane < count)
+                                    #pragma unroll 8
+                                    for (int i = 0; i < rows; ++i) dx[i * a.dxr + lane * a.dxk] = *out_at<D>(out, i, lane);
+                                __syncwarp();
                             }
                         }
-                    } else {
-                        float* p = a.dw_part + t.split * a.dw_split_stride +
-                                   ((a.dw_tile0 + (int64_t)t.m * a.n_tiles + n) * BN + col) * kBM + quarter * 32 + lane;
-                        if (!a.first)
-                            #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] += p[j * kBM];
-                        #pragma unroll
-                        for (int j = 0; j < 32; ++j) p[j * kBM] = v[j];
                     }
                 }
             }
@@ -607,6 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_const
     }
     tc::fence_before();
     __syncthreads();
+    tc::cluster_sync();   // neither CTA leaves while the other's MMAs or arrivals may reach it
     tc::fence_after();
     if (warp == 1) tc::tmem_free(tmem, 2 * BN);
 }
@@ -650,10 +648,11 @@ __global__ void __launch_bounds__(256) xent_setup_kernel(SetupArgs a) {
     }
 }
 
-// Marks left-out rows of a 16-bit x read in place that hold a value that is no number; a warp a row.
+// Looks for left-out rows of a 16-bit x read in place that hold a value that is no number (0 x it
+// would be NaN in dw, whose sum runs over the rows); a warp a row.
 __global__ void __launch_bounds__(256) xent_poison_kernel(const int64_t* __restrict__ labels, int64_t n,
                                                           const uint16_t* __restrict__ x, int64_t xr, int64_t d, int bf16,
-                                                          uint32_t* poison, Meta* meta) {
+                                                          Meta* meta) {
     const int lane = threadIdx.x & 31;
     const uint32_t inf = bf16 ? 0x7f80 : 0x7c00;
     for (int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32; r < n; r += (int64_t)gridDim.x * blockDim.x / 32) {
@@ -668,10 +667,7 @@ __global__ void __launch_bounds__(256) xent_poison_kernel(const int64_t* __restr
             for (int i = 0; i < 4; ++i) b |= (u[i] & inf) == inf || (u[i] >> 16 & inf) == inf;
         }
         if (lane < d % 8) b |= (x[r * xr + d / 8 * 8 + lane] & inf) == inf;
-        if (__any_sync(0xffffffffu, b) && lane == 0) {
-            atomicOr(&poison[r / 32], 1u << (r % 32));
-            meta->poison = 1;
-        }
+        if (__any_sync(0xffffffffu, b) && lane == 0) meta->poison = 1;
     }
 }
 
@@ -840,26 +836,32 @@ __global__ void __launch_bounds__(256) xent_planes_rows_kernel(const float* __re
     }
 }
 
-// Factors that undo the scales of a gradient of x: 2^(s_k - t - u) as two that fp32 holds.
+// Factors that undo the scales of the gradients, each as two that fp32 holds: 2^(s_k - t - u) of dx,
+// then 2^(-s_k - u) of dw.
 __global__ void __launch_bounds__(256) xent_undo_kernel(const uint32_t* __restrict__ colmax, int64_t d, int64_t pitch,
                                                         const Meta* __restrict__ meta, float* __restrict__ undo) {
     const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (k >= pitch) return;
-    const int e = (k < d ? fit_exponent(colmax[k]) : 0) - w_exponent(meta, 1) - g_exponent(meta, 1);
-    const int c = min(252, max(-252, e)), h = c / 2;
-    undo[k] = pow2i(h);
-    undo[pitch + k] = pow2i(c - h);
+    const int s = k < d ? fit_exponent(colmax[k]) : 0, u = g_exponent(meta, 1);
+    const int e[2] = {s - w_exponent(meta, 1) - u, -s - u};
+    for (int i = 0; i < 2; ++i) {
+        const int c = min(252, max(-252, e[i])), h = c / 2;
+        undo[2 * i * pitch + k] = pow2i(h);
+        undo[(2 * i + 1) * pitch + k] = pow2i(c - h);
+    }
 }
 
 // rows x d of any strides -> planes [rows][dp], a 64 x 64 tile a block; rows with a negative label
-// become zeros.  fp32: hi and lo fp16 of the scaled value; 16 bits: a copy.
+// become zeros.  fp32: hi and lo fp16 of the scaled value; 16 bits: a copy (if_poison: only where
+// one is needed).
 template <typename T, typename E>
 __global__ void __launch_bounds__(256) xent_planes_kernel(const T* __restrict__ x, int64_t xr, int64_t xk,
                                                           const int64_t* __restrict__ labels, int64_t n, int64_t d,
                                                           int64_t dp, const uint32_t* __restrict__ colmax,
-                                                          const Meta* __restrict__ meta, int is_w, E* __restrict__ hi,
-                                                          E* __restrict__ lo) {
+                                                          const Meta* __restrict__ meta, int is_w, int if_poison,
+                                                          E* __restrict__ hi, E* __restrict__ lo) {
     __shared__ float t[64][65];      // [feature][row]
+    if (if_poison && meta->poison == 0) return;
     const int64_t tiles_k = (dp + 63) / 64;
     const int64_t k0 = (blockIdx.x % tiles_k) * 64, r0 = (blockIdx.x / tiles_k) * 64;
     const bool down = xr == 1 && xk != 1;
@@ -929,50 +931,45 @@ __global__ void __launch_bounds__(256) xent_colsum_kernel(const float* __restric
     }
 }
 
-// dw from the splits' partial sums, and dbias.  A block makes 32 classes x F features, 8 warps
-// in turn a feature each: 32 where there are few splits, 8 where each output adds up many.
-template <typename T, int F>
-__global__ void __launch_bounds__(256) xent_dw_kernel(const float* __restrict__ part, int splits, int64_t split_stride,
-                                                      int64_t n_tiles, int bn, int64_t c, int64_t d,
-                                                      const uint32_t* __restrict__ colmax, int scaled, int half_g,
-                                                      const Meta* __restrict__ meta, T* __restrict__ dw,
-                                                      const double* __restrict__ bias_part, int bias_splits,
-                                                      float* __restrict__ dbias) {
-    __shared__ float t[F][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+// dbias from its splits; and NaN in dw where a kernel's wait gave up.
+template <typename T>
+__global__ void __launch_bounds__(256) xent_finish_kernel(int64_t c, int64_t d, int half_g, const Meta* __restrict__ meta,
+                                                          T* __restrict__ dw, const double* __restrict__ bias_part,
+                                                          int bias_splits, float* __restrict__ dbias) {
     const bool failed = meta->err != 0;
-    const int ue = g_exponent(meta, half_g);
-    const int64_t tiles_k = (d + F - 1) / F;
-    const int64_t k0 = (blockIdx.x % tiles_k) * F, c0 = (blockIdx.x / tiles_k) * 32;
-    if (dbias && k0 == 0 && ty == 0 && c0 + tx < c) {
-        double v = 0.0;
-        for (int s = 0; s < bias_splits; ++s) v += bias_part[s * c + c0 + tx];
-        dbias[c0 + tx] = failed ? NAN : (float)ldexp(v, -ue);
-    }
-    if (!dw) return;
-    #pragma unroll
-    for (int j = ty; j < F; j += 8) {
-        float out = 0.f;
-        if (k0 + j < d && c0 + tx < c) {
-            const int64_t k = k0 + j;
-            const float* p = part + (((c0 / kBM) * n_tiles + k / bn) * bn + k % bn) * kBM + c0 % kBM + tx;
-            if (splits == 1) {
-                out = *p;
-            } else {
-                double v = 0.0;
-                #pragma unroll 8
-                for (int s = 0; s < splits; ++s) v += (double)p[s * split_stride];
-                out = (float)v;
-            }
-            out = scale2(out, -ue - (scaled ? fit_exponent(colmax[k]) : 0));
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
+    if (dbias)
+        for (int64_t j = at / 32; j < c; j += all / 32) {   // a warp a class
+            double v = 0.0;
+            for (int s = threadIdx.x & 31; s < bias_splits; s += 32) v += bias_part[s * c + j];
+            #pragma unroll
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if ((threadIdx.x & 31) == 0) dbias[j] = failed ? NAN : (float)ldexp(v, -g_exponent(meta, half_g));
         }
-        t[j][tx] = out;
+    if (dw && failed)
+        for (int64_t i = at; i < c * d; i += all) dw[i] = from_float<T>(NAN);
+}
+
+// dw from several splits' partial sums: a block makes 32 classes x 8 features, a warp a feature.
+template <typename T>
+__global__ void __launch_bounds__(256) xent_dw_kernel(const float* __restrict__ part, int splits, int64_t split_stride,
+                                                      int n_tiles, int bn, int c, int d, const float* __restrict__ undo,
+                                                      int64_t undo_pitch, int half_g, const Meta* __restrict__ meta,
+                                                      T* __restrict__ dw) {
+    __shared__ float t[8][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int tiles_k = (d + 7) / 8;
+    const int k0 = (int)(blockIdx.x % tiles_k) * 8, c0 = (int)(blockIdx.x / tiles_k) * 32, k = k0 + ty;
+    if (k < d && c0 + tx < c) {
+        const float* p = part + (((int64_t)(c0 / kBM) * n_tiles + k / bn) * bn + k % bn) * kBM + c0 % kBM + tx;
+        double v = 0.0;
+        #pragma unroll 8
+        for (int s = 0; s < splits; ++s) v += (double)p[s * split_stride];
+        t[ty][tx] = undo ? (float)v * undo[k] * undo[undo_pitch + k] : scale2((float)v, -g_exponent(meta, half_g));
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * F; i += 256) {
-        const int j = i / F, k = i % F;
-        if (c0 + j < c && k0 + k < d) dw[(c0 + j) * d + k0 + k] = from_float<T>(failed ? NAN : t[k][j]);
-    }
+    const int j = threadIdx.x >> 3, i = threadIdx.x & 7;
+    if (c0 + j < c && k0 + i < d) dw[(int64_t)(c0 + j) * d + k0 + i] = from_float<T>(t[i][j]);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -1035,11 +1032,13 @@ struct Plan {
     int planes, bn_c, bn_d;
     bool x_in_place, w_in_place;
     int64_t dp;
-    int64_t m_tiles, c_tiles;        // of the whole call
+    int64_t m_tiles, c_tiles;        // of the whole call, 256 rows and bn_c classes
     int splits, per_split;           // LSE
     int64_t piece_rows, piece_classes, ldg;
     int64_t dw_c_tiles, dw_d_tiles;  // 128 classes x bn_d features
+    int64_t dw_stride;               // floats of a split's partial
     int dw_splits, dw_per_split;
+    bool dw_direct;                  // one split: dw leaves the products' kernel
     int bias_splits;
     bool products;                   // dx or dw or dbias wanted
     // workspace
@@ -1047,7 +1046,7 @@ struct Plan {
     uint32_t* colmax;
     size_t meta_bytes;
     float* bias2;
-    uint32_t* poison;
+    uint16_t* xc;                    // x without left-out rows, made where one of those holds no number
     uint16_t *xh, *xl, *wh, *wl, *gh, *gl;
     float2* part;
     float* zy;
@@ -1065,57 +1064,66 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
     Plan p{};
     p.planes = a.type == GAFIME_TYPE_FP32 ? 2 : 1;
     p.bn_c = tile_n(a.c);
-    p.bn_d = tile_n(a.d);
+    p.bn_d = std::max(128, tile_n(a.d));   // a CTA's half of it is whole 64-value lines
+    const int pairs = sms / 2;
     p.x_in_place = in_place(a.type, a.x, a.xr, a.xk, a.d);
     p.w_in_place = in_place(a.type, a.w, a.wr, a.wk, a.d);
     p.dp = up(a.d, 8);
-    p.m_tiles = std::max<int64_t>(1, cdiv(a.n, kBM));
+    p.m_tiles = std::max<int64_t>(1, cdiv(a.n, kPM));
     p.c_tiles = cdiv(a.c, p.bn_c);
-    // LSE: enough units of (row tile, run of class tiles) for every SM
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(p.c_tiles, cdiv(2 * sms, p.m_tiles)));
-    p.per_split = (int)cdiv(p.c_tiles, p.m_tiles >= 2 * sms ? 1 : want);
+    // LSE: units of (row tile, run of class tiles), the longest runs that leave the pairs of CTAs
+    // about as evenly loaded as any
+    auto load = [&](int64_t run) { return cdiv(p.m_tiles * cdiv(p.c_tiles, run), pairs) * run; };
+    int64_t best = load(p.c_tiles);
+    for (int64_t run = 1; run < p.c_tiles && run <= 64; ++run) best = std::min(best, load(run));
+    int64_t run = p.c_tiles;
+    if (load(run) > best + best / 32)
+        for (run = std::min<int64_t>(64, p.c_tiles); run > 1 && load(run) > best + best / 32;) --run;
+    p.per_split = (int)run;
     p.splits = (int)cdiv(p.c_tiles, p.per_split);
     p.products = a.gradient && (a.dx || a.dw || a.dbias) && a.n > 0;
 
     Carver cv(ws);
     p.meta = cv.take<Meta>(1);
     p.colmax = cv.take<uint32_t>(p.planes == 2 ? a.d : 0);
-    if (a.gradient && a.dw && p.x_in_place && a.n > 0) p.poison = cv.take<uint32_t>(cdiv(a.n, 32) + 2);
     p.meta_bytes = cv.used;
     p.bias2 = cv.take<float>(p.c_tiles * p.bn_c + 256);
     if (p.planes == 2 || !p.x_in_place) p.xh = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
     if (p.planes == 2) p.xl = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
     if (p.planes == 2 || !p.w_in_place) p.wh = cv.take<uint16_t>(a.c * p.dp);
     if (p.planes == 2) p.wl = cv.take<uint16_t>(a.c * p.dp);
+    if (a.gradient && a.dw && p.x_in_place) p.xc = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
     p.part = cv.take<float2>(a.n * 2 * p.splits);
     p.zy = cv.take<float>(a.n);
     if (p.products) {
         p.shift = cv.take<float2>(a.n);
         // a piece of g: rows for one row tile an SM, then as many classes as kPieceBytes hold
         const int64_t es = 2 * p.planes;
-        p.piece_rows = std::min<int64_t>(up(a.n, kBM), (int64_t)sms * kBM);
+        p.piece_rows = std::min<int64_t>(up(a.n, kPM), (int64_t)pairs * kPM);
         p.piece_classes = std::max<int64_t>(1024, (int64_t)(kPieceBytes / (p.piece_rows * es)) / 256 * 256);
         if (p.piece_classes >= a.c) {
             p.piece_classes = a.c;
             // few classes: more rows at once, still whole rounds of the SMs
             const int64_t more = (int64_t)(kPieceBytes / (p.piece_rows * es * up(a.c, 8)));
-            if (more > 1) p.piece_rows = std::min<int64_t>(up(a.n, kBM), p.piece_rows * more);
+            if (more > 1) p.piece_rows = std::min<int64_t>(up(a.n, kPM), p.piece_rows * more);
         }
         p.ldg = up(p.piece_classes, 64);   // whole 128-byte lines: TMA boxes meet no line twice
         p.gh = cv.take<uint16_t>(p.piece_rows * p.ldg);
         if (p.planes == 2) p.gl = cv.take<uint16_t>(p.piece_rows * p.ldg);
         p.dw_d_tiles = cdiv(a.d, p.bn_d);
-        p.dw_c_tiles = cdiv(a.c, kBM);
+        p.dw_c_tiles = cdiv(a.c, kPM) * 2;
+        p.dw_stride = p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM;
         p.undo_pitch = p.dw_d_tiles * p.bn_d;
-        if (a.dx && p.planes == 2) p.undo = cv.take<float>(2 * p.undo_pitch);
+        if (p.planes == 2) p.undo = cv.take<float>(4 * p.undo_pitch);
         if (a.dx && p.piece_classes < a.c)
-            p.dx_acc = cv.take<float>(cdiv(p.piece_rows, kBM) * p.dw_d_tiles * p.bn_d * kBM);
+            p.dx_acc = cv.take<float>(p.piece_rows * p.dw_d_tiles * p.bn_d);
         if (a.dw) {
-            const int64_t tiles = cdiv(p.piece_classes, kBM) * p.dw_d_tiles, blocks = cdiv(std::min(a.n, p.piece_rows), kBK);
-            const int64_t s = std::max<int64_t>(1, std::min<int64_t>(sms / tiles, blocks / 4));
+            const int64_t tiles = cdiv(p.piece_classes, kPM) * p.dw_d_tiles, blocks = cdiv(std::min(a.n, p.piece_rows), kBK);
+            const int64_t s = std::max<int64_t>(1, std::min<int64_t>(pairs / tiles, blocks / 4));
             p.dw_per_split = (int)cdiv(blocks, s);
             p.dw_splits = (int)cdiv(blocks, p.dw_per_split);
-            p.dw_part = cv.take<float>(p.dw_splits * p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM);
+            p.dw_direct = p.dw_splits == 1;
+            if (!p.dw_direct || a.n > p.piece_rows) p.dw_part = cv.take<float>(p.dw_splits * p.dw_stride);
         }
         if (a.dbias) {
             const int64_t blocks = cdiv(p.piece_classes, 32);
@@ -1139,7 +1147,7 @@ cudaError_t launch_bn(const TcArgs& t, int sms, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     if (attr.numRegs * kThreads < 128 * kControlRegs + 256 * kEpiRegs) return cudaErrorLaunchOutOfResources;
     KernelTimer kt(stream, GAFIME_KERNEL_XENT_TC);
-    fn<<<std::min(sms, t.units), kThreads, smem_of(BN), stream>>>(t);
+    fn<<<2 * std::min(sms / 2, t.units), kThreads, smem_of(BN), stream>>>(t);
     return cudaGetLastError();
 }
 template <int MODE, typename E, int kPlanes>
@@ -1160,7 +1168,7 @@ cudaError_t launch(const TcArgs& t, int bn, int sms, cudaStream_t stream) {
 
 template <typename T, typename E>
 cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const int64_t* labels, int64_t rows, int64_t d,
-                   bool is_w, uint16_t* hi, uint16_t* lo, int sms, cudaStream_t stream) {
+                   bool is_w, bool if_poison, uint16_t* hi, uint16_t* lo, int sms, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         if (rows_vector(src, sr, sk)) {
             const int64_t blocks_k = cdiv(p.dp, 1024);
@@ -1174,7 +1182,7 @@ cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const in
     const int64_t blocks = cdiv(p.dp, 64) * cdiv(rows, 64);
     KernelTimer kt(stream, GAFIME_KERNEL_XENT);
     xent_planes_kernel<T, E><<<(unsigned)blocks, 256, 0, stream>>>(src, sr, sk, labels, rows, d, p.dp, p.colmax, p.meta,
-                                                                   is_w, (E*)hi, (E*)lo);
+                                                                   is_w, if_poison, (E*)hi, (E*)lo);
     return cudaGetLastError();
 }
 
@@ -1204,11 +1212,12 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         xent_setup_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(8 * sms, cdiv(threads, 256))), 256, 0, st>>>(s);
         XENT_TRY(cudaGetLastError());
     }
-    if (p.poison) {
+    if (p.xc) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
         xent_poison_kernel<<<(unsigned)std::min<int64_t>(8 * sms, cdiv(a.n, 8)), 256, 0, st>>>(
-            a.labels, a.n, (const uint16_t*)a.x, a.xr, a.d, kBf16, p.poison, p.meta);
+            a.labels, a.n, (const uint16_t*)a.x, a.xr, a.d, kBf16, p.meta);
         XENT_TRY(cudaGetLastError());
+        XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, true, p.xc, nullptr, sms, st)));
     }
     if (scaled) {
         {
@@ -1225,8 +1234,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             (const float*)a.w, a.wr, a.wk, a.c, a.d, p.colmax, p.meta);
         XENT_TRY(cudaGetLastError());
     }
-    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, p.xh, p.xl, sms, st)));
-    if (p.wh) XENT_TRY((planes<T, E>(p, (const T*)a.w, a.wr, a.wk, nullptr, a.c, a.d, true, p.wh, p.wl, sms, st)));
+    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, false, p.xh, p.xl, sms, st)));
+    if (p.wh) XENT_TRY((planes<T, E>(p, (const T*)a.w, a.wr, a.wk, nullptr, a.c, a.d, true, false, p.wh, p.wl, sms, st)));
     // where the operands are read
     const void *xs[2] = {p.xh ? (const void*)p.xh : a.x, p.xl}, *ws[2] = {p.wh ? (const void*)p.wh : a.w, p.wl};
     const int64_t ldx = p.xh ? p.dp : a.xr, ldw = p.wh ? p.dp : a.wr;
@@ -1237,7 +1246,10 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     };
 
     TcArgs t{};
-    t.chunk = p.planes == 2 ? 1 : 8;
+    // fp32: 4 products of the large planes to a block, each cutting about 2^-24 of the sum; two
+    // blocks (6e-7) keep the drains of tensor memory, 128 KB a CTA beside the running MMAs, behind
+    // them.  16 bits: 32 products and more are nothing beside the operands' rounding.
+    t.chunk = p.planes == 2 ? 2 : 8;
     t.scaled = scaled;
     t.half_g = !kBf16;
     t.meta = p.meta;
@@ -1250,7 +1262,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     if (forward) {
         TcArgs l = t;
         XENT_TRY(map(l.a, xs, a.d, a.n, ldx, kBM));
-        XENT_TRY(map(l.b, ws, a.d, a.c, ldw, p.bn_c));
+        XENT_TRY(map(l.b, ws, a.d, a.c, ldw, p.bn_c / 2));
         l.m_tiles = (int)p.m_tiles;
         l.n_tiles = (int)p.c_tiles;
         l.per_split = p.per_split;
@@ -1284,8 +1296,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             const int64_t classes = std::min(p.piece_classes, a.c - c0);
             TcArgs g = t;
             XENT_TRY(map(g.a, xs, a.d, a.n, ldx, kBM));
-            XENT_TRY(map(g.b, ws, a.d, a.c, ldw, p.bn_c));
-            g.m_tiles = (int)cdiv(rows, kBM);
+            XENT_TRY(map(g.b, ws, a.d, a.c, ldw, p.bn_c / 2));
+            g.m_tiles = (int)cdiv(rows, kPM);
             g.n_tiles = (int)cdiv(classes, p.bn_c);
             g.units = g.m_tiles * g.n_tiles;
             g.k_blocks = (int)cdiv(a.d, kBK);
@@ -1304,7 +1316,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             g.bias_part = a.dbias ? p.bias_sums : nullptr;
             XENT_TRY((launch<G, E, kPlanes>(g, p.bn_c, sms, st)));
             if (a.dbias) {
-                const int64_t lines = g.m_tiles * 4;
+                const int64_t lines = g.m_tiles * 8;
                 KernelTimer kt(st, GAFIME_KERNEL_XENT);
                 xent_colsum_kernel<<<dim3((unsigned)cdiv(classes, 32), (unsigned)p.bias_splits), 256, 0, st>>>(
                     p.bias_sums, p.ldg, lines, classes, cdiv(p.piece_rows / 32, p.bias_splits), r0 == 0, p.bias_part,
@@ -1317,10 +1329,11 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 // the piece's classes of w
                 const void* wp[2] = {(const uint16_t*)ws[0] + c0 * ldw, ws[1] ? (const uint16_t*)ws[1] + c0 * ldw : nullptr};
                 XENT_TRY(map(x.b, wp, a.d, classes, ldw, kBK));
-                x.m_tiles = (int)cdiv(rows, kBM);
+                x.m_tiles = (int)cdiv(rows, kPM);
                 x.n_tiles = (int)p.dw_d_tiles;
                 x.units = x.m_tiles * x.n_tiles;
                 x.k_blocks = (int)cdiv(classes, kBK);
+                if (p.planes == 1) x.chunk = 16;
                 x.rows = rows;
                 x.row0 = r0;
                 x.cols = a.d;
@@ -1338,33 +1351,46 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 TcArgs w = t;
                 XENT_TRY(map(w.a, gs, classes, rows, p.ldg, kBK));
                 XENT_TRY(map(w.b, xs, a.d, a.n, ldx, kBK));
-                w.m_tiles = (int)cdiv(classes, kBM);
+                w.m_tiles = (int)cdiv(classes, kPM);
                 w.n_tiles = (int)p.dw_d_tiles;
                 w.units = w.m_tiles * w.n_tiles * p.dw_splits;
                 w.per_split = p.dw_per_split;
                 w.k_blocks = (int)cdiv(rows, kBK);
+                if (p.planes == 1) w.chunk = 16;
                 w.b_row0 = (int)r0;
-                w.row0 = r0;
-                w.n_total = a.n;
+                w.row0 = c0;
                 w.rows = classes;
                 w.cols = a.d;
                 w.first = r0 == 0;
+                w.last = r0 + rows == a.n;
                 w.dw_part = p.dw_part;
-                w.dw_split_stride = p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM;
+                w.dw_split_stride = p.dw_stride;
                 w.dw_tile0 = c0 / kBM * p.dw_d_tiles;
-                w.poison = p.poison;
+                w.dw_direct = p.dw_direct;
+                w.dx = a.dw;
+                w.dxr = a.d;
+                w.dxk = 1;
+                w.dx_map = (uintptr_t)a.dw % 16 == 0 && a.d * (int64_t)sizeof(T) % 16 == 0;
+                if (w.dx_map && !make_out_map(&w.out[0], a.type, a.dw, a.d, a.c, a.d)) return cudaErrorInvalidValue;
+                w.undo = p.undo ? p.undo + 2 * p.undo_pitch : nullptr;
+                w.undo_pitch = p.undo_pitch;
+                w.cleaned = p.xc != nullptr;
+                if (p.xc && !make_map(&w.b[1], kBf16, p.xc, a.d, a.n, p.dp, kBK)) return cudaErrorInvalidValue;
                 XENT_TRY((launch<DW, E, kPlanes>(w, p.bn_d, sms, st)));
             }
         }
     }
-    if (a.dw || a.dbias) {
-        const bool many = a.dw && p.dw_splits > 4;
-        const int64_t blocks = cdiv(a.c, 32) * (a.dw ? cdiv(a.d, many ? 8 : 32) : 1);
-        auto fn = many ? xent_dw_kernel<T, 8> : xent_dw_kernel<T, 32>;
+    if (a.dw && !p.dw_direct) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        fn<<<(unsigned)blocks, 256, 0, st>>>(p.dw_part, p.dw_splits, p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM, p.dw_d_tiles,
-                                             p.bn_d, a.c, a.dw ? a.d : 1, p.colmax, scaled, !kBf16, p.meta, (T*)a.dw,
-                                             p.bias_part, p.bias_splits, a.dbias);
+        xent_dw_kernel<T><<<(unsigned)(cdiv(a.c, 32) * cdiv(a.d, 8)), 256, 0, st>>>(
+            p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_d, (int)a.c, (int)a.d,
+            p.undo ? p.undo + 2 * p.undo_pitch : nullptr, p.undo_pitch, !kBf16, p.meta, (T*)a.dw);
+        XENT_TRY(cudaGetLastError());
+    }
+    if (a.dw || a.dbias) {
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_finish_kernel<T><<<(unsigned)std::min<int64_t>(2 * sms, cdiv(a.c, 8)), 256, 0, st>>>(
+            a.c, a.d, !kBf16, p.meta, (T*)a.dw, p.bias_part, p.bias_splits, a.dbias);
         XENT_TRY(cudaGetLastError());
     }
     return cudaSuccess;
