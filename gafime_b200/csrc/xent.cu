@@ -61,6 +61,181 @@ __global__ void __launch_bounds__(1024) xent_few_sum_kernel(const float* __restr
     }
 }
 
+// ---- a few rows, any number of classes ----------------------------------------------------
+// Losses of up to kRowsFew rows (serving's single rows): bound by reading w once.  A warp takes
+// classes in turn, its lanes the features, and keeps every row's running maximum and sum; the
+// tensor cores would spend a tile of 256 rows on each class tile.
+constexpr int kRowsFew = 8;
+constexpr int64_t kRowsFewValues = 12288;   // of x, fp32 in shared memory
+constexpr int kRowsThreads = 256;
+
+// 16 bytes of w, or one value where its rows are not made of them
+template <typename T, bool VEC>
+struct WLoad {
+    static constexpr int kCount = VEC ? 16 / sizeof(T) : 1;
+    static __device__ __forceinline__ void load(float (&v)[kCount], const T* p) {
+        if constexpr (!VEC) {
+            v[0] = to_float(*p);
+        } else {
+            const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+            if constexpr (sizeof(T) == 4) {
+                v[0] = __uint_as_float(t.x);
+                v[1] = __uint_as_float(t.y);
+                v[2] = __uint_as_float(t.z);
+                v[3] = __uint_as_float(t.w);
+            } else {
+                few::load4(reinterpret_cast<float(&)[4]>(v[0]), reinterpret_cast<const uint8_t*>(&t), T{});
+                few::load4(reinterpret_cast<float(&)[4]>(v[4]), reinterpret_cast<const uint8_t*>(&t) + 8, T{});
+            }
+        }
+    }
+};
+
+struct RowsArgs {
+    const void* x;
+    int64_t xr, xk;
+    const void* w;
+    int64_t wr, wk;
+    const float* bias;
+    const int64_t* labels;
+    int n, d;
+    int64_t c;
+    float2* part;       // [n][warps of the grid]
+    float* zy;          // [n], the label's logit
+};
+
+// N rows; x in shared memory as [units][N][values of a unit], zero past the features
+template <typename T, int N, bool VEC>
+__global__ void __launch_bounds__(kRowsThreads) xent_rows_kernel(const RowsArgs a) {
+    constexpr int V = WLoad<T, VEC>::kCount;
+    extern __shared__ __align__(16) float xs[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int units = (a.d + V - 1) / V, whole = a.d / V;
+    for (int i = threadIdx.x; i < units * V * N; i += kRowsThreads) {
+        const int v = i % V, r = i / V % N, k = i / (V * N) * V + v;
+        xs[i] = r < a.n && k < a.d ? to_float(((const T*)a.x)[r * a.xr + k * a.xk]) : 0.f;
+    }
+    __syncthreads();
+    float top[N], sum[N];
+    int64_t y[N];
+    #pragma unroll
+    for (int r = 0; r < N; ++r) {
+        top[r] = -INFINITY;
+        sum[r] = 0.f;
+        y[r] = r < a.n ? a.labels[r] : -1;
+    }
+    const int64_t first = (int64_t)blockIdx.x * (kRowsThreads / 32) + warp, step = (int64_t)gridDim.x * (kRowsThreads / 32);
+    for (int64_t j = first; j < a.c; j += step) {
+        const T* w = (const T*)a.w + j * a.wr;
+        float z[N];
+        #pragma unroll
+        for (int r = 0; r < N; ++r) z[r] = 0.f;
+        #pragma unroll 4
+        for (int q = lane; q < whole; q += 32) {
+            float v[V];
+            WLoad<T, VEC>::load(v, w + (int64_t)q * V * (VEC ? 1 : a.wk));
+            #pragma unroll
+            for (int r = 0; r < N; ++r)
+                #pragma unroll
+                for (int i = 0; i < V; ++i) z[r] = fmaf(v[i], xs[(q * N + r) * V + i], z[r]);
+        }
+        if (VEC && whole * V + lane < a.d) {   // the features past the last unit
+            const float v = to_float(w[whole * V + lane]);
+            #pragma unroll
+            for (int r = 0; r < N; ++r) z[r] = fmaf(v, xs[(whole * N + r) * V + lane], z[r]);
+        }
+        #pragma unroll
+        for (int r = 0; r < N; ++r)
+            #pragma unroll
+            for (int o = 16; o; o >>= 1) z[r] += __shfl_xor_sync(0xffffffffu, z[r], o);
+        const float b = a.bias ? a.bias[j] : 0.f;
+        #pragma unroll
+        for (int r = 0; r < N; ++r) {
+            const float v = z[r] + b, m = fmaxf(top[r], v), shift = m == -INFINITY ? 0.f : m;
+            sum[r] = sum[r] * expf(top[r] - shift) + expf(v - shift);
+            top[r] = m;
+            if (j == y[r] && lane == 0) a.zy[r] = v;
+        }
+    }
+    if (lane == 0)
+        #pragma unroll
+        for (int r = 0; r < N; ++r)
+            if (r < a.n) a.part[r * step + first] = make_float2(top[r], sum[r]);
+}
+
+// a block a row: loss and lse from the warps' maxima and sums, in a fixed order
+__global__ void __launch_bounds__(256) xent_rows_join_kernel(const float2* __restrict__ part, int64_t parts, int64_t c,
+                                                             const float* __restrict__ zy,
+                                                             const int64_t* __restrict__ labels, float* loss, float* lse) {
+    __shared__ float s[8];
+    const int r = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float2* p = part + r * parts;
+    float m = -INFINITY;
+    for (int64_t i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, p[i].x);
+    #pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s[warp] = m;
+    __syncthreads();
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, s[i]);
+    if (m == -INFINITY) m = 0.f;
+    float t = 0.f;
+    for (int64_t i = threadIdx.x; i < parts; i += 256) t += p[i].y * expf(p[i].x - m);
+    #pragma unroll
+    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    __syncthreads();
+    if (lane == 0) s[warp] = t;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    t = 0.f;
+    for (int i = 0; i < 8; ++i) t += s[i];
+    const int64_t y = labels[r];
+    const float l = logf(t);
+    loss[r] = y < 0 ? 0.f : y < c ? (m - zy[r]) + l : NAN;
+    if (lse) lse[r] = y < 0 ? 0.f : m + l;
+}
+
+bool rows_fit(const XentCall& a) {
+    return !a.gradient && a.n >= 1 && a.n <= kRowsFew && a.n * a.d <= kRowsFewValues && a.c >= 32;
+}
+int rows_grid(const XentCall& a, int sms) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(4 * sms, (a.c + 8 * 2 - 1) / (8 * 2)));   // two classes a warp at least
+}
+size_t rows_carve(const XentCall& a, int sms, uint8_t* ws, float2*& part, float*& zy) {
+    Carver cv(ws);
+    part = cv.take<float2>((size_t)a.n * rows_grid(a, sms) * (kRowsThreads / 32));
+    zy = cv.take<float>(a.n);
+    return cv.used;
+}
+template <typename T, int N>
+cudaError_t rows_launch(const RowsArgs& r, int grid, cudaStream_t st) {
+    const bool vec = r.wk == 1 && (uintptr_t)r.w % 16 == 0 && r.wr * (int64_t)sizeof(T) % 16 == 0;
+    const int V = vec ? 16 / sizeof(T) : 1;
+    const size_t smem = (size_t)((r.d + V - 1) / V) * V * N * sizeof(float);
+    auto fn = vec ? xent_rows_kernel<T, N, true> : xent_rows_kernel<T, N, false>;
+    const cudaError_t e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    KernelTimer kt(st, GAFIME_KERNEL_XENT);
+    fn<<<grid, kRowsThreads, smem, st>>>(r);
+    return cudaGetLastError();
+}
+template <typename T>
+cudaError_t rows_run(const XentCall& a, int sms) {
+    RowsArgs r{};
+    r.x = a.x; r.xr = a.xr; r.xk = a.xk; r.w = a.w; r.wr = a.wr; r.wk = a.wk;
+    r.bias = a.bias; r.labels = a.labels; r.n = (int)a.n; r.d = (int)a.d; r.c = a.c;
+    rows_carve(a, sms, a.ws, r.part, r.zy);
+    const int grid = rows_grid(a, sms);
+    cudaError_t e = a.n == 1   ? rows_launch<T, 1>(r, grid, a.stream)
+                    : a.n == 2 ? rows_launch<T, 2>(r, grid, a.stream)
+                    : a.n <= 4 ? rows_launch<T, 4>(r, grid, a.stream)
+                               : rows_launch<T, 8>(r, grid, a.stream);
+    if (e != cudaSuccess) return e;
+    KernelTimer kt(a.stream, GAFIME_KERNEL_XENT);
+    xent_rows_join_kernel<<<(unsigned)a.n, 256, 0, a.stream>>>(r.part, (int64_t)grid * (kRowsThreads / 32), a.c, r.zy,
+                                                               a.labels, a.loss, a.lse);
+    return cudaGetLastError();
+}
+
 FewPlan few_plan(const XentCall& a, int sms) {
     FewPlan p{};
     const int d = (int)a.d, c = (int)a.c, es = (int)xent_type_size(a.type);
@@ -173,6 +348,11 @@ bool sizes_ok(int type, int64_t n, int64_t d, int64_t c) {
 
 size_t workspace_of(const XentCall& a) {
     const int sms = sm_count_of_current();
+    if (rows_fit(a)) {
+        float2* part;
+        float* zy;
+        return rows_carve(a, sms, nullptr, part, zy);
+    }
     return xent_few_fits(a) ? xent_few_workspace(a, sms) : xent_tc_workspace(a, sms);
 }
 
@@ -182,7 +362,13 @@ int run_xent(const XentCall& a) {
     const size_t need = workspace_of(a);
     if (need > a.ws_bytes || (need && (!a.ws || (uintptr_t)a.ws % 256))) return GAFIME_ERROR_INVALID_ARGS;
     const int sms = sm_count_of_current();
-    const cudaError_t e = xent_few_fits(a) ? xent_few(a, sms) : xent_tc(a, sms);
+    cudaError_t e;
+    if (rows_fit(a))
+        e = a.type == GAFIME_TYPE_FP32   ? rows_run<float>(a, sms)
+            : a.type == GAFIME_TYPE_FP16 ? rows_run<__half>(a, sms)
+                                         : rows_run<__nv_bfloat16>(a, sms);
+    else
+        e = xent_few_fits(a) ? xent_few(a, sms) : xent_tc(a, sms);
     return e == cudaSuccess ? GAFIME_SUCCESS : status_from(e);
 }
 

@@ -622,6 +622,7 @@ struct SetupArgs {
     float* bias2;
     int64_t c, c_pad;
     float* zy;                // nullable: cleared to NaN
+    uint32_t* keep;           // nullable: bit r of word r / 32: row r counts
     Meta* meta;
 };
 
@@ -630,13 +631,17 @@ __global__ void __launch_bounds__(256) xent_setup_kernel(SetupArgs a) {
     const int64_t gt = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
     for (int64_t i = gt; i < a.c_pad; i += all)
         a.bias2[i] = i < a.c ? (a.bias ? a.bias[i] * kLog2e : 0.f) : -INFINITY;
-    if (!a.want_weight && !a.zy) return;
+    if (!a.want_weight && !a.zy && !a.keep) return;
     float top = 0.f;
     for (int64_t w = gt / 32; w < (a.n + 31) / 32; w += all / 32) {
         const int64_t r = w * 32 + lane;
         const bool in = r < a.n;
         const bool kept = in && a.labels[r] >= 0;
         if (a.zy && in) a.zy[r] = NAN;
+        if (a.keep) {
+            const uint32_t bits = __ballot_sync(0xffffffffu, kept);
+            if (lane == 0) a.keep[w] = bits;
+        }
         if (a.want_weight && kept) {
             const float v = fabsf((a.weight ? a.weight[r * a.weight_stride] : 1.f) * a.scale);
             if (v <= 3.402823466e38f) top = fmaxf(top, v);
@@ -722,54 +727,65 @@ __device__ __forceinline__ float finite_abs(float v) {
     return v <= 3.402823466e38f ? v : 0.f;
 }
 
-// Largest finite |x_k| over the rows that count.  A block takes `rows` rows and, row by row, a
-// run of 4 x 256 features (a thread four of them, several rows at once where the features are
-// fewer), else 32 features with a warp going down one of them at a time.
+__device__ __forceinline__ bool row_counts(const uint32_t* keep, int64_t r) { return (keep[r >> 5] >> (r & 31)) & 1; }
+
+// Largest finite |x_k| over the rows that count (the bits of `keep`).
+//   kRows    x row by row in 16-byte units: a block takes `rows` rows of 1024 features, a thread four
+//            of them, several rows at once where the features are fewer
+//   kColumns x column by column: a block takes `rows` rows of one feature
+//   kAny     a block takes `rows` rows of 32 features
+enum { kRows = 0, kColumns = 1, kAny = 2 };
 __global__ void __launch_bounds__(256) xent_colmax_kernel(const float* __restrict__ x, int64_t xr, int64_t xk,
-                                                          const int64_t* __restrict__ labels, int64_t n, int64_t d,
-                                                          int64_t rows, int vector, uint32_t* colmax) {
+                                                          const uint32_t* __restrict__ keep, int64_t n, int64_t d,
+                                                          int64_t rows, int order, uint32_t* colmax) {
     __shared__ uint32_t top[1024];
-    const int64_t width = vector ? 1024 : 32, blocks_k = (d + width - 1) / width;
+    const int64_t width = order == kRows ? 1024 : order == kColumns ? 1 : 32, blocks_k = (d + width - 1) / width;
     const int64_t k0 = (blockIdx.x % blocks_k) * width, r0 = (blockIdx.x / blocks_k) * rows, r1 = min(n, r0 + rows);
     for (int i = threadIdx.x; i < width; i += 256) top[i] = 0;
     __syncthreads();
-    if (vector) {
+    if (order == kRows) {
         const int quads = (int)min((int64_t)256, (d - k0 + 3) / 4), at_once = 256 / quads;
         const int quad = threadIdx.x % quads, ro = threadIdx.x / quads;
         if (ro < at_once) {
             float m[4] = {0.f, 0.f, 0.f, 0.f};
-            #pragma unroll 4
+            #pragma unroll 8
             for (int64_t r = r0 + ro; r < r1; r += at_once) {
                 const float4 v = load_quad(x + r * xr, k0 + 4 * quad, d);
-                if (labels[r] < 0) continue;
-                m[0] = fmaxf(m[0], finite_abs(v.x));
-                m[1] = fmaxf(m[1], finite_abs(v.y));
-                m[2] = fmaxf(m[2], finite_abs(v.z));
-                m[3] = fmaxf(m[3], finite_abs(v.w));
+                const bool in = row_counts(keep, r);
+                m[0] = fmaxf(m[0], in ? finite_abs(v.x) : 0.f);
+                m[1] = fmaxf(m[1], in ? finite_abs(v.y) : 0.f);
+                m[2] = fmaxf(m[2], in ? finite_abs(v.z) : 0.f);
+                m[3] = fmaxf(m[3], in ? finite_abs(v.w) : 0.f);
             }
             for (int i = 0; i < 4; ++i) atomicMax(&top[4 * quad + i], __float_as_uint(m[i]));
         }
-    } else if (xr == 1 && xk != 1) {
-        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-        for (int j = ty; j < 32 && k0 + j < d; j += 8) {
-            float m = 0.f;
-            #pragma unroll 8
-            for (int64_t r = r0 + tx; r < r1; r += 32) {
-                const float v = finite_abs(x[r + (k0 + j) * xk]);
-                if (labels[r] >= 0) m = fmaxf(m, v);
+    } else if (order == kColumns) {
+        const float* p = x + k0 * xk;
+        float m = 0.f;
+        if ((uintptr_t)p % 16 == 0) {   // r0 is a multiple of 32
+            #pragma unroll 4
+            for (int64_t r = r0 + 4 * threadIdx.x; r < r1; r += 1024) {
+                const float4 v = load_quad(p, r, n);
+                const uint32_t bits = keep[r >> 5] >> (r & 31);
+                m = fmaxf(m, bits & 1 ? finite_abs(v.x) : 0.f);
+                m = fmaxf(m, bits & 2 ? finite_abs(v.y) : 0.f);
+                m = fmaxf(m, bits & 4 ? finite_abs(v.z) : 0.f);
+                m = fmaxf(m, bits & 8 ? finite_abs(v.w) : 0.f);
             }
-            const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-            if (tx == 0) top[j] = w;
+        } else {
+            #pragma unroll 8
+            for (int64_t r = r0 + threadIdx.x; r < r1; r += 256)
+                if (row_counts(keep, r)) m = fmaxf(m, finite_abs(p[r]));
         }
+        const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+        if ((threadIdx.x & 31) == 0) atomicMax(&top[0], w);
     } else {
         const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
         float m = 0.f;
         if (k0 + tx < d)
             #pragma unroll 4
-            for (int64_t r = r0 + ty; r < r1; r += 8) {
-                const float v = finite_abs(x[r * xr + (k0 + tx) * xk]);
-                if (labels[r] >= 0) m = fmaxf(m, v);
-            }
+            for (int64_t r = r0 + ty; r < r1; r += 8)
+                if (row_counts(keep, r)) m = fmaxf(m, finite_abs(x[r * xr + (k0 + tx) * xk]));
         atomicMax(&top[tx], __float_as_uint(m));
     }
     __syncthreads();
@@ -807,7 +823,7 @@ __device__ __forceinline__ void split2(float v0, float v1, uint32_t& hi, uint32_
 // fp32 rows in 16-byte units -> planes [rows][dp], hi and lo fp16 of the scaled values; rows with
 // a negative label become zeros.  A thread keeps four features and their scales over its rows.
 __global__ void __launch_bounds__(256) xent_planes_rows_kernel(const float* __restrict__ x, int64_t xr,
-                                                               const int64_t* __restrict__ labels, int64_t n, int64_t d,
+                                                               const uint32_t* __restrict__ keep, int64_t n, int64_t d,
                                                                int64_t dp, int64_t rows, const uint32_t* __restrict__ colmax,
                                                                const Meta* __restrict__ meta, int is_w,
                                                                __half* __restrict__ hi, __half* __restrict__ lo) {
@@ -827,7 +843,7 @@ __global__ void __launch_bounds__(256) xent_planes_rows_kernel(const float* __re
     #pragma unroll 4
     for (int64_t r = r0 + ro; r < r1; r += at_once) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!labels || labels[r] >= 0) v = load_quad(x + r * xr, k, d);
+        if (!keep || row_counts(keep, r)) v = load_quad(x + r * xr, k, d);
         uint2 h, l;
         split2(v.x * f0[0] * f1[0], v.y * f0[1] * f1[1], h.x, l.x);
         split2(v.z * f0[2] * f1[2], v.w * f0[3] * f1[3], h.y, l.y);
@@ -856,7 +872,7 @@ __global__ void __launch_bounds__(256) xent_undo_kernel(const uint32_t* __restri
 // one is needed).
 template <typename T, typename E>
 __global__ void __launch_bounds__(256) xent_planes_kernel(const T* __restrict__ x, int64_t xr, int64_t xk,
-                                                          const int64_t* __restrict__ labels, int64_t n, int64_t d,
+                                                          const uint32_t* __restrict__ keep, int64_t n, int64_t d,
                                                           int64_t dp, const uint32_t* __restrict__ colmax,
                                                           const Meta* __restrict__ meta, int is_w, int if_poison,
                                                           E* __restrict__ hi, E* __restrict__ lo) {
@@ -865,12 +881,34 @@ __global__ void __launch_bounds__(256) xent_planes_kernel(const T* __restrict__ 
     const int64_t tiles_k = (dp + 63) / 64;
     const int64_t k0 = (blockIdx.x % tiles_k) * 64, r0 = (blockIdx.x / tiles_k) * 64;
     const bool down = xr == 1 && xk != 1;
-    #pragma unroll 4
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = down ? i & 63 : i >> 6, k = down ? i >> 6 : i & 63;
-        float v = 0.f;
-        if (r0 + r < n && k0 + k < d && (!labels || labels[r0 + r] >= 0)) v = to_float(x[(r0 + r) * xr + (k0 + k) * xk]);
-        t[k][r] = v;
+    if (down && sizeof(T) == 4 && (uintptr_t)x % 16 == 0 && xk % 4 == 0) {
+        // four rows of a feature at a time
+        #pragma unroll
+        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+            const int r = (i & 15) * 4, k = i >> 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r0 + r < n && k0 + k < d) {
+                v = load_quad((const float*)x + (k0 + k) * xk, r0 + r, n);
+                const uint32_t bits = keep ? keep[(r0 + r) >> 5] >> ((r0 + r) & 31) : 15;
+                if (!(bits & 1)) v.x = 0.f;
+                if (!(bits & 2)) v.y = 0.f;
+                if (!(bits & 4)) v.z = 0.f;
+                if (!(bits & 8)) v.w = 0.f;
+            }
+            t[k][r] = v.x;
+            t[k][r + 1] = v.y;
+            t[k][r + 2] = v.z;
+            t[k][r + 3] = v.w;
+        }
+    } else {
+        #pragma unroll 8
+        for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+            const int r = down ? i & 63 : i >> 6, k = down ? i >> 6 : i & 63;
+            float v = 0.f;
+            if (r0 + r < n && k0 + k < d && (!keep || row_counts(keep, r0 + r)))
+                v = to_float(x[(r0 + r) * xr + (k0 + k) * xk]);
+            t[k][r] = v;
+        }
     }
     __syncthreads();
     // 8 features of a row to a thread, 16 bytes of a plane
@@ -1029,13 +1067,14 @@ bool in_place(int type, const void* p, int64_t row, int64_t col, int64_t len) {
 }
 
 struct Plan {
-    int planes, bn_c, bn_d;
+    int planes, bn_c, bn_dx, bn_dw;
     bool x_in_place, w_in_place;
     int64_t dp;
     int64_t m_tiles, c_tiles;        // of the whole call, 256 rows and bn_c classes
     int splits, per_split;           // LSE
     int64_t piece_rows, piece_classes, ldg;
-    int64_t dw_c_tiles, dw_d_tiles;  // 128 classes x bn_d features
+    int64_t dx_d_tiles;              // of bn_dx features
+    int64_t dw_c_tiles, dw_d_tiles;  // 128 classes x bn_dw features
     int64_t dw_stride;               // floats of a split's partial
     int dw_splits, dw_per_split;
     bool dw_direct;                  // one split: dw leaves the products' kernel
@@ -1046,6 +1085,7 @@ struct Plan {
     uint32_t* colmax;
     size_t meta_bytes;
     float* bias2;
+    uint32_t* keep;
     uint16_t* xc;                    // x without left-out rows, made where one of those holds no number
     uint16_t *xh, *xl, *wh, *wl, *gh, *gl;
     float2* part;
@@ -1064,7 +1104,6 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
     Plan p{};
     p.planes = a.type == GAFIME_TYPE_FP32 ? 2 : 1;
     p.bn_c = tile_n(a.c);
-    p.bn_d = std::max(128, tile_n(a.d));   // a CTA's half of it is whole 64-value lines
     const int pairs = sms / 2;
     p.x_in_place = in_place(a.type, a.x, a.xr, a.xk, a.d);
     p.w_in_place = in_place(a.type, a.w, a.wr, a.wk, a.d);
@@ -1088,6 +1127,7 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
     p.colmax = cv.take<uint32_t>(p.planes == 2 ? a.d : 0);
     p.meta_bytes = cv.used;
     p.bias2 = cv.take<float>(p.c_tiles * p.bn_c + 256);
+    p.keep = cv.take<uint32_t>(cdiv(a.n, 32) + 2);
     if (p.planes == 2 || !p.x_in_place) p.xh = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
     if (p.planes == 2) p.xl = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
     if (p.planes == 2 || !p.w_in_place) p.wh = cv.take<uint16_t>(a.c * p.dp);
@@ -1110,18 +1150,42 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
         p.ldg = up(p.piece_classes, 64);   // whole 128-byte lines: TMA boxes meet no line twice
         p.gh = cv.take<uint16_t>(p.piece_rows * p.ldg);
         if (p.planes == 2) p.gl = cv.take<uint16_t>(p.piece_rows * p.ldg);
-        p.dw_d_tiles = cdiv(a.d, p.bn_d);
+        // Feature tiles of 128 or 256 (a CTA's half is whole 64-value lines): the ones with the fewer
+        // rounds of the pairs, where a round of 128 takes about 0.6 of one of 256; dw's rows are split
+        // over pairs that its tiles leave idle, in runs of at least 4 blocks
+        double dx_cost = 1e300, dw_cost = 1e300;
+        const int64_t m_dx = cdiv(std::min(p.piece_rows, a.n), kPM), m_dw = cdiv(p.piece_classes, kPM);
+        const int64_t blocks = cdiv(std::min(a.n, p.piece_rows), kBK);
+        for (int bn : {256, 128}) {
+            if (bn == 256 && a.d <= 128) continue;
+            const int64_t nt = cdiv(a.d, bn);
+            const double tile = bn == 256 ? 1.0 : 0.6;
+            const double dx = cdiv(m_dx * nt, pairs) * tile;
+            if (dx < dx_cost) {
+                dx_cost = dx;
+                p.bn_dx = bn;
+            }
+            for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(pairs, blocks / 4)); ++s) {
+                const int64_t per = cdiv(blocks, s);
+                if (s > 1 && m_dw * nt * cdiv(blocks, per) > 2 * pairs) break;
+                const double dw = cdiv(m_dw * nt * cdiv(blocks, per), pairs) * (per + 4.0) * tile;
+                if (dw < dw_cost * 0.97) {
+                    dw_cost = dw;
+                    p.bn_dw = bn;
+                    p.dw_per_split = (int)per;
+                }
+            }
+        }
+        p.dw_splits = (int)cdiv(blocks, p.dw_per_split);
+        p.dx_d_tiles = cdiv(a.d, p.bn_dx);
+        p.dw_d_tiles = cdiv(a.d, p.bn_dw);
         p.dw_c_tiles = cdiv(a.c, kPM) * 2;
-        p.dw_stride = p.dw_c_tiles * p.dw_d_tiles * p.bn_d * kBM;
-        p.undo_pitch = p.dw_d_tiles * p.bn_d;
+        p.dw_stride = p.dw_c_tiles * p.dw_d_tiles * p.bn_dw * kBM;
+        p.undo_pitch = up(a.d, 256);
         if (p.planes == 2) p.undo = cv.take<float>(4 * p.undo_pitch);
         if (a.dx && p.piece_classes < a.c)
-            p.dx_acc = cv.take<float>(p.piece_rows * p.dw_d_tiles * p.bn_d);
+            p.dx_acc = cv.take<float>(p.piece_rows * p.dx_d_tiles * p.bn_dx);
         if (a.dw) {
-            const int64_t tiles = cdiv(p.piece_classes, kPM) * p.dw_d_tiles, blocks = cdiv(std::min(a.n, p.piece_rows), kBK);
-            const int64_t s = std::max<int64_t>(1, std::min<int64_t>(pairs / tiles, blocks / 4));
-            p.dw_per_split = (int)cdiv(blocks, s);
-            p.dw_splits = (int)cdiv(blocks, p.dw_per_split);
             p.dw_direct = p.dw_splits == 1;
             if (!p.dw_direct || a.n > p.piece_rows) p.dw_part = cv.take<float>(p.dw_splits * p.dw_stride);
         }
@@ -1167,7 +1231,7 @@ cudaError_t launch(const TcArgs& t, int bn, int sms, cudaStream_t stream) {
     } while (0)
 
 template <typename T, typename E>
-cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const int64_t* labels, int64_t rows, int64_t d,
+cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const uint32_t* keep, int64_t rows, int64_t d,
                    bool is_w, bool if_poison, uint16_t* hi, uint16_t* lo, int sms, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         if (rows_vector(src, sr, sk)) {
@@ -1175,13 +1239,13 @@ cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const in
             const int64_t per = std::max<int64_t>(16, cdiv(rows * blocks_k, 16 * sms));
             KernelTimer kt(stream, GAFIME_KERNEL_XENT);
             xent_planes_rows_kernel<<<(unsigned)(blocks_k * cdiv(rows, per)), 256, 0, stream>>>(
-                src, sr, labels, rows, d, p.dp, per, p.colmax, p.meta, is_w, (__half*)hi, (__half*)lo);
+                src, sr, keep, rows, d, p.dp, per, p.colmax, p.meta, is_w, (__half*)hi, (__half*)lo);
             return cudaGetLastError();
         }
     }
     const int64_t blocks = cdiv(p.dp, 64) * cdiv(rows, 64);
     KernelTimer kt(stream, GAFIME_KERNEL_XENT);
-    xent_planes_kernel<T, E><<<(unsigned)blocks, 256, 0, stream>>>(src, sr, sk, labels, rows, d, p.dp, p.colmax, p.meta,
+    xent_planes_kernel<T, E><<<(unsigned)blocks, 256, 0, stream>>>(src, sr, sk, keep, rows, d, p.dp, p.colmax, p.meta,
                                                                    is_w, if_poison, (E*)hi, (E*)lo);
     return cudaGetLastError();
 }
@@ -1206,6 +1270,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         s.want_weight = p.products && !kBf16;
         s.bias = a.bias; s.bias2 = p.bias2; s.c = a.c; s.c_pad = p.c_tiles * p.bn_c + 256;
         s.zy = forward ? p.zy : nullptr;
+        s.keep = p.xh || p.xc ? p.keep : nullptr;
         s.meta = p.meta;
         const int64_t threads = std::max<int64_t>(s.c_pad, a.n);
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
@@ -1217,16 +1282,16 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         xent_poison_kernel<<<(unsigned)std::min<int64_t>(8 * sms, cdiv(a.n, 8)), 256, 0, st>>>(
             a.labels, a.n, (const uint16_t*)a.x, a.xr, a.d, kBf16, p.meta);
         XENT_TRY(cudaGetLastError());
-        XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, true, p.xc, nullptr, sms, st)));
+        XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, p.keep, a.n, a.d, false, true, p.xc, nullptr, sms, st)));
     }
     if (scaled) {
         {
-            const int vector = rows_vector(a.x, a.xr, a.xk);
-            const int64_t blocks_k = cdiv(a.d, vector ? 1024 : 32);
-            const int64_t rows = std::max<int64_t>(64, cdiv(a.n * blocks_k, 8 * sms));
+            const int order = rows_vector(a.x, a.xr, a.xk) ? kRows : a.xr == 1 && a.xk != 1 ? kColumns : kAny;
+            const int64_t blocks_k = cdiv(a.d, order == kRows ? 1024 : order == kColumns ? 1 : 32);
+            const int64_t rows = up(std::max<int64_t>(order == kColumns ? 1024 : 64, cdiv(a.n * blocks_k, 8 * sms)), 32);
             KernelTimer kt(st, GAFIME_KERNEL_XENT);
             xent_colmax_kernel<<<(unsigned)(blocks_k * cdiv(a.n, rows)), 256, 0, st>>>(
-                (const float*)a.x, a.xr, a.xk, a.labels, a.n, a.d, rows, vector, p.colmax);
+                (const float*)a.x, a.xr, a.xk, p.keep, a.n, a.d, rows, order, p.colmax);
             XENT_TRY(cudaGetLastError());
         }
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
@@ -1234,7 +1299,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             (const float*)a.w, a.wr, a.wk, a.c, a.d, p.colmax, p.meta);
         XENT_TRY(cudaGetLastError());
     }
-    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, a.labels, a.n, a.d, false, false, p.xh, p.xl, sms, st)));
+    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, p.keep, a.n, a.d, false, false, p.xh, p.xl, sms, st)));
     if (p.wh) XENT_TRY((planes<T, E>(p, (const T*)a.w, a.wr, a.wk, nullptr, a.c, a.d, true, false, p.wh, p.wl, sms, st)));
     // where the operands are read
     const void *xs[2] = {p.xh ? (const void*)p.xh : a.x, p.xl}, *ws[2] = {p.wh ? (const void*)p.wh : a.w, p.wl};
@@ -1330,7 +1395,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 const void* wp[2] = {(const uint16_t*)ws[0] + c0 * ldw, ws[1] ? (const uint16_t*)ws[1] + c0 * ldw : nullptr};
                 XENT_TRY(map(x.b, wp, a.d, classes, ldw, kBK));
                 x.m_tiles = (int)cdiv(rows, kPM);
-                x.n_tiles = (int)p.dw_d_tiles;
+                x.n_tiles = (int)p.dx_d_tiles;
                 x.units = x.m_tiles * x.n_tiles;
                 x.k_blocks = (int)cdiv(classes, kBK);
                 if (p.planes == 1) x.chunk = 16;
@@ -1345,7 +1410,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 x.dx_acc = p.dx_acc;
                 x.first = c0 == 0;
                 x.last = c0 + classes == a.c;
-                XENT_TRY((launch<DX, E, kPlanes>(x, p.bn_d, sms, st)));
+                XENT_TRY((launch<DX, E, kPlanes>(x, p.bn_dx, sms, st)));
             }
             if (a.dw) {
                 TcArgs w = t;
@@ -1376,14 +1441,14 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 w.undo_pitch = p.undo_pitch;
                 w.cleaned = p.xc != nullptr;
                 if (p.xc && !make_map(&w.b[1], kBf16, p.xc, a.d, a.n, p.dp, kBK)) return cudaErrorInvalidValue;
-                XENT_TRY((launch<DW, E, kPlanes>(w, p.bn_d, sms, st)));
+                XENT_TRY((launch<DW, E, kPlanes>(w, p.bn_dw, sms, st)));
             }
         }
     }
     if (a.dw && !p.dw_direct) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
         xent_dw_kernel<T><<<(unsigned)(cdiv(a.c, 32) * cdiv(a.d, 8)), 256, 0, st>>>(
-            p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_d, (int)a.c, (int)a.d,
+            p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_dw, (int)a.c, (int)a.d,
             p.undo ? p.undo + 2 * p.undo_pitch : nullptr, p.undo_pitch, !kBf16, p.meta, (T*)a.dw);
         XENT_TRY(cudaGetLastError());
     }
