@@ -25,8 +25,8 @@ namespace gafime {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGridPerSm = 4;
-constexpr int kMaxGrid = 1024;
+constexpr int kGridPerSm = 8;
+constexpr int kMaxGrid = 2048;
 constexpr int kChunk = 16384;      // elements a CTA takes at a time
 constexpr int kFewTensors = 32, kManyTensors = 1024;   // of one launch
 
@@ -129,7 +129,7 @@ __device__ void chunk_scale(const T* p, T* o, int len, float f) {
         unpack(v, q[i], T{});
         #pragma unroll
         for (int j = 0; j < V; ++j) v[j] *= f;
-        w[i] = repack(v, T{});
+        __stcs(w + i, repack(v, T{}));
     }
     const int rest = len - head - vecs * V;
     if ((int)threadIdx.x < head + rest) {

@@ -104,10 +104,11 @@ struct RowsArgs {
     float* zy;          // [n], the label's logit
 };
 
-// N rows; x in shared memory as [units][N][values of a unit], zero past the features
+// N rows; x in shared memory as [units][N][values of a unit], zero past the features.  J classes
+// at a time keep as many loads under way.
 template <typename T, int N, bool VEC>
 __global__ void __launch_bounds__(kRowsThreads) xent_rows_kernel(const RowsArgs a) {
-    constexpr int V = WLoad<T, VEC>::kCount;
+    constexpr int V = WLoad<T, VEC>::kCount, J = N <= 2 ? 4 : N <= 4 ? 2 : 1;
     extern __shared__ __align__(16) float xs[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int units = (a.d + V - 1) / V, whole = a.d / V;
@@ -125,36 +126,54 @@ __global__ void __launch_bounds__(kRowsThreads) xent_rows_kernel(const RowsArgs 
         y[r] = r < a.n ? a.labels[r] : -1;
     }
     const int64_t first = (int64_t)blockIdx.x * (kRowsThreads / 32) + warp, step = (int64_t)gridDim.x * (kRowsThreads / 32);
-    for (int64_t j = first; j < a.c; j += step) {
-        const T* w = (const T*)a.w + j * a.wr;
-        float z[N];
+    for (int64_t j0 = first * J; j0 < a.c; j0 += step * J) {
+        const T* w[J];
         #pragma unroll
-        for (int r = 0; r < N; ++r) z[r] = 0.f;
-        #pragma unroll 4
+        for (int j = 0; j < J; ++j) w[j] = (const T*)a.w + min(j0 + j, a.c - 1) * a.wr;
+        float z[J][N];
+        #pragma unroll
+        for (int j = 0; j < J; ++j)
+            #pragma unroll
+            for (int r = 0; r < N; ++r) z[j][r] = 0.f;
+        #pragma unroll 2
         for (int q = lane; q < whole; q += 32) {
-            float v[V];
-            WLoad<T, VEC>::load(v, w + (int64_t)q * V * (VEC ? 1 : a.wk));
+            float v[J][V];
+            #pragma unroll
+            for (int j = 0; j < J; ++j) WLoad<T, VEC>::load(v[j], w[j] + (int64_t)q * V * (VEC ? 1 : a.wk));
             #pragma unroll
             for (int r = 0; r < N; ++r)
                 #pragma unroll
-                for (int i = 0; i < V; ++i) z[r] = fmaf(v[i], xs[(q * N + r) * V + i], z[r]);
+                for (int i = 0; i < V; ++i) {
+                    const float xv = xs[(q * N + r) * V + i];
+                    #pragma unroll
+                    for (int j = 0; j < J; ++j) z[j][r] = fmaf(v[j][i], xv, z[j][r]);
+                }
         }
         if (VEC && whole * V + lane < a.d) {   // the features past the last unit
-            const float v = to_float(w[whole * V + lane]);
             #pragma unroll
-            for (int r = 0; r < N; ++r) z[r] = fmaf(v, xs[(whole * N + r) * V + lane], z[r]);
+            for (int j = 0; j < J; ++j) {
+                const float v = to_float(w[j][whole * V + lane]);
+                #pragma unroll
+                for (int r = 0; r < N; ++r) z[j][r] = fmaf(v, xs[(whole * N + r) * V + lane], z[j][r]);
+            }
         }
         #pragma unroll
-        for (int r = 0; r < N; ++r)
+        for (int o = 16; o; o >>= 1)
             #pragma unroll
-            for (int o = 16; o; o >>= 1) z[r] += __shfl_xor_sync(0xffffffffu, z[r], o);
-        const float b = a.bias ? a.bias[j] : 0.f;
+            for (int j = 0; j < J; ++j)
+                #pragma unroll
+                for (int r = 0; r < N; ++r) z[j][r] += __shfl_xor_sync(0xffffffffu, z[j][r], o);
         #pragma unroll
-        for (int r = 0; r < N; ++r) {
-            const float v = z[r] + b, m = fmaxf(top[r], v), shift = m == -INFINITY ? 0.f : m;
-            sum[r] = sum[r] * expf(top[r] - shift) + expf(v - shift);
-            top[r] = m;
-            if (j == y[r] && lane == 0) a.zy[r] = v;
+        for (int j = 0; j < J; ++j) {
+            if (j0 + j >= a.c) break;
+            const float b = a.bias ? a.bias[j0 + j] : 0.f;
+            #pragma unroll
+            for (int r = 0; r < N; ++r) {
+                const float v = z[j][r] + b, m = fmaxf(top[r], v), shift = m == -INFINITY ? 0.f : m;
+                sum[r] = sum[r] * expf(top[r] - shift) + expf(v - shift);
+                top[r] = m;
+                if (j0 + j == y[r] && lane == 0) a.zy[r] = v;
+            }
         }
     }
     if (lane == 0)
@@ -198,7 +217,7 @@ bool rows_fit(const XentCall& a) {
     return !a.gradient && a.n >= 1 && a.n <= kRowsFew && a.n * a.d <= kRowsFewValues && a.c >= 32;
 }
 int rows_grid(const XentCall& a, int sms) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(4 * sms, (a.c + 8 * 2 - 1) / (8 * 2)));   // two classes a warp at least
+    return (int)std::max<int64_t>(1, std::min<int64_t>(4 * sms, (a.c + 8 * 4 - 1) / (8 * 4)));   // four classes a warp
 }
 size_t rows_carve(const XentCall& a, int sms, uint8_t* ws, float2*& part, float*& zy) {
     Carver cv(ws);

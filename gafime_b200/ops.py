@@ -9,8 +9,10 @@ comes from torch's allocator.  The kernels are those of ``gafime_xent_*`` and
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
+import operator
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -19,6 +21,14 @@ from . import _native
 
 TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _DX, _DW, _DBIAS, _GRADIENT = 1, 2, 4, 8
+# over lists of hundreds of tensors, without a Python frame for each
+_numel, _pointer, _device = torch.Tensor.numel, torch.Tensor.data_ptr, torch.Tensor.get_device
+_contiguous = torch.Tensor.is_contiguous
+_dtype = operator.attrgetter("dtype")
+
+
+def _address(values: array.array) -> int:
+    return values.buffer_info()[0]
 
 
 class XentGrad(NamedTuple):
@@ -61,48 +71,54 @@ def _check(x, w, labels, bias, row_weight):
         raise ValueError(f"bias must be a float32 ({c},) tensor")
     if row_weight is not None and (row_weight.shape != (n,) or row_weight.dtype != torch.float32):
         raise ValueError(f"row_weight must be a float32 ({n},) tensor")
-    device = x.device
-    for name, t in (("x", x), ("w", w), ("labels", labels), ("bias", bias), ("row_weight", row_weight)):
-        if t is not None and (not t.is_cuda or t.device != device):
-            raise ValueError(f"{name} must be on the GPU that holds x, got {t.device}")
+    index = x.get_device()
+    if index < 0 or w.get_device() != index or labels.get_device() != index or (
+            bias is not None and bias.get_device() != index) or (
+            row_weight is not None and row_weight.get_device() != index):
+        raise ValueError("x, w, labels, bias and row_weight must be on one GPU (there is no CPU path)")
     return n, d, c
+
+
+def _on_device(index: int, name: str, fn, args) -> None:
+    """fn(*args, stream) on torch's current stream of device `index`."""
+    if torch.cuda.current_device() == index:
+        code = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if code:
+        _native.check(name, code)
 
 
 def _call(x, w, labels, bias, n, d, c, want, row_weight=None, scale=1.0, loss=None, lse=None, dx=None, dw=None,
           dbias=None):
     """One library call on the current stream of x's device; loss and lse given: read, not written."""
     lib = _native.load()
-    type_id = TYPES[x.dtype]
+    type_id, device, index = TYPES[x.dtype], x.device, x.get_device()
     xp, wp = x.data_ptr(), w.data_ptr()
     xr, xk = x.stride()
     wr, wk = w.stride()
-    index = x.device.index
     have = loss is not None
     if labels.dtype != torch.int64 or (n > 1 and labels.stride(0) != 1):
         labels = labels.to(torch.int64).contiguous()
     if bias is not None and c > 1 and bias.stride(0) != 1:
         bias = bias.contiguous()
-    with torch.cuda.device(index):
-        size = _workspace_bytes(index, type_id, xp % 16, xr, xk, wp % 16, wr, wk, n, d, c, want)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        if not have:
-            loss = torch.empty(n, dtype=torch.float32, device=x.device)
-            lse = torch.empty(n, dtype=torch.float32, device=x.device)
-        stream = torch.cuda.current_stream(index).cuda_stream
-        bias_p = None if bias is None else bias.data_ptr()
-        ws_p = None if ws is None else ws.data_ptr()
-        if want == 0:
-            _native.check("gafime_xent_forward", lib.gafime_xent_forward(
-                type_id, xp, xr, xk, wp, wr, wk, bias_p, labels.data_ptr(), n, d, c, loss.data_ptr(),
-                lse.data_ptr(), ws_p, size, stream))
-        else:
-            _native.check("gafime_xent_gradient", lib.gafime_xent_gradient(
-                type_id, xp, xr, xk, wp, wr, wk, bias_p, labels.data_ptr(), n, d, c,
-                None if row_weight is None else row_weight.data_ptr(),
-                0 if row_weight is None else row_weight.stride(0), scale, int(have), loss.data_ptr(),
-                lse.data_ptr(), None if dx is None else dx.data_ptr(), 0 if dx is None else dx.stride(0),
-                0 if dx is None else dx.stride(1), None if dw is None else dw.data_ptr(),
-                None if dbias is None else dbias.data_ptr(), ws_p, size, stream))
+    size = _workspace_bytes(index, type_id, xp % 16, xr, xk, wp % 16, wr, wk, n, d, c, want)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    if not have:
+        loss = torch.empty(n, dtype=torch.float32, device=device)
+        lse = torch.empty(n, dtype=torch.float32, device=device)
+    args = (type_id, xp, xr, xk, wp, wr, wk, None if bias is None else bias.data_ptr(), labels.data_ptr(), n, d, c)
+    end = (None if ws is None else ws.data_ptr(), size)
+    if want == 0:
+        args += (loss.data_ptr(), lse.data_ptr())
+        _on_device(index, "gafime_xent_forward", lib.gafime_xent_forward, args + end)
+    else:
+        args += (None, 0) if row_weight is None else (row_weight.data_ptr(), row_weight.stride(0))
+        args += (scale, int(have), loss.data_ptr(), lse.data_ptr())
+        args += (None, 0, 0) if dx is None else (dx.data_ptr(), dx.stride(0), dx.stride(1))
+        args += (None if dw is None else dw.data_ptr(), None if dbias is None else dbias.data_ptr())
+        _on_device(index, "gafime_xent_gradient", lib.gafime_xent_gradient, args + end)
     return loss, lse
 
 
@@ -176,8 +192,7 @@ def softmax_xent_grad(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, bi
                           bias is not None)
 
 
-def _grad_norm(tensors: Sequence[torch.Tensor], out, max_norm: float) -> torch.Tensor:
-    tensors = list(tensors)
+def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
     count = len(tensors)
     if count == 0:
         raise ValueError("at least one tensor is needed")
@@ -185,36 +200,33 @@ def _grad_norm(tensors: Sequence[torch.Tensor], out, max_norm: float) -> torch.T
     if device.type != "cuda":
         raise ValueError(f"the tensors must be on one GPU, got {device}")
     index = device.index
-    ptrs, sizes, types = [], [], []
-    for t in tensors:
-        type_id = TYPES.get(t.dtype)
-        if type_id is None:
-            raise TypeError(f"tensors must be float32, float16 or bfloat16, got {t.dtype}")
-        if t.get_device() != index or not t.is_contiguous():
-            raise ValueError("the tensors must be contiguous and on one GPU")
-        ptrs.append(t.data_ptr())
-        sizes.append(t.numel())
-        types.append(type_id)
+    # whole lists at C speed: 64-bit arrays that the library reads in place
+    sizes = array.array("q", map(_numel, tensors))
+    dtypes = list(map(_dtype, tensors))
+    if not set(dtypes) <= TYPES.keys():
+        raise TypeError(f"tensors must be float32, float16 or bfloat16, got {set(dtypes) - TYPES.keys()}")
+    if set(map(_device, tensors)) != {index} or not all(map(_contiguous, tensors)):
+        raise ValueError("the tensors must be contiguous and on one GPU")
     lib = _native.load()
     outs = None
-    if out is not None:
+    ptrs = array.array("q", map(_pointer, tensors))
+    if out is tensors:
+        outs = ptrs
+    elif out is not None:
         out = list(out)
         if len(out) != count:
             raise ValueError(f"{count} tensors, but {len(out)} outs")
-        outs = []
-        for t, o in zip(tensors, out):
-            if o is not t and (o.dtype != t.dtype or o.shape != t.shape or o.get_device() != index
-                               or not o.is_contiguous()):
-                raise ValueError("every out must have its tensor's shape, type and device, and be contiguous")
-            outs.append(o.data_ptr())
-        outs = (ctypes.c_void_p * count)(*outs)
-    with torch.cuda.device(index):
-        size = _norm_workspace(count)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        _native.check("gafime_grad_norm", lib.gafime_grad_norm(
-            (ctypes.c_void_p * count)(*ptrs), (ctypes.c_int64 * count)(*sizes), (ctypes.c_int * count)(*types), count,
-            outs, max_norm, norm.data_ptr(), ws.data_ptr(), size, torch.cuda.current_stream(index).cuda_stream))
+        if (list(map(_dtype, out)) != dtypes or array.array("q", map(_numel, out)) != sizes
+                or set(map(_device, out)) != {index} or not all(map(_contiguous, out))):
+            raise ValueError("every out must have its tensor's size, type and device, and be contiguous")
+        outs = array.array("q", map(_pointer, out))
+    size = _norm_workspace(count)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    types = array.array("i", map(TYPES.__getitem__, dtypes))
+    args = (_address(ptrs), _address(sizes), _address(types), count, None if outs is None else _address(outs), max_norm,
+            norm.data_ptr(), ws.data_ptr(), size)
+    _on_device(index, "gafime_grad_norm", lib.gafime_grad_norm, args)
     return norm
 
 
@@ -230,14 +242,14 @@ def _norm_workspace(count: int) -> int:
 def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     """2-norm over all elements of the tensors together, a float32 scalar on their GPU.  The
     tensors are contiguous, float32, float16 or bfloat16 in any mix; squares are summed in fp64."""
-    return _grad_norm(tensors, None, 0.0)
+    return _grad_norm(list(tensors), None, 0.0)
 
 
 @torch.no_grad()
 def clip_grad_norm(tensors: Sequence[torch.Tensor], max_norm: float,
                    out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scale the tensors by min(1, max_norm / norm) of their norm together, in place or into
-    ``out`` (one contiguous tensor each, alike in shape and type, apart from one another and
+    ``out`` (one contiguous tensor each, alike in size and type, apart from one another and
     from the tensors), and return the norm before it.  A norm that is not finite leaves the
     values as they are: the caller sees it in the result and skips the step."""
     max_norm = float(max_norm)
