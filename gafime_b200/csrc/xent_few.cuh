@@ -135,16 +135,37 @@ __device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64
             }
         }
     } else {
-        // any strides: element by element, neighbouring lanes on neighbouring elements
+        // any strides: element by element, neighbouring lanes on neighbouring elements of a line (or
+        // of several short lines), eight loads under way
+        constexpr int E = COLS ? R : F, W = E < 32 ? E : 32;  // elements of a line, and of those at a time
+        constexpr int L = 32 / W;                             // lines at a time
         const int full = COLS ? R : (feats + V - 1) / V * V;
-        for (int l = 0; l < lines; ++l)
-            for (int e = lane; e < full; e += 32) {
-                if constexpr (sizeof(T) == 4) {
-                    copy4(dst + Geo::at(l, e), e < len ? x + l * ls + e * es : x, e < len ? 4 : 0);
-                } else {
-                    *reinterpret_cast<T*>(tile + Geo::at(l, e)) = e < len ? x[l * ls + e * es] : from_float<T>(0.f);
+        const int e0 = lane % W, l0 = lane / W;
+        for (int h = 0; h < E / W; ++h) {
+            const int e = e0 + h * W;
+            if (e >= full) break;
+            const bool in = e < len;
+            const T* src = x + l0 * ls + (in ? e * es : 0);
+            const int64_t hop = L * ls;
+            const int unit = e * (int)sizeof(T) >> 4, rest = e * (int)sizeof(T) & 15;
+            if constexpr (sizeof(T) == 4) {
+                #pragma unroll 8
+                for (int l = l0; l < lines; l += L, src += hop) copy4(dst + Geo::unit(l, unit) + rest, in ? src : x, in ? 4 : 0);
+            } else {
+                for (int l = l0; l < lines; l += 8 * L) {
+                    T v[8];
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        v[i] = from_float<T>(0.f);
+                        if (in && l + i * L < lines) v[i] = src[i * hop];
+                    }
+                    src += 8 * hop;
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (l + i * L < lines) *reinterpret_cast<T*>(tile + Geo::unit(l + i * L, unit) + rest) = v[i];
                 }
             }
+        }
     }
     if (!COLS && left < R) {
         // rows past the table: their lanes read them in step 1

@@ -31,6 +31,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <type_traits>
 
@@ -793,15 +794,37 @@ __global__ void __launch_bounds__(256) xent_colmax_kernel(const float* __restric
         if (k0 + i < d && top[i]) atomicMax(&colmax[k0 + i], top[i]);
 }
 
-// largest exponent of w_jk 2^-s_k
+// largest exponent of w_jk 2^-s_k: a block takes `rows` classes of 1024 features (kRows) or of 32
 __global__ void __launch_bounds__(256) xent_wmax_kernel(const float* __restrict__ w, int64_t wr, int64_t wk, int64_t c,
-                                                        int64_t d, const uint32_t* __restrict__ colmax, Meta* meta) {
+                                                        int64_t d, int64_t rows, int order,
+                                                        const uint32_t* __restrict__ colmax, Meta* meta) {
+    const int64_t width = order == kRows ? 1024 : 32, blocks_k = (d + width - 1) / width;
+    const int64_t k0 = (blockIdx.x % blocks_k) * width, r0 = (blockIdx.x / blocks_k) * rows, r1 = min(c, r0 + rows);
     int top = 0;
-    const int64_t all = c * d;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t j = wk == 1 ? i / d : i % c, k = wk == 1 ? i % d : i / c;
-        const uint32_t b = __float_as_uint(w[j * wr + k * wk]) & 0x7fffffffu;
-        if (b && b < 0x7f800000u) top = max(top, (int)(b >> 23) - 127 - fit_exponent(colmax[k]) + kExpBias);
+    auto exponent = [](float v, int s) {
+        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+        return b && b < 0x7f800000u ? (int)(b >> 23) - 127 - s + kExpBias : 0;
+    };
+    if (order == kRows) {
+        const int quads = (int)min((int64_t)256, (d - k0 + 3) / 4), at_once = 256 / quads;
+        const int quad = threadIdx.x % quads, ro = threadIdx.x / quads;
+        const int64_t k = k0 + 4 * quad;
+        int s[4];
+        for (int i = 0; i < 4; ++i) s[i] = k + i < d ? fit_exponent(colmax[k + i]) : 0;
+        if (ro < at_once)
+            #pragma unroll 8
+            for (int64_t r = r0 + ro; r < r1; r += at_once) {
+                const float4 v = load_quad(w + r * wr, k, d);
+                top = max(max(top, exponent(v.x, s[0])), exponent(v.y, s[1]));
+                top = max(max(top, exponent(v.z, s[2])), exponent(v.w, s[3]));
+            }
+    } else {
+        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+        if (k0 + tx < d) {
+            const int s = fit_exponent(colmax[k0 + tx]);
+            #pragma unroll 8
+            for (int64_t r = r0 + ty; r < r1; r += 8) top = max(top, exponent(w[r * wr + (k0 + tx) * wk], s));
+        }
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0 && top) atomicMax(&meta->w_exp, (uint32_t)top);
@@ -1203,13 +1226,20 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
 template <int MODE, int BN, typename E, int kPlanes>
 cudaError_t launch_bn(const TcArgs& t, int sms, cudaStream_t stream) {
     auto fn = xent_tc_kernel<MODE, BN, E, kPlanes>;
-    cudaError_t e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(BN));
+    static std::atomic<uint64_t> ready{0};   // devices on which the kernel has its shared memory
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    // the epilogues take their registers from the launch's: one that has fewer would wait for good
-    cudaFuncAttributes attr;
-    e = cudaFuncGetAttributes(&attr, (const void*)fn);
-    if (e != cudaSuccess) return e;
-    if (attr.numRegs * kThreads < 128 * kControlRegs + 256 * kEpiRegs) return cudaErrorLaunchOutOfResources;
+    if (dev >= 64 || !((ready.load(std::memory_order_relaxed) >> dev) & 1)) {
+        e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(BN));
+        if (e != cudaSuccess) return e;
+        // the epilogues take their registers from the launch's: one that has fewer would wait for good
+        cudaFuncAttributes attr;
+        e = cudaFuncGetAttributes(&attr, (const void*)fn);
+        if (e != cudaSuccess) return e;
+        if (attr.numRegs * kThreads < 128 * kControlRegs + 256 * kEpiRegs) return cudaErrorLaunchOutOfResources;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     KernelTimer kt(stream, GAFIME_KERNEL_XENT_TC);
     fn<<<2 * std::min(sms / 2, t.units), kThreads, smem_of(BN), stream>>>(t);
     return cudaGetLastError();
@@ -1294,9 +1324,12 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 (const float*)a.x, a.xr, a.xk, p.keep, a.n, a.d, rows, order, p.colmax);
             XENT_TRY(cudaGetLastError());
         }
+        const int order = rows_vector(a.w, a.wr, a.wk) ? kRows : kAny;
+        const int64_t blocks_k = cdiv(a.d, order == kRows ? 1024 : 32);
+        const int64_t rows = std::max<int64_t>(16, cdiv(a.c * blocks_k, 8 * sms));
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_wmax_kernel<<<(unsigned)std::min<int64_t>(8 * sms, cdiv(a.c * a.d, 1024)), 256, 0, st>>>(
-            (const float*)a.w, a.wr, a.wk, a.c, a.d, p.colmax, p.meta);
+        xent_wmax_kernel<<<(unsigned)(blocks_k * cdiv(a.c, rows)), 256, 0, st>>>(
+            (const float*)a.w, a.wr, a.wk, a.c, a.d, rows, order, p.colmax, p.meta);
         XENT_TRY(cudaGetLastError());
     }
     if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, p.keep, a.n, a.d, false, false, p.xh, p.xl, sms, st)));

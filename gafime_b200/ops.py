@@ -144,8 +144,7 @@ class _SoftmaxXent(torch.autograd.Function):
     def forward(ctx, x, w, labels, bias):
         n, d, c = x.shape[0], x.shape[1], w.shape[0]
         loss, lse = _call(x, w, labels, bias, n, d, c, 0)
-        # the values as computed here: the caller may write into the loss it gets
-        ctx.save_for_backward(x, w, labels, bias, loss.clone(), lse)
+        ctx.save_for_backward(x, w, labels, bias, loss, lse)
         return loss
 
     @staticmethod
