@@ -133,12 +133,11 @@ struct TcArgs {
     int dx_map;               // out[0] is valid; else element stores
     const float* undo;        // DX, DW in fp32: two factors a feature, undo_pitch apart
     int64_t undo_pitch;
-    float* dx_acc;            // DX: sums of earlier class pieces, [tile][BN][128]
     int first, last;          // DX: first / last class piece; DW: first / last row piece
-    float* dw_part;           // DW: [split][128-class tile][feature tile][BN][128]
-    int dw_direct;            // DW: one split, whose last piece goes to dx (dw) with out[0]
-    int64_t dw_split_stride;
-    int64_t dw_tile0;         // first tile of the class piece
+    float* sums;              // DX, DW: [split][128-row tile][feature tile][BN][128] of pieces and splits
+    int64_t split_stride;
+    int64_t tile0;            // DW: first tile of the class piece
+    int direct;               // one split, whose last piece leaves as dx or dw
     int cleaned;              // DW: b[1] is a copy of x without such rows, there when meta->poison is set
 };
 
@@ -199,9 +198,6 @@ __device__ __forceinline__ Unit unit_of(const TcArgs& a, int u) {
     } else if (MODE == G) {
         t.m = u % a.m_tiles;
         t.n = u / a.m_tiles;
-    } else if (MODE == DX) {
-        t.n = u % a.n_tiles;
-        t.m = u / a.n_tiles;
     } else {
         const int tiles = a.m_tiles * a.n_tiles, tile = u % tiles;
         t.split = u / tiles;
@@ -532,15 +528,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             if (cb + lane < a.ldg) a.bias_part[((int64_t)mt * 4 + quarter) * a.ldg + cb + lane] = c;
                         }
                     } else {
-                        // sums of earlier pieces: dx of class pieces, a place a unit; dw of row pieces
-                        float* keep = MODE == DX ? a.dx_acc + ((int64_t)(2 * u + rank) * BN + col) * kBM
-                                                 : a.dw_part + t.split * a.dw_split_stride +
-                                                       ((a.dw_tile0 + (int64_t)mt * a.n_tiles + n) * BN + col) * kBM;
-                        keep += quarter * 32 + lane;
+                        // sums of earlier pieces: dx of class pieces, dw of row pieces
+                        float* keep = a.sums + t.split * a.split_stride +
+                                      ((a.tile0 + (int64_t)mt * a.n_tiles + n) * BN + col) * kBM + quarter * 32 + lane;
                         if (!a.first)
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] += keep[j * kBM];
-                        if (!a.last || (MODE == DW && !a.dw_direct)) {
+                        if (!a.last || !a.direct) {
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) keep[j * kBM] = v[j];
                             continue;
@@ -1011,26 +1005,33 @@ __global__ void __launch_bounds__(256) xent_finish_kernel(int64_t c, int64_t d, 
         for (int64_t i = at; i < c * d; i += all) dw[i] = from_float<T>(NAN);
 }
 
-// dw from several splits' partial sums: a block makes 32 classes x 8 features, a warp a feature.
+// dw or dx from several splits' sums: a block makes 32 rows x 8 features, a warp a feature.  Rows
+// with a negative label (dx) are zero.
 template <typename T>
-__global__ void __launch_bounds__(256) xent_dw_kernel(const float* __restrict__ part, int splits, int64_t split_stride,
-                                                      int n_tiles, int bn, int c, int d, const float* __restrict__ undo,
-                                                      int64_t undo_pitch, int half_g, const Meta* __restrict__ meta,
-                                                      T* __restrict__ dw) {
+__global__ void __launch_bounds__(256) xent_sum_kernel(const float* __restrict__ sums, int splits, int64_t split_stride,
+                                                       int n_tiles, int bn, int64_t rows, int d,
+                                                       const float* __restrict__ undo, int64_t undo_pitch, int half_g,
+                                                       const Meta* __restrict__ meta, const int64_t* __restrict__ labels,
+                                                       T* __restrict__ out, int64_t out_row, int64_t out_col) {
     __shared__ float t[8][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int tiles_k = (d + 7) / 8;
-    const int k0 = (int)(blockIdx.x % tiles_k) * 8, c0 = (int)(blockIdx.x / tiles_k) * 32, k = k0 + ty;
-    if (k < d && c0 + tx < c) {
-        const float* p = part + (((int64_t)(c0 / kBM) * n_tiles + k / bn) * bn + k % bn) * kBM + c0 % kBM + tx;
+    const int k0 = (int)(blockIdx.x % tiles_k) * 8, k = k0 + ty;
+    const int64_t r0 = (int64_t)(blockIdx.x / tiles_k) * 32;
+    if (k < d && r0 + tx < rows) {
+        const float* p = sums + ((r0 / kBM * n_tiles + k / bn) * bn + k % bn) * kBM + r0 % kBM + tx;
         double v = 0.0;
         #pragma unroll 8
         for (int s = 0; s < splits; ++s) v += (double)p[s * split_stride];
-        t[ty][tx] = undo ? (float)v * undo[k] * undo[undo_pitch + k] : scale2((float)v, -g_exponent(meta, half_g));
+        float f = undo ? (float)v * undo[k] * undo[undo_pitch + k] : scale2((float)v, -g_exponent(meta, half_g));
+        if (labels && labels[r0 + tx] < 0) f = 0.f;
+        t[ty][tx] = f;
     }
     __syncthreads();
-    const int j = threadIdx.x >> 3, i = threadIdx.x & 7;
-    if (c0 + j < c && k0 + i < d) dw[(int64_t)(c0 + j) * d + k0 + i] = from_float<T>(t[i][j]);
+    // neighbouring threads on neighbouring elements of the output
+    const bool down = out_row == 1;
+    const int j = down ? tx : threadIdx.x >> 3, i = down ? ty : threadIdx.x & 7;
+    if (r0 + j < rows && k0 + i < d) out[(r0 + j) * out_row + (k0 + i) * out_col] = from_float<T>(t[i][j]);
 }
 
 // ---- host ------------------------------------------------------------------------------
@@ -1097,6 +1098,9 @@ struct Plan {
     int splits, per_split;           // LSE
     int64_t piece_rows, piece_classes, ldg;
     int64_t dx_d_tiles;              // of bn_dx features
+    int64_t dx_stride;               // floats of a split's sums
+    int dx_splits, dx_per_split;
+    bool dx_direct;                  // one split: dx leaves the products' kernel
     int64_t dw_c_tiles, dw_d_tiles;  // 128 classes x bn_dw features
     int64_t dw_stride;               // floats of a split's partial
     int dw_splits, dw_per_split;
@@ -1114,7 +1118,7 @@ struct Plan {
     float2* part;
     float* zy;
     float2* shift;
-    float* dx_acc;
+    float* dx_sums;
     float* undo;
     int64_t undo_pitch;
     float* dw_part;
@@ -1173,41 +1177,41 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
         p.ldg = up(p.piece_classes, 64);   // whole 128-byte lines: TMA boxes meet no line twice
         p.gh = cv.take<uint16_t>(p.piece_rows * p.ldg);
         if (p.planes == 2) p.gl = cv.take<uint16_t>(p.piece_rows * p.ldg);
-        // Feature tiles of 128 or 256 (a CTA's half is whole 64-value lines): the ones with the fewer
-        // rounds of the pairs, where a round of 128 takes about 0.6 of one of 256; dw's rows are split
-        // over pairs that its tiles leave idle, in runs of at least 4 blocks
-        double dx_cost = 1e300, dw_cost = 1e300;
-        const int64_t m_dx = cdiv(std::min(p.piece_rows, a.n), kPM), m_dw = cdiv(p.piece_classes, kPM);
-        const int64_t blocks = cdiv(std::min(a.n, p.piece_rows), kBK);
-        for (int bn : {256, 128}) {
-            if (bn == 256 && a.d <= 128) continue;
-            const int64_t nt = cdiv(a.d, bn);
-            const double tile = bn == 256 ? 1.0 : 0.6;
-            const double dx = cdiv(m_dx * nt, pairs) * tile;
-            if (dx < dx_cost) {
-                dx_cost = dx;
-                p.bn_dx = bn;
-            }
-            for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(pairs, blocks / 4)); ++s) {
-                const int64_t per = cdiv(blocks, s);
-                if (s > 1 && m_dw * nt * cdiv(blocks, per) > 2 * pairs) break;
-                const double dw = cdiv(m_dw * nt * cdiv(blocks, per), pairs) * (per + 4.0) * tile;
-                if (dw < dw_cost * 0.97) {
-                    dw_cost = dw;
-                    p.bn_dw = bn;
-                    p.dw_per_split = (int)per;
+        // Feature tiles of 128 or 256 (a CTA's half is whole 64-value lines), and the sum over classes
+        // (dx) or rows (dw) split over pairs that the tiles leave idle, in runs of at least 4 blocks:
+        // what takes the fewest rounds, where a block of 128 takes about 0.6 of one of 256
+        auto choose = [&](int64_t row_tiles, int64_t blocks, int& bn_out, int& per_out) {
+            double best = 1e300;
+            for (int bn : {256, 128}) {
+                if (bn == 256 && a.d <= 128) continue;
+                const int64_t tiles = row_tiles * cdiv(a.d, bn);
+                for (int64_t s = 1; s <= std::max<int64_t>(1, std::min<int64_t>(pairs, blocks / 4)); ++s) {
+                    const int64_t per = cdiv(blocks, s);
+                    if (s > 1 && tiles * cdiv(blocks, per) > 2 * pairs) break;
+                    const double cost = cdiv(tiles * cdiv(blocks, per), pairs) * (per + 4.0) * (bn == 256 ? 1.0 : 0.6);
+                    if (cost < best * 0.97) {
+                        best = cost;
+                        bn_out = bn;
+                        per_out = (int)per;
+                    }
                 }
             }
-        }
+        };
+        const int64_t rows_at_once = std::min(a.n, p.piece_rows), blocks = cdiv(rows_at_once, kBK);
+        const int64_t class_blocks = cdiv(p.piece_classes, kBK);
+        choose(cdiv(rows_at_once, kPM), class_blocks, p.bn_dx, p.dx_per_split);
+        choose(cdiv(p.piece_classes, kPM), blocks, p.bn_dw, p.dw_per_split);
+        p.dx_splits = (int)cdiv(class_blocks, p.dx_per_split);
+        p.dx_direct = p.dx_splits == 1;
         p.dw_splits = (int)cdiv(blocks, p.dw_per_split);
         p.dx_d_tiles = cdiv(a.d, p.bn_dx);
         p.dw_d_tiles = cdiv(a.d, p.bn_dw);
+        p.dx_stride = p.piece_rows * p.dx_d_tiles * p.bn_dx;
         p.dw_c_tiles = cdiv(a.c, kPM) * 2;
         p.dw_stride = p.dw_c_tiles * p.dw_d_tiles * p.bn_dw * kBM;
         p.undo_pitch = up(a.d, 256);
         if (p.planes == 2) p.undo = cv.take<float>(4 * p.undo_pitch);
-        if (a.dx && p.piece_classes < a.c)
-            p.dx_acc = cv.take<float>(p.piece_rows * p.dx_d_tiles * p.bn_dx);
+        if (a.dx && (!p.dx_direct || p.piece_classes < a.c)) p.dx_sums = cv.take<float>(p.dx_splits * p.dx_stride);
         if (a.dw) {
             p.dw_direct = p.dw_splits == 1;
             if (!p.dw_direct || a.n > p.piece_rows) p.dw_part = cv.take<float>(p.dw_splits * p.dw_stride);
@@ -1429,7 +1433,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 XENT_TRY(map(x.b, wp, a.d, classes, ldw, kBK));
                 x.m_tiles = (int)cdiv(rows, kPM);
                 x.n_tiles = (int)p.dx_d_tiles;
-                x.units = x.m_tiles * x.n_tiles;
+                x.units = x.m_tiles * x.n_tiles * p.dx_splits;
+                x.per_split = p.dx_per_split;
                 x.k_blocks = (int)cdiv(classes, kBK);
                 if (p.planes == 1) x.chunk = 16;
                 x.rows = rows;
@@ -1440,10 +1445,19 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 if (x.dx_map && !make_out_map(&x.out[0], a.type, a.dx, a.d, a.n, a.dxr)) return cudaErrorInvalidValue;
                 x.undo = p.undo;
                 x.undo_pitch = p.undo_pitch;
-                x.dx_acc = p.dx_acc;
+                x.sums = p.dx_sums;
+                x.split_stride = p.dx_stride;
+                x.direct = p.dx_direct;
                 x.first = c0 == 0;
                 x.last = c0 + classes == a.c;
                 XENT_TRY((launch<DX, E, kPlanes>(x, p.bn_dx, sms, st)));
+                if (x.last && !p.dx_direct) {
+                    KernelTimer kt(st, GAFIME_KERNEL_XENT);
+                    xent_sum_kernel<T><<<(unsigned)(cdiv(rows, 32) * cdiv(a.d, 8)), 256, 0, st>>>(
+                        p.dx_sums, p.dx_splits, p.dx_stride, (int)p.dx_d_tiles, p.bn_dx, rows, (int)a.d, p.undo, p.undo_pitch,
+                        !kBf16, p.meta, a.labels + r0, (T*)a.dx + r0 * a.dxr, a.dxr, a.dxk);
+                    XENT_TRY(cudaGetLastError());
+                }
             }
             if (a.dw) {
                 TcArgs w = t;
@@ -1461,10 +1475,10 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 w.cols = a.d;
                 w.first = r0 == 0;
                 w.last = r0 + rows == a.n;
-                w.dw_part = p.dw_part;
-                w.dw_split_stride = p.dw_stride;
-                w.dw_tile0 = c0 / kBM * p.dw_d_tiles;
-                w.dw_direct = p.dw_direct;
+                w.sums = p.dw_part;
+                w.split_stride = p.dw_stride;
+                w.tile0 = c0 / kBM * p.dw_d_tiles;
+                w.direct = p.dw_direct;
                 w.dx = a.dw;
                 w.dxr = a.d;
                 w.dxk = 1;
@@ -1480,9 +1494,9 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     }
     if (a.dw && !p.dw_direct) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_dw_kernel<T><<<(unsigned)(cdiv(a.c, 32) * cdiv(a.d, 8)), 256, 0, st>>>(
-            p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_dw, (int)a.c, (int)a.d,
-            p.undo ? p.undo + 2 * p.undo_pitch : nullptr, p.undo_pitch, !kBf16, p.meta, (T*)a.dw);
+        xent_sum_kernel<T><<<(unsigned)(cdiv(a.c, 32) * cdiv(a.d, 8)), 256, 0, st>>>(
+            p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_dw, a.c, (int)a.d,
+            p.undo ? p.undo + 2 * p.undo_pitch : nullptr, p.undo_pitch, !kBf16, p.meta, nullptr, (T*)a.dw, a.d, 1);
         XENT_TRY(cudaGetLastError());
     }
     if (a.dw || a.dbias) {
