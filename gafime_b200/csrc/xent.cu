@@ -271,7 +271,7 @@ FewPlan few_plan(const XentCall& a, int sms) {
     p.features = few_features(p.grad);
     k.d_pad = (d + p.features - 1) / p.features * p.features;
     const int64_t line_stride = p.cols ? a.xk : a.xr;
-    k.vec_ok = (p.cols ? a.xr == 1 : a.xk == 1) && (uintptr_t)a.x % 16 == 0 && line_stride >= 0 &&
+    p.vec = (p.cols ? a.xr == 1 : a.xk == 1) && (uintptr_t)a.x % 16 == 0 && line_stride >= 0 &&
                line_stride * es % 16 == 0;
     k.warps = p.grad ? k.d_pad / p.features : 1;
     k.groups = std::max(1, (p.grad ? 4 : 8) / k.warps);

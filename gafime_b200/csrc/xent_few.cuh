@@ -60,7 +60,6 @@ struct FewArgs {
     double* part_bias;   // [groups][c]
     int d_pad;           // features rounded up to whole tiles
     int rows, log_rows;  // of a tile: 8, 16 or 32
-    int vec_ok;          // 16-byte copies allowed
     int warps;           // W, side by side
     int groups;          // of W warps in a CTA
     int n_tiles;         // of rows
@@ -70,6 +69,7 @@ struct FewPlan {
     FewArgs k;
     int cp, grid, threads, features;
     bool cols, grad;
+    bool vec;            // 16-byte copies of x: unit stride, aligned lines
     size_t smem;
 };
 
@@ -104,9 +104,51 @@ struct Tile {
     }
 };
 
+// The same for any strides: element by element, neighbouring lanes on neighbouring elements of a
+// line (or of several short lines), eight loads under way.
+template <typename T, bool COLS, int R, int F>
+__device__ __forceinline__ void load_tile_any(const FewArgs& a, uint8_t* tile, int64_t r0, int k0, int lane) {
+    using Geo = Tile<T, COLS, R, F>;
+    constexpr int V = 16 / sizeof(T);
+    const int left = (int)min((int64_t)R, a.n - r0), feats = min(F, a.d - k0);
+    const T* x = (const T*)a.x + r0 * a.xr + (int64_t)k0 * a.xk;
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(tile);
+    const int lines = COLS ? feats : left, len = COLS ? left : feats;
+    const int64_t ls = COLS ? a.xk : a.xr, es = COLS ? a.xr : a.xk;
+    constexpr int E = COLS ? R : F, W = E < 32 ? E : 32;  // elements of a line, and of those at a time
+    constexpr int L = 32 / W;                             // lines at a time
+    const int full = COLS ? R : (feats + V - 1) / V * V;
+    const int e0 = lane % W, l0 = lane / W;
+    for (int h = 0; h < E / W; ++h) {
+        const int e = e0 + h * W;
+        if (e >= full) break;
+        const bool in = e < len;
+        const T* src = x + l0 * ls + (in ? e * es : 0);
+        const int64_t hop = L * ls;
+        const int unit = e * (int)sizeof(T) >> 4, rest = e * (int)sizeof(T) & 15;
+        if constexpr (sizeof(T) == 4) {
+            #pragma unroll 8
+            for (int l = l0; l < lines; l += L, src += hop) copy4(dst + Geo::unit(l, unit) + rest, in ? src : x, in ? 4 : 0);
+        } else {
+            for (int l = l0; l < lines; l += 8 * L) {
+                T v[8];
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    v[i] = from_float<T>(0.f);
+                    if (in && l + i * L < lines) v[i] = src[i * hop];
+                }
+                src += 8 * hop;
+                #pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (l + i * L < lines) *reinterpret_cast<T*>(tile + Geo::unit(l + i * L, unit) + rest) = v[i];
+            }
+        }
+    }
+}
+
 // Queue a warp's copies of rows [r0, r0 + R) x features [k0, k0 + 128).  Rows and features past
 // the table read zero in units that hold some of it; other units are never used.
-template <typename T, bool COLS, int R, int F>
+template <typename T, bool COLS, int R, int F, bool VEC>
 __device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64_t r0, int k0, int lane) {
     using Geo = Tile<T, COLS, R, F>;
     constexpr int V = 16 / sizeof(T), U = Geo::kUnits;
@@ -115,8 +157,8 @@ __device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64
     const T* x = (const T*)a.x + r0 * a.xr + (int64_t)k0 * a.xk;
     const uint32_t dst = (uint32_t)__cvta_generic_to_shared(tile);
     const int lines = COLS ? feats : left, len = COLS ? left : feats;
-    const int64_t ls = COLS ? a.xk : a.xr, es = COLS ? a.xr : a.xk;
-    if (a.vec_ok) {
+    const int64_t ls = COLS ? a.xk : a.xr;
+    if constexpr (VEC) {
         const int l0 = lane / U, q = lane % U;
         const int bytes = max(0, min(V, len - q * V)) * (int)sizeof(T);
         const T* src = x + l0 * ls + (bytes ? q * V : 0);
@@ -135,37 +177,7 @@ __device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64
             }
         }
     } else {
-        // any strides: element by element, neighbouring lanes on neighbouring elements of a line (or
-        // of several short lines), eight loads under way
-        constexpr int E = COLS ? R : F, W = E < 32 ? E : 32;  // elements of a line, and of those at a time
-        constexpr int L = 32 / W;                             // lines at a time
-        const int full = COLS ? R : (feats + V - 1) / V * V;
-        const int e0 = lane % W, l0 = lane / W;
-        for (int h = 0; h < E / W; ++h) {
-            const int e = e0 + h * W;
-            if (e >= full) break;
-            const bool in = e < len;
-            const T* src = x + l0 * ls + (in ? e * es : 0);
-            const int64_t hop = L * ls;
-            const int unit = e * (int)sizeof(T) >> 4, rest = e * (int)sizeof(T) & 15;
-            if constexpr (sizeof(T) == 4) {
-                #pragma unroll 8
-                for (int l = l0; l < lines; l += L, src += hop) copy4(dst + Geo::unit(l, unit) + rest, in ? src : x, in ? 4 : 0);
-            } else {
-                for (int l = l0; l < lines; l += 8 * L) {
-                    T v[8];
-                    #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        v[i] = from_float<T>(0.f);
-                        if (in && l + i * L < lines) v[i] = src[i * hop];
-                    }
-                    src += 8 * hop;
-                    #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (l + i * L < lines) *reinterpret_cast<T*>(tile + Geo::unit(l + i * L, unit) + rest) = v[i];
-                }
-            }
-        }
+        load_tile_any<T, COLS, R, F>(a, tile, r0, k0, lane);
     }
     if (!COLS && left < R) {
         // rows past the table: their lanes read them in step 1
@@ -271,14 +283,17 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
         #pragma unroll
         for (int c0 = 0; c0 < C; c0 += B) {
             float part[4][B];
-            Pair sum[2][B];
+            constexpr int Q = B <= 4 ? 2 : 1;   // sets of sums, of alternate lines: shorter chains
+            Pair sum[Q][2][B];
             #pragma unroll
-            for (int c = 0; c < B; ++c) sum[0][c] = sum[1][c] = 0;
+            for (int q = 0; q < Q; ++q)
+                #pragma unroll
+                for (int c = 0; c < B; ++c) sum[q][0][c] = sum[q][1][c] = 0;
             // lines share, share + S, ...: S a multiple of 4, so two exchanges in turn
             const uint8_t* p0 = tile + Geo::at(share, 4 * group);
             const uint8_t* p1 = tile + Geo::at(share + S, 4 * group);
             const float* wk = w + share * CL + c0;
-            auto line = [&](const uint8_t* p, const float* wl) {
+            auto line = [&](const uint8_t* p, const float* wl, Pair (&to)[2][B]) {
                 float xv[4], wv[B];
                 load4(xv, p, T{});
                 #pragma unroll
@@ -291,24 +306,35 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
                 #pragma unroll
                 for (int c = 0; c < B; ++c) {
                     const Pair ww = pair(wv[c], wv[c]);
-                    fma2(sum[0][c], a, ww);
-                    fma2(sum[1][c], b, ww);
+                    fma2(to[0][c], a, ww);
+                    fma2(to[1][c], b, ww);
                 }
             };
             int k = share;
-            #pragma unroll 2
+            #pragma unroll 4
             for (; k + S < feats; k += 2 * S) {
-                line(p0, wk);
-                line(p1, wk + S * CL);
+                line(p0, wk, sum[0]);
+                line(p1, wk + S * CL, sum[Q - 1]);
                 p0 += 2 * S * Geo::kLine;
                 p1 += 2 * S * Geo::kLine;
                 wk += 2 * S * CL;
             }
-            if (k < feats) line(p0, wk);
+            if (k < feats) line(p0, wk, sum[0]);
+            if constexpr (Q == 2) {
+                #pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    #pragma unroll
+                    for (int c = 0; c < B; ++c) {
+                        float l0, h0, l1, h1;
+                        unpair(l0, h0, sum[0][h][c]);
+                        unpair(l1, h1, sum[1][h][c]);
+                        sum[0][h][c] = pair(l0 + l1, h0 + h1);
+                    }
+            }
             #pragma unroll
             for (int c = 0; c < B; ++c) {
-                unpair(part[0][c], part[1][c], sum[0][c]);
-                unpair(part[2][c], part[3][c], sum[1][c]);
+                unpair(part[0][c], part[1][c], sum[0][0][c]);
+                unpair(part[2][c], part[3][c], sum[0][1][c]);
             }
             // the lane keeps row i = share & 3 of its four: the first two steps of the sum over the
             // lanes halve what is held, as in column_sums
@@ -372,58 +398,71 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
         // lines lane + 32 f exchange alike; four rows of a line at a time
         const uint8_t* line = tile + lane * Geo::kLine;
         const int x0 = ((lane >> Geo::kShift) & Geo::kMask) << 4;
-        constexpr int B = C <= 8 ? C : 8;                     // classes at a time: g of four rows in registers
-        #pragma unroll
-        for (int c0 = 0; c0 < C; c0 += B) {
-            #pragma unroll 2
-            for (int r = 0; r < R; r += 4) {
-                Pair g0[B], g1[B];
-                load_pairs<B>(g0, g + (r / 2 * CL + c0) * 2);
-                load_pairs<B>(g1, g + ((r / 2 + 1) * CL + c0) * 2);
-                const int b = r * (int)sizeof(T);
-                const uint8_t* p = line + (((b >> 4 << 4) ^ x0) + (b & 15));
-                #pragma unroll
-                for (int f = 0; f < F / 32; ++f) {
-                    if (32 * f >= feats) break;
-                    float xv[4];
-                    load4(xv, p + 32 * f * Geo::kLine, T{});
-                    if (bad)
-                        #pragma unroll
-                        for (int v = 0; v < 4; ++v)
-                            if ((bad >> (r + v)) & 1) xv[v] = 0.f;
-                    const Pair a = pair(xv[0], xv[1]), b2 = pair(xv[2], xv[3]);
+        constexpr int B = C <= 6 ? C : 4;                     // classes at a time
+        auto pass = [&](auto plain) {                         // plain: a whole tile of numbers, no checks
+            #pragma unroll
+            for (int c0 = 0; c0 < C; c0 += B) {
+                #pragma unroll 2
+                for (int r = 0; r < R; r += 4) {
+                    Pair g0[B], g1[B];
+                    load_pairs<B>(g0, g + (r / 2 * CL + c0) * 2);
+                    load_pairs<B>(g1, g + ((r / 2 + 1) * CL + c0) * 2);
+                    const int b = r * (int)sizeof(T);
+                    const uint8_t* p = line + (((b >> 4 << 4) ^ x0) + (b & 15));
                     #pragma unroll
-                    for (int c = 0; c < B; ++c) {
-                        fma2(acc[f][c0 + c], a, g0[c]);
-                        fma2(acc[f][c0 + c], b2, g1[c]);
+                    for (int f = 0; f < F / 32; ++f) {
+                        if (!plain() && 32 * f >= feats) break;
+                        float xv[4];
+                        load4(xv, p + 32 * f * Geo::kLine, T{});
+                        if (!plain())
+                            #pragma unroll
+                            for (int v = 0; v < 4; ++v)
+                                if ((bad >> (r + v)) & 1) xv[v] = 0.f;
+                        const Pair a = pair(xv[0], xv[1]), b2 = pair(xv[2], xv[3]);
+                        #pragma unroll
+                        for (int c = 0; c < B; ++c) {
+                            fma2(acc[f][c0 + c], a, g0[c]);
+                            fma2(acc[f][c0 + c], b2, g1[c]);
+                        }
                     }
                 }
             }
-        }
+        };
+        if (bad == 0 && feats == F)
+            pass([] { return true; });
+        else
+            pass([] { return false; });
     } else {
         constexpr int N = F / 32;                             // neighbouring features of a lane
         const int b = N * lane * (int)sizeof(T);
         const int own = (b >> 4) << 4;
         const uint8_t* p = tile + (b & 15);
-        #pragma unroll 8
-        for (int r = 0; r < R; ++r) {
-            if ((bad >> r) & 1) continue;
-            float xv[N];
-            Pair gv[C];
-            load_some(xv, p + r * Geo::kLine + (own ^ ((r & 7) << 4)), T{});
-            load_pairs<C>(gv, g + r * CL * 2);
-            #pragma unroll
-            for (int f = 0; f < N; f += 2) {
-                const Pair x = pair(xv[f], xv[f + 1]);
+        auto pass = [&](auto plain) {
+            #pragma unroll 8
+            for (int r = 0; r < R; ++r) {
+                if (!plain() && ((bad >> r) & 1)) continue;
+                float xv[N];
+                Pair gv[C];
+                load_some(xv, p + r * Geo::kLine + (own ^ ((r & 7) << 4)), T{});
+                load_pairs<C>(gv, g + r * CL * 2);
                 #pragma unroll
-                for (int c = 0; c < C; ++c) fma2(acc[f / 2][c], x, gv[c]);
+                for (int f = 0; f < N; f += 2) {
+                    const Pair x = pair(xv[f], xv[f + 1]);
+                    #pragma unroll
+                    for (int c = 0; c < C; ++c) fma2(acc[f / 2][c], x, gv[c]);
+                }
             }
-        }
+        };
+        if (bad == 0)
+            pass([] { return true; });
+        else
+            pass([] { return false; });
     }
 }
 
-// C: classes the code has room for (a.c of them exist); GRAD: dw and dbias wanted or dx
-template <typename T, int C, bool COLS, bool GRAD, bool DX, int F>
+// C: classes the code has room for (a.c of them exist); GRAD: dw, dbias or dx wanted; F: features of
+// a warp's tile; VEC: x in 16-byte copies (kernels of their own, for the registers)
+template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC>
 __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : 3) xent_few_kernel(const FewArgs a) {
     constexpr int CL = padded<C>(), NF = GRAD ? F / 32 : 1;   // NF: features a lane sums in step 3
     constexpr int NP = !GRAD ? 1 : COLS ? NF : NF / 2;         // its sums: pairs over rows, or over features
@@ -513,11 +552,11 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : 3) xent_few_kerne
     const int k_first = GRAD ? kw : 0, k_step = GRAD ? a.d_pad : F;
     auto load = [&](int64_t t, int k0) {
         if (R == 32)
-            load_tile<T, COLS, 32, F>(a, tile, t * R, k0, lane);
+            load_tile<T, COLS, 32, F, VEC>(a, tile, t * R, k0, lane);
         else if (R == 16)
-            load_tile<T, COLS, 16, F>(a, tile, t * R, k0, lane);
+            load_tile<T, COLS, 16, F, VEC>(a, tile, t * R, k0, lane);
         else
-            load_tile<T, COLS, 8, F>(a, tile, t * R, k0, lane);
+            load_tile<T, COLS, 8, F, VEC>(a, tile, t * R, k0, lane);
     };
     struct Meta {
         int64_t y;
@@ -677,9 +716,9 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : 3) xent_few_kerne
     }
 }
 
-template <typename T, int C, bool COLS, bool GRAD, bool DX, int F>
+template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC>
 cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
-    auto fn = xent_few_kernel<T, C, COLS, GRAD, DX, F>;
+    auto fn = xent_few_kernel<T, C, COLS, GRAD, DX, F, VEC>;
     const cudaError_t e =
         cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
     if (e != cudaSuccess) return e;
@@ -690,7 +729,8 @@ cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
 
 template <typename T, int C, bool COLS, bool GRAD, bool DX>
 cudaError_t launch(const FewPlan& p, cudaStream_t s) {
-    return launch_f<T, C, COLS, GRAD, DX, few_features(GRAD)>(p, s);
+    constexpr int F = few_features(GRAD);
+    return p.vec ? launch_f<T, C, COLS, GRAD, DX, F, true>(p, s) : launch_f<T, C, COLS, GRAD, DX, F, false>(p, s);
 }
 
 template <typename T, int C>
