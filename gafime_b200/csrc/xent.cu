@@ -283,9 +283,9 @@ FewPlan few_plan(const XentCall& a, int sms) {
                                 (p.grad && k.warps > 1 ? 2 * (size_t)warps * p.cp * 32 : 0)) +
                (p.grad ? sizeof(double) * k.groups * p.cp * 32 : 0);
     };
-    // CTAs an SM holds: registers allow 24 warps of 85 or 16 of 128
+    // CTAs an SM holds: registers allow 24 warps of 80 or 16 of 128
     auto resident = [&](int rows) {
-        return (int)std::min<size_t>((p.grad ? 16 : 24) / warps, (227 * 1024) / (smem(rows) + 1024));
+        return (int)std::min<size_t>((p.grad ? 16 : 8 * few_loss_ctas(p.cp)) / warps, (227 * 1024) / (smem(rows) + 1024));
     };
     // Rows of a tile: 32, half of that where fewer than ten warps an SM would be left, and fewer
     // still where SMs would be left without a tile

@@ -36,6 +36,8 @@ namespace gafime {
 constexpr int kFewMaxC = 16, kFewMaxGrad = 8;
 // Features of a warp's tile: 128 with gradients, 64 without (24 warps an SM in place of 12).
 constexpr int few_features(bool grad) { return grad ? 128 : 64; }
+// CTAs of eight warps that an SM holds without gradients, by registers.
+constexpr int few_loss_ctas(int c) { return c >= 6 ? 2 : 3; }
 constexpr int kRowsMost = 32;
 constexpr int kFlushRows = 256;
 
@@ -283,7 +285,7 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
         #pragma unroll
         for (int c0 = 0; c0 < C; c0 += B) {
             float part[4][B];
-            constexpr int Q = B <= 4 ? 2 : 1;   // sets of sums, of alternate lines: shorter chains
+            constexpr int Q = C <= 4 ? 2 : 1;   // sets of sums, of alternate lines: shorter chains
             Pair sum[Q][2][B];
             #pragma unroll
             for (int q = 0; q < Q; ++q)
@@ -398,7 +400,7 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
         // lines lane + 32 f exchange alike; four rows of a line at a time
         const uint8_t* line = tile + lane * Geo::kLine;
         const int x0 = ((lane >> Geo::kShift) & Geo::kMask) << 4;
-        constexpr int B = C <= 6 ? C : 4;                     // classes at a time
+        constexpr int B = C <= 8 ? C : 4;                     // classes at a time
         auto pass = [&](auto plain) {                         // plain: a whole tile of numbers, no checks
             #pragma unroll
             for (int c0 = 0; c0 < C; c0 += B) {
@@ -428,7 +430,8 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
                 }
             }
         };
-        if (bad == 0 && feats == F)
+        // (from five classes on two copies of the loop cost more in registers than the checks)
+        if (C <= 4 && bad == 0 && feats == F)
             pass([] { return true; });
         else
             pass([] { return false; });
@@ -463,7 +466,7 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
 // C: classes the code has room for (a.c of them exist); GRAD: dw, dbias or dx wanted; F: features of
 // a warp's tile; VEC: x in 16-byte copies (kernels of their own, for the registers)
 template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC>
-__global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : 3) xent_few_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C)) xent_few_kernel(const FewArgs a) {
     constexpr int CL = padded<C>(), NF = GRAD ? F / 32 : 1;   // NF: features a lane sums in step 3
     constexpr int NP = !GRAD ? 1 : COLS ? NF : NF / 2;         // its sums: pairs over rows, or over features
     constexpr int GL = COLS ? CL : 2 * CL;                     // floats of a row of g
