@@ -105,8 +105,9 @@ __device__ __forceinline__ void store_2d(const CUtensorMap* map, uint32_t src, i
 }
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // A warp's wait for lane 0's stores: their source may be written again / they are done.
+template <int N>   // all but the last N
 __device__ __forceinline__ void store_wait_read() {
-    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
     __syncwarp();
 }
 __device__ __forceinline__ void store_wait_all() {

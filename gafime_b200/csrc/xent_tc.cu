@@ -60,11 +60,16 @@ constexpr size_t kPieceBytes = (size_t)256 << 20;   // of g
 enum { LSE = 0, G = 1, DX = 2, DW = 3 };
 
 constexpr int stage_bytes(int bn) { return kABytes + bn / 2 * kBK * 2; }   // of one CTA
-constexpr int stages_of(int bn) { return bn == 256 ? 6 : 8; }
-// an epilogue warp's outgoing 32 x 32 block: fp32, or hi and lo in 16 bits
-constexpr int kOutBytes = 4096;
-constexpr size_t smem_of(int bn) { return (size_t)stages_of(bn) * stage_bytes(bn) + kEpiWarps * kOutBytes + 1024 + 256; }
-static_assert(smem_of(256) <= 232448 && smem_of(128) <= 232448 && smem_of(64) <= 232448, "shared memory per CTA");
+constexpr int stages_of(int bn, int out) { return bn == 256 ? (out > 4096 ? 5 : 6) : bn == 128 ? (out > 4096 ? 6 : 8) : 8; }
+// An epilogue warp's outgoing 32 x 32 blocks: two of one plane of g, or of hi and lo, in turn (a
+// store is read while the next block is made); one of dx or dw.
+constexpr int out_bytes(int mode, int planes) { return mode == 1 && planes == 2 ? 8192 : 4096; }
+constexpr size_t smem_of(int bn, int out) {
+    return (size_t)stages_of(bn, out) * stage_bytes(bn) + kEpiWarps * out + 1024 + 256;
+}
+static_assert(smem_of(256, 4096) <= 232448 && smem_of(128, 4096) <= 232448 && smem_of(64, 4096) <= 232448 &&
+                  smem_of(256, 8192) <= 232448 && smem_of(128, 8192) <= 232448 && smem_of(64, 8192) <= 232448,
+              "shared memory per CTA");
 
 // What the kernels of one call share on the device; cleared at its start.
 struct Meta {
@@ -239,7 +244,8 @@ __device__ __forceinline__ float pick(const float* v, int i) {
 // E: type of the operand planes; kPlanes: 1, or hi and lo of fp32
 template <int MODE, int BN, typename E, int kPlanes>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_constant__ TcArgs a) {
-    constexpr int S = stages_of(BN), kCols = BN / 2;   // ring stages; columns of an epilogue thread
+    constexpr int kOut = out_bytes(MODE, kPlanes);
+    constexpr int S = stages_of(BN, kOut), kCols = BN / 2;   // ring stages; columns of an epilogue thread
     constexpr bool kAMn = MODE == DW, kBMn = MODE == DX || MODE == DW;
     constexpr bool kBf16 = sizeof(E) == 2 && !std::is_same<E, __half>::value;
     constexpr uint32_t kId = tc::idesc(BN, kBf16, kAMn, kBMn);
@@ -247,7 +253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
     const uint32_t base = (tc::smem_addr(raw) + 1023) & ~1023u;
     uint8_t* gbase = raw + (base - tc::smem_addr(raw));
     const uint32_t outs = base + S * stage_bytes(BN);         // a multiple of 1024
-    const uint32_t bars = outs + kEpiWarps * kOutBytes;
+    const uint32_t bars = outs + kEpiWarps * kOut;
     const uint32_t full0 = bars, empty0 = bars + 8 * S, afull0 = bars + 16 * S, aempty0 = afull0 + 16,
                    drain = afull0 + 32, slot = afull0 + 40;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -388,9 +394,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-        const uint32_t out_addr = outs + (warp - 4) * kOutBytes;
+        const uint32_t out_addr = outs + (warp - 4) * kOut;
         uint8_t* out = gbase + (out_addr - base);
-        uint32_t acc = 0;
+        uint32_t acc = 0, turn = 0;
         bool ok = true;
         const int te = w_exponent(a.meta, a.scaled), ue = g_exponent(a.meta, a.half_g);
         const float f = pow2i(-te) * kLog2e;
@@ -471,15 +477,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     uint32_t hit = 0;
                     if (MODE == LSE || MODE == G) hit = __ballot_sync(0xffffffffu, here);
                     if (MODE == LSE) {
-                        float m = top;
-                        #pragma unroll
-                        for (int j = 0; j < 32; ++j) m = fmaxf(m, v[j]);
-                        const float shift = m == -INFINITY ? 0.f : m;   // nothing but excluded classes so far
-                        float s = 0.f;
-                        #pragma unroll
-                        for (int j = 0; j < 32; ++j) s += exp2_fast(v[j] - shift);
-                        sum = sum * exp2_fast(top - shift) + s;
-                        top = m;
                         if (hit) {
                             const float q = pick(v, (int)rel & 31);
                             if (here) zy = q;
@@ -490,9 +487,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             const float p = exp2_fast(v[j] - sh.x) * ws;
                             v[j] = y >= 0 ? p : 0.f;
                         }
-                        tc::store_wait_read();       // the block's last store has read it
-                        out_write<E>(out, lane, v);
-                        if (here) *out_at<E>(out, lane, (int)rel) = from_float<E>(gy);
+                        uint8_t* blk = out + turn * (2048 * kPlanes);
+                        const uint32_t blk_addr = out_addr + turn * (2048 * kPlanes);
+                        turn ^= 1;
+                        tc::store_wait_read<1>();    // the block's last store has read it
+                        out_write<E>(blk, lane, v);
+                        if (here) *out_at<E>(blk, lane, (int)rel) = from_float<E>(gy);
                         if (kPlanes == 2) {
                             #pragma unroll
                             for (int j = 0; j < 32; j += 8) {
@@ -503,16 +503,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                                     const float h1 = to_float(from_float<E>(v[j + 2 * i + 1]));
                                     q[i] = pack(v[j + 2 * i] - h0, v[j + 2 * i + 1] - h1, E{});
                                 }
-                                *reinterpret_cast<uint4*>(out + 2048 + out_unit<E>(lane, j / 8)) =
+                                *reinterpret_cast<uint4*>(blk + 2048 + out_unit<E>(lane, j / 8)) =
                                     make_uint4(q[0], q[1], q[2], q[3]);
                             }
-                            if (here) *out_at<E>(out + 2048, lane, (int)rel) = from_float<E>(gy - to_float(from_float<E>(gy)));
+                            if (here) *out_at<E>(blk + 2048, lane, (int)rel) = from_float<E>(gy - to_float(from_float<E>(gy)));
                         }
                         tc::fence_async_smem();
                         __syncwarp();
                         if (lane == 0 && y0 < a.rows) {
-                            tc::store_2d(&a.out[0], out_addr, (int)cb, (int)y0);
-                            if (kPlanes == 2) tc::store_2d(&a.out[1], out_addr + 2048, (int)cb, (int)y0);
+                            tc::store_2d(&a.out[0], blk_addr, (int)cb, (int)y0);
+                            if (kPlanes == 2) tc::store_2d(&a.out[1], blk_addr + 2048, (int)cb, (int)y0);
                             tc::store_commit();
                         }
                         if (a.bias_part) {
@@ -568,7 +568,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                                 for (int j = 0; j < 32; ++j)
                                     if (j < count) dx[lane + j * a.dxk] = from_float<D>(v[j]);
                         } else {
-                            tc::store_wait_read();
+                            tc::store_wait_read<0>();
                             out_write<D>(out, lane, v);
                             if (a.dx_map) {
                                 tc::fence_async_smem();
@@ -588,6 +588,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             }
                         }
                     }
+                }
+                if (MODE == LSE) {
+                    // columns past the classes hold -inf from their bias (or, a whole block past them, are cut)
+                    const int blocks = (int)min((int64_t)(kCols / 32), max((int64_t)0, (a.cols - (int64_t)n * BN - half * kCols + 31) / 32));
+                    float m4[4] = {top, top, top, top};
+                    #pragma unroll
+                    for (int ch = 0; ch < kCols / 32; ++ch)
+                        if (ch < blocks)
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], sums[ch * 32 + j]);
+                    const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    const float shift = m == -INFINITY ? 0.f : m;   // nothing but excluded classes so far
+                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                    #pragma unroll
+                    for (int ch = 0; ch < kCols / 32; ++ch)
+                        if (ch < blocks)
+                            #pragma unroll
+                            for (int j = 0; j < 32; ++j) s4[j & 3] += exp2_fast(sums[ch * 32 + j] - shift);
+                    sum = sum * exp2_fast(top - shift) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+                    top = m;
                 }
             }
             if (MODE == LSE && valid) {
@@ -1235,7 +1255,7 @@ cudaError_t launch_bn(const TcArgs& t, int sms, cudaStream_t stream) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !((ready.load(std::memory_order_relaxed) >> dev) & 1)) {
-        e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(BN));
+        e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(BN, out_bytes(MODE, kPlanes)));
         if (e != cudaSuccess) return e;
         // the epilogues take their registers from the launch's: one that has fewer would wait for good
         cudaFuncAttributes attr;
@@ -1245,7 +1265,7 @@ cudaError_t launch_bn(const TcArgs& t, int sms, cudaStream_t stream) {
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     KernelTimer kt(stream, GAFIME_KERNEL_XENT_TC);
-    fn<<<2 * std::min(sms / 2, t.units), kThreads, smem_of(BN), stream>>>(t);
+    fn<<<2 * std::min(sms / 2, t.units), kThreads, smem_of(BN, out_bytes(MODE, kPlanes)), stream>>>(t);
     return cudaGetLastError();
 }
 template <int MODE, typename E, int kPlanes>
