@@ -62,6 +62,19 @@ cudaError_t xent_few(const XentCall& a, int sms);
 size_t xent_tc_workspace(const XentCall& a, int sms);
 cudaError_t xent_tc(const XentCall& a, int sms);
 
+// Packed pairs of floats: one instruction works on both (f32x2).
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ void unpair(float& lo, float& hi, Pair p) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
 template <typename T>
 __device__ __forceinline__ float to_float(T v) {
     return (float)v;

@@ -188,16 +188,6 @@ __device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64
     }
 }
 
-// Packed pairs of floats: one instruction multiplies and adds both (fma.rn.f32x2).
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float lo, float hi) {
-    Pair p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
-    return p;
-}
-__device__ __forceinline__ void unpair(float& lo, float& hi, Pair p) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
-__device__ __forceinline__ void fma2(Pair& d, Pair a, Pair b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b)); }
-
 // Classes of a line in shared memory, padded so that C pairs are whole 16-byte units.
 template <int C>
 constexpr int padded() { return (C + 1) / 2 * 2; }
@@ -308,8 +298,8 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
                 #pragma unroll
                 for (int c = 0; c < B; ++c) {
                     const Pair ww = pair(wv[c], wv[c]);
-                    fma2(to[0][c], a, ww);
-                    fma2(to[1][c], b, ww);
+                    to[0][c] = fma2(a, ww, to[0][c]);
+                    to[1][c] = fma2(b, ww, to[1][c]);
                 }
             };
             int k = share;
@@ -371,7 +361,7 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
                     const Pair x = pair(xv[v], xv[v + 1]);
                     load_pairs<C>(wv, w + (q * V + 4 * h + v) * CL);
                     #pragma unroll
-                    for (int c = 0; c < C; ++c) fma2(sum[c], x, wv[c]);
+                    for (int c = 0; c < C; ++c) sum[c] = fma2(x, wv[c], sum[c]);
                 }
             }
         }
@@ -423,8 +413,8 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
                         const Pair a = pair(xv[0], xv[1]), b2 = pair(xv[2], xv[3]);
                         #pragma unroll
                         for (int c = 0; c < B; ++c) {
-                            fma2(acc[f][c0 + c], a, g0[c]);
-                            fma2(acc[f][c0 + c], b2, g1[c]);
+                            acc[f][c0 + c] = fma2(a, g0[c], acc[f][c0 + c]);
+                            acc[f][c0 + c] = fma2(b2, g1[c], acc[f][c0 + c]);
                         }
                     }
                 }
@@ -452,7 +442,7 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
                 for (int f = 0; f < N; f += 2) {
                     const Pair x = pair(xv[f], xv[f + 1]);
                     #pragma unroll
-                    for (int c = 0; c < C; ++c) fma2(acc[f / 2][c], x, gv[c]);
+                    for (int c = 0; c < C; ++c) acc[f / 2][c] = fma2(x, gv[c], acc[f / 2][c]);
                 }
             }
         };
