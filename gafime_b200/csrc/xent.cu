@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(1024) xent_few_sum_kernel(const float* __restr
 constexpr int kRowsFew = 8;
 constexpr int64_t kRowsFewValues = 12288;   // of x, fp32 in shared memory
 constexpr int kRowsThreads = 256;
+constexpr int rows_ctas(int64_t n) { return n <= 1 ? 3 : 2; }   // an SM holds, by registers
 
 // 16 bytes of w, or one value where its rows are not made of them
 template <typename T, bool VEC>
@@ -107,7 +108,7 @@ struct RowsArgs {
 // N rows; x in shared memory as [units][N][values of a unit], zero past the features.  J classes
 // at a time keep as many loads under way.
 template <typename T, int N, bool VEC>
-__global__ void __launch_bounds__(kRowsThreads) xent_rows_kernel(const RowsArgs a) {
+__global__ void __launch_bounds__(kRowsThreads, rows_ctas(N)) xent_rows_kernel(const RowsArgs a) {
     constexpr int V = WLoad<T, VEC>::kCount, J = N <= 2 ? 4 : N <= 4 ? 2 : 1;
     extern __shared__ __align__(16) float xs[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -217,7 +218,7 @@ bool rows_fit(const XentCall& a) {
     return !a.gradient && a.n >= 1 && a.n <= kRowsFew && a.n * a.d <= kRowsFewValues && a.c >= 32;
 }
 int rows_grid(const XentCall& a, int sms) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>(4 * sms, (a.c + 8 * 4 - 1) / (8 * 4)));   // four classes a warp
+    return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)rows_ctas(a.n) * sms, (a.c + 8 * 4 - 1) / (8 * 4)));   // four classes a warp
 }
 size_t rows_carve(const XentCall& a, int sms, uint8_t* ws, float2*& part, float*& zy) {
     Carver cv(ws);

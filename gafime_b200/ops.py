@@ -186,9 +186,7 @@ def softmax_xent_grad(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, bi
     and need_dx=False that is one pass over x.  The gradient of a bias that is None is None.
     Arguments as softmax_xent; row_weight (n,) float32, None for ones."""
     n, d, c = _check(x, w, labels, bias, row_weight)
-    with torch.no_grad():
-        return _gradients(x.detach(), w.detach(), labels, bias, n, d, c, row_weight, float(scale), need_dx, need_dw,
-                          bias is not None)
+    return _gradients(x, w, labels, bias, n, d, c, row_weight, float(scale), need_dx, need_dw, bias is not None)
 
 
 def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
