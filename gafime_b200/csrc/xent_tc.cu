@@ -61,8 +61,8 @@ enum { LSE = 0, G = 1, DX = 2, DW = 3 };
 
 constexpr int stage_bytes(int bn) { return kABytes + bn / 2 * kBK * 2; }   // of one CTA
 constexpr int stages_of(int bn, int out) { return bn == 256 ? (out > 4096 ? 5 : 6) : bn == 128 ? (out > 4096 ? 6 : 8) : 8; }
-// An epilogue warp's outgoing 32 x 32 blocks: two of one plane of g, or of hi and lo, in turn (a
-// store is read while the next block is made); one of dx or dw.
+// An epilogue warp's outgoing blocks: 32 rows x 128 bytes of each plane of g (64 bytes where a tile
+// has 64 columns), or of dx or dw (64 bytes in 16 bits).
 constexpr int out_bytes(int mode, int planes) { return mode == 1 && planes == 2 ? 8192 : 4096; }
 constexpr size_t smem_of(int bn, int out) {
     return (size_t)stages_of(bn, out) * stage_bytes(bn) + kEpiWarps * out + 1024 + 256;
@@ -176,6 +176,11 @@ __device__ __forceinline__ void out_write(uint8_t* block, int row, const float* 
                            pack(v[8 * q + 4], v[8 * q + 5], T{}), pack(v[8 * q + 6], v[8 * q + 7], T{}));
         *reinterpret_cast<uint4*>(block + out_unit<T>(row, q)) = u;
     }
+}
+// the same of g's blocks, SPAN x 32 columns of 16 bits
+template <int SPAN>
+__device__ __forceinline__ int g_unit(int row, int q) {
+    return SPAN == 2 ? row * 128 + ((q ^ (row & 7)) << 4) : row * 64 + ((q ^ ((row >> 1) & 3)) << 4);
 }
 template <typename T>
 __device__ __forceinline__ T* out_at(uint8_t* block, int row, int col) {
@@ -396,7 +401,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const uint32_t out_addr = outs + (warp - 4) * kOut;
         uint8_t* out = gbase + (out_addr - base);
-        uint32_t acc = 0, turn = 0;
+        uint32_t acc = 0;
         bool ok = true;
         const int te = w_exponent(a.meta, a.scaled), ue = g_exponent(a.meta, a.half_g);
         const float f = pow2i(-te) * kLog2e;
@@ -487,33 +492,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             const float p = exp2_fast(v[j] - sh.x) * ws;
                             v[j] = y >= 0 ? p : 0.f;
                         }
-                        uint8_t* blk = out + turn * (2048 * kPlanes);
-                        const uint32_t blk_addr = out_addr + turn * (2048 * kPlanes);
-                        turn ^= 1;
-                        tc::store_wait_read<1>();    // the block's last store has read it
-                        out_write<E>(blk, lane, v);
-                        if (here) *out_at<E>(blk, lane, (int)rel) = from_float<E>(gy);
-                        if (kPlanes == 2) {
-                            #pragma unroll
-                            for (int j = 0; j < 32; j += 8) {
-                                uint32_t q[4];
+                        // 64 columns a store where the thread has as many: whole 128-byte lines
+                        constexpr int kSpan = kCols >= 64 ? 2 : 1;       // blocks of 32 columns in one
+                        constexpr int kPlane = 2048 * kSpan;
+                        const int q0 = (ch % kSpan) * 4;
+                        if (q0 == 0) tc::store_wait_read<0>();          // the last store has read them
+                        #pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            *reinterpret_cast<uint4*>(out + g_unit<kSpan>(lane, q0 + q)) =
+                                make_uint4(pack(v[8 * q], v[8 * q + 1], E{}), pack(v[8 * q + 2], v[8 * q + 3], E{}),
+                                           pack(v[8 * q + 4], v[8 * q + 5], E{}), pack(v[8 * q + 6], v[8 * q + 7], E{}));
+                            if (kPlanes == 2) {
+                                uint32_t r[4];
                                 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
-                                    const float h0 = to_float(from_float<E>(v[j + 2 * i]));
-                                    const float h1 = to_float(from_float<E>(v[j + 2 * i + 1]));
-                                    q[i] = pack(v[j + 2 * i] - h0, v[j + 2 * i + 1] - h1, E{});
+                                    const float h0 = to_float(from_float<E>(v[8 * q + 2 * i]));
+                                    const float h1 = to_float(from_float<E>(v[8 * q + 2 * i + 1]));
+                                    r[i] = pack(v[8 * q + 2 * i] - h0, v[8 * q + 2 * i + 1] - h1, E{});
                                 }
-                                *reinterpret_cast<uint4*>(blk + 2048 + out_unit<E>(lane, j / 8)) =
-                                    make_uint4(q[0], q[1], q[2], q[3]);
+                                *reinterpret_cast<uint4*>(out + kPlane + g_unit<kSpan>(lane, q0 + q)) =
+                                    make_uint4(r[0], r[1], r[2], r[3]);
                             }
-                            if (here) *out_at<E>(blk + 2048, lane, (int)rel) = from_float<E>(gy - to_float(from_float<E>(gy)));
                         }
-                        tc::fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0 && y0 < a.rows) {
-                            tc::store_2d(&a.out[0], blk_addr, (int)cb, (int)y0);
-                            if (kPlanes == 2) tc::store_2d(&a.out[1], blk_addr + 2048, (int)cb, (int)y0);
-                            tc::store_commit();
+                        if (here) {
+                            E* p = reinterpret_cast<E*>(out + g_unit<kSpan>(lane, q0 + (int)rel / 8)) + rel % 8;
+                            *p = from_float<E>(gy);
+                            if (kPlanes == 2) p[kPlane / 2] = from_float<E>(gy - to_float(from_float<E>(gy)));
+                        }
+                        // (past the last class the second block holds what it held: nobody reads there)
+                        if (ch % kSpan == kSpan - 1 || cb + 32 >= a.cols) {
+                            tc::fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && y0 < a.rows) {
+                                tc::store_2d(&a.out[0], out_addr, (int)cb - 8 * q0, (int)y0);
+                                if (kPlanes == 2) tc::store_2d(&a.out[1], out_addr + kPlane, (int)cb - 8 * q0, (int)y0);
+                                tc::store_commit();
+                            }
                         }
                         if (a.bias_part) {
                             // the bias's gradient from g before its rounding: 32 rows' sums a column
@@ -1069,21 +1083,21 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return fn;
 }
 
-// rows of `inner` values, `ld` apart, written in blocks of 32 x 32
-bool make_out_map(CUtensorMap* map, int type, const void* base, int64_t inner, int64_t rows, int64_t ld) {
+// rows of `inner` values, `ld` apart, written in blocks of 32 rows x `cols`
+bool make_out_map(CUtensorMap* map, int type, const void* base, int64_t inner, int64_t rows, int64_t ld, int cols = 32) {
     auto enc = encoder();
     if (!enc) return false;
     const bool wide = type == GAFIME_TYPE_FP32;
     cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld * (wide ? 4 : 2)};
-    cuuint32_t box[2] = {32, 32};
+    cuuint32_t box[2] = {(cuuint32_t)cols, 32};
     cuuint32_t estr[2] = {1, 1};
     return enc(map,
                wide                          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                : type == GAFIME_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               wide ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               cols * (wide ? 4 : 2) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1432,7 +1446,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             g.shift = p.shift;
             g.loss = a.loss;
             for (int i = 0; i < p.planes; ++i)
-                if (!make_out_map(&g.out[i], kBf16 ? GAFIME_TYPE_BF16 : GAFIME_TYPE_FP16, gs[i], p.ldg, rows, p.ldg))
+                if (!make_out_map(&g.out[i], kBf16 ? GAFIME_TYPE_BF16 : GAFIME_TYPE_FP16, gs[i], p.ldg, rows, p.ldg,
+                                  p.bn_c >= 128 ? 64 : 32))
                     return cudaErrorInvalidValue;
             g.ldg = p.ldg;
             g.bias_part = a.dbias ? p.bias_sums : nullptr;
