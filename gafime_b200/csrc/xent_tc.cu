@@ -1,6 +1,6 @@
 // xent_tc.cu -- softmax cross entropy of a linear head with many classes, on the tensor cores.
 //
-// The n x c logits never exist as a whole.  A forward call forms 128 x BN tiles of them in tensor
+// The n x c logits never exist as a whole.  A forward call forms 256 x BN tiles of them in tensor
 // memory and keeps, per row, the running maximum and sum of exponentials.  A gradient call forms
 // them again piece by piece (kPieceBytes at a time), writes a piece's
 //   g_ij = r_i (exp(z_ij - lse_i) - [j = y(i)])
@@ -24,6 +24,18 @@
 // pair's first CTA issues the MMAs into one of two tensor-memory accumulators; warps 4-11 turn
 // the other accumulator's 128 rows of their CTA into sums, g, dx or dw.  Every mbarrier wait is
 // bounded; one that gives up records a code, and the call's losses and gradients of w become NaN.
+//
+// What bounds it, measured on a B200 (1,645 TFLOP/s bf16 in a burst, 1,381 sustained under the
+// power cap):
+//   16 bits, 8192 x 1024, 32768 classes (0.55 TFLOP a product): lse 0.41 ms, g 0.47, dx 0.45, dw
+//     0.45 = 1,150 to 1,340 TFLOP/s, 83 to 97 % of the sustained rate.  With the MMAs left out the
+//     loads alone take 0.29 ms; g adds its exponentials, packing, stores and column sums.
+//   fp32, 200000 x 256, 1000 classes (3 products of 0.10 TFLOP): lse 0.26 ms, g 0.45, dx 0.32, dw
+//     0.30 = 680 to 1,200 TFLOP/s of 16-bit products.  The drains of tensor memory every two blocks
+//     and the epilogues bound it: without its epilogue's arithmetic g takes 0.24 ms.
+// Pairs of CTAs against single ones of 128 x 256: lse 0.54 -> 0.41 ms together with even runs of
+// class tiles, dw 0.47 -> 0.45.  Pieces of 256 MB against 128: 0.62 -> 0.32 ms for dx in fp32,
+// together with tabled scales (one round of the pairs to a launch exposes its start and end).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -55,7 +67,7 @@ constexpr int kBK = 64;                      // 16-bit values of K to a stage
 constexpr int kABytes = kBM * kBK * 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr size_t kPieceBytes = (size_t)256 << 20;   // of g
+constexpr size_t kPieceBytes = (size_t)256 << 20;   // of g: several rounds of the pairs, not the n x c whole
 
 enum { LSE = 0, G = 1, DX = 2, DW = 3 };
 

@@ -440,7 +440,8 @@ int gafime_contiguous_bucket_mark_updated(ContiguousBucket bucket);
  * of the current device without waiting, and allocate nothing: scratch memory is the caller's
  * workspace, which belongs to the call until the stream has passed it (two calls that may
  * overlap need two).  They can be captured into a CUDA graph.  Bad arguments return
- * GAFIME_ERROR_INVALID_ARGS before any work.
+ * GAFIME_ERROR_INVALID_ARGS before any work: sizes, NULL where a buffer is needed, pointers off
+ * their elements' boundaries, negative strides, a workspace too small or misaligned.
  */
 #define GAFIME_TYPE_FP32 0
 #define GAFIME_TYPE_FP16 1
@@ -481,7 +482,8 @@ int gafime_xent_forward(int type, const void* d_x, int64_t x_row, int64_t x_col,
  * have_lse = 0: computes d_loss and (unless NULL) d_lse as gafime_xent_forward does; with few
  * classes the loss, dw and dbias take one pass over x.  have_lse = 1: d_loss and d_lse are those
  * of a forward call on the same inputs and are only read.
- * The outputs may not overlap the inputs.
+ * The outputs may not overlap the inputs; dx of rows left out is zero.  A kernel whose bounded
+ * waits gave up leaves NaN in every loss (have_lse = 0) and in dw.
  */
 int gafime_xent_gradient(int type, const void* d_x, int64_t x_row, int64_t x_col, const void* d_w, int64_t w_row,
                          int64_t w_col, const float* d_bias, const int64_t* d_labels, int64_t n, int64_t d, int64_t c,

@@ -68,6 +68,21 @@ def test_entry_points_refuse_bad_arguments(lib):
         assert gradient(lib, ws=None) == -1 and gradient(lib, ws=WS + 16, size=1 << 30) == -1
 
 
+def test_pointers_and_strides_are_checked(lib):
+    """Off an element's boundary, negative, or two elements of dx in one place: refused before any work."""
+    def call(x=X, xs=(40, 1), w=W, ws=(40, 1), bias=None, labels=L, weight=None, wstride=0, loss=OUT, lse=OUT + 4096,
+             dx=OUT + 8192, dxs=(40, 1), dw=OUT + 65536, dbias=None):
+        return lib.gafime_xent_gradient(0, x, *xs, w, *ws, bias, labels, 100, 40, 300, weight, wstride, 1.0, 0, loss, lse,
+                                        dx, *dxs, dw, dbias, WS, 0, None)
+    good = -1 if lib.gafime_cuda_available() == 1 else -2      # (no workspace is given)
+    assert call() == good
+    for bad in (dict(x=X + 2), dict(w=W + 1), dict(bias=OUT + 2), dict(labels=L + 4), dict(weight=OUT + 1),
+                dict(loss=OUT + 2), dict(lse=OUT + 1), dict(dx=OUT + 3), dict(dw=OUT + 2), dict(dbias=OUT + 2),
+                dict(xs=(-40, 1)), dict(xs=(40, -1)), dict(ws=(-1, 1)), dict(ws=(40, -1)), dict(weight=OUT, wstride=-1),
+                dict(dxs=(0, 1)), dict(dxs=(40, 0)), dict(dxs=(1, 1)), dict(dxs=(-40, 1))):
+        assert call(**bad) == -1, bad
+
+
 def norm(lib, tensors=(X, W), sizes=(10, 20), types=(0, 1), outs=None, max_norm=1.0, out=OUT, ws=WS, size=1 << 20, n=None):
     count = len(tensors) if n is None else n
     p = (ctypes.c_void_p * len(tensors))(*tensors)
@@ -79,7 +94,7 @@ def norm(lib, tensors=(X, W), sizes=(10, 20), types=(0, 1), outs=None, max_norm=
 
 def test_norm_refuses_bad_arguments(lib):
     bad = [dict(sizes=(10, -1)), dict(types=(0, 3)), dict(tensors=(X, None)), dict(tensors=(X + 2, W)),
-           dict(out=None), dict(ws=None), dict(ws=WS + 8), dict(size=8), dict(n=-1), dict(outs=(X, None)),
+           dict(out=None), dict(out=OUT + 2), dict(ws=None), dict(ws=WS + 8), dict(size=8), dict(n=-1), dict(outs=(X, None)),
            dict(outs=(X, W + 1)), dict(outs=(X, W), max_norm=-1.0), dict(outs=(X, W), max_norm=float("nan")),
            dict(outs=(X, W), max_norm=float("inf")),
            dict(outs=(X, X + 4)),                                   # written twice
