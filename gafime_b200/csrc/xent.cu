@@ -270,7 +270,7 @@ FewPlan few_plan(const XentCall& a, int sms) {
     k.weight = a.weight; k.weight_stride = a.weight_stride; k.scale = a.scale;
     k.have_lse = a.have_lse;
     k.loss = a.loss; k.lse = a.lse; k.dx = a.dx; k.dxr = a.dxr; k.dxk = a.dxk;
-    p.features = few_features(p.grad);
+    p.features = few_features(p.grad, d <= 64);
     k.d_pad = (d + p.features - 1) / p.features * p.features;
     const int64_t line_stride = p.cols ? a.xk : a.xr;
     p.vec = (p.cols ? a.xr == 1 : a.xk == 1) && (uintptr_t)a.x % 16 == 0 && line_stride >= 0 &&
@@ -285,15 +285,17 @@ FewPlan few_plan(const XentCall& a, int sms) {
                                 (p.grad && k.warps > 1 ? 2 * (size_t)warps * p.cp * 32 : 0)) +
                (p.grad ? sizeof(double) * k.groups * p.cp * 32 : 0);
     };
-    // CTAs an SM holds: registers allow 24 warps of 80 or 16 of 128
+    // CTAs an SM holds
     auto resident = [&](int rows) {
-        return (int)std::min<size_t>((p.grad ? 16 : 8 * few_loss_ctas(p.cp)) / warps, (227 * 1024) / (smem(rows) + 1024));
+        return (int)std::min<size_t>(few_warps(p.cp, p.features, p.grad) / warps, (227 * 1024) / (smem(rows) + 1024));
     };
     // Rows of a tile: 32, half of that where fewer than ten warps an SM would be left, and fewer
     // still where SMs would be left without a tile
     int rows = kRowsMost;
     if (resident(rows) * warps < 10 && resident(16) * warps > resident(rows) * warps) rows = 16;
     while (rows > 8 && ((a.n + rows - 1) / rows < 4 * sms || resident(rows) < 1)) rows /= 2;
+    // By columns the tiles of a CTA's groups lie side by side: longer pieces of a column
+    p.beside = p.grad && p.cols && p.vec && rows == 32 && (k.groups == 4 || k.groups == 2) ? k.groups : 1;
     k.rows = rows;
     k.log_rows = rows == 32 ? 5 : rows == 16 ? 4 : 3;
     k.n_tiles = (int)((a.n + rows - 1) / rows);
@@ -335,20 +337,22 @@ size_t xent_few_workspace(const XentCall& a, int sms) {
     return few_carve(a, p, nullptr);
 }
 
+template <typename T>
+static cudaError_t few_run(const XentCall& a, const FewPlan& p) {
+    if (a.n > 0) {
+        const cudaError_t e = p.cols ? few_launch_columns(p, a.stream, T{}) : few_launch_rows(p, a.stream, T{});
+        if (e != cudaSuccess) return e;
+    }
+    return p.grad && (a.dw || a.dbias) ? few_sum<T>(a, p) : cudaSuccess;
+}
+
 cudaError_t xent_few(const XentCall& a, int sms) {
     FewPlan p = few_plan(a, sms);
     few_carve(a, p, a.ws);
-    if (a.n > 0) {
-        const cudaError_t e = a.type == GAFIME_TYPE_FP32   ? few_launch_fp32(p, a.stream)
-                              : a.type == GAFIME_TYPE_FP16 ? few_launch_fp16(p, a.stream)
-                                                           : few_launch_bf16(p, a.stream);
-        if (e != cudaSuccess) return e;
-    }
-    if (!p.grad || (!a.dw && !a.dbias)) return cudaSuccess;
     switch (a.type) {
-        case GAFIME_TYPE_FP32: return few_sum<float>(a, p);
-        case GAFIME_TYPE_FP16: return few_sum<__half>(a, p);
-        default: return few_sum<__nv_bfloat16>(a, p);
+        case GAFIME_TYPE_FP32: return few_run<float>(a, p);
+        case GAFIME_TYPE_FP16: return few_run<__half>(a, p);
+        default: return few_run<__nv_bfloat16>(a, p);
     }
 }
 

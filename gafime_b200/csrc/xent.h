@@ -1,5 +1,6 @@
-// xent.h -- softmax cross entropy of a linear head: what its two paths share.
-//   xent.cu      entry points, argument checks, the choice of path, the few-class path
+// xent.h -- softmax cross entropy of a linear head: what its paths share.
+//   xent.cu      entry points, argument checks, the choice of path, losses of a few rows
+//   xent_few.cuh few classes: one pass over x (xent_few_*.cu: an instance a type)
 //   xent_tc.cu   many classes: logits, gradients of x and w as tcgen05 products
 #pragma once
 
@@ -53,7 +54,7 @@ struct Carver {
     }
 };
 
-// Few classes (xent.cu): true when the class and feature counts fit its registers.
+// Few classes: true when the class and feature counts fit its registers.
 bool xent_few_fits(const XentCall& a);
 size_t xent_few_workspace(const XentCall& a, int sms);
 cudaError_t xent_few(const XentCall& a, int sms);

@@ -20,7 +20,7 @@
 // chains, added in fp64 in a fixed order by xent_few_sum_kernel at the end.
 //
 // Measured on a B200 (copy rate 6,551 GB/s): steps of 1e6 x 256 with 2 classes 0.182 ms by rows
-// (5,700 GB/s) and 0.215 ms by columns (4,800), of 4e6 x 128 with 3 classes 0.39 and 0.48 ms; the
+// (5,700 GB/s) and 0.195 ms by columns (5,300), of 4e6 x 128 with 3 classes 0.39 and 0.41 ms; the
 // loss of 300001 x 2048 with 5 classes 0.40 ms (6,130 GB/s).  By columns the loss alone of 4e6 x 128
 // stays at 4,700 GB/s: 128-byte pieces of columns 16 MB apart.  From six classes on the
 // multiply-adds bound it: 500000 x 512 with 8 classes takes 0.45 ms by rows, 0.55 by columns.
@@ -41,9 +41,13 @@ namespace gafime {
 // fp32: 1.5 to 3.1 ms a step, the tensor cores' path 1.5 ms); without, 16 (0.34 ms against 1.04 ms).
 constexpr int kFewMaxC = 16, kFewMaxGrad = 8;
 // Features of a warp's tile: 128 with gradients, 64 without (24 warps an SM in place of 12).
-constexpr int few_features(bool grad) { return grad ? 128 : 64; }
-// CTAs of eight warps that an SM holds without gradients, by registers.
-constexpr int few_loss_ctas(int c) { return c >= 6 ? 2 : 3; }
+constexpr int few_features(bool grad, bool narrow) { return grad && !narrow ? 128 : 64; }
+// Warps that an SM holds, by registers: 24 of 80, 20 of 96 or 16 of 128.
+constexpr int few_warps(int c, int features, bool grad) {
+    return features == 128 || c >= 6 ? 16 : grad && c > 2 ? 20 : 24;
+}
+// Threads of a CTA, at most.
+constexpr int few_threads(int features, bool grad) { return features == 128 ? 512 : grad ? 128 : 256; }
 constexpr int kRowsMost = 32;
 constexpr int kFlushRows = 256;
 
@@ -77,14 +81,19 @@ struct FewPlan {
     FewArgs k;
     int cp, grid, threads, features;
     bool cols, grad;
+    int beside;          // groups whose tiles lie side by side (by columns, with gradients), or 1
     bool vec;            // 16-byte copies of x: unit stride, aligned lines
     size_t smem;
 };
 
-// One per type (xent_few_*.cu): launches the kernel of the plan.
-cudaError_t few_launch_fp32(const FewPlan& p, cudaStream_t s);
-cudaError_t few_launch_fp16(const FewPlan& p, cudaStream_t s);
-cudaError_t few_launch_bf16(const FewPlan& p, cudaStream_t s);
+// Launches the kernel of the plan: one per type (the last argument names it) and order of x, each
+// in a file of its own (xent_few_*.cu), which compile side by side.
+cudaError_t few_launch_rows(const FewPlan& p, cudaStream_t s, float);
+cudaError_t few_launch_rows(const FewPlan& p, cudaStream_t s, __half);
+cudaError_t few_launch_rows(const FewPlan& p, cudaStream_t s, __nv_bfloat16);
+cudaError_t few_launch_columns(const FewPlan& p, cudaStream_t s, float);
+cudaError_t few_launch_columns(const FewPlan& p, cudaStream_t s, __half);
+cudaError_t few_launch_columns(const FewPlan& p, cudaStream_t s, __nv_bfloat16);
 
 namespace few {
 
@@ -95,11 +104,12 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) 
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// Geometry of a tile of R rows: bytes of a line, and the exchange of its 16-byte units.  The
-// pattern repeats every 8 lines, so unrolled loops need a few precomputed offsets only.
-template <typename T, bool COLS, int R, int F>
+// Geometry of a tile of R rows (of G groups' tiles side by side, by columns): bytes of a line, and
+// the exchange of its 16-byte units.  The pattern repeats every 8 lines, so unrolled loops need a
+// few precomputed offsets only.
+template <typename T, bool COLS, int R, int F, int G = 1>
 struct Tile {
-    static constexpr int kLine = (COLS ? R : F) * (int)sizeof(T);
+    static constexpr int kLine = (COLS ? G * R : F) * (int)sizeof(T);
     static constexpr int kUnits = kLine / 16;                 // of a line
     static constexpr int kMask = kUnits >= 8 ? 7 : kUnits - 1;
     static constexpr int kShift = kUnits >= 8 ? 0 : kUnits == 4 ? 1 : kUnits == 2 ? 2 : 3;
@@ -194,6 +204,26 @@ __device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64
     }
 }
 
+// The tiles of G groups side by side, x by columns: the groups' warps over the same features fill
+// one tile of G x 32 rows together.  A column is then read in pieces of 512 bytes (fp32, four
+// groups) in place of 128; by columns that lie pages apart it costs less than the two barriers
+// of the CTA that it takes.  Steps by columns, fp32, apart and side by side: 4e6 x 128 with 3
+// classes 502 and 411 us, 1e6 x 256 with 2 classes 226 and 195; 2e6 x 50 151 and 156.
+template <typename T, int F, int G>
+__device__ __forceinline__ void load_side_by_side(const FewArgs& a, uint8_t* tile, int64_t r0, int k0, int group, int lane) {
+    using Geo = Tile<T, true, 32, F, G>;
+    constexpr int V = 16 / sizeof(T), U = Geo::kUnits, LS = 32 / U;   // LS: lines of a warp at a time
+    const int len = (int)min((int64_t)(32 * G), a.n - r0), feats = min(F, a.d - k0);
+    const int l0 = lane / U, q = lane % U;
+    const int bytes = max(0, min(V, len - q * V)) * (int)sizeof(T);
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(tile);
+    const T* src = (const T*)a.x + r0 * a.xr + (int64_t)(k0 + group * LS + l0) * a.xk + (bytes ? q * V : 0);
+    const int64_t hop = (int64_t)LS * G * a.xk;
+    #pragma unroll 8
+    for (int l = group * LS + l0; l < feats; l += LS * G, src += hop)
+        copy16(dst + Geo::unit(l, q), bytes ? src : (const T*)a.x, bytes);
+}
+
 // Classes of a line in shared memory, padded so that C pairs are whole 16-byte units.
 template <int C>
 constexpr int padded() { return (C + 1) / 2 * 2; }
@@ -270,14 +300,14 @@ struct Lanes {
 // Step 1: dot products of the tile's rows with w, all of row Lanes::row(lane) in z at the end.
 // w: columns [features][classes], pairs of rows multiplied together, a value of w for four rows;
 // rows [feature pairs][classes][2], pairs of features.
-template <typename T, int C, bool COLS, int R, int F>
-__device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const float* w, int feats, int lane) {
-    using Geo = Tile<T, COLS, R, F>;
+template <typename T, int C, bool COLS, int R, int F, int G = 1>
+__device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const float* w, int feats, int lane, int beside = 0) {
+    using Geo = Tile<T, COLS, R, F, G>;
     using L = Lanes<COLS, R>;
     constexpr int CL = padded<C>(), S = L::kShares;
     if constexpr (COLS) {
-        constexpr int G = L::kGroups, B = C <= 6 ? C : 4;     // B: classes at a time
-        const int group = lane % G, share = lane / G;
+        constexpr int K = L::kGroups, B = C <= 6 ? C : 4;     // B: classes at a time
+        const int group = lane % K, share = lane / K, own = beside * R + 4 * group;
         #pragma unroll
         for (int c0 = 0; c0 < C; c0 += B) {
             float part[4][B];
@@ -288,8 +318,8 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
                 #pragma unroll
                 for (int c = 0; c < B; ++c) sum[q][0][c] = sum[q][1][c] = 0;
             // lines share, share + S, ...: S a multiple of 4, so two exchanges in turn
-            const uint8_t* p0 = tile + Geo::at(share, 4 * group);
-            const uint8_t* p1 = tile + Geo::at(share + S, 4 * group);
+            const uint8_t* p0 = tile + Geo::at(share, own);
+            const uint8_t* p1 = tile + Geo::at(share + S, own);
             const float* wk = w + share * CL + c0;
             auto line = [&](const uint8_t* p, const float* wl, Pair (&to)[2][B]) {
                 float xv[4], wv[B];
@@ -341,10 +371,10 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
                 const bool odd = share & 1, high = share & 2;
                 const float s0 = odd ? part[0][c] : part[1][c], k0 = odd ? part[1][c] : part[0][c];
                 const float s1 = odd ? part[2][c] : part[3][c], k1 = odd ? part[3][c] : part[2][c];
-                const float u0 = k0 + __shfl_xor_sync(0xffffffffu, s0, G), u1 = k1 + __shfl_xor_sync(0xffffffffu, s1, G);
-                float t = (high ? u1 : u0) + __shfl_xor_sync(0xffffffffu, high ? u0 : u1, 2 * G);
+                const float u0 = k0 + __shfl_xor_sync(0xffffffffu, s0, K), u1 = k1 + __shfl_xor_sync(0xffffffffu, s1, K);
+                float t = (high ? u1 : u0) + __shfl_xor_sync(0xffffffffu, high ? u0 : u1, 2 * K);
                 #pragma unroll
-                for (int o = 4 * G; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+                for (int o = 4 * K; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
                 if (c0 + c < C) z[c0 + c] += t;
             }
         }
@@ -387,10 +417,10 @@ __device__ __forceinline__ void dots(float (&z)[C], const uint8_t* tile, const f
 // count.  `bad`: rows left out that hold no numbers (0 x NaN is NaN), skipped.
 //   columns: pairs of rows, g as [row pairs][classes][2]; the two sums of a pair meet at a flush
 //   rows: pairs of features, g as [rows][classes][2 alike]
-template <typename T, int C, bool COLS, int R, int F>
+template <typename T, int C, bool COLS, int R, int F, int G = 1>
 __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], const uint8_t* tile, const float* g,
-                                     uint32_t bad, int feats, int lane) {
-    using Geo = Tile<T, COLS, R, F>;
+                                     uint32_t bad, int feats, int lane, int beside = 0) {
+    using Geo = Tile<T, COLS, R, F, G>;
     constexpr int CL = padded<C>();
     if (COLS) {
         // lines lane + 32 f exchange alike; four rows of a line at a time
@@ -405,7 +435,7 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
                     Pair g0[B], g1[B];
                     load_pairs<B>(g0, g + (r / 2 * CL + c0) * 2);
                     load_pairs<B>(g1, g + ((r / 2 + 1) * CL + c0) * 2);
-                    const int b = r * (int)sizeof(T);
+                    const int b = (beside * R + r) * (int)sizeof(T);
                     const uint8_t* p = line + (((b >> 4 << 4) ^ x0) + (b & 15));
                     #pragma unroll
                     for (int f = 0; f < F / 32; ++f) {
@@ -460,9 +490,10 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
 }
 
 // C: classes the code has room for (a.c of them exist); GRAD: dw, dbias or dx wanted; F: features of
-// a warp's tile; VEC: x in 16-byte copies (kernels of their own, for the registers)
-template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC>
-__global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C)) xent_few_kernel(const FewArgs a) {
+// a warp's tile; VEC: x in 16-byte copies (kernels of their own, for the registers); G: groups
+// whose tiles lie side by side
+template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC, int G>
+__global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 32 / few_threads(F, GRAD)) xent_few_kernel(const FewArgs a) {
     constexpr int CL = padded<C>(), NF = GRAD ? F / 32 : 1;   // NF: features a lane sums in step 3
     constexpr int NP = !GRAD ? 1 : COLS ? NF : NF / 2;         // its sums: pairs over rows, or over features
     constexpr int GL = COLS ? CL : 2 * CL;                     // floats of a row of g
@@ -472,7 +503,7 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C))
     const int R = a.rows;
     const int warps = W * a.groups;
     const int tile_bytes = R * F * (int)sizeof(T);
-    uint8_t* tile = smem + (size_t)warp * tile_bytes;
+    uint8_t* tile = smem + (size_t)(G > 1 ? wg * G : warp) * tile_bytes;   // G > 1: one for the G groups
     float* ws = reinterpret_cast<float*>(smem + (size_t)warps * tile_bytes);   // w, [d_pad][CL] or [d_pad / 2][CL][2]
     float* gs = ws + (size_t)a.d_pad * CL + (size_t)warp * (GRAD ? kRowsMost * GL : 0);   // g, a warp's own
     float* red = ws + (size_t)a.d_pad * CL + (size_t)warps * (GRAD ? kRowsMost * GL : 0);   // [2][groups][W][C][32]
@@ -508,7 +539,8 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C))
     // The groups of a CTA take neighbouring tiles (of a wide table's columns they then read the
     // same pages); where there are few tiles, one group of every CTA comes first.
     const int64_t step = (int64_t)a.groups * gridDim.x;
-    const int64_t first = a.n_tiles >= step ? (int64_t)blockIdx.x * a.groups + group : (int64_t)group * gridDim.x + blockIdx.x;
+    const int64_t first = G > 1 || a.n_tiles >= step ? (int64_t)blockIdx.x * a.groups + group
+                                                     : (int64_t)group * gridDim.x + blockIdx.x;
     const size_t part_at = (size_t)first * a.c * a.d_pad;
     int parity = 0, since = 0;
     bool flushed = false;
@@ -572,23 +604,34 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C))
         return m;
     };
     Meta meta = meta_of(first);
-    for (int64_t t = first; t < a.n_tiles; t += step) {
+    // (side by side, the groups of a CTA go on together: rows past the table's end are zeros)
+    for (int64_t t = first; G > 1 ? t - group < a.n_tiles : t < a.n_tiles; t += step) {
         const int64_t r0 = t * R, gr = r0 + row;
         float z[C];
         #pragma unroll
         for (int c = 0; c < C; ++c) z[c] = 0.f;
         Meta next = meta;
         for (int k0 = k_first; k0 < a.d; k0 += k_step) {
-            __syncwarp();                                  // the tile's last readers are done
-            load(t, k0);
+            if constexpr (G > 1) {
+                __syncthreads();                           // the tiles' last readers are done
+                load_side_by_side<T, F, G>(a, tile, (t - group) * R, k0, group, lane);
+            } else {
+                __syncwarp();                              // the tile's last readers are done
+                load(t, k0);
+            }
             asm volatile("cp.async.commit_group;" ::: "memory");
             if (k0 == k_first) next = meta_of(t + step);
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncwarp();
+            if constexpr (G > 1)
+                __syncthreads();
+            else
+                __syncwarp();
             // 1. a lane is a row
             const int feats = min(F, a.d - k0);
             const float* wk = ws + (size_t)k0 * CL;                // k0 / 2 pairs of 2 CL
-            if (R == 32)
+            if constexpr (G > 1)
+                dots<T, C, COLS, 32, F, G>(z, tile, wk, feats, lane, group);
+            else if (R == 32)
                 dots<T, C, COLS, 32, F>(z, tile, wk, feats, lane);
             else if (R == 16)
                 dots<T, C, COLS, 16, F>(z, tile, wk, feats, lane);
@@ -603,7 +646,12 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C))
             float* mine = red + ((size_t)(parity * a.groups + group) * W) * C * 32;
             #pragma unroll
             for (int c = 0; c < C; ++c) mine[(wg * C + c) * 32 + lane] = z[c];
-            asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(W * 32) : "memory");
+            // (two groups at most; a barrier named by a register would reserve all 16, and an SM has
+            // those of four CTAs)
+            if (group)
+                asm volatile("bar.sync 2, %0;" ::"r"(W * 32) : "memory");
+            else
+                asm volatile("bar.sync 1, %0;" ::"r"(W * 32) : "memory");
             #pragma unroll
             for (int c = 0; c < C; ++c) z[c] = 0.f;
             #pragma unroll 2
@@ -690,7 +738,9 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C))
             if constexpr (GRAD) {
                 if (a.part && __any_sync(0xffffffffu, kept)) {
                     const int feats = min(F, a.d - kw);
-                    if (R == 32)
+                    if constexpr (G > 1)
+                        sums<T, C, COLS, 32, F, G>(acc, tile, gs, bad, feats, lane, group);
+                    else if (R == 32)
                         sums<T, C, COLS, 32, F>(acc, tile, gs, bad, feats, lane);
                     else if (R == 16)
                         sums<T, C, COLS, 16, F>(acc, tile, gs, bad, feats, lane);
@@ -715,9 +765,9 @@ __global__ void __launch_bounds__(GRAD ? 512 : 256, GRAD ? 1 : few_loss_ctas(C))
     }
 }
 
-template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC>
+template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC, int G>
 cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
-    auto fn = xent_few_kernel<T, C, COLS, GRAD, DX, F, VEC>;
+    auto fn = xent_few_kernel<T, C, COLS, GRAD, DX, F, VEC, G>;
     const cudaError_t e =
         cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
     if (e != cudaSuccess) return e;
@@ -726,31 +776,40 @@ cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <typename T, int C, bool COLS, bool GRAD, bool DX>
-cudaError_t launch(const FewPlan& p, cudaStream_t s) {
-    constexpr int F = few_features(GRAD);
-    return p.vec ? launch_f<T, C, COLS, GRAD, DX, F, true>(p, s) : launch_f<T, C, COLS, GRAD, DX, F, false>(p, s);
+template <typename T, int C, bool COLS, bool GRAD, bool DX, int F>
+cudaError_t launch_g(const FewPlan& p, cudaStream_t s) {
+    if constexpr (COLS && GRAD) {
+        if (p.beside == 4) return launch_f<T, C, COLS, GRAD, DX, F, true, 4>(p, s);
+        if constexpr (F == 128)
+            if (p.beside == 2) return launch_f<T, C, COLS, GRAD, DX, F, true, 2>(p, s);
+    }
+    return p.vec ? launch_f<T, C, COLS, GRAD, DX, F, true, 1>(p, s) : launch_f<T, C, COLS, GRAD, DX, F, false, 1>(p, s);
 }
 
-template <typename T, int C>
+template <typename T, int C, bool COLS, bool GRAD, bool DX>
+cudaError_t launch(const FewPlan& p, cudaStream_t s) {
+    if constexpr (GRAD)
+        if (p.features == 128) return launch_g<T, C, COLS, GRAD, DX, 128>(p, s);
+    return launch_g<T, C, COLS, GRAD, DX, 64>(p, s);
+}
+
+template <typename T, int C, bool COLS>
 cudaError_t launch_c(const FewPlan& p, cudaStream_t s) {
-    if (!p.grad) return p.cols ? launch<T, C, true, false, false>(p, s) : launch<T, C, false, false, false>(p, s);
-    if constexpr (C <= kFewMaxGrad) {
-        if (!p.k.dx) return p.cols ? launch<T, C, true, true, false>(p, s) : launch<T, C, false, true, false>(p, s);
-        return p.cols ? launch<T, C, true, true, true>(p, s) : launch<T, C, false, true, true>(p, s);
-    }
+    if (!p.grad) return launch<T, C, COLS, false, false>(p, s);
+    if constexpr (C <= kFewMaxGrad)
+        return p.k.dx ? launch<T, C, COLS, true, true>(p, s) : launch<T, C, COLS, true, false>(p, s);
     return cudaErrorInvalidValue;
 }
 
-template <typename T>
+template <typename T, bool COLS>
 cudaError_t launch_t(const FewPlan& p, cudaStream_t s) {
     switch (p.cp) {
-        case 2: return launch_c<T, 2>(p, s);
-        case 3: return launch_c<T, 3>(p, s);
-        case 4: return launch_c<T, 4>(p, s);
-        case 6: return launch_c<T, 6>(p, s);
-        case 8: return launch_c<T, 8>(p, s);
-        case 16: return launch_c<T, 16>(p, s);
+        case 2: return launch_c<T, 2, COLS>(p, s);
+        case 3: return launch_c<T, 3, COLS>(p, s);
+        case 4: return launch_c<T, 4, COLS>(p, s);
+        case 6: return launch_c<T, 6, COLS>(p, s);
+        case 8: return launch_c<T, 8, COLS>(p, s);
+        case 16: return launch_c<T, 16, COLS>(p, s);
     }
     return cudaErrorInvalidValue;
 }

@@ -168,6 +168,22 @@ def test_orders_of_x(ops, n, d, c, order, dtype):
     check(ops, *data(n, d, c, dtype, order=order, left_out=0.1, seed=3))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("order", ["columns", "rows"])
+@pytest.mark.parametrize("d", [1, 16, 33, 64, 65, 128, 129, 256, 300])
+@pytest.mark.parametrize("n,c", [(20008, 2), (19040, 3), (33056, 5), (20008, 8)])
+def test_whole_tiles_of_rows(ops, n, d, c, order, dtype):
+    """Enough rows that every SM has tiles of 32 rows, and some at the end without any."""
+    x, w, labels, b, r = data(n, d, c, dtype, order=order, left_out=0.1, seed=12)
+    out = labels < 0
+    x[out.nonzero()[::3, 0]] = float("nan")
+    want = reference(x, w, labels, b, r)
+    for need_dx in (False, True):
+        g = ops.softmax_xent_grad(x, w, labels, b, row_weight=r, need_dx=need_dx)
+        for name in ("loss", "lse", "dw", "dbias") + (("dx",) if need_dx else ()):
+            compare(name, getattr(g, name), want[name])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("order", ["columns", "pitched", "aligned", "every other"])
 @pytest.mark.parametrize("n,d,c", [(100, 45, 3), (140, 72, 70)])
