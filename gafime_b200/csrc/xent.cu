@@ -26,28 +26,37 @@ namespace {
 constexpr int kFewMaxD = 2048;
 constexpr size_t kFewMaxSmem = 226 * 1024;
 
-// dw[c][k] = sum over p of part[p][c][k], and the bias's, fp64 in a fixed order: 32 warps split
-// the partials of 32 neighbouring outputs
+// dw[c][k] = sum over p of part[p][c][k], and the bias's, fp64 in a fixed order.  A CTA adds
+// eight neighbouring outputs (a sector of each partial): 128 threads share an output's partials,
+// of which there are up to 24 an SM, so that two batches of loads read them (4e6 x 16 with 2
+// classes: 9 us; 32 outputs a CTA, 19).
+constexpr int kSumOut = 8;
 template <typename T>
 __global__ void __launch_bounds__(1024) xent_few_sum_kernel(const float* __restrict__ part,
                                                             const double* __restrict__ part_bias, int parts, int c, int d,
                                                             int d_pad, T* __restrict__ dw, float* __restrict__ dbias) {
-    __shared__ double s[32][33];
+    constexpr int kShare = 1024 / kSumOut;
+    __shared__ double s[32][kSumOut + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int blocks_k = (d + 31) / 32;
+    const int out = threadIdx.x % kSumOut, share = threadIdx.x / kSumOut;
+    const int blocks_k = (d + kSumOut - 1) / kSumOut;
     const bool is_bias = !dw || (int)blockIdx.x >= c * blocks_k;
-    const int cls = is_bias ? 0 : blockIdx.x / blocks_k, k = is_bias ? lane : (blockIdx.x % blocks_k) * 32 + lane;
+    const int cls = is_bias ? 0 : blockIdx.x / blocks_k, k = is_bias ? out : (blockIdx.x % blocks_k) * kSumOut + out;
     double v = 0.0;
     if (is_bias) {
         if (k < c)
-            for (int p = warp; p < parts; p += 32) v += part_bias[(size_t)p * c + k];
+            #pragma unroll 16
+            for (int p = share; p < parts; p += kShare) v += part_bias[(size_t)p * c + k];
     } else if (k < d) {
         const float* q = part + (size_t)cls * d_pad + k;
-        #pragma unroll 8
-        for (int p = warp; p < parts; p += 32) v += (double)q[(size_t)p * c * d_pad];
+        #pragma unroll 16
+        for (int p = share; p < parts; p += kShare) v += (double)q[(size_t)p * c * d_pad];
     }
-    s[warp][lane] = v;
+    #pragma unroll
+    for (int o = 16; o >= kSumOut; o >>= 1) v += __shfl_down_sync(0xffffffffu, v, o);
+    if (lane < kSumOut) s[warp][lane] = v;
     __syncthreads();
+    if (warp >= kSumOut) return;
     // transposed: a warp adds one output's 32 sums
     v = s[lane][warp];
     #pragma unroll
@@ -56,10 +65,11 @@ __global__ void __launch_bounds__(1024) xent_few_sum_kernel(const float* __restr
     if (is_bias) {
         if (warp < c && dbias) dbias[warp] = (float)v;
     } else {
-        const int ko = (blockIdx.x % blocks_k) * 32 + warp;
+        const int ko = (blockIdx.x % blocks_k) * kSumOut + warp;
         if (ko < d) dw[(size_t)cls * d + ko] = from_float<T>((float)v);
     }
 }
+static_assert(kFewMaxGrad <= kSumOut, "the bias's sums are one CTA's");
 
 // ---- a few rows, any number of classes ----------------------------------------------------
 // Losses of up to kRowsFew rows (serving's single rows): bound by reading w once.  A warp takes
@@ -316,7 +326,7 @@ size_t few_carve(const XentCall& a, FewPlan& p, uint8_t* ws) {
 
 template <typename T>
 cudaError_t few_sum(const XentCall& a, const FewPlan& p) {
-    const int blocks = (a.dw ? (int)a.c * (((int)a.d + 31) / 32) : 0) + (a.dbias ? 1 : 0);
+    const int blocks = (a.dw ? (int)a.c * (((int)a.d + kSumOut - 1) / kSumOut) : 0) + (a.dbias ? 1 : 0);
     KernelTimer kt(a.stream, GAFIME_KERNEL_XENT);
     xent_few_sum_kernel<T><<<blocks, 1024, 0, a.stream>>>(p.k.part, p.k.part_bias, a.n > 0 ? p.grid * p.k.groups : 0,
                                                           (int)a.c, (int)a.d, p.k.d_pad, (T*)a.dw, a.dbias);

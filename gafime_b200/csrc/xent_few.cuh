@@ -427,7 +427,8 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
         const uint8_t* line = tile + lane * Geo::kLine;
         const int x0 = ((lane >> Geo::kShift) & Geo::kMask) << 4;
         constexpr int B = C <= 8 ? C : 4;                     // classes at a time
-        auto pass = [&](auto plain) {                         // plain: a whole tile of numbers, no checks
+        // plain: numbers alone, no checks; features past the table give sums that nothing reads
+        auto pass = [&](auto plain) {
             #pragma unroll
             for (int c0 = 0; c0 < C; c0 += B) {
                 #pragma unroll 2
@@ -457,7 +458,7 @@ __device__ __forceinline__ void sums(Pair (&acc)[COLS ? F / 32 : F / 64][C], con
             }
         };
         // (from five classes on two copies of the loop cost more in registers than the checks)
-        if (C <= 4 && bad == 0 && feats == F)
+        if (C <= 4 && bad == 0 && (F == 64 || 2 * feats > F))
             pass([] { return true; });
         else
             pass([] { return false; });
@@ -548,24 +549,32 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
     // sums so far to the group's partial
     auto flush = [&]() {
         if (a.part) {
+            // several loads under way before their stores
+            constexpr int B = NP * C <= 16 ? NP : 1, V = COLS ? 1 : 2;
+            float* p = a.part + part_at + kw + (COLS ? lane : NF * lane);
             #pragma unroll
-            for (int f = 0; f < NP; ++f) {
+            for (int f0 = 0; f0 < NP; f0 += B) {
+                float old[B][C][V] = {};
+                if (flushed)
+                    #pragma unroll
+                    for (int f = 0; f < B; ++f)
+                        #pragma unroll
+                        for (int c = 0; c < C; ++c)
+                            #pragma unroll
+                            for (int v = 0; v < V; ++v)
+                                if (c < a.c) old[f][c][v] = p[(size_t)c * a.d_pad + (COLS ? 32 : 2) * (f0 + f) + v];
                 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    float lo, hi;
-                    unpair(lo, hi, acc[f][c]);
-                    acc[f][c] = 0;
-                    if (c >= a.c) continue;
-                    float* p = a.part + part_at + (size_t)c * a.d_pad + kw;
-                    if (COLS) {
-                        p += lane + 32 * f;
-                        *p = flushed ? *p + (lo + hi) : lo + hi;
-                    } else {
-                        p += NF * lane + 2 * f;
-                        p[0] = flushed ? p[0] + lo : lo;
-                        p[1] = flushed ? p[1] + hi : hi;
+                for (int f = 0; f < B; ++f)
+                    #pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        float lo, hi;
+                        unpair(lo, hi, acc[f0 + f][c]);
+                        acc[f0 + f][c] = 0;
+                        if (c >= a.c) continue;
+                        float* q = p + (size_t)c * a.d_pad + (COLS ? 32 : 2) * (f0 + f);
+                        q[0] = old[f][c][0] + (COLS ? lo + hi : lo);
+                        if (!COLS) q[V - 1] = old[f][c][V - 1] + hi;
                     }
-                }
             }
         }
         if (wg == 0)
