@@ -7,6 +7,7 @@
 // in 16 bits and multiplies it with both sides:
 //   lse   z = x w^T, online softmax in the epilogue              2 n d c FLOP
 //   g     z again, g in the epilogue                             2 n d c
+//   both  where one tile holds every class (256 and fewer): loss and g from the same z
 //   dx    g w        (classes summed; fp32 sums kept between class pieces)
 //   dw    g^T x      (rows summed; split over rows where the c x d tiles are few)
 //
@@ -69,13 +70,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr size_t kPieceBytes = (size_t)256 << 20;   // of g: several rounds of the pairs, not the n x c whole
 
-enum { LSE = 0, G = 1, DX = 2, DW = 3 };
+enum { LSE = 0, G = 1, DX = 2, DW = 3, BOTH = 4 };
 
 constexpr int stage_bytes(int bn) { return kABytes + bn / 2 * kBK * 2; }   // of one CTA
 constexpr int stages_of(int bn, int out) { return bn == 256 ? (out > 4096 ? 5 : 6) : bn == 128 ? (out > 4096 ? 6 : 8) : 8; }
 // An epilogue warp's outgoing blocks: 32 rows x 128 bytes of each plane of g (64 bytes where a tile
 // has 64 columns), or of dx or dw (64 bytes in 16 bits).
-constexpr int out_bytes(int mode, int planes) { return mode == 1 && planes == 2 ? 8192 : 4096; }
+constexpr int out_bytes(int mode, int planes) { return (mode == G || mode == BOTH) && planes == 2 ? 8192 : 4096; }
 constexpr size_t smem_of(int bn, int out) {
     return (size_t)stages_of(bn, out) * stage_bytes(bn) + kEpiWarps * out + 1024 + 256;
 }
@@ -136,6 +137,7 @@ struct TcArgs {
     const uint32_t* colmax;   // [d] largest |x_k| as float bits (fp32)
     const float* bias2;       // bias in base 2, -inf past the classes
     const int64_t* labels;
+    float *loss_out, *lse_out;   // BOTH: [n]; the second may be null
     float2* part;             // LSE: [n][2 splits] maximum, sum
     float* zy;                // LSE: label's logit, base 2
     const float2* shift;      // G: [n] maximum and log2 of the sum
@@ -217,7 +219,7 @@ __device__ __forceinline__ Unit unit_of(const TcArgs& a, int u) {
         t.split = u / a.m_tiles;
         t.n = t.split * a.per_split;
         t.tiles = min(a.per_split, a.n_tiles - t.n);
-    } else if (MODE == G) {
+    } else if (MODE == G || MODE == BOTH) {
         t.m = u % a.m_tiles;
         t.n = u / a.m_tiles;
     } else {
@@ -263,6 +265,7 @@ template <int MODE, int BN, typename E, int kPlanes>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_constant__ TcArgs a) {
     constexpr int kOut = out_bytes(MODE, kPlanes);
     constexpr int S = stages_of(BN, kOut), kCols = BN / 2;   // ring stages; columns of an epilogue thread
+    constexpr bool kG = MODE == G || MODE == BOTH, kZ = kG || MODE == LSE;
     constexpr bool kAMn = MODE == DW, kBMn = MODE == DX || MODE == DW;
     constexpr bool kBf16 = sizeof(E) == 2 && !std::is_same<E, __half>::value;
     constexpr uint32_t kId = tc::idesc(BN, kBf16, kAMn, kBMn);
@@ -426,17 +429,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
             int64_t y = -1;
             float top = -INFINITY, sum = 0.f, zy = NAN;    // LSE
             float2 sh = make_float2(0.f, 0.f);             // G
-            float wt = 0.f, ws = 0.f, gy = 0.f;            // ws: the weight over the row's sum
+            float wt = 0.f, ws = 0.f, gy = 0.f;            // G: ws the weight over the row's sum
             if (MODE != DW && valid) {
                 y = a.labels[a.row0 + row];
-                if (MODE == G && y >= 0) {
-                    sh = a.shift[a.row0 + row];
+                if (kG && y >= 0) {
                     wt = (a.weight ? a.weight[(a.row0 + row) * a.weight_stride] : 1.f) * a.scale;
                     wt = scale2(wt, ue);
-                    // exp(z_y - lse) - 1 from the loss, without the cancellation
-                    gy = expm1f(-a.loss[a.row0 + row]) * wt;
                     if (y >= a.c_total) wt = NAN;
-                    ws = wt * exp2f(-sh.y);
+                    if (MODE == G) {
+                        sh = a.shift[a.row0 + row];
+                        // exp(z_y - lse) - 1 from the loss, without the cancellation
+                        gy = expm1f(-a.loss[a.row0 + row]) * wt;
+                        ws = wt * exp2f(-sh.y);
+                    }
                 }
             }
             for (int r = 0; ok && r < t.tiles && t.kn > 0; ++r) {
@@ -470,6 +475,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             for (int j = 0; j < 32; ++j) sums[ch * 32 + 32 + j] += w[j];
                     }
                 }
+                if constexpr (MODE == BOTH) {
+                    // the row's maximum and sum over this half's classes, its exponentials left in sums
+                    const int blocks = (int)min((int64_t)(kCols / 32), max((int64_t)0, (a.cols - half * kCols + 31) / 32));
+                    float m4[4] = {top, top, top, top};
+                    #pragma unroll
+                    for (int ch = 0; ch < kCols / 32; ++ch) {
+                        if (ch >= blocks) break;
+                        float* v = sums + ch * 32;
+                        const int cb = half * kCols + ch * 32;
+                        const float4* b4 = reinterpret_cast<const float4*>(a.bias2 + cb);
+                        #pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float4 b = __ldg(b4 + j);
+                            v[4 * j] = fmaf(v[4 * j], f, b.x);
+                            v[4 * j + 1] = fmaf(v[4 * j + 1], f, b.y);
+                            v[4 * j + 2] = fmaf(v[4 * j + 2], f, b.z);
+                            v[4 * j + 3] = fmaf(v[4 * j + 3], f, b.w);
+                        }
+                        #pragma unroll
+                        for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
+                        const int64_t rel = y - cb;
+                        const bool here = rel >= 0 && rel < 32 && y < a.c_total;
+                        if (__any_sync(0xffffffffu, here)) {
+                            const float q = pick(v, (int)rel & 31);
+                            if (here) zy = q;
+                        }
+                    }
+                    top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    const float own = top == -INFINITY ? 0.f : top;   // nothing but excluded classes
+                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                    #pragma unroll
+                    for (int ch = 0; ch < kCols / 32; ++ch) {
+                        if (ch >= blocks) break;
+                        float* v = sums + ch * 32;
+                        #pragma unroll
+                        for (int j = 0; j < 32; ++j) s4[j & 3] += v[j] = exp2_fast(v[j] - own);
+                    }
+                    sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                    // and over the other half's, from the warp that has it.  A warp whose wait gave up
+                    // comes here too, so that neither waits for good.
+                    tc::store_wait_read<0>();          // the last store has read the block
+                    reinterpret_cast<float4*>(out)[lane] = make_float4(top, sum, zy, ok ? 1.f : 0.f);
+                    asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");
+                    const float4 o = reinterpret_cast<const float4*>(out + (half ? -4 : 4) * kOut)[lane];
+                    asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");   // read before g is written there
+                    ok = ok && o.w != 0.f;
+                    const float m = fmaxf(top, o.x), shift = m == -INFINITY ? 0.f : m;
+                    const float l = log2f(sum * exp2f(top - shift) + o.y * exp2f(o.x - shift));
+                    if (isnan(zy)) zy = o.z;
+                    const float loss = y >= 0 ? ((shift - zy) + l) * kLn2 : 0.f;
+                    if (half == 0 && valid) {
+                        a.loss_out[a.row0 + row] = loss;
+                        if (a.lse_out)
+                            a.lse_out[a.row0 + row] = y >= 0 ? (float)(((double)shift + (double)l) * 0.69314718055994530942) : 0.f;
+                    }
+                    gy = expm1f(-loss) * wt;
+                    // (with no class of its own a half's exponentials are zeros, whatever their shift)
+                    ws = wt * (top == -INFINITY ? 0.f : exp2f((own - shift) - l));
+                }
                 if (!ok) break;
                 #pragma unroll
                 for (int ch = 0; ch < kCols / 32; ++ch) {
@@ -477,7 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     const int64_t cb = (int64_t)n * BN + col;         // column of the piece
                     if (cb >= a.cols) break;
                     float* v = sums + ch * 32;
-                    if (MODE == LSE || MODE == G) {
+                    if (MODE == LSE || MODE == G) {   // (BOTH: done)
                         const float4* b4 = reinterpret_cast<const float4*>(a.bias2 + a.c0 + cb);
                         #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -490,18 +554,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     }
                     // the row's label among these columns
                     const int64_t rel = y - a.c0 - cb;
-                    const bool here = (MODE == LSE || MODE == G) && rel >= 0 && rel < 32 && y < a.c_total;
+                    const bool here = kZ && rel >= 0 && rel < 32 && y < a.c_total;
                     uint32_t hit = 0;
-                    if (MODE == LSE || MODE == G) hit = __ballot_sync(0xffffffffu, here);
+                    if (kZ) hit = __ballot_sync(0xffffffffu, here);
                     if (MODE == LSE) {
                         if (hit) {
                             const float q = pick(v, (int)rel & 31);
                             if (here) zy = q;
                         }
-                    } else if (MODE == G) {
+                    } else if (kG) {
                         #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float p = exp2_fast(v[j] - sh.x) * ws;
+                            const float p = (MODE == BOTH ? v[j] : exp2_fast(v[j] - sh.x)) * ws;
                             v[j] = y >= 0 ? p : 0.f;
                         }
                         // 64 columns a store where the thread has as many: whole 128-byte lines
@@ -1032,11 +1096,12 @@ __global__ void __launch_bounds__(256) xent_colsum_kernel(const float* __restric
     }
 }
 
-// dbias from its splits; and NaN in dw where a kernel's wait gave up.
+// dbias from its splits; and NaN in dw (BOTH: losses) where a kernel's wait gave up.
 template <typename T>
 __global__ void __launch_bounds__(256) xent_finish_kernel(int64_t c, int64_t d, int half_g, const Meta* __restrict__ meta,
                                                           T* __restrict__ dw, const double* __restrict__ bias_part,
-                                                          int bias_splits, float* __restrict__ dbias) {
+                                                          int bias_splits, float* __restrict__ dbias, int64_t n,
+                                                          float* __restrict__ loss, float* __restrict__ lse) {
     const bool failed = meta->err != 0;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
     if (dbias)
@@ -1049,6 +1114,11 @@ __global__ void __launch_bounds__(256) xent_finish_kernel(int64_t c, int64_t d, 
         }
     if (dw && failed)
         for (int64_t i = at; i < c * d; i += all) dw[i] = from_float<T>(NAN);
+    if (loss && failed)
+        for (int64_t i = at; i < n; i += all) {
+            loss[i] = NAN;
+            if (lse) lse[i] = NAN;
+        }
 }
 
 // dw or dx from several splits' sums: a block makes 32 rows x 8 features, a warp a feature.  Rows
@@ -1343,7 +1413,9 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         return cudaSuccess;
     }
     XENT_TRY(cudaMemsetAsync(p.meta, 0, p.meta_bytes, st));
-    const bool forward = !a.have_lse;
+    // one tile of classes: the call's losses come with its g
+    const bool both = p.products && !a.have_lse && p.c_tiles == 1;
+    const bool forward = !a.have_lse && !both;
     {
         SetupArgs s{};
         s.labels = a.labels; s.n = a.n; s.weight = a.weight; s.weight_stride = a.weight_stride; s.scale = a.scale;
@@ -1422,7 +1494,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         l.zy = p.zy;
         XENT_TRY((launch<LSE, E, kPlanes>(l, p.bn_c, sms, st)));
     }
-    if (forward || p.products) {
+    if (!both && (forward || p.products)) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
         const int lanes = forward && p.splits >= 16 ? 32 : 1;
         xent_join_kernel<<<(unsigned)cdiv(a.n * lanes, 256), 256, 0, st>>>(p.part, 2 * p.splits, lanes, p.zy, a.labels, a.n,
@@ -1463,7 +1535,12 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                     return cudaErrorInvalidValue;
             g.ldg = p.ldg;
             g.bias_part = a.dbias ? p.bias_sums : nullptr;
-            XENT_TRY((launch<G, E, kPlanes>(g, p.bn_c, sms, st)));
+            g.loss_out = a.loss;
+            g.lse_out = a.lse;
+            if (both)
+                XENT_TRY((launch<BOTH, E, kPlanes>(g, p.bn_c, sms, st)));
+            else
+                XENT_TRY((launch<G, E, kPlanes>(g, p.bn_c, sms, st)));
             if (a.dbias) {
                 const int64_t lines = g.m_tiles * 8;
                 KernelTimer kt(st, GAFIME_KERNEL_XENT);
@@ -1546,10 +1623,10 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             p.undo ? p.undo + 2 * p.undo_pitch : nullptr, p.undo_pitch, !kBf16, p.meta, nullptr, (T*)a.dw, a.d, 1);
         XENT_TRY(cudaGetLastError());
     }
-    if (a.dw || a.dbias) {
+    if (a.dw || a.dbias || both) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
         xent_finish_kernel<T><<<(unsigned)std::min<int64_t>(2 * sms, cdiv(a.c, 8)), 256, 0, st>>>(
-            a.c, a.d, !kBf16, p.meta, (T*)a.dw, p.bias_part, p.bias_splits, a.dbias);
+            a.c, a.d, !kBf16, p.meta, (T*)a.dw, p.bias_part, p.bias_splits, a.dbias, a.n, both ? a.loss : nullptr, a.lse);
         XENT_TRY(cudaGetLastError());
     }
     return cudaSuccess;

@@ -197,6 +197,44 @@ def test_several_pieces_of_the_gradient(ops, n, d, c, dtype):
     check(ops, *data(n, d, c, dtype, left_out=0.1, seed=5))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("c", [17, 32, 33, 64, 65, 96, 128, 129, 200, 256, 257])
+def test_every_class_in_one_tile(ops, c, dtype):
+    """Loss and gradients from one computation of the logits, and from a loss call before."""
+    x, w, labels, b, r = data(389, 70, c, dtype, left_out=0.2, seed=13)
+    x[(labels < 0).nonzero()[::2, 0]] = float("nan")
+    want = reference(x, w, labels, b, r)
+    g = ops.softmax_xent_grad(x, w, labels, b, row_weight=r)
+    for name in ("loss", "lse", "dw", "dx", "dbias"):
+        compare(name, getattr(g, name), want[name])
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    loss = ops.softmax_xent(leaves[0], leaves[1], labels, leaves[2])
+    compare("loss", loss.detach(), want["loss"])
+    loss.backward(r)
+    for name, leaf in zip(("dx", "dw", "dbias"), leaves):
+        compare(name + " of the backward pass", leaf.grad, want[name])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c,kept", [(256, (0, 128)), (256, (128, 256)), (100, (0, 50)), (100, (64, 100)), (40, (39, 40))])
+def test_a_run_of_classes_excluded(ops, c, kept, dtype):
+    x, w, labels, b, r = data(200, 32, c, dtype, seed=14)
+    out = torch.ones(c, dtype=torch.bool, device="cuda")
+    out[kept[0]:kept[1]] = False
+    labels = labels % (kept[1] - kept[0]) + kept[0]
+    for shift in (0.0, -300.0, 300.0):
+        bias = torch.where(out, float("-inf"), b + shift)
+        want = reference(x, w, labels, bias, r)
+        g = ops.softmax_xent_grad(x, w, labels, bias, row_weight=r)
+        for name in ("loss", "lse", "dx"):
+            compare(name, getattr(g, name), want[name])
+        assert not g.dw[out].any() and not g.dbias[out].any()
+
+
+def test_one_tile_of_classes_in_several_pieces(ops):
+    check(ops, *data(300_000, 8, 200, F32, left_out=0.1, seed=15))
+
+
 @pytest.mark.parametrize("c", [2, 60])
 def test_without_a_bias(ops, c):
     check(ops, *data(300, 40, c, F32, bias=False, seed=6))
