@@ -421,8 +421,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
         const int te = w_exponent(a.meta, a.scaled), ue = g_exponent(a.meta, a.half_g);
         const float f = pow2i(-te) * kLog2e;
         const uint32_t aempty_l = tc::in_leader(aempty0);
+        // What a unit needs of its rows is loaded while the unit before it is worked on.
+        struct Row {
+            int64_t y;
+            float weight, loss;
+            float2 shift;
+        };
+        auto row_of = [&](int u) {
+            Row r = {-1, 1.f, 0.f, make_float2(0.f, 0.f)};
+            if (MODE == DW || u >= a.units) return r;
+            const int64_t row = (int64_t)(2 * unit_of<MODE>(a, u).m + rank) * kBM + quarter * 32 + lane;
+            if (row >= a.rows) return r;
+            r.y = a.labels[a.row0 + row];
+            if (kG && a.weight) r.weight = a.weight[(a.row0 + row) * a.weight_stride];
+            if (MODE == G) {
+                r.loss = a.loss[a.row0 + row];
+                r.shift = a.shift[a.row0 + row];
+            }
+            return r;
+        };
+        Row next = row_of(pair);
         for (int u = pair; ok && u < a.units; u += pairs) {
             const Unit t = unit_of<MODE>(a, u);
+            const Row own_row = next;
+            next = row_of(u + pairs);
             const int mt = 2 * t.m + rank;                 // this CTA's 128 rows
             const int64_t y0 = (int64_t)mt * kBM + quarter * 32, row = y0 + lane;
             const bool valid = row < a.rows;
@@ -430,18 +452,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
             float top = -INFINITY, sum = 0.f, zy = NAN;    // LSE
             float2 sh = make_float2(0.f, 0.f);             // G
             float wt = 0.f, ws = 0.f, gy = 0.f;            // G: ws the weight over the row's sum
-            if (MODE != DW && valid) {
-                y = a.labels[a.row0 + row];
-                if (kG && y >= 0) {
-                    wt = (a.weight ? a.weight[(a.row0 + row) * a.weight_stride] : 1.f) * a.scale;
-                    wt = scale2(wt, ue);
-                    if (y >= a.c_total) wt = NAN;
-                    if (MODE == G) {
-                        sh = a.shift[a.row0 + row];
-                        // exp(z_y - lse) - 1 from the loss, without the cancellation
-                        gy = expm1f(-a.loss[a.row0 + row]) * wt;
-                        ws = wt * exp2f(-sh.y);
-                    }
+            if (MODE != DW) y = own_row.y;
+            if (kG && y >= 0) {
+                wt = scale2(own_row.weight * a.scale, ue);
+                if (y >= a.c_total) wt = NAN;
+                if (MODE == G) {
+                    sh = own_row.shift;
+                    // exp(z_y - lse) - 1 from the loss, without the cancellation
+                    gy = expm1f(-own_row.loss) * wt;
+                    ws = wt * exp2f(-sh.y);
                 }
             }
             for (int r = 0; ok && r < t.tiles && t.kn > 0; ++r) {
