@@ -304,8 +304,13 @@ FewPlan few_plan(const XentCall& a, int sms) {
     int rows = kRowsMost;
     if (resident(rows) * warps < 10 && resident(16) * warps > resident(rows) * warps) rows = 16;
     while (rows > 8 && ((a.n + rows - 1) / rows < 4 * sms || resident(rows) < 1)) rows /= 2;
-    // By columns the tiles of a CTA's groups lie side by side: longer pieces of a column
-    p.beside = p.grad && p.cols && p.vec && rows == 32 && (k.groups == 4 || k.groups == 2) ? k.groups : 1;
+    // By columns the tiles of a CTA's groups (without gradients, of two sets of them) lie side by
+    // side: longer pieces of a column
+    p.beside = 1;
+    if (p.cols && p.vec && rows == 32) {
+        if (!p.grad && p.cp <= kBesideMaxC && d >= kBesideMinD) p.beside = 4;
+        if (p.grad && (k.groups == 4 || k.groups == 2)) p.beside = k.groups;
+    }
     k.rows = rows;
     k.log_rows = rows == 32 ? 5 : rows == 16 ? 4 : 3;
     k.n_tiles = (int)((a.n + rows - 1) / rows);

@@ -8,22 +8,24 @@
 // A warp owns a tile of 32 rows (fewer in small calls) x 64 or 128 features in shared memory,
 // which it fills with its own asynchronous copies; W warps side by side cover the features.
 // Tiles are not double-buffered: a warp that waits for its copies leaves the SM to up to 23
-// others, which costs no barrier and no second tile (measured against two buffers of half the
+// others, which costs no second tile (measured against two buffers of half the
 // rows: 64-byte pieces of columns instead of 128 cost more than the overlap gained).
 //   1. a lane is a row: partial dot products with c accumulators, w broadcast from shared memory
 //      (fewer rows than lanes: the lanes of a row share the features)
 //   2. the W partial logits are added through shared memory (the only barrier); a lane computes
 //      its row's softmax, loss and g, and leaves g in shared memory
-//   3. a lane is two or four features: c sums each of g x over the tile's rows
-// Without gradients a warp walks over the features by itself, and there is no barrier at all.
+//   3. a lane is two or four features: c sums each of g x over the tile's rows (a whole tile, past
+//      the table's features too: those sums are not read)
+// Without gradients a warp walks over the features by itself, without that barrier.
 // The sums of step 3 move to a partial in global memory every kFlushRows rows: short fp32
 // chains, added in fp64 in a fixed order by xent_few_sum_kernel at the end.
 //
-// Measured on a B200 (copy rate 6,551 GB/s): steps of 1e6 x 256 with 2 classes 0.182 ms by rows
-// (5,700 GB/s) and 0.195 ms by columns (5,300), of 4e6 x 128 with 3 classes 0.39 and 0.41 ms; the
-// loss of 300001 x 2048 with 5 classes 0.40 ms (6,130 GB/s).  By columns the loss alone of 4e6 x 128
-// stays at 4,700 GB/s: 128-byte pieces of columns 16 MB apart.  From six classes on the
-// multiply-adds bound it: 500000 x 512 with 8 classes takes 0.45 ms by rows, 0.55 by columns.
+// Measured on a B200 (copy rate 6,551 GB/s): steps of 1e6 x 256 with 2 classes 0.176 ms by rows
+// (5,900 GB/s) and 0.182 ms by columns (5,700), of 4e6 x 128 with 3 classes 0.37 and 0.36 ms; their
+// losses 0.168 and 0.163 (6,350), 0.33 and 0.31 ms (6,650); the loss of 300001 x 2048 with 5 classes
+// 0.40 ms by rows.  Narrow tables are bound by a row's own work (softmax, g, the sums of lanes): the
+// step of 4e6 x 16 with 2 classes 0.139 ms.  From six classes on the multiply-adds bound it:
+// 500000 x 512 with 8 classes takes 0.45 ms by rows, 0.52 by columns.
 //
 // Tile layout: 16-byte units, unit q of line L at q ^ (L >> shift & mask), so that both the
 // reads along lines and those across them meet no bank twice.  A line is a row (x row by row)
@@ -38,9 +40,11 @@
 namespace gafime {
 
 // Most classes of this path.  With gradients 8: at 16 their sums leave no registers (200000 x 1024
-// fp32: 1.5 to 3.1 ms a step, the tensor cores' path 1.5 ms); without, 16 (0.34 ms against 1.04 ms).
+// fp32: 1.5 to 3.1 ms a step, the tensor cores' path 1.04 ms); without, 16 (0.34 ms against 1.04 ms).
 constexpr int kFewMaxC = 16, kFewMaxGrad = 8;
-// Features of a warp's tile: 128 with gradients, 64 without (24 warps an SM in place of 12).
+// Features of a warp's tile: 128 with gradients, 64 without and for narrow tables (up to 24 warps
+// an SM in place of 12 to 16: steps of 4e6 x 16 with 2 classes 217 -> 174 us, 500000 x 33 with 8
+// classes 102 -> 67).
 constexpr int few_features(bool grad, bool narrow) { return grad && !narrow ? 128 : 64; }
 // Warps that an SM holds, by registers: 24 of 80, 20 of 96 or 16 of 128.
 constexpr int few_warps(int c, int features, bool grad) {
@@ -49,6 +53,10 @@ constexpr int few_warps(int c, int features, bool grad) {
 // Threads of a CTA, at most.
 constexpr int few_threads(int features, bool grad) { return features == 128 ? 512 : grad ? 128 : 256; }
 constexpr int kRowsMost = 32;
+// Losses by columns: tiles side by side for 4 classes and 32 features or more (below; with more
+// classes or fewer features the barriers cost more: 500000 x 512 with 8 classes 187 -> 200 us,
+// 4e6 x 16 with 2 classes 72 -> 78).
+constexpr int kBesideMaxC = 4, kBesideMinD = 32;
 constexpr int kFlushRows = 256;
 
 struct FewArgs {
@@ -208,7 +216,8 @@ __device__ __forceinline__ void load_tile(const FewArgs& a, uint8_t* tile, int64
 // one tile of G x 32 rows together.  A column is then read in pieces of 512 bytes (fp32, four
 // groups) in place of 128; by columns that lie pages apart it costs less than the two barriers
 // of the CTA that it takes.  Steps by columns, fp32, apart and side by side: 4e6 x 128 with 3
-// classes 502 and 411 us, 1e6 x 256 with 2 classes 226 and 195; 2e6 x 50 151 and 156.
+// classes 502 and 411 us, 1e6 x 256 with 2 classes 226 and 195; 2e6 x 50 151 and 156; losses 441
+// and 314, 190 and 163, 78 and 72.
 template <typename T, int F, int G>
 __device__ __forceinline__ void load_side_by_side(const FewArgs& a, uint8_t* tile, int64_t r0, int k0, int group, int lane) {
     using Geo = Tile<T, true, 32, F, G>;
@@ -504,7 +513,8 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
     const int R = a.rows;
     const int warps = W * a.groups;
     const int tile_bytes = R * F * (int)sizeof(T);
-    uint8_t* tile = smem + (size_t)(G > 1 ? wg * G : warp) * tile_bytes;   // G > 1: one for the G groups
+    const int gi = G > 1 ? group % G : 0;                 // among the G groups that share a tile
+    uint8_t* tile = smem + (size_t)(G > 1 ? wg * G + group - gi : warp) * tile_bytes;
     float* ws = reinterpret_cast<float*>(smem + (size_t)warps * tile_bytes);   // w, [d_pad][CL] or [d_pad / 2][CL][2]
     float* gs = ws + (size_t)a.d_pad * CL + (size_t)warp * (GRAD ? kRowsMost * GL : 0);   // g, a warp's own
     float* red = ws + (size_t)a.d_pad * CL + (size_t)warps * (GRAD ? kRowsMost * GL : 0);   // [2][groups][W][C][32]
@@ -598,6 +608,15 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
         else
             load_tile<T, COLS, 8, F, VEC>(a, tile, t * R, k0, lane);
     };
+    // the warps of the groups that share a tile wait for each other (without gradients, two sets)
+    auto together = [&]() {
+        if (GRAD)
+            __syncthreads();
+        else if (group < G)
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * G) : "memory");
+        else
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * G) : "memory");
+    };
     struct Meta {
         int64_t y;
         float weight, lse;
@@ -622,8 +641,8 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
         Meta next = meta;
         for (int k0 = k_first; k0 < a.d; k0 += k_step) {
             if constexpr (G > 1) {
-                __syncthreads();                           // the tiles' last readers are done
-                load_side_by_side<T, F, G>(a, tile, (t - group) * R, k0, group, lane);
+                together();                                // the tiles' last readers are done
+                load_side_by_side<T, F, G>(a, tile, (t - gi) * R, k0, gi, lane);
             } else {
                 __syncwarp();                              // the tile's last readers are done
                 load(t, k0);
@@ -632,14 +651,14 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
             if (k0 == k_first) next = meta_of(t + step);
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             if constexpr (G > 1)
-                __syncthreads();
+                together();
             else
                 __syncwarp();
             // 1. a lane is a row
             const int feats = min(F, a.d - k0);
             const float* wk = ws + (size_t)k0 * CL;                // k0 / 2 pairs of 2 CL
             if constexpr (G > 1)
-                dots<T, C, COLS, 32, F, G>(z, tile, wk, feats, lane, group);
+                dots<T, C, COLS, 32, F, G>(z, tile, wk, feats, lane, gi);
             else if (R == 32)
                 dots<T, C, COLS, 32, F>(z, tile, wk, feats, lane);
             else if (R == 16)
@@ -748,7 +767,7 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
                 if (a.part && __any_sync(0xffffffffu, kept)) {
                     const int feats = min(F, a.d - kw);
                     if constexpr (G > 1)
-                        sums<T, C, COLS, 32, F, G>(acc, tile, gs, bad, feats, lane, group);
+                        sums<T, C, COLS, 32, F, G>(acc, tile, gs, bad, feats, lane, gi);
                     else if (R == 32)
                         sums<T, C, COLS, 32, F>(acc, tile, gs, bad, feats, lane);
                     else if (R == 16)
@@ -787,9 +806,9 @@ cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
 
 template <typename T, int C, bool COLS, bool GRAD, bool DX, int F>
 cudaError_t launch_g(const FewPlan& p, cudaStream_t s) {
-    if constexpr (COLS && GRAD) {
+    if constexpr (COLS && (GRAD || C <= kBesideMaxC)) {
         if (p.beside == 4) return launch_f<T, C, COLS, GRAD, DX, F, true, 4>(p, s);
-        if constexpr (F == 128)
+        if constexpr (GRAD && F == 128)
             if (p.beside == 2) return launch_f<T, C, COLS, GRAD, DX, F, true, 2>(p, s);
     }
     return p.vec ? launch_f<T, C, COLS, GRAD, DX, F, true, 1>(p, s) : launch_f<T, C, COLS, GRAD, DX, F, false, 1>(p, s);

@@ -178,6 +178,7 @@ def test_whole_tiles_of_rows(ops, n, d, c, order, dtype):
     out = labels < 0
     x[out.nonzero()[::3, 0]] = float("nan")
     want = reference(x, w, labels, b, r)
+    compare("loss", ops.softmax_xent(x, w, labels, b), want["loss"])
     for need_dx in (False, True):
         g = ops.softmax_xent_grad(x, w, labels, b, row_weight=r, need_dx=need_dx)
         for name in ("loss", "lse", "dw", "dbias") + (("dx",) if need_dx else ()):
