@@ -2,7 +2,7 @@
 //
 // The n x c logits never exist as a whole.  A forward call forms 256 x BN tiles of them in tensor
 // memory and keeps, per row, the running maximum and sum of exponentials.  A gradient call forms
-// them again piece by piece (kPieceBytes at a time), writes a piece's
+// them again piece by piece (piece_bytes at a time), writes a piece's
 //   g_ij = r_i (exp(z_ij - lse_i) - [j = y(i)])
 // in 16 bits and multiplies it with both sides:
 //   lse   z = x w^T, online softmax in the epilogue              2 n d c FLOP
@@ -13,12 +13,15 @@
 //
 // Types.  16-bit x and w are multiplied as they are (TMA reads them in place where their
 // strides allow, else from a copy); g is rounded once to their type (half a step, 2^-8 or 2^-11
-// relative, independent from element to element, which is what rounding the result costs too).
-// fp32 is split into hi + lo fp16 (22 bits) after a power-of-two scale per feature, and every
-// product is hi hi + hi lo + lo hi, so its products hold about 2^-22:
-//   x'_ik = x_ik 2^s_k, |x'| < 2^14     w'_jk = w_jk 2^(t - s_k), |w'| < 2^14
-//   z = 2^-t sum x' w'      dw_jk = 2^(-u - s_k) sum g' x'      dx_ik = 2^(s_k - t - u) sum g' w'
-// with g' = g 2^u (u from the largest row weight, in fp16 too; u = 0 in bf16).
+// relative, independent from element to element, which is what rounding the result costs too); in
+// fp16 it is scaled by a power of two first, from the largest row weight, and held to 2^-38 of that.
+// An fp32 value is held as three bf16 planes, its bits eight by eight, x = h + m + l exactly
+// (below 2^-110, to 2^-134), and so is g in fp32.  bf16 has fp32's exponents, so there is nothing to
+// scale and no value changes another's bits: a row, a feature, a class or a row weight far above the
+// others leaves them as they are.  A product is
+//   l h + h l + m m + m h + h m + h h        (left out: m l, l m, l l, below 3 x 2^-23 of |x||w|)
+// six 16-bit products, with everything that a 24-bit product holds but its last bit or two.  Two
+// fp16 planes with common scales would take three, but hold only 38 bits below the largest value.
 //
 // Kernel (pairs of CTAs, one CTA an SM, persistent, 12 warps; a pair makes 256 x BN tiles): warp 0
 // queues its CTA's TMA loads of 128 x 64 of A and BN / 2 x 64 of B into a ring; warp 1 of the
@@ -68,30 +71,32 @@ constexpr int kBK = 64;                      // 16-bit values of K to a stage
 constexpr int kABytes = kBM * kBK * 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr size_t kPieceBytes = (size_t)256 << 20;   // of g: several rounds of the pairs, not the n x c whole
+// Of a piece of g: several rounds of the pairs, not the n x c whole.  Three planes get as many values
+// as two would in 256 MB.
+constexpr size_t piece_bytes(int planes) { return (size_t)(planes == 3 ? 384 : 256) << 20; }
 
 enum { LSE = 0, G = 1, DX = 2, DW = 3, BOTH = 4 };
 
 constexpr int stage_bytes(int bn) { return kABytes + bn / 2 * kBK * 2; }   // of one CTA
-constexpr int stages_of(int bn, int out) { return bn == 256 ? (out > 4096 ? 5 : 6) : bn == 128 ? (out > 4096 ? 6 : 8) : 8; }
+// Ring stages.  fp32 holds three of them for a block of K and hands the first back a third of the
+// way through its products, so four keep the next block's loads under way.
+constexpr int stages_of(int bn, int out) { return bn == 256 ? (out > 4096 ? 4 : 6) : bn == 128 ? (out > 4096 ? 5 : 8) : out > 4096 ? 6 : 8; }
 // An epilogue warp's outgoing blocks: 32 rows x 128 bytes of each plane of g (64 bytes where a tile
 // has 64 columns), or of dx or dw (64 bytes in 16 bits).
-constexpr int out_bytes(int mode, int planes) { return (mode == G || mode == BOTH) && planes == 2 ? 8192 : 4096; }
+constexpr int out_bytes(int mode, int planes) { return (mode == G || mode == BOTH) && planes == 3 ? 12288 : 4096; }
 constexpr size_t smem_of(int bn, int out) {
     return (size_t)stages_of(bn, out) * stage_bytes(bn) + kEpiWarps * out + 1024 + 256;
 }
 static_assert(smem_of(256, 4096) <= 232448 && smem_of(128, 4096) <= 232448 && smem_of(64, 4096) <= 232448 &&
-                  smem_of(256, 8192) <= 232448 && smem_of(128, 8192) <= 232448 && smem_of(64, 8192) <= 232448,
+                  smem_of(256, 12288) <= 232448 && smem_of(128, 12288) <= 232448 && smem_of(64, 12288) <= 232448,
               "shared memory per CTA");
 
 // What the kernels of one call share on the device; cleared at its start.
 struct Meta {
     int err;                 // code of a wait that gave up
     uint32_t weight_bits;    // largest finite |row weight| as float bits
-    uint32_t w_exp;          // largest exponent of w_jk 2^-s_k, + kExpBias
     uint32_t poison;         // some left-out row of an x read in place holds a value that is not finite
 };
-constexpr int kExpBias = 4096;
 
 // exponent that brings a largest magnitude below 2^14 (0 for nothing to bring)
 __device__ __forceinline__ int fit_exponent(uint32_t max_bits) {
@@ -112,16 +117,11 @@ __device__ __forceinline__ float exp2_fast(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ int w_exponent(const Meta* m, int scaled) {
-    if (!scaled || m->w_exp == 0) return 0;
-    return min(126, max(-126, 13 - ((int)m->w_exp - kExpBias)));
-}
 __device__ __forceinline__ int g_exponent(const Meta* m, int half_g) { return half_g ? fit_exponent(m->weight_bits) : 0; }
 
 struct TcArgs {
-    CUtensorMap a[2], b[2];   // planes hi, lo
-    CUtensorMap out[2];       // G: planes of g; DX: dx
-    int scaled;               // fp32: power-of-two scales in force
+    CUtensorMap a[3], b[3];   // planes: one, or h, m, l of fp32 (b[1] also: see cleaned)
+    CUtensorMap out[3];       // G: planes of g; DX, DW: dx, dw
     int half_g;               // g in fp16 (scaled by 2^u), else bf16
     int units, m_tiles, n_tiles, splits;
     int per_split;            // LSE: class tiles of a split; DW: k blocks of a split
@@ -134,7 +134,6 @@ struct TcArgs {
     int64_t c_total;
     int c0;                   // first class of the piece
     Meta* meta;
-    const uint32_t* colmax;   // [d] largest |x_k| as float bits (fp32)
     const float* bias2;       // bias in base 2, -inf past the classes
     const int64_t* labels;
     float *loss_out, *lse_out;   // BOTH: [n]; the second may be null
@@ -150,8 +149,6 @@ struct TcArgs {
     void* dx;                 // DX; DW: dw
     int64_t dxr, dxk;
     int dx_map;               // out[0] is valid; else element stores
-    const float* undo;        // DX, DW in fp32: two factors a feature, undo_pitch apart
-    int64_t undo_pitch;
     int first, last;          // DX: first / last class piece; DW: first / last row piece
     float* sums;              // DX, DW: [split][128-row tile][feature tile][BN][128] of pieces and splits
     int64_t split_stride;
@@ -167,6 +164,15 @@ __device__ __forceinline__ uint32_t pack(float a, float b, __half) {
 __device__ __forceinline__ uint32_t pack(float a, float b, __nv_bfloat16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The bf16 thirds of two fp32 values, a in the lower halves: h the upper 8 bits, cut (rounding could
+// leave the type), m the next 8 of what is left, rounded, and l the rest.
+__device__ __forceinline__ void thirds(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    h = __byte_perm(ua, ub, 0x7632);
+    const float ra = a - __uint_as_float(ua & 0xffff0000u), rb = b - __uint_as_float(ub & 0xffff0000u);
+    m = pack(ra, rb, __nv_bfloat16{});
+    l = pack(ra - __uint_as_float(m << 16), rb - __uint_as_float(m & 0xffff0000u), __nv_bfloat16{});
 }
 
 // Outgoing blocks of 32 rows (the lanes) x 32 columns in shared memory, as TMA stores read them:
@@ -260,7 +266,7 @@ __device__ __forceinline__ float pick(const float* v, int i) {
     return t[0];
 }
 
-// E: type of the operand planes; kPlanes: 1, or hi and lo of fp32
+// E: type of the operand planes; kPlanes: 1, or the three of fp32
 template <int MODE, int BN, typename E, int kPlanes>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc_kernel(const __grid_constant__ TcArgs a) {
     constexpr int kOut = out_bytes(MODE, kPlanes);
@@ -313,11 +319,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     const int m0 = t.m * kPM + rank * kBM;
                     for (int r = 0; ok && r < t.tiles; ++r) {
                         const int n0 = (t.n + r) * BN + rank * (BN / 2);
-                        // two planes: a block of K takes two stages, (A hi, B lo) and (A lo, B hi)
+                        // three planes: a block of K takes three stages, l, h and m of both sides
                         for (int i = 0; i < t.kn * kPlanes; ++i, ++k) {
                             const int kb = t.kb + i / kPlanes;
-                            const CUtensorMap* ma = &a.a[i % kPlanes];
-                            const CUtensorMap* mb = &a.b[clean ? 1 : kPlanes - 1 - i % kPlanes];
+                            const int plane = kPlanes == 1 ? 0 : (i % kPlanes + 2) % kPlanes;
+                            const CUtensorMap* ma = &a.a[plane];
+                            const CUtensorMap* mb = &a.b[clean ? 1 : plane];
                             const uint32_t s = k % S, full = full_l + 8 * s;
                             // (a wait of a second is over long after the copies before it)
                             if (k >= S && !(ok = tc::bar_wait(empty0 + 8 * s, ((k / S) - 1) & 1, err, 1))) break;
@@ -375,27 +382,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             __syncwarp();
                         }
                     } else {
-                        // the chunk's small products first, hi lo and lo hi, as its stages arrive
-                        // (A hi with B lo, A lo with B hi); then hi hi across each pair of stages:
-                        // what the tensor cores cut off is a part of the sum so far
-                        const uint32_t k0 = k;
-                        for (; i < stop; ++i) {
-                            for (int h = 0; ok && h < 2; ++h, ++k) {
-                                const uint32_t s = k % S;
-                                if (!(ok = tc::bar_wait_warp(full0 + 8 * s, (k / S) & 1, err, 4))) break;
-                                tc::fence_after();
-                                if (lane == 0) multiply(s, s);
-                                __syncwarp();
+                        // (one block of K to a chunk) the small products first, as the stages arrive: what
+                        // the tensor cores cut off is a part of the sum so far
+                        for (; i < stop; ++i, k += 3) {
+                            const uint32_t sl = k % S, sh = (k + 1) % S, sm = (k + 2) % S;
+                            auto arrived = [&](uint32_t q) {
+                                ok = ok && tc::bar_wait_warp(full0 + 8 * (q % S), (q / S) & 1, err, 4);
+                                return ok;
+                            };
+                            if (!arrived(k) || !arrived(k + 1)) break;
+                            tc::fence_after();
+                            if (lane == 0) {
+                                multiply(sl, sh);
+                                multiply(sh, sl);
+                                tc::commit_both(empty0 + 8 * sl);
                             }
-                            if (!ok) break;
+                            __syncwarp();
+                            if (!arrived(k + 2)) break;
+                            tc::fence_after();
+                            if (lane == 0) {
+                                multiply(sm, sm);
+                                multiply(sm, sh);
+                                multiply(sh, sm);
+                                tc::commit_both(empty0 + 8 * sm);
+                                multiply(sh, sh);
+                                tc::commit_both(empty0 + 8 * sh);
+                            }
+                            __syncwarp();
                         }
-                        if (ok && lane == 0)
-                            for (uint32_t q = k0; q < k; q += 2) {
-                                multiply(q % S, (q + 1) % S);
-                                tc::commit_both(empty0 + 8 * (q % S));
-                                tc::commit_both(empty0 + 8 * ((q + 1) % S));
-                            }
-                        __syncwarp();
                     }
                     if (ok && lane == 0) tc::commit_both(afull0 + 8 * (acc & 1));
                     ++acc;
@@ -418,8 +432,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
         uint8_t* out = gbase + (out_addr - base);
         uint32_t acc = 0;
         bool ok = true;
-        const int te = w_exponent(a.meta, a.scaled), ue = g_exponent(a.meta, a.half_g);
-        const float f = pow2i(-te) * kLog2e;
+        const int ue = g_exponent(a.meta, a.half_g);
+        const float f = kLog2e;
         const uint32_t aempty_l = tc::in_leader(aempty0);
         // What a unit needs of its rows is loaded while the unit before it is worked on.
         struct Row {
@@ -594,25 +608,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                         if (q0 == 0) tc::store_wait_read<0>();          // the last store has read them
                         #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            *reinterpret_cast<uint4*>(out + g_unit<kSpan>(lane, q0 + q)) =
-                                make_uint4(pack(v[8 * q], v[8 * q + 1], E{}), pack(v[8 * q + 2], v[8 * q + 3], E{}),
-                                           pack(v[8 * q + 4], v[8 * q + 5], E{}), pack(v[8 * q + 6], v[8 * q + 7], E{}));
-                            if (kPlanes == 2) {
-                                uint32_t r[4];
-                                #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float h0 = to_float(from_float<E>(v[8 * q + 2 * i]));
-                                    const float h1 = to_float(from_float<E>(v[8 * q + 2 * i + 1]));
-                                    r[i] = pack(v[8 * q + 2 * i] - h0, v[8 * q + 2 * i + 1] - h1, E{});
-                                }
-                                *reinterpret_cast<uint4*>(out + kPlane + g_unit<kSpan>(lane, q0 + q)) =
-                                    make_uint4(r[0], r[1], r[2], r[3]);
+                            uint8_t* to = out + g_unit<kSpan>(lane, q0 + q);
+                            uint32_t h[4], m[4], l[4];
+                            #pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (kPlanes == 3)
+                                    thirds(v[8 * q + 2 * i], v[8 * q + 2 * i + 1], h[i], m[i], l[i]);
+                                else
+                                    h[i] = pack(v[8 * q + 2 * i], v[8 * q + 2 * i + 1], E{});
+                            }
+                            *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                            if (kPlanes == 3) {
+                                *reinterpret_cast<uint4*>(to + kPlane) = make_uint4(m[0], m[1], m[2], m[3]);
+                                *reinterpret_cast<uint4*>(to + 2 * kPlane) = make_uint4(l[0], l[1], l[2], l[3]);
                             }
                         }
                         if (here) {
-                            E* p = reinterpret_cast<E*>(out + g_unit<kSpan>(lane, q0 + (int)rel / 8)) + rel % 8;
-                            *p = from_float<E>(gy);
-                            if (kPlanes == 2) p[kPlane / 2] = from_float<E>(gy - to_float(from_float<E>(gy)));
+                            uint16_t* p = reinterpret_cast<uint16_t*>(out + g_unit<kSpan>(lane, q0 + (int)rel / 8)) + rel % 8;
+                            if (kPlanes == 3) {
+                                uint32_t h, m, l;
+                                thirds(gy, 0.f, h, m, l);
+                                p[0] = (uint16_t)h;
+                                p[kPlane / 2] = (uint16_t)m;
+                                p[kPlane] = (uint16_t)l;
+                            } else {
+                                p[0] = (uint16_t)pack(gy, 0.f, E{});
+                            }
                         }
                         // (past the last class the second block holds what it held: nobody reads there)
                         if (ch % kSpan == kSpan - 1 || cb + 32 >= a.cols) {
@@ -620,7 +641,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             __syncwarp();
                             if (lane == 0 && y0 < a.rows) {
                                 tc::store_2d(&a.out[0], out_addr, (int)cb - 8 * q0, (int)y0);
-                                if (kPlanes == 2) tc::store_2d(&a.out[1], out_addr + kPlane, (int)cb - 8 * q0, (int)y0);
+                                if (kPlanes == 3) {
+                                    tc::store_2d(&a.out[1], out_addr + kPlane, (int)cb - 8 * q0, (int)y0);
+                                    tc::store_2d(&a.out[2], out_addr + 2 * kPlane, (int)cb - 8 * q0, (int)y0);
+                                }
                                 tc::store_commit();
                             }
                         }
@@ -648,20 +672,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             for (int j = 0; j < 32; ++j) keep[j * kBM] = v[j];
                             continue;
                         }
-                        using D = typename std::conditional<kPlanes == 2, float, E>::type;
+                        using D = typename std::conditional<kPlanes == 3, float, E>::type;
                         const int count = (int)min((int64_t)32, a.cols - cb);
-                        if (kPlanes == 2) {
-                            const float4* f4 = reinterpret_cast<const float4*>(a.undo + cb);
-                            const float4* g4 = reinterpret_cast<const float4*>(a.undo + a.undo_pitch + cb);
-                            #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float4 p = __ldg(f4 + j), q = __ldg(g4 + j);
-                                v[4 * j] = v[4 * j] * p.x * q.x;
-                                v[4 * j + 1] = v[4 * j + 1] * p.y * q.y;
-                                v[4 * j + 2] = v[4 * j + 2] * p.z * q.z;
-                                v[4 * j + 3] = v[4 * j + 3] * p.w * q.w;
-                            }
-                        } else {
+                        if (a.half_g) {
                             const float q = pow2i(-ue);
                             #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] *= q;
@@ -846,196 +859,74 @@ __device__ __forceinline__ float4 load_quad(const float* row, int64_t k, int64_t
     if (k + 4 <= d) return *reinterpret_cast<const float4*>(row + k);
     return make_float4(k < d ? row[k] : 0.f, k + 1 < d ? row[k + 1] : 0.f, k + 2 < d ? row[k + 2] : 0.f, 0.f);
 }
-__device__ __forceinline__ float finite_abs(float v) {
-    v = fabsf(v);
-    return v <= 3.402823466e38f ? v : 0.f;
-}
-
 __device__ __forceinline__ bool row_counts(const uint32_t* keep, int64_t r) { return (keep[r >> 5] >> (r & 31)) & 1; }
 
-// Largest finite |x_k| over the rows that count (the bits of `keep`).
-//   kRows    x row by row in 16-byte units: a block takes `rows` rows of 1024 features, a thread four
-//            of them, several rows at once where the features are fewer
-//   kColumns x column by column: a block takes `rows` rows of one feature
-//   kAny     a block takes `rows` rows of 32 features
-enum { kRows = 0, kColumns = 1, kAny = 2 };
-__global__ void __launch_bounds__(256) xent_colmax_kernel(const float* __restrict__ x, int64_t xr, int64_t xk,
-                                                          const uint32_t* __restrict__ keep, int64_t n, int64_t d,
-                                                          int64_t rows, int order, uint32_t* colmax) {
-    __shared__ uint32_t top[1024];
-    const int64_t width = order == kRows ? 1024 : order == kColumns ? 1 : 32, blocks_k = (d + width - 1) / width;
-    const int64_t k0 = (blockIdx.x % blocks_k) * width, r0 = (blockIdx.x / blocks_k) * rows, r1 = min(n, r0 + rows);
-    for (int i = threadIdx.x; i < width; i += 256) top[i] = 0;
-    __syncthreads();
-    if (order == kRows) {
-        const int quads = (int)min((int64_t)256, (d - k0 + 3) / 4), at_once = 256 / quads;
-        const int quad = threadIdx.x % quads, ro = threadIdx.x / quads;
-        if (ro < at_once) {
-            float m[4] = {0.f, 0.f, 0.f, 0.f};
-            #pragma unroll 8
-            for (int64_t r = r0 + ro; r < r1; r += at_once) {
-                const float4 v = load_quad(x + r * xr, k0 + 4 * quad, d);
-                const bool in = row_counts(keep, r);
-                m[0] = fmaxf(m[0], in ? finite_abs(v.x) : 0.f);
-                m[1] = fmaxf(m[1], in ? finite_abs(v.y) : 0.f);
-                m[2] = fmaxf(m[2], in ? finite_abs(v.z) : 0.f);
-                m[3] = fmaxf(m[3], in ? finite_abs(v.w) : 0.f);
-            }
-            for (int i = 0; i < 4; ++i) atomicMax(&top[4 * quad + i], __float_as_uint(m[i]));
-        }
-    } else if (order == kColumns) {
-        const float* p = x + k0 * xk;
-        float m = 0.f;
-        if ((uintptr_t)p % 16 == 0) {   // r0 is a multiple of 32
-            #pragma unroll 4
-            for (int64_t r = r0 + 4 * threadIdx.x; r < r1; r += 1024) {
-                const float4 v = load_quad(p, r, n);
-                const uint32_t bits = keep[r >> 5] >> (r & 31);
-                m = fmaxf(m, bits & 1 ? finite_abs(v.x) : 0.f);
-                m = fmaxf(m, bits & 2 ? finite_abs(v.y) : 0.f);
-                m = fmaxf(m, bits & 4 ? finite_abs(v.z) : 0.f);
-                m = fmaxf(m, bits & 8 ? finite_abs(v.w) : 0.f);
-            }
-        } else {
-            #pragma unroll 8
-            for (int64_t r = r0 + threadIdx.x; r < r1; r += 256)
-                if (row_counts(keep, r)) m = fmaxf(m, finite_abs(p[r]));
-        }
-        const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-        if ((threadIdx.x & 31) == 0) atomicMax(&top[0], w);
-    } else {
-        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-        float m = 0.f;
-        if (k0 + tx < d)
-            #pragma unroll 4
-            for (int64_t r = r0 + ty; r < r1; r += 8)
-                if (row_counts(keep, r)) m = fmaxf(m, finite_abs(x[r * xr + (k0 + tx) * xk]));
-        atomicMax(&top[tx], __float_as_uint(m));
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < width; i += 256)
-        if (k0 + i < d && top[i]) atomicMax(&colmax[k0 + i], top[i]);
+// thirds() of two values; one that is not finite is h alone
+__device__ __forceinline__ void split3(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
+    thirds(a, b, h, m, l);
+    // (a NaN that holds its bits in the lower half would be cut to infinity)
+    const bool fa = fabsf(a) <= 3.402823466e38f, fb = fabsf(b) <= 3.402823466e38f;
+    if (fa && fb) return;
+    h = pack(fa ? __uint_as_float(h << 16) : a, fb ? __uint_as_float(h & 0xffff0000u) : b, __nv_bfloat16{});
+    const uint32_t keep = (fa ? 0xffffu : 0u) | (fb ? 0xffff0000u : 0u);
+    m &= keep;
+    l &= keep;
 }
 
-// largest exponent of w_jk 2^-s_k: a block takes `rows` classes of 1024 features (kRows) or of 32
-__global__ void __launch_bounds__(256) xent_wmax_kernel(const float* __restrict__ w, int64_t wr, int64_t wk, int64_t c,
-                                                        int64_t d, int64_t rows, int order,
-                                                        const uint32_t* __restrict__ colmax, Meta* meta) {
-    const int64_t width = order == kRows ? 1024 : 32, blocks_k = (d + width - 1) / width;
-    const int64_t k0 = (blockIdx.x % blocks_k) * width, r0 = (blockIdx.x / blocks_k) * rows, r1 = min(c, r0 + rows);
-    int top = 0;
-    auto exponent = [](float v, int s) {
-        const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-        return b && b < 0x7f800000u ? (int)(b >> 23) - 127 - s + kExpBias : 0;
-    };
-    if (order == kRows) {
-        const int quads = (int)min((int64_t)256, (d - k0 + 3) / 4), at_once = 256 / quads;
-        const int quad = threadIdx.x % quads, ro = threadIdx.x / quads;
-        const int64_t k = k0 + 4 * quad;
-        int s[4];
-        for (int i = 0; i < 4; ++i) s[i] = k + i < d ? fit_exponent(colmax[k + i]) : 0;
-        if (ro < at_once)
-            #pragma unroll 8
-            for (int64_t r = r0 + ro; r < r1; r += at_once) {
-                const float4 v = load_quad(w + r * wr, k, d);
-                top = max(max(top, exponent(v.x, s[0])), exponent(v.y, s[1]));
-                top = max(max(top, exponent(v.z, s[2])), exponent(v.w, s[3]));
-            }
-    } else {
-        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-        if (k0 + tx < d) {
-            const int s = fit_exponent(colmax[k0 + tx]);
-            #pragma unroll 8
-            for (int64_t r = r0 + ty; r < r1; r += 8) top = max(top, exponent(w[r * wr + (k0 + tx) * wk], s));
-        }
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0 && top) atomicMax(&meta->w_exp, (uint32_t)top);
-}
+// What the operands' copies are made of and go to: rows x d -> planes [rows][dp], zero past the
+// features and in rows with a negative label.
+struct PlaneArgs {
+    const void* x;
+    int64_t xr, xk;
+    const uint32_t* keep;     // nullable: bit r of word r / 32: row r counts
+    int64_t rows, d, dp;
+    int64_t per_block;        // xent_planes_rows_kernel: rows a block
+    const Meta* meta;
+    int if_poison;            // nothing to do unless meta->poison is set
+    uint16_t* to[3];          // one plane of 16 bits, or h, m, l of fp32
+};
 
-// Exponent that a plane's values of feature k are scaled by.
-__device__ __forceinline__ int plane_exponent(const uint32_t* colmax, const Meta* meta, int64_t k, int64_t d, int is_w) {
-    const int e = k < d ? fit_exponent(colmax[k]) : 0;
-    return is_w ? w_exponent(meta, 1) - e : e;
-}
-// hi and lo of two scaled values; nothing below a value that is not finite
-__device__ __forceinline__ void split2(float v0, float v1, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(v0, v1);
-    const float2 f = __half22float2(h);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = pack(isfinite(f.x) ? v0 - f.x : 0.f, isfinite(f.y) ? v1 - f.y : 0.f, __half{});
-}
-
-// fp32 rows in 16-byte units -> planes [rows][dp], hi and lo fp16 of the scaled values; rows with
-// a negative label become zeros.  A thread keeps four features and their scales over its rows.
-__global__ void __launch_bounds__(256) xent_planes_rows_kernel(const float* __restrict__ x, int64_t xr,
-                                                               const uint32_t* __restrict__ keep, int64_t n, int64_t d,
-                                                               int64_t dp, int64_t rows, const uint32_t* __restrict__ colmax,
-                                                               const Meta* __restrict__ meta, int is_w,
-                                                               __half* __restrict__ hi, __half* __restrict__ lo) {
-    const int64_t blocks_k = (dp + 1023) / 1024;
-    const int64_t k0 = (blockIdx.x % blocks_k) * 1024, r0 = (blockIdx.x / blocks_k) * rows, r1 = min(n, r0 + rows);
-    const int quads = (int)min((int64_t)256, (dp - k0) / 4), at_once = 256 / quads;
+// fp32 rows in 16-byte units: a block takes some rows of 1024 features, a thread four of them,
+// several rows at once where the features are fewer.
+__global__ void __launch_bounds__(256) xent_planes_rows_kernel(const PlaneArgs a) {
+    const int64_t blocks_k = (a.dp + 1023) / 1024;
+    const int64_t k0 = (blockIdx.x % blocks_k) * 1024, r0 = (blockIdx.x / blocks_k) * a.per_block;
+    const int64_t r1 = min(a.rows, r0 + a.per_block);
+    const int quads = (int)min((int64_t)256, (a.dp - k0) / 4), at_once = 256 / quads;
     const int quad = threadIdx.x % quads, ro = threadIdx.x / quads;
     if (ro >= at_once) return;
     const int64_t k = k0 + 4 * quad;
-    float f0[4], f1[4];
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int e = plane_exponent(colmax, meta, k + i, d, is_w), h = e / 2;
-        f0[i] = pow2i(h);
-        f1[i] = pow2i(e - h);
-    }
     #pragma unroll 4
     for (int64_t r = r0 + ro; r < r1; r += at_once) {
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!keep || row_counts(keep, r)) v = load_quad(x + r * xr, k, d);
-        uint2 h, l;
-        split2(v.x * f0[0] * f1[0], v.y * f0[1] * f1[1], h.x, l.x);
-        split2(v.z * f0[2] * f1[2], v.w * f0[3] * f1[3], h.y, l.y);
-        *reinterpret_cast<uint2*>(hi + r * dp + k) = h;
-        *reinterpret_cast<uint2*>(lo + r * dp + k) = l;
+        if (!a.keep || row_counts(a.keep, r)) v = load_quad((const float*)a.x + r * a.xr, k, a.d);
+        uint2 h, m, l;
+        split3(v.x, v.y, h.x, m.x, l.x);
+        split3(v.z, v.w, h.y, m.y, l.y);
+        *reinterpret_cast<uint2*>(a.to[0] + r * a.dp + k) = h;
+        *reinterpret_cast<uint2*>(a.to[1] + r * a.dp + k) = m;
+        *reinterpret_cast<uint2*>(a.to[2] + r * a.dp + k) = l;
     }
 }
 
-// Factors that undo the scales of the gradients, each as two that fp32 holds: 2^(s_k - t - u) of dx,
-// then 2^(-s_k - u) of dw.
-__global__ void __launch_bounds__(256) xent_undo_kernel(const uint32_t* __restrict__ colmax, int64_t d, int64_t pitch,
-                                                        const Meta* __restrict__ meta, float* __restrict__ undo) {
-    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (k >= pitch) return;
-    const int s = k < d ? fit_exponent(colmax[k]) : 0, u = g_exponent(meta, 1);
-    const int e[2] = {s - w_exponent(meta, 1) - u, -s - u};
-    for (int i = 0; i < 2; ++i) {
-        const int c = min(252, max(-252, e[i])), h = c / 2;
-        undo[2 * i * pitch + k] = pow2i(h);
-        undo[(2 * i + 1) * pitch + k] = pow2i(c - h);
-    }
-}
-
-// rows x d of any strides -> planes [rows][dp], a 64 x 64 tile a block; rows with a negative label
-// become zeros.  fp32: hi and lo fp16 of the scaled value; 16 bits: a copy (if_poison: only where
-// one is needed).
+// any strides, a 64 x 64 tile a block; T: type of x, E: of the planes
 template <typename T, typename E>
-__global__ void __launch_bounds__(256) xent_planes_kernel(const T* __restrict__ x, int64_t xr, int64_t xk,
-                                                          const uint32_t* __restrict__ keep, int64_t n, int64_t d,
-                                                          int64_t dp, const uint32_t* __restrict__ colmax,
-                                                          const Meta* __restrict__ meta, int is_w, int if_poison,
-                                                          E* __restrict__ hi, E* __restrict__ lo) {
+__global__ void __launch_bounds__(256) xent_planes_kernel(const PlaneArgs a) {
     __shared__ float t[64][65];      // [feature][row]
-    if (if_poison && meta->poison == 0) return;
-    const int64_t tiles_k = (dp + 63) / 64;
+    if (a.if_poison && a.meta->poison == 0) return;
+    const int64_t tiles_k = (a.dp + 63) / 64;
     const int64_t k0 = (blockIdx.x % tiles_k) * 64, r0 = (blockIdx.x / tiles_k) * 64;
-    const bool down = xr == 1 && xk != 1;
-    if (down && sizeof(T) == 4 && (uintptr_t)x % 16 == 0 && xk % 4 == 0) {
+    const T* x = (const T*)a.x;
+    const bool down = a.xr == 1 && a.xk != 1;
+    if (down && sizeof(T) == 4 && (uintptr_t)x % 16 == 0 && a.xk % 4 == 0) {
         // four rows of a feature at a time
         #pragma unroll
         for (int i = threadIdx.x; i < 64 * 16; i += 256) {
             const int r = (i & 15) * 4, k = i >> 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r0 + r < n && k0 + k < d) {
-                v = load_quad((const float*)x + (k0 + k) * xk, r0 + r, n);
-                const uint32_t bits = keep ? keep[(r0 + r) >> 5] >> ((r0 + r) & 31) : 15;
+            if (r0 + r < a.rows && k0 + k < a.d) {
+                v = load_quad((const float*)x + (k0 + k) * a.xk, r0 + r, a.rows);
+                const uint32_t bits = a.keep ? a.keep[(r0 + r) >> 5] >> ((r0 + r) & 31) : 15;
                 if (!(bits & 1)) v.x = 0.f;
                 if (!(bits & 2)) v.y = 0.f;
                 if (!(bits & 4)) v.z = 0.f;
@@ -1051,42 +942,33 @@ __global__ void __launch_bounds__(256) xent_planes_kernel(const T* __restrict__ 
         for (int i = threadIdx.x; i < 64 * 64; i += 256) {
             const int r = down ? i & 63 : i >> 6, k = down ? i >> 6 : i & 63;
             float v = 0.f;
-            if (r0 + r < n && k0 + k < d && (!keep || row_counts(keep, r0 + r)))
-                v = to_float(x[(r0 + r) * xr + (k0 + k) * xk]);
+            if (r0 + r < a.rows && k0 + k < a.d && (!a.keep || row_counts(a.keep, r0 + r)))
+                v = to_float(x[(r0 + r) * a.xr + (k0 + k) * a.xk]);
             t[k][r] = v;
         }
     }
     __syncthreads();
     // 8 features of a row to a thread, 16 bytes of a plane
     const int k = (threadIdx.x & 7) * 8;
-    if (k0 + k >= dp) return;
-    float f0[8], f1[8];
-    if constexpr (sizeof(T) == 4) {
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int e = plane_exponent(colmax, meta, k0 + k + i, d, is_w), h = e / 2;
-            f0[i] = pow2i(h);
-            f1[i] = pow2i(e - h);
-        }
-    }
+    if (k0 + k >= a.dp) return;
     #pragma unroll
     for (int r = threadIdx.x >> 3; r < 64; r += 32) {
-        if (r0 + r >= n) break;
-        const int64_t at = (r0 + r) * dp + k0 + k;
-        uint32_t h[4], l[4];
+        if (r0 + r >= a.rows) break;
+        const int64_t at = (r0 + r) * a.dp + k0 + k;
+        uint32_t h[4], m[4], l[4];
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float v0 = t[k + 2 * i][r], v1 = t[k + 2 * i + 1][r];
-            if constexpr (sizeof(T) == 4) {
-                v0 = v0 * f0[2 * i] * f1[2 * i];
-                v1 = v1 * f0[2 * i + 1] * f1[2 * i + 1];
-                split2(v0, v1, h[i], l[i]);
-            } else {
+            const float v0 = t[k + 2 * i][r], v1 = t[k + 2 * i + 1][r];
+            if constexpr (sizeof(T) == 4)
+                split3(v0, v1, h[i], m[i], l[i]);
+            else
                 h[i] = pack(v0, v1, E{});
-            }
         }
-        *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+        *reinterpret_cast<uint4*>(a.to[0] + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<uint4*>(a.to[1] + at) = make_uint4(m[0], m[1], m[2], m[3]);
+            *reinterpret_cast<uint4*>(a.to[2] + at) = make_uint4(l[0], l[1], l[2], l[3]);
+        }
     }
 }
 
@@ -1144,8 +1026,7 @@ __global__ void __launch_bounds__(256) xent_finish_kernel(int64_t c, int64_t d, 
 // with a negative label (dx) are zero.
 template <typename T>
 __global__ void __launch_bounds__(256) xent_sum_kernel(const float* __restrict__ sums, int splits, int64_t split_stride,
-                                                       int n_tiles, int bn, int64_t rows, int d,
-                                                       const float* __restrict__ undo, int64_t undo_pitch, int half_g,
+                                                       int n_tiles, int bn, int64_t rows, int d, int half_g,
                                                        const Meta* __restrict__ meta, const int64_t* __restrict__ labels,
                                                        T* __restrict__ out, int64_t out_row, int64_t out_col) {
     __shared__ float t[8][33];
@@ -1158,7 +1039,7 @@ __global__ void __launch_bounds__(256) xent_sum_kernel(const float* __restrict__
         double v = 0.0;
         #pragma unroll 8
         for (int s = 0; s < splits; ++s) v += (double)p[s * split_stride];
-        float f = undo ? (float)v * undo[k] * undo[undo_pitch + k] : scale2((float)v, -g_exponent(meta, half_g));
+        float f = scale2((float)v, -g_exponent(meta, half_g));
         if (labels && labels[r0 + tx] < 0) f = 0.f;
         t[ty][tx] = f;
     }
@@ -1244,18 +1125,14 @@ struct Plan {
     bool products;                   // dx or dw or dbias wanted
     // workspace
     Meta* meta;
-    uint32_t* colmax;
-    size_t meta_bytes;
     float* bias2;
     uint32_t* keep;
     uint16_t* xc;                    // x without left-out rows, made where one of those holds no number
-    uint16_t *xh, *xl, *wh, *wl, *gh, *gl;
+    uint16_t *x[3], *w[3], *g[3];    // planes; null where the operands are read in place
     float2* part;
     float* zy;
     float2* shift;
     float* dx_sums;
-    float* undo;
-    int64_t undo_pitch;
     float* dw_part;
     float* bias_sums;
     double* bias_part;
@@ -1264,7 +1141,7 @@ struct Plan {
 
 Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
     Plan p{};
-    p.planes = a.type == GAFIME_TYPE_FP32 ? 2 : 1;
+    p.planes = a.type == GAFIME_TYPE_FP32 ? 3 : 1;
     p.bn_c = tile_n(a.c);
     const int pairs = sms / 2;
     p.x_in_place = in_place(a.type, a.x, a.xr, a.xk, a.d);
@@ -1286,32 +1163,29 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
 
     Carver cv(ws);
     p.meta = cv.take<Meta>(1);
-    p.colmax = cv.take<uint32_t>(p.planes == 2 ? a.d : 0);
-    p.meta_bytes = cv.used;
     p.bias2 = cv.take<float>(p.c_tiles * p.bn_c + 256);
     p.keep = cv.take<uint32_t>(cdiv(a.n, 32) + 2);
-    if (p.planes == 2 || !p.x_in_place) p.xh = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
-    if (p.planes == 2) p.xl = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
-    if (p.planes == 2 || !p.w_in_place) p.wh = cv.take<uint16_t>(a.c * p.dp);
-    if (p.planes == 2) p.wl = cv.take<uint16_t>(a.c * p.dp);
+    for (int i = 0; i < p.planes; ++i) {
+        if (!p.x_in_place) p.x[i] = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
+        if (!p.w_in_place) p.w[i] = cv.take<uint16_t>(a.c * p.dp);
+    }
     if (a.gradient && a.dw && p.x_in_place) p.xc = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
     p.part = cv.take<float2>(a.n * 2 * p.splits);
     p.zy = cv.take<float>(a.n);
     if (p.products) {
         p.shift = cv.take<float2>(a.n);
-        // a piece of g: rows for one row tile an SM, then as many classes as kPieceBytes hold
+        // a piece of g: rows for one row tile an SM, then as many classes as piece_bytes hold
         const int64_t es = 2 * p.planes;
         p.piece_rows = std::min<int64_t>(up(a.n, kPM), (int64_t)pairs * kPM);
-        p.piece_classes = std::max<int64_t>(1024, (int64_t)(kPieceBytes / (p.piece_rows * es)) / 256 * 256);
+        p.piece_classes = std::max<int64_t>(1024, (int64_t)(piece_bytes(p.planes) / (p.piece_rows * es)) / 256 * 256);
         if (p.piece_classes >= a.c) {
             p.piece_classes = a.c;
             // few classes: more rows at once, still whole rounds of the SMs
-            const int64_t more = (int64_t)(kPieceBytes / (p.piece_rows * es * up(a.c, 8)));
+            const int64_t more = (int64_t)(piece_bytes(p.planes) / (p.piece_rows * es * up(a.c, 8)));
             if (more > 1) p.piece_rows = std::min<int64_t>(up(a.n, kPM), p.piece_rows * more);
         }
         p.ldg = up(p.piece_classes, 64);   // whole 128-byte lines: TMA boxes meet no line twice
-        p.gh = cv.take<uint16_t>(p.piece_rows * p.ldg);
-        if (p.planes == 2) p.gl = cv.take<uint16_t>(p.piece_rows * p.ldg);
+        for (int i = 0; i < p.planes; ++i) p.g[i] = cv.take<uint16_t>(p.piece_rows * p.ldg);
         // Feature tiles of 128 or 256 (a CTA's half is whole 64-value lines), and the sum over classes
         // (dx) or rows (dw) split over pairs that the tiles leave idle, in runs of at least 4 blocks:
         // what takes the fewest rounds, where a block of 128 takes about 0.6 of one of 256
@@ -1344,8 +1218,6 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
         p.dx_stride = p.piece_rows * p.dx_d_tiles * p.bn_dx;
         p.dw_c_tiles = cdiv(a.c, kPM) * 2;
         p.dw_stride = p.dw_c_tiles * p.dw_d_tiles * p.bn_dw * kBM;
-        p.undo_pitch = up(a.d, 256);
-        if (p.planes == 2) p.undo = cv.take<float>(4 * p.undo_pitch);
         if (a.dx && (!p.dx_direct || p.piece_classes < a.c)) p.dx_sums = cv.take<float>(p.dx_splits * p.dx_stride);
         if (a.dw) {
             p.dw_direct = p.dw_splits == 1;
@@ -1400,22 +1272,18 @@ cudaError_t launch(const TcArgs& t, int bn, int sms, cudaStream_t stream) {
     } while (0)
 
 template <typename T, typename E>
-cudaError_t planes(const Plan& p, const T* src, int64_t sr, int64_t sk, const uint32_t* keep, int64_t rows, int64_t d,
-                   bool is_w, bool if_poison, uint16_t* hi, uint16_t* lo, int sms, cudaStream_t stream) {
+cudaError_t planes(PlaneArgs s, int sms, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
-        if (rows_vector(src, sr, sk)) {
-            const int64_t blocks_k = cdiv(p.dp, 1024);
-            const int64_t per = std::max<int64_t>(16, cdiv(rows * blocks_k, 16 * sms));
+        if (rows_vector(s.x, s.xr, s.xk)) {
+            const int64_t blocks_k = cdiv(s.dp, 1024);
+            s.per_block = std::max<int64_t>(16, cdiv(s.rows * blocks_k, 16 * sms));
             KernelTimer kt(stream, GAFIME_KERNEL_XENT);
-            xent_planes_rows_kernel<<<(unsigned)(blocks_k * cdiv(rows, per)), 256, 0, stream>>>(
-                src, sr, keep, rows, d, p.dp, per, p.colmax, p.meta, is_w, (__half*)hi, (__half*)lo);
+            xent_planes_rows_kernel<<<(unsigned)(blocks_k * cdiv(s.rows, s.per_block)), 256, 0, stream>>>(s);
             return cudaGetLastError();
         }
     }
-    const int64_t blocks = cdiv(p.dp, 64) * cdiv(rows, 64);
     KernelTimer kt(stream, GAFIME_KERNEL_XENT);
-    xent_planes_kernel<T, E><<<(unsigned)blocks, 256, 0, stream>>>(src, sr, sk, keep, rows, d, p.dp, p.colmax, p.meta,
-                                                                   is_w, if_poison, (E*)hi, (E*)lo);
+    xent_planes_kernel<T, E><<<(unsigned)(cdiv(s.dp, 64) * cdiv(s.rows, 64)), 256, 0, stream>>>(s);
     return cudaGetLastError();
 }
 
@@ -1423,15 +1291,14 @@ template <typename T, typename E>
 cudaError_t run_tc(const XentCall& a, int sms) {
     const Plan p = make_plan(a, sms, a.ws);
     constexpr bool kBf16 = std::is_same<E, __nv_bfloat16>::value;
-    constexpr int kPlanes = std::is_same<T, float>::value ? 2 : 1;
-    const bool scaled = p.planes == 2;
+    constexpr int kPlanes = std::is_same<T, float>::value ? 3 : 1;
     cudaStream_t st = a.stream;
     if (a.n == 0) {   // gradients of no rows
         if (a.dw) XENT_TRY(cudaMemsetAsync(a.dw, 0, (size_t)(a.c * a.d) * sizeof(T), st));
         if (a.dbias) XENT_TRY(cudaMemsetAsync(a.dbias, 0, a.c * 4, st));
         return cudaSuccess;
     }
-    XENT_TRY(cudaMemsetAsync(p.meta, 0, p.meta_bytes, st));
+    XENT_TRY(cudaMemsetAsync(p.meta, 0, sizeof(Meta), st));
     // one tile of classes: the call's losses come with its g
     const bool both = p.products && !a.have_lse && p.c_tiles == 1;
     const bool forward = !a.have_lse && !both;
@@ -1441,7 +1308,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         s.want_weight = p.products && !kBf16;
         s.bias = a.bias; s.bias2 = p.bias2; s.c = a.c; s.c_pad = p.c_tiles * p.bn_c + 256;
         s.zy = forward ? p.zy : nullptr;
-        s.keep = p.xh || p.xc ? p.keep : nullptr;
+        s.keep = p.x[0] || p.xc ? p.keep : nullptr;
         s.meta = p.meta;
         const int64_t threads = std::max<int64_t>(s.c_pad, a.n);
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
@@ -1453,46 +1320,33 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         xent_poison_kernel<<<(unsigned)std::min<int64_t>(8 * sms, cdiv(a.n, 8)), 256, 0, st>>>(
             a.labels, a.n, (const uint16_t*)a.x, a.xr, a.d, kBf16, p.meta);
         XENT_TRY(cudaGetLastError());
-        XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, p.keep, a.n, a.d, false, true, p.xc, nullptr, sms, st)));
+        PlaneArgs s{a.x, a.xr, a.xk, p.keep, a.n, a.d, p.dp, 0, p.meta, 1, {p.xc, nullptr, nullptr}};
+        XENT_TRY((planes<T, E>(s, sms, st)));
     }
-    if (scaled) {
-        {
-            const int order = rows_vector(a.x, a.xr, a.xk) ? kRows : a.xr == 1 && a.xk != 1 ? kColumns : kAny;
-            const int64_t blocks_k = cdiv(a.d, order == kRows ? 1024 : order == kColumns ? 1 : 32);
-            const int64_t rows = up(std::max<int64_t>(order == kColumns ? 1024 : 64, cdiv(a.n * blocks_k, 8 * sms)), 32);
-            KernelTimer kt(st, GAFIME_KERNEL_XENT);
-            xent_colmax_kernel<<<(unsigned)(blocks_k * cdiv(a.n, rows)), 256, 0, st>>>(
-                (const float*)a.x, a.xr, a.xk, p.keep, a.n, a.d, rows, order, p.colmax);
-            XENT_TRY(cudaGetLastError());
-        }
-        const int order = rows_vector(a.w, a.wr, a.wk) ? kRows : kAny;
-        const int64_t blocks_k = cdiv(a.d, order == kRows ? 1024 : 32);
-        const int64_t rows = std::max<int64_t>(16, cdiv(a.c * blocks_k, 8 * sms));
-        KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_wmax_kernel<<<(unsigned)(blocks_k * cdiv(a.c, rows)), 256, 0, st>>>(
-            (const float*)a.w, a.wr, a.wk, a.c, a.d, rows, order, p.colmax, p.meta);
-        XENT_TRY(cudaGetLastError());
+    if (p.x[0]) {
+        PlaneArgs s{a.x, a.xr, a.xk, p.keep, a.n, a.d, p.dp, 0, p.meta, 0, {p.x[0], p.x[1], p.x[2]}};
+        XENT_TRY((planes<T, E>(s, sms, st)));
     }
-    if (p.xh) XENT_TRY((planes<T, E>(p, (const T*)a.x, a.xr, a.xk, p.keep, a.n, a.d, false, false, p.xh, p.xl, sms, st)));
-    if (p.wh) XENT_TRY((planes<T, E>(p, (const T*)a.w, a.wr, a.wk, nullptr, a.c, a.d, true, false, p.wh, p.wl, sms, st)));
+    if (p.w[0]) {
+        PlaneArgs s{a.w, a.wr, a.wk, nullptr, a.c, a.d, p.dp, 0, p.meta, 0, {p.w[0], p.w[1], p.w[2]}};
+        XENT_TRY((planes<T, E>(s, sms, st)));
+    }
     // where the operands are read
-    const void *xs[2] = {p.xh ? (const void*)p.xh : a.x, p.xl}, *ws[2] = {p.wh ? (const void*)p.wh : a.w, p.wl};
-    const int64_t ldx = p.xh ? p.dp : a.xr, ldw = p.wh ? p.dp : a.wr;
-    auto map = [&](CUtensorMap (&m)[2], const void* const (&base)[2], int64_t inner, int64_t rows, int64_t ld, int box) {
+    const void *xs[3] = {p.x[0] ? (const void*)p.x[0] : a.x, p.x[1], p.x[2]};
+    const void *ws[3] = {p.w[0] ? (const void*)p.w[0] : a.w, p.w[1], p.w[2]};
+    const int64_t ldx = p.x[0] ? p.dp : a.xr, ldw = p.w[0] ? p.dp : a.wr;
+    auto map = [&](CUtensorMap (&m)[3], const void* const (&base)[3], int64_t inner, int64_t rows, int64_t ld, int box) {
         for (int i = 0; i < p.planes; ++i)
             if (!make_map(&m[i], kBf16, base[i], inner, rows, ld, box)) return cudaErrorInvalidValue;
         return cudaSuccess;
     };
 
     TcArgs t{};
-    // fp32: 4 products of the large planes to a block, each cutting about 2^-24 of the sum; two
-    // blocks (6e-7) keep the drains of tensor memory, 128 KB a CTA beside the running MMAs, behind
-    // them.  16 bits: 32 products and more are nothing beside the operands' rounding.
-    t.chunk = p.planes == 2 ? 2 : 8;
-    t.scaled = scaled;
+    // k blocks summed in tensor memory at a time.  fp32: one, 4 products of the h planes, each cutting
+    // about 2^-24 of the sum.  16 bits: 32 products and more are nothing beside the operands' rounding.
+    t.chunk = p.planes == 3 ? 1 : 8;
     t.half_g = !kBf16;
     t.meta = p.meta;
-    t.colmax = p.colmax;
     t.bias2 = p.bias2;
     t.labels = a.labels;
     t.weight = a.weight; t.weight_stride = a.weight_stride; t.scale = a.scale;
@@ -1523,12 +1377,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     }
     if (!p.products) return cudaSuccess;
 
-    if (p.undo) {
-        KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_undo_kernel<<<(unsigned)cdiv(p.undo_pitch, 256), 256, 0, st>>>(p.colmax, a.d, p.undo_pitch, p.meta, p.undo);
-        XENT_TRY(cudaGetLastError());
-    }
-    const void* gs[2] = {p.gh, p.gl};
+    const void* gs[3] = {p.g[0], p.g[1], p.g[2]};
     for (int64_t r0 = 0; r0 < a.n; r0 += p.piece_rows) {
         const int64_t rows = std::min(p.piece_rows, a.n - r0);
         for (int64_t c0 = 0; c0 < a.c; c0 += p.piece_classes) {
@@ -1572,7 +1421,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 TcArgs x = t;
                 XENT_TRY(map(x.a, gs, classes, rows, p.ldg, kBM));
                 // the piece's classes of w
-                const void* wp[2] = {(const uint16_t*)ws[0] + c0 * ldw, ws[1] ? (const uint16_t*)ws[1] + c0 * ldw : nullptr};
+                const void* wp[3];
+                for (int i = 0; i < p.planes; ++i) wp[i] = (const uint16_t*)ws[i] + c0 * ldw;
                 XENT_TRY(map(x.b, wp, a.d, classes, ldw, kBK));
                 x.m_tiles = (int)cdiv(rows, kPM);
                 x.n_tiles = (int)p.dx_d_tiles;
@@ -1586,8 +1436,6 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 x.dx = a.dx; x.dxr = a.dxr; x.dxk = a.dxk;
                 x.dx_map = a.dxk == 1 && (uintptr_t)a.dx % 16 == 0 && a.dxr >= a.d && a.dxr * (int64_t)sizeof(T) % 16 == 0;
                 if (x.dx_map && !make_out_map(&x.out[0], a.type, a.dx, a.d, a.n, a.dxr)) return cudaErrorInvalidValue;
-                x.undo = p.undo;
-                x.undo_pitch = p.undo_pitch;
                 x.sums = p.dx_sums;
                 x.split_stride = p.dx_stride;
                 x.direct = p.dx_direct;
@@ -1597,7 +1445,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 if (x.last && !p.dx_direct) {
                     KernelTimer kt(st, GAFIME_KERNEL_XENT);
                     xent_sum_kernel<T><<<(unsigned)(cdiv(rows, 32) * cdiv(a.d, 8)), 256, 0, st>>>(
-                        p.dx_sums, p.dx_splits, p.dx_stride, (int)p.dx_d_tiles, p.bn_dx, rows, (int)a.d, p.undo, p.undo_pitch,
+                        p.dx_sums, p.dx_splits, p.dx_stride, (int)p.dx_d_tiles, p.bn_dx, rows, (int)a.d,
                         !kBf16, p.meta, a.labels + r0, (T*)a.dx + r0 * a.dxr, a.dxr, a.dxk);
                     XENT_TRY(cudaGetLastError());
                 }
@@ -1627,8 +1475,6 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 w.dxk = 1;
                 w.dx_map = (uintptr_t)a.dw % 16 == 0 && a.d * (int64_t)sizeof(T) % 16 == 0;
                 if (w.dx_map && !make_out_map(&w.out[0], a.type, a.dw, a.d, a.c, a.d)) return cudaErrorInvalidValue;
-                w.undo = p.undo ? p.undo + 2 * p.undo_pitch : nullptr;
-                w.undo_pitch = p.undo_pitch;
                 w.cleaned = p.xc != nullptr;
                 if (p.xc && !make_map(&w.b[1], kBf16, p.xc, a.d, a.n, p.dp, kBK)) return cudaErrorInvalidValue;
                 XENT_TRY((launch<DW, E, kPlanes>(w, p.bn_dw, sms, st)));
@@ -1638,8 +1484,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     if (a.dw && !p.dw_direct) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
         xent_sum_kernel<T><<<(unsigned)(cdiv(a.c, 32) * cdiv(a.d, 8)), 256, 0, st>>>(
-            p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_dw, a.c, (int)a.d,
-            p.undo ? p.undo + 2 * p.undo_pitch : nullptr, p.undo_pitch, !kBf16, p.meta, nullptr, (T*)a.dw, a.d, 1);
+            p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_dw, a.c, (int)a.d, !kBf16, p.meta, nullptr, (T*)a.dw, a.d, 1);
         XENT_TRY(cudaGetLastError());
     }
     if (a.dw || a.dbias || both) {
@@ -1657,7 +1502,7 @@ size_t xent_tc_workspace(const XentCall& a, int sms) { return make_plan(a, sms, 
 
 cudaError_t xent_tc(const XentCall& a, int sms) {
     switch (a.type) {
-        case GAFIME_TYPE_FP32: return run_tc<float, __half>(a, sms);
+        case GAFIME_TYPE_FP32: return run_tc<float, __nv_bfloat16>(a, sms);
         case GAFIME_TYPE_FP16: return run_tc<__half, __half>(a, sms);
         default: return run_tc<__nv_bfloat16, __nv_bfloat16>(a, sms);
     }
