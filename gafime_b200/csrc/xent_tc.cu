@@ -22,6 +22,8 @@
 //   l h + h l + m m + m h + h m + h h        (left out: m l, l m, l l, below 3 x 2^-23 of |x||w|)
 // six 16-bit products, with everything that a 24-bit product holds but its last bit or two.  Two
 // fp16 planes with common scales would take three, but hold only 38 bits below the largest value.
+// A weight of +-infinity sits in a fourth plane of its own, which only x's h meets (its m and l have
+// signs of their own, and 0 x inf is no number): a product more where there is such a weight.
 //
 // Kernel (pairs of CTAs, one CTA an SM, persistent, 12 warps; a pair makes 256 x BN tiles): warp 0
 // queues its CTA's TMA loads of 128 x 64 of A and BN / 2 x 64 of B into a ring; warp 1 of the
@@ -48,6 +50,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <iterator>
 #include <mutex>
 #include <type_traits>
 
@@ -95,6 +98,7 @@ static_assert(smem_of(256, 4096) <= 232448 && smem_of(128, 4096) <= 232448 && sm
 struct Meta {
     int err;                 // code of a wait that gave up
     uint32_t weight_bits;    // largest finite |row weight| as float bits
+    uint32_t wild;           // fp32: some weight is infinite
     uint32_t poison;         // some left-out row of an x read in place holds a value that is not finite
 };
 
@@ -120,7 +124,7 @@ __device__ __forceinline__ float exp2_fast(float v) {
 __device__ __forceinline__ int g_exponent(const Meta* m, int half_g) { return half_g ? fit_exponent(m->weight_bits) : 0; }
 
 struct TcArgs {
-    CUtensorMap a[3], b[3];   // planes: one, or h, m, l of fp32 (b[1] also: see cleaned)
+    CUtensorMap a[3], b[4];   // planes: one, or h, m, l of fp32, w's infinities (b[1] also: see cleaned)
     CUtensorMap out[3];       // G: planes of g; DX, DW: dx, dw
     int half_g;               // g in fp16 (scaled by 2^u), else bf16
     int units, m_tiles, n_tiles, splits;
@@ -286,6 +290,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
     const int rank = (int)tc::cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     int* err = &a.meta->err;
+    const bool wild = kPlanes == 3 && MODE != DW && a.meta->wild != 0;
+    const int stages = kPlanes + wild;                        // of a block of K
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -319,12 +325,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     const int m0 = t.m * kPM + rank * kBM;
                     for (int r = 0; ok && r < t.tiles; ++r) {
                         const int n0 = (t.n + r) * BN + rank * (BN / 2);
-                        // three planes: a block of K takes three stages, l, h and m of both sides
-                        for (int i = 0; i < t.kn * kPlanes; ++i, ++k) {
-                            const int kb = t.kb + i / kPlanes;
-                            const int plane = kPlanes == 1 ? 0 : (i % kPlanes + 2) % kPlanes;
+                        // three planes: a block of K takes three stages, l, h and m of both sides, and
+                        // where some weight is infinite a fourth, h and the infinities
+                        for (int i = 0; i < t.kn * stages; ++i, ++k) {
+                            const int kb = t.kb + i / stages, q = i % stages;
+                            const int plane = kPlanes == 1 || q == 3 ? 0 : (q + 2) % 3;
                             const CUtensorMap* ma = &a.a[plane];
-                            const CUtensorMap* mb = &a.b[clean ? 1 : plane];
+                            const CUtensorMap* mb = &a.b[clean ? 1 : q == 3 ? 3 : plane];
                             const uint32_t s = k % S, full = full_l + 8 * s;
                             // (a wait of a second is over long after the copies before it)
                             if (k >= S && !(ok = tc::bar_wait(empty0 + 8 * s, ((k / S) - 1) & 1, err, 1))) break;
@@ -338,8 +345,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                             }
                             if (kBMn) {
                                 #pragma unroll
-                                for (int q = 0; q < BN / 128; ++q)
-                                    tc::load_2d(sb + q * 8192, mb, full, n0 + q * 64, a.b_row0 + kb * kBK);
+                                for (int h = 0; h < BN / 128; ++h)
+                                    tc::load_2d(sb + h * 8192, mb, full, n0 + h * 64, a.b_row0 + kb * kBK);
                             } else {
                                 tc::load_2d(sb, mb, full, kb * kBK, a.b_row0 + n0);
                             }
@@ -384,8 +391,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     } else {
                         // (one block of K to a chunk) the small products first, as the stages arrive: what
                         // the tensor cores cut off is a part of the sum so far
-                        for (; i < stop; ++i, k += 3) {
-                            const uint32_t sl = k % S, sh = (k + 1) % S, sm = (k + 2) % S;
+                        for (; i < stop; ++i, k += stages) {
+                            const uint32_t sl = k % S, sh = (k + 1) % S, sm = (k + 2) % S, si = (k + 3) % S;
                             auto arrived = [&](uint32_t q) {
                                 ok = ok && tc::bar_wait_warp(full0 + 8 * (q % S), (q / S) & 1, err, 4);
                                 return ok;
@@ -398,13 +405,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                                 tc::commit_both(empty0 + 8 * sl);
                             }
                             __syncwarp();
-                            if (!arrived(k + 2)) break;
+                            if (!arrived(k + 2) || (wild && !arrived(k + 3))) break;
                             tc::fence_after();
                             if (lane == 0) {
                                 multiply(sm, sm);
                                 multiply(sm, sh);
                                 multiply(sh, sm);
                                 tc::commit_both(empty0 + 8 * sm);
+                                if (wild) {
+                                    multiply(si, si);
+                                    tc::commit_both(empty0 + 8 * si);
+                                }
                                 multiply(sh, sh);
                                 tc::commit_both(empty0 + 8 * sh);
                             }
@@ -881,10 +892,18 @@ struct PlaneArgs {
     const uint32_t* keep;     // nullable: bit r of word r / 32: row r counts
     int64_t rows, d, dp;
     int64_t per_block;        // xent_planes_rows_kernel: rows a block
-    const Meta* meta;
+    Meta* meta;
     int if_poison;            // nothing to do unless meta->poison is set
-    uint16_t* to[3];          // one plane of 16 bits, or h, m, l of fp32
+    uint16_t* to[4];          // one plane of 16 bits, or h, m, l of fp32, and (nullable) its infinities
 };
+// Infinities go from two values to a plane of their own; true when there are any.
+__device__ __forceinline__ bool take_infinities(float& a, float& b, uint32_t& plane) {
+    const bool ia = isinf(a), ib = isinf(b);
+    plane = pack(ia ? a : 0.f, ib ? b : 0.f, __nv_bfloat16{});
+    if (ia) a = 0.f;
+    if (ib) b = 0.f;
+    return ia || ib;
+}
 
 // fp32 rows in 16-byte units: a block takes some rows of 1024 features, a thread four of them,
 // several rows at once where the features are fewer.
@@ -901,6 +920,12 @@ __global__ void __launch_bounds__(256) xent_planes_rows_kernel(const PlaneArgs a
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (!a.keep || row_counts(a.keep, r)) v = load_quad((const float*)a.x + r * a.xr, k, a.d);
         uint2 h, m, l;
+        if (a.to[3]) {
+            uint2 f;
+            const bool some = take_infinities(v.x, v.y, f.x) | take_infinities(v.z, v.w, f.y);
+            *reinterpret_cast<uint2*>(a.to[3] + r * a.dp + k) = f;
+            if (some) a.meta->wild = 1;
+        }
         split3(v.x, v.y, h.x, m.x, l.x);
         split3(v.z, v.w, h.y, m.y, l.y);
         *reinterpret_cast<uint2*>(a.to[0] + r * a.dp + k) = h;
@@ -955,15 +980,23 @@ __global__ void __launch_bounds__(256) xent_planes_kernel(const PlaneArgs a) {
     for (int r = threadIdx.x >> 3; r < 64; r += 32) {
         if (r0 + r >= a.rows) break;
         const int64_t at = (r0 + r) * a.dp + k0 + k;
-        uint32_t h[4], m[4], l[4];
+        uint32_t h[4], m[4], l[4], f[4];
+        bool some = false;
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float v0 = t[k + 2 * i][r], v1 = t[k + 2 * i + 1][r];
-            if constexpr (sizeof(T) == 4)
+            float v0 = t[k + 2 * i][r], v1 = t[k + 2 * i + 1][r];
+            if constexpr (sizeof(T) == 4) {
+                if (a.to[3]) some |= take_infinities(v0, v1, f[i]);
                 split3(v0, v1, h[i], m[i], l[i]);
-            else
+            } else {
                 h[i] = pack(v0, v1, E{});
+            }
         }
+        if constexpr (sizeof(T) == 4)
+            if (a.to[3]) {
+                *reinterpret_cast<uint4*>(a.to[3] + at) = make_uint4(f[0], f[1], f[2], f[3]);
+                if (some) a.meta->wild = 1;
+            }
         *reinterpret_cast<uint4*>(a.to[0] + at) = make_uint4(h[0], h[1], h[2], h[3]);
         if constexpr (sizeof(T) == 4) {
             *reinterpret_cast<uint4*>(a.to[1] + at) = make_uint4(m[0], m[1], m[2], m[3]);
@@ -1128,7 +1161,7 @@ struct Plan {
     float* bias2;
     uint32_t* keep;
     uint16_t* xc;                    // x without left-out rows, made where one of those holds no number
-    uint16_t *x[3], *w[3], *g[3];    // planes; null where the operands are read in place
+    uint16_t *x[3], *w[4], *g[3];    // planes; null where the operands are read in place
     float2* part;
     float* zy;
     float2* shift;
@@ -1169,6 +1202,7 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
         if (!p.x_in_place) p.x[i] = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
         if (!p.w_in_place) p.w[i] = cv.take<uint16_t>(a.c * p.dp);
     }
+    if (p.planes == 3) p.w[3] = cv.take<uint16_t>(a.c * p.dp);
     if (a.gradient && a.dw && p.x_in_place) p.xc = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
     p.part = cv.take<float2>(a.n * 2 * p.splits);
     p.zy = cv.take<float>(a.n);
@@ -1320,7 +1354,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         xent_poison_kernel<<<(unsigned)std::min<int64_t>(8 * sms, cdiv(a.n, 8)), 256, 0, st>>>(
             a.labels, a.n, (const uint16_t*)a.x, a.xr, a.d, kBf16, p.meta);
         XENT_TRY(cudaGetLastError());
-        PlaneArgs s{a.x, a.xr, a.xk, p.keep, a.n, a.d, p.dp, 0, p.meta, 1, {p.xc, nullptr, nullptr}};
+        PlaneArgs s{a.x, a.xr, a.xk, p.keep, a.n, a.d, p.dp, 0, p.meta, 1, {p.xc}};
         XENT_TRY((planes<T, E>(s, sms, st)));
     }
     if (p.x[0]) {
@@ -1328,15 +1362,15 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         XENT_TRY((planes<T, E>(s, sms, st)));
     }
     if (p.w[0]) {
-        PlaneArgs s{a.w, a.wr, a.wk, nullptr, a.c, a.d, p.dp, 0, p.meta, 0, {p.w[0], p.w[1], p.w[2]}};
+        PlaneArgs s{a.w, a.wr, a.wk, nullptr, a.c, a.d, p.dp, 0, p.meta, 0, {p.w[0], p.w[1], p.w[2], p.w[3]}};
         XENT_TRY((planes<T, E>(s, sms, st)));
     }
     // where the operands are read
     const void *xs[3] = {p.x[0] ? (const void*)p.x[0] : a.x, p.x[1], p.x[2]};
-    const void *ws[3] = {p.w[0] ? (const void*)p.w[0] : a.w, p.w[1], p.w[2]};
+    const void *ws[4] = {p.w[0] ? (const void*)p.w[0] : a.w, p.w[1], p.w[2], p.w[3]};
     const int64_t ldx = p.x[0] ? p.dp : a.xr, ldw = p.w[0] ? p.dp : a.wr;
-    auto map = [&](CUtensorMap (&m)[3], const void* const (&base)[3], int64_t inner, int64_t rows, int64_t ld, int box) {
-        for (int i = 0; i < p.planes; ++i)
+    auto map = [&](auto& m, const auto& base, int64_t inner, int64_t rows, int64_t ld, int box) {
+        for (size_t i = 0; i < std::size(base) && base[i]; ++i)
             if (!make_map(&m[i], kBf16, base[i], inner, rows, ld, box)) return cudaErrorInvalidValue;
         return cudaSuccess;
     };
@@ -1421,8 +1455,8 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                 TcArgs x = t;
                 XENT_TRY(map(x.a, gs, classes, rows, p.ldg, kBM));
                 // the piece's classes of w
-                const void* wp[3];
-                for (int i = 0; i < p.planes; ++i) wp[i] = (const uint16_t*)ws[i] + c0 * ldw;
+                const void* wp[4] = {};
+                for (int i = 0; i < 4 && ws[i]; ++i) wp[i] = (const uint16_t*)ws[i] + c0 * ldw;
                 XENT_TRY(map(x.b, wp, a.d, classes, ldw, kBK));
                 x.m_tiles = (int)cdiv(rows, kPM);
                 x.n_tiles = (int)p.dx_d_tiles;

@@ -190,3 +190,37 @@ def test_row_weights_in_16_bits(ops, big, dtype):
     if dtype == F16:     # g itself: 2^-38 of the largest row weight
         tol = tol + 2.0 ** -37 * w.double().abs().sum(0)
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("n,c", [(20, 5), (200, 40), (300, 300), (20, 16), (4, 64)])
+def test_a_weight_of_minus_infinity_excludes_its_class(ops, n, c):
+    """z of that class is -inf in rows whose feature is positive: no part in their softmax, as with a
+    bias of -inf; a row whose feature is negative gets +inf and a loss that is no number."""
+    x, w, labels, b, _ = data(n, 24, c, seed=9)
+    w[4, 2] = float("-inf")
+    x[:, 2] = x[:, 2].abs() + 0.1
+    x[0, 2] *= -1.0
+    labels = torch.where(labels == 4, torch.zeros_like(labels), labels)
+    z = x[1:].double() @ torch.where(torch.isinf(w), 0.0, w.double()).t() + b.double()
+    z[:, 4] = float("-inf")
+    want = torch.logsumexp(z - z.gather(1, labels[1:, None]), 1)
+    for got in (ops.softmax_xent(x, w, labels, b), ops.softmax_xent_grad(x, w, labels, b).loss):
+        assert torch.isnan(got[0])
+        assert ((got[1:].double() - want).abs() <= 64 * U * (want.abs() + 16)).all()
+    # without the row of +inf: dw as with the class left out
+    g = ops.softmax_xent_grad(x[1:], w, labels[1:], b, need_dx=False)
+    p = torch.softmax(z, 1)
+    p.scatter_add_(1, labels[1:, None], -torch.ones((n - 1, 1), device="cuda", dtype=torch.float64))
+    size = p.abs().t() @ x[1:].double().abs()
+    assert ((g.dw.double() - p.t() @ x[1:].double()).abs() <= 256 * U * size + 1e-30).all()
+    assert not g.dw[4].any() and g.dbias[4] == 0
+    # dx: 0 x inf is no number, as the definition has it; the other features hold theirs
+    g = ops.softmax_xent_grad(x[1:], w, labels[1:], b)
+    assert torch.isnan(g.dx[:, 2]).all()
+    rest = [k for k in range(24) if k != 2]
+    size = p.abs() @ w.double().abs()[:, rest]
+    assert ((g.dx[:, rest].double() - p @ w.double()[:, rest]).abs() <= 256 * U * size + 1e-30).all()
+    # its label: an infinite loss
+    labels[1] = 4
+    got = ops.softmax_xent(x, w, labels, b)
+    assert math.isinf(float(got[1])) and float(got[1]) > 0
