@@ -73,7 +73,6 @@ constexpr int kPM = 256;                     // rows of a pair's tile
 constexpr int kBK = 64;                      // 16-bit values of K to a stage
 constexpr int kABytes = kBM * kBK * 2;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 // Of a piece of g: several rounds of the pairs, not the n x c whole.  Three planes get as many values
 // as two would in 256 MB.
 constexpr size_t piece_bytes(int planes) { return (size_t)(planes == 3 ? 384 : 256) << 20; }
@@ -115,10 +114,12 @@ __device__ __forceinline__ float scale2(float v, int e) {
     const int h = e / 2;
     return v * pow2i(h) * pow2i(e - h);
 }
-// 2^v; below 2^-126 zero, which is nothing beside the sums it enters (2^-22 relative otherwise)
-__device__ __forceinline__ float exp2_fast(float v) {
+// e^v; below 2^-126 zero, which is nothing beside the sums it enters (2^-22 relative otherwise, and
+// 2^-24 |v|).  Logits stay in base e up to the difference that comes here: one of the type's lowest
+// value, a mask's, has no finite double in base 2.
+__device__ __forceinline__ float exp_fast(float v) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * kLog2e));
     return r;
 }
 __device__ __forceinline__ int g_exponent(const Meta* m, int half_g) { return half_g ? fit_exponent(m->weight_bits) : 0; }
@@ -138,12 +139,12 @@ struct TcArgs {
     int64_t c_total;
     int c0;                   // first class of the piece
     Meta* meta;
-    const float* bias2;       // bias in base 2, -inf past the classes
+    const float* bias;        // -inf past the classes
     const int64_t* labels;
     float *loss_out, *lse_out;   // BOTH: [n]; the second may be null
     float2* part;             // LSE: [n][2 splits] maximum, sum
-    float* zy;                // LSE: label's logit, base 2
-    const float2* shift;      // G: [n] maximum and log2 of the sum
+    float* zy;                // LSE: label's logit
+    const float2* shift;      // G: [n] maximum and log of the sum
     const float* loss;        // G
     const float* weight;
     int64_t weight_stride;
@@ -444,7 +445,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
         uint32_t acc = 0;
         bool ok = true;
         const int ue = g_exponent(a.meta, a.half_g);
-        const float f = kLog2e;
         const uint32_t aempty_l = tc::in_leader(aempty0);
         // What a unit needs of its rows is loaded while the unit before it is worked on.
         struct Row {
@@ -485,7 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     sh = own_row.shift;
                     // exp(z_y - lse) - 1 from the loss, without the cancellation
                     gy = expm1f(-own_row.loss) * wt;
-                    ws = wt * exp2f(-sh.y);
+                    ws = wt * expf(-sh.y);
                 }
             }
             for (int r = 0; ok && r < t.tiles && t.kn > 0; ++r) {
@@ -528,14 +528,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                         if (ch >= blocks) break;
                         float* v = sums + ch * 32;
                         const int cb = half * kCols + ch * 32;
-                        const float4* b4 = reinterpret_cast<const float4*>(a.bias2 + cb);
+                        const float4* b4 = reinterpret_cast<const float4*>(a.bias + cb);
                         #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const float4 b = __ldg(b4 + j);
-                            v[4 * j] = fmaf(v[4 * j], f, b.x);
-                            v[4 * j + 1] = fmaf(v[4 * j + 1], f, b.y);
-                            v[4 * j + 2] = fmaf(v[4 * j + 2], f, b.z);
-                            v[4 * j + 3] = fmaf(v[4 * j + 3], f, b.w);
+                            v[4 * j] += b.x;
+                            v[4 * j + 1] += b.y;
+                            v[4 * j + 2] += b.z;
+                            v[4 * j + 3] += b.w;
                         }
                         #pragma unroll
                         for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], v[j]);
@@ -554,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                         if (ch >= blocks) break;
                         float* v = sums + ch * 32;
                         #pragma unroll
-                        for (int j = 0; j < 32; ++j) s4[j & 3] += v[j] = exp2_fast(v[j] - own);
+                        for (int j = 0; j < 32; ++j) s4[j & 3] += v[j] = exp_fast(v[j] - own);
                     }
                     sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
                     // and over the other half's, from the warp that has it.  A warp whose wait gave up
@@ -566,17 +566,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory");   // read before g is written there
                     ok = ok && o.w != 0.f;
                     const float m = fmaxf(top, o.x), shift = m == -INFINITY ? 0.f : m;
-                    const float l = log2f(sum * exp2f(top - shift) + o.y * exp2f(o.x - shift));
+                    const float l = logf(sum * expf(top - shift) + o.y * expf(o.x - shift));
                     if (isnan(zy)) zy = o.z;
-                    const float loss = y >= 0 ? ((shift - zy) + l) * kLn2 : 0.f;
+                    const float loss = y >= 0 ? (shift - zy) + l : 0.f;
                     if (half == 0 && valid) {
                         a.loss_out[a.row0 + row] = loss;
                         if (a.lse_out)
-                            a.lse_out[a.row0 + row] = y >= 0 ? (float)(((double)shift + (double)l) * 0.69314718055994530942) : 0.f;
+                            a.lse_out[a.row0 + row] = y >= 0 ? shift + l : 0.f;
                     }
                     gy = expm1f(-loss) * wt;
                     // (with no class of its own a half's exponentials are zeros, whatever their shift)
-                    ws = wt * (top == -INFINITY ? 0.f : exp2f((own - shift) - l));
+                    ws = wt * (top == -INFINITY ? 0.f : expf((own - shift) - l));
                 }
                 if (!ok) break;
                 #pragma unroll
@@ -586,14 +586,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     if (cb >= a.cols) break;
                     float* v = sums + ch * 32;
                     if (MODE == LSE || MODE == G) {   // (BOTH: done)
-                        const float4* b4 = reinterpret_cast<const float4*>(a.bias2 + a.c0 + cb);
+                        const float4* b4 = reinterpret_cast<const float4*>(a.bias + a.c0 + cb);
                         #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const float4 b = __ldg(b4 + j);
-                            v[4 * j] = fmaf(v[4 * j], f, b.x);
-                            v[4 * j + 1] = fmaf(v[4 * j + 1], f, b.y);
-                            v[4 * j + 2] = fmaf(v[4 * j + 2], f, b.z);
-                            v[4 * j + 3] = fmaf(v[4 * j + 3], f, b.w);
+                            v[4 * j] += b.x;
+                            v[4 * j + 1] += b.y;
+                            v[4 * j + 2] += b.z;
+                            v[4 * j + 3] += b.w;
                         }
                     }
                     // the row's label among these columns
@@ -609,7 +609,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     } else if (kG) {
                         #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float p = (MODE == BOTH ? v[j] : exp2_fast(v[j] - sh.x)) * ws;
+                            const float p = (MODE == BOTH ? v[j] : exp_fast(v[j] - sh.x)) * ws;
                             v[j] = y >= 0 ? p : 0.f;
                         }
                         // 64 columns a store where the thread has as many: whole 128-byte lines
@@ -738,8 +738,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     for (int ch = 0; ch < kCols / 32; ++ch)
                         if (ch < blocks)
                             #pragma unroll
-                            for (int j = 0; j < 32; ++j) s4[j & 3] += exp2_fast(sums[ch * 32 + j] - shift);
-                    sum = sum * exp2_fast(top - shift) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+                            for (int j = 0; j < 32; ++j) s4[j & 3] += exp_fast(sums[ch * 32 + j] - shift);
+                    sum = sum * exp_fast(top - shift) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
                     top = m;
                 }
             }
@@ -767,7 +767,7 @@ struct SetupArgs {
     float scale;
     int want_weight;          // largest row weight
     const float* bias;
-    float* bias2;
+    float* bias_pad;
     int64_t c, c_pad;
     float* zy;                // nullable: cleared to NaN
     uint32_t* keep;           // nullable: bit r of word r / 32: row r counts
@@ -778,7 +778,7 @@ __global__ void __launch_bounds__(256) xent_setup_kernel(SetupArgs a) {
     const int lane = threadIdx.x & 31;
     const int64_t gt = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, all = (int64_t)gridDim.x * blockDim.x;
     for (int64_t i = gt; i < a.c_pad; i += all)
-        a.bias2[i] = i < a.c ? (a.bias ? a.bias[i] * kLog2e : 0.f) : -INFINITY;
+        a.bias_pad[i] = i < a.c ? (a.bias ? a.bias[i] : 0.f) : -INFINITY;
     if (!a.want_weight && !a.zy && !a.keep) return;
     float top = 0.f;
     for (int64_t w = gt / 32; w < (a.n + 31) / 32; w += all / 32) {
@@ -834,9 +834,7 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     const int lane = (int)(at % lanes);
     if (r >= n) return;
     if (have_lse) {
-        const double l2 = (double)lse[r] * 1.4426950408889634074;
-        const float hi = (float)l2;
-        shift[r] = make_float2(hi, isfinite(hi) ? (float)(l2 - hi) : 0.f);
+        shift[r] = make_float2(lse[r], 0.f);
         return;
     }
     float m = -INFINITY;
@@ -848,18 +846,18 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     float s = 0.f;
     for (int i = lane; i < parts; i += lanes) {
         const float2 p = part[r * parts + i];
-        s += p.y * exp2f(p.x - sh);
+        s += p.y * expf(p.x - sh);
     }
     if (lanes == 32)
         #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane != 0) return;
-    const float l = log2f(s);
+    const float l = logf(s);
     if (shift) shift[r] = make_float2(sh, l);
     const bool kept = labels[r] >= 0;
     const bool failed = meta->err != 0;
-    loss[r] = failed ? NAN : kept ? ((sh - zy[r]) + l) * kLn2 : 0.f;
-    if (lse) lse[r] = failed ? NAN : kept ? (float)(((double)sh + (double)l) * 0.69314718055994530942) : 0.f;
+    loss[r] = failed ? NAN : kept ? (sh - zy[r]) + l : 0.f;
+    if (lse) lse[r] = failed ? NAN : kept ? sh + l : 0.f;
 }
 
 // Rows read four features at a time: unit features, 16-byte aligned rows.
@@ -1158,7 +1156,7 @@ struct Plan {
     bool products;                   // dx or dw or dbias wanted
     // workspace
     Meta* meta;
-    float* bias2;
+    float* bias;
     uint32_t* keep;
     uint16_t* xc;                    // x without left-out rows, made where one of those holds no number
     uint16_t *x[3], *w[4], *g[3];    // planes; null where the operands are read in place
@@ -1196,7 +1194,7 @@ Plan make_plan(const XentCall& a, int sms, uint8_t* ws) {
 
     Carver cv(ws);
     p.meta = cv.take<Meta>(1);
-    p.bias2 = cv.take<float>(p.c_tiles * p.bn_c + 256);
+    p.bias = cv.take<float>(p.c_tiles * p.bn_c + 256);
     p.keep = cv.take<uint32_t>(cdiv(a.n, 32) + 2);
     for (int i = 0; i < p.planes; ++i) {
         if (!p.x_in_place) p.x[i] = cv.take<uint16_t>(std::max<int64_t>(1, a.n) * p.dp);
@@ -1340,7 +1338,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         SetupArgs s{};
         s.labels = a.labels; s.n = a.n; s.weight = a.weight; s.weight_stride = a.weight_stride; s.scale = a.scale;
         s.want_weight = p.products && !kBf16;
-        s.bias = a.bias; s.bias2 = p.bias2; s.c = a.c; s.c_pad = p.c_tiles * p.bn_c + 256;
+        s.bias = a.bias; s.bias_pad = p.bias; s.c = a.c; s.c_pad = p.c_tiles * p.bn_c + 256;
         s.zy = forward ? p.zy : nullptr;
         s.keep = p.x[0] || p.xc ? p.keep : nullptr;
         s.meta = p.meta;
@@ -1381,7 +1379,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     t.chunk = p.planes == 3 ? 1 : 8;
     t.half_g = !kBf16;
     t.meta = p.meta;
-    t.bias2 = p.bias2;
+    t.bias = p.bias;
     t.labels = a.labels;
     t.weight = a.weight; t.weight_stride = a.weight_stride; t.scale = a.scale;
     t.c_total = a.c;

@@ -1,0 +1,85 @@
+"""Biases that mask classes by a low value."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+U = 2.0 ** -24
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from gafime_b200 import _native, ops as o
+    _native.load()
+    return o
+
+
+def data(n, c, d=24, dtype=F32, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((n, d), generator=g, device="cuda").to(dtype)
+    w = (torch.randn((c, d), generator=g, device="cuda") * 0.3).to(dtype)
+    b = torch.randn(c, generator=g, device="cuda")
+    labels = torch.randint(0, c, (n,), generator=g, device="cuda")
+    return x, w, labels, b
+
+
+def through_autograd(ops, x, w, labels, b):
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    loss = ops.softmax_xent(leaves[0], leaves[1], labels, leaves[2])
+    loss.sum().backward()
+    return loss.detach(), leaves[0].grad, leaves[1].grad, leaves[2].grad
+
+
+PATHS = [(20, 5), (200, 40), (300, 300), (20, 16)]     # few classes, one tile, several, few with tiles
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,c", PATHS + [(1, 40), (5, 300)])
+@pytest.mark.parametrize("how", ["step"])
+def test_a_mask_of_the_lowest_value_that_leaves_nothing(ops, how, n, c, dtype):
+    """Every logit is the type's lowest value (the product is lost beside it): all classes alike."""
+    x, w, labels, b = data(n, c, dtype=dtype)
+    b.fill_(LOWEST)
+    want = torch.full((n,), math.log(c), device="cuda")
+    tol = 8 * U * (1 + math.log(c))
+    assert ((ops.softmax_xent(x, w, labels, b) - want).abs() <= tol).all()
+    if how == "step":
+        loss, _, dx, dw, db = ops.softmax_xent_grad(x, w, labels, b)
+    else:
+        loss, dx, dw, db = through_autograd(ops, x, w, labels, b)
+    assert ((loss - want).abs() <= tol).all()
+    # each class has p = 1 / c of every row, and its labels
+    p = torch.full((n, c), 1.0 / c, device="cuda", dtype=torch.float64)
+    p.scatter_add_(1, labels[:, None], -torch.ones((n, 1), device="cuda", dtype=torch.float64))
+    half = torch.finfo(dtype).eps / 2 if dtype != F32 else 0.0
+    A = p.abs()
+    for name, got, value, size in (("dx", dx, p @ w.double(), A @ w.double().abs()),
+                                   ("dw", dw, p.t() @ x.double(), A.t() @ x.double().abs()),
+                                   ("dbias", db, p.sum(0), A.sum(0))):
+        slack = (half + 64 * U) * size + (torch.finfo(got.dtype).eps / 2) * value.abs() + 2.0 ** -24
+        assert ((got.double() - value).abs() <= slack).all(), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,c", PATHS + [(4, 64)])
+@pytest.mark.parametrize("low", [LOWEST, -2.5e38, -1e30])
+def test_a_label_of_a_class_masked_by_a_low_value(ops, n, c, low, dtype):
+    """The loss is the distance to it, a finite number."""
+    x, w, labels, b = data(n, c, dtype=dtype, seed=1)
+    b[3] = low
+    labels[1] = 3
+    labels = torch.where((labels == 3) & (torch.arange(n, device="cuda") != 1), torch.zeros_like(labels), labels)
+    z = x.double() @ w.double().t() + b.double()
+    want = torch.logsumexp(z - z.gather(1, labels[:, None]), 1)
+    got = ops.softmax_xent(x, w, labels, b)
+    assert torch.isfinite(got).all()
+    assert ((got.double() - want).abs() <= 64 * U * (want.abs() + 16)).all()
+    g = ops.softmax_xent_grad(x, w, labels, b)
+    assert ((g.loss.double() - want).abs() <= 64 * U * (want.abs() + 16)).all()
+    for t in (g.dx, g.dw, g.dbias) + through_autograd(ops, x, w, labels, b)[1:]:
+        assert torch.isfinite(t).all()
