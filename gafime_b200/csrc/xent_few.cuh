@@ -71,7 +71,7 @@ struct FewArgs {
     const float* weight;
     int64_t weight_stride;
     float scale;
-    int have_lse;
+    int have_lse;        // loss and lse are there already
     float* loss;
     float* lse;
     void* dx;
@@ -619,15 +619,14 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
     };
     struct Meta {
         int64_t y;
-        float weight, lse;
+        float weight;
     };
     auto meta_of = [&](int64_t t) {
-        Meta m = {-1, 0.f, 0.f};
+        Meta m = {-1, 0.f};
         const int64_t gr = t * R + row;
         if (t < a.n_tiles && gr < a.n) {
             m.y = a.labels[gr];
             if (GRAD) m.weight = (a.weight ? a.weight[gr * a.weight_stride] : 1.f) * a.scale;
-            if (a.have_lse) m.lse = a.lse[gr];
         }
         return m;
     };
@@ -667,7 +666,7 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
                 dots<T, C, COLS, 8, F>(z, tile, wk, feats, lane);
         }
         const int64_t y64 = meta.y;
-        const float rw = meta.weight, shift_in = meta.lse;
+        const float rw = meta.weight;
         meta = next;
         // 2. logits of all warps, softmax, loss, g
         if (GRAD && W > 1) {
@@ -711,15 +710,15 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
             if (a.lse) a.lse[gr] = kept ? m + ls : 0.f;
         }
         if (GRAD) {
-            // with this call's own sum, e / s; else exp of the difference to the given lse
+            // e / s, whether the loss is there or not: logits far from zero leave a given lse, rounded
+            // to its last bit, too coarse for exp(z - lse)
             const float inv = 1.f / s;
             // bit r: row r is left out and holds something that is no number
             uint32_t bad = 0;
             if (__any_sync(0xffffffffu, !kept && !finite)) bad = __reduce_or_sync(0xffffffffu, !kept && !finite ? 1u << row : 0u);
             #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const float p = a.have_lse ? expf(z[c] - shift_in) : e[c] * inv;
-                float g = kept ? (p - (c == y ? 1.f : 0.f)) * rw : 0.f;
+                float g = kept ? (e[c] * inv - (c == y ? 1.f : 0.f)) * rw : 0.f;
                 if (kept && y < 0) g = NAN;
                 if (c >= a.c) g = 0.f;
                 e[c] = g;

@@ -824,19 +824,14 @@ __global__ void __launch_bounds__(256) xent_poison_kernel(const int64_t* __restr
     }
 }
 
-// lse and loss of a row from its partial maxima and sums; with the sums given (have_lse), only
-// the shift that g subtracts
+// lse and loss of a row from its partial maxima and sums
 __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part, int parts, int lanes,
-                                                        const float* zy, const int64_t* labels, int64_t n, int have_lse,
+                                                        const float* zy, const int64_t* labels, int64_t n,
                                                         float* loss, float* lse, float2* shift, const Meta* meta) {
     // `lanes` neighbouring threads to a row, 1 or 32
     const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, r = at / lanes;
     const int lane = (int)(at % lanes);
     if (r >= n) return;
-    if (have_lse) {
-        shift[r] = make_float2(lse[r], 0.f);
-        return;
-    }
     float m = -INFINITY;
     for (int i = lane; i < parts; i += lanes) m = fmaxf(m, part[r * parts + i].x);
     if (lanes == 32)
@@ -858,6 +853,39 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     const bool failed = meta->err != 0;
     loss[r] = failed ? NAN : kept ? (sh - zy[r]) + l : 0.f;
     if (lse) lse[r] = failed ? NAN : kept ? sh + l : 0.f;
+}
+
+// The shift that g subtracts where loss and lse are given: lse, which is rounded to its last bit.
+// Past kFarLse that bit (2^-19 and more) shows in every probability of the row, and where the
+// logits are the type's lowest value nothing is left beside it of the log of their sum; there the
+// shift is the label's logit, formed once more, and the loss, held in two floats.
+constexpr float kFarLse = 64.f;
+template <typename T>
+__global__ void __launch_bounds__(256) xent_shift_kernel(const T* __restrict__ x, int64_t xr, int64_t xk,
+                                                         const T* __restrict__ w, int64_t wr, int64_t wk,
+                                                         const float* __restrict__ bias, const int64_t* __restrict__ labels,
+                                                         int64_t n, int64_t d, int64_t c, const float* __restrict__ loss,
+                                                         const float* __restrict__ lse, float2* __restrict__ shift) {
+    const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int lane = threadIdx.x & 31;
+    const int64_t y = r < n ? labels[r] : -1;
+    float2 s = make_float2(r < n ? lse[r] : 0.f, 0.f);
+    uint32_t far = __ballot_sync(0xffffffffu, y >= 0 && y < c && fabsf(s.x) > kFarLse && fabsf(s.x) <= 3.402823466e38f);
+    while (far) {
+        const int l = __ffs(far) - 1;
+        far &= far - 1;
+        const int64_t row = r - lane + l, cls = __shfl_sync(0xffffffffu, y, l);
+        float v = 0.f;
+        for (int64_t k = lane; k < d; k += 32) v = fmaf(to_float(x[row * xr + k * xk]), to_float(w[cls * wr + k * wk]), v);
+        #pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == l) {
+            // the sum and, exactly, what it rounded off
+            const float z = v + bias[cls], q = loss[r], sum = z + q, part = sum - z;
+            if (isfinite(sum)) s = make_float2(sum, (z - (sum - part)) + (q - part));
+        }
+    }
+    if (r < n) shift[r] = s;
 }
 
 // Rows read four features at a time: unit features, 16-byte aligned rows.
@@ -1399,12 +1427,17 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         l.zy = p.zy;
         XENT_TRY((launch<LSE, E, kPlanes>(l, p.bn_c, sms, st)));
     }
-    if (!both && (forward || p.products)) {
+    if (forward) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        const int lanes = forward && p.splits >= 16 ? 32 : 1;
+        const int lanes = p.splits >= 16 ? 32 : 1;
         xent_join_kernel<<<(unsigned)cdiv(a.n * lanes, 256), 256, 0, st>>>(p.part, 2 * p.splits, lanes, p.zy, a.labels, a.n,
-                                                                           !forward, a.loss, a.lse,
-                                                                           p.products ? p.shift : nullptr, p.meta);
+                                                                           a.loss, a.lse, p.products ? p.shift : nullptr,
+                                                                           p.meta);
+        XENT_TRY(cudaGetLastError());
+    } else if (p.products && !both) {
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_shift_kernel<T><<<(unsigned)cdiv(a.n, 256), 256, 0, st>>>((const T*)a.x, a.xr, a.xk, (const T*)a.w, a.wr, a.wk,
+                                                                      p.bias, a.labels, a.n, a.d, a.c, a.loss, a.lse, p.shift);
         XENT_TRY(cudaGetLastError());
     }
     if (!p.products) return cudaSuccess;

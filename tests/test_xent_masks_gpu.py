@@ -1,4 +1,4 @@
-"""Biases that mask classes by a low value."""
+"""Biases that mask classes by a low value, and logits that lie far from zero."""
 import math
 
 import pytest
@@ -40,7 +40,7 @@ PATHS = [(20, 5), (200, 40), (300, 300), (20, 16)]     # few classes, one tile, 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("n,c", PATHS + [(1, 40), (5, 300)])
-@pytest.mark.parametrize("how", ["step"])
+@pytest.mark.parametrize("how", ["step", "autograd"])
 def test_a_mask_of_the_lowest_value_that_leaves_nothing(ops, how, n, c, dtype):
     """Every logit is the type's lowest value (the product is lost beside it): all classes alike."""
     x, w, labels, b = data(n, c, dtype=dtype)
@@ -83,3 +83,17 @@ def test_a_label_of_a_class_masked_by_a_low_value(ops, n, c, low, dtype):
     assert ((g.loss.double() - want).abs() <= 64 * U * (want.abs() + 16)).all()
     for t in (g.dx, g.dw, g.dbias) + through_autograd(ops, x, w, labels, b)[1:]:
         assert torch.isfinite(t).all()
+
+
+@pytest.mark.parametrize("n,c", PATHS)
+@pytest.mark.parametrize("offset", [0.0, 900.0, 3e4, -1e6, 1e8, -3e10])
+def test_logits_far_from_zero(ops, n, c, offset):
+    """The backward pass's probabilities are normalised whatever the logits' common size: every row's
+    g sums to zero, which shows in the bias's gradient."""
+    x, w, labels, b = data(n, c, seed=2)
+    b = b * max(1.0, abs(offset) * 2.0 ** -20) + offset
+    loss, dx, dw, db = through_autograd(ops, x, w, labels, b)
+    g = ops.softmax_xent_grad(x, w, labels, b)
+    # sums of c probabilities of fp32, n rows of them, and each row's label
+    assert abs(float(db.double().sum())) <= n * (c + 64) * 4 * U
+    assert abs(float(g.dbias.double().sum())) <= n * (c + 64) * 4 * U
