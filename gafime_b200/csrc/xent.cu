@@ -24,7 +24,6 @@ namespace gafime {
 namespace {
 
 constexpr int kFewMaxD = 2048;
-constexpr size_t kFewMaxSmem = 226 * 1024;
 
 // dw[c][k] = sum over p of part[p][c][k], and the bias's, fp64 in a fixed order.  A CTA adds
 // eight neighbouring outputs (a sector of each partial): 128 threads share an output's partials,
@@ -78,6 +77,7 @@ static_assert(kFewMaxGrad <= kSumOut, "the bias's sums are one CTA's");
 // bf16: 24 us (4,200 GB/s; 31 on the tensor cores' path with 128-row tiles, 42 with pairs).
 constexpr int kRowsFew = 8;
 constexpr int64_t kRowsFewValues = 12288;   // of x, fp32 in shared memory
+constexpr size_t kRowsMaxSmem = 80 * 1024;   // eight rows' room for five of 2457 values, in whole units
 constexpr int kRowsThreads = 256;
 constexpr int rows_ctas(int64_t n) { return n <= 1 ? 3 : 2; }   // an SM holds, by registers
 
@@ -237,17 +237,22 @@ size_t rows_carve(const XentCall& a, int sms, uint8_t* ws, float2*& part, float*
     zy = cv.take<float>(a.n);
     return cv.used;
 }
-template <typename T, int N>
-cudaError_t rows_launch(const RowsArgs& r, int grid, cudaStream_t st) {
-    const bool vec = r.wk == 1 && (uintptr_t)r.w % 16 == 0 && r.wr * (int64_t)sizeof(T) % 16 == 0;
-    const int V = vec ? 16 / sizeof(T) : 1;
+template <typename T, int N, bool VEC>
+cudaError_t rows_launch_as(const RowsArgs& r, int grid, cudaStream_t st) {
+    constexpr int V = WLoad<T, VEC>::kCount;
     const size_t smem = (size_t)((r.d + V - 1) / V) * V * N * sizeof(float);
-    auto fn = vec ? xent_rows_kernel<T, N, true> : xent_rows_kernel<T, N, false>;
-    const cudaError_t e = cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    auto fn = xent_rows_kernel<T, N, VEC>;
+    static SharedMemory shared;
+    const cudaError_t e = shared.allow((const void*)fn, kRowsMaxSmem);
     if (e != cudaSuccess) return e;
     KernelTimer kt(st, GAFIME_KERNEL_XENT);
     fn<<<grid, kRowsThreads, smem, st>>>(r);
     return cudaGetLastError();
+}
+template <typename T, int N>
+cudaError_t rows_launch(const RowsArgs& r, int grid, cudaStream_t st) {
+    const bool vec = r.wk == 1 && (uintptr_t)r.w % 16 == 0 && r.wr * (int64_t)sizeof(T) % 16 == 0;
+    return vec ? rows_launch_as<T, N, true>(r, grid, st) : rows_launch_as<T, N, false>(r, grid, st);
 }
 template <typename T>
 cudaError_t rows_run(const XentCall& a, int sms) {

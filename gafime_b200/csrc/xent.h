@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/gafime_b200.h"
 
 namespace gafime {
@@ -52,6 +54,25 @@ struct Carver {
         used += (count * sizeof(T) + 255) / 256 * 256;
         return base ? reinterpret_cast<T*>(base + at) : nullptr;
     }
+};
+
+// A kernel's dynamic shared memory, allowed once a device.  The limit belongs to the kernel, not to a
+// launch: were it set to each call's own size, a smaller call of another thread could lower it
+// between a call's setting and its launch.  One object for each kernel, always with the same size.
+class SharedMemory {
+public:
+    cudaError_t allow(const void* kernel, size_t bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 64 && ((allowed_.load(std::memory_order_relaxed) >> dev) & 1)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess && dev < 64) allowed_.fetch_or(1ull << dev, std::memory_order_relaxed);
+        return e;
+    }
+
+private:
+    std::atomic<uint64_t> allowed_{0};
 };
 
 // Few classes: true when the class and feature counts fit its registers.

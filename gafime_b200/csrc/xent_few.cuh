@@ -58,6 +58,7 @@ constexpr int kRowsMost = 32;
 // 4e6 x 16 with 2 classes 72 -> 78).
 constexpr int kBesideMaxC = 4, kBesideMinD = 32;
 constexpr int kFlushRows = 256;
+constexpr size_t kFewMaxSmem = 226 * 1024;   // of a CTA, at most
 
 struct FewArgs {
     const void* x;
@@ -795,8 +796,8 @@ __global__ void __launch_bounds__(few_threads(F, GRAD), few_warps(C, F, GRAD) * 
 template <typename T, int C, bool COLS, bool GRAD, bool DX, int F, bool VEC, int G>
 cudaError_t launch_f(const FewPlan& p, cudaStream_t stream) {
     auto fn = xent_few_kernel<T, C, COLS, GRAD, DX, F, VEC, G>;
-    const cudaError_t e =
-        cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+    static SharedMemory shared;
+    const cudaError_t e = shared.allow((const void*)fn, kFewMaxSmem);
     if (e != cudaSuccess) return e;
     KernelTimer kt(stream, GAFIME_KERNEL_XENT);
     fn<<<p.grid, p.threads, p.smem, stream>>>(p.k);
