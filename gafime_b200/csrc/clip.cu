@@ -117,10 +117,10 @@ __device__ double chunk_squares(const T* p, int len) {
 }
 
 template <typename T>
-__device__ void chunk_scale(const T* p, T* o, int len, float f) {
+__device__ void chunk_scale(const T* p, T* o, int len, float f, float f2) {
     constexpr int V = 16 / sizeof(T);
     if ((uintptr_t)p % 16 != (uintptr_t)o % 16) {
-        for (int e = threadIdx.x; e < len; e += kThreads) o[e] = from_float<T>(to_float(p[e]) * f);
+        for (int e = threadIdx.x; e < len; e += kThreads) o[e] = from_float<T>(to_float(p[e]) * f2 * f);
         return;
     }
     const int head = head_of(p, len), vecs = (len - head) / V;
@@ -131,13 +131,13 @@ __device__ void chunk_scale(const T* p, T* o, int len, float f) {
         float v[V];
         unpack(v, q[i], T{});
         #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= f;
+        for (int j = 0; j < V; ++j) v[j] = v[j] * f2 * f;
         __stcs(w + i, repack(v, T{}));
     }
     const int rest = len - head - vecs * V;
     if ((int)threadIdx.x < head + rest) {
         const int e = (int)threadIdx.x < head ? threadIdx.x : head + vecs * V + threadIdx.x - head;
-        o[e] = from_float<T>(to_float(p[e]) * f);
+        o[e] = from_float<T>(to_float(p[e]) * f2 * f);
     }
 }
 
@@ -201,19 +201,21 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
                                                               int parts, float max_norm, float* norm) {
     const double v = norm_of(part, parts);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)v;
-    // a norm that is not finite has no scale that would mend its tensors
-    const float f = isfinite(v) && v > (double)max_norm ? (float)((double)max_norm / v) : 1.f;
+    // A norm that is not finite has no scale that would mend its tensors; nor is one past fp32, which
+    // the caller sees as infinity.  A factor below fp32's normal numbers comes as two.
+    const double q = isfinite((float)v) && v > (double)max_norm ? (double)max_norm / v : 1.0;
+    const float f2 = q < 0x1p-126 ? 0x1p-126f : 1.f, f = (float)(q / (double)f2);
     for (uint32_t c = blockIdx.x; c < t.chunk0[t.count]; c += gridDim.x) {
         const int i = tensor_of(t, c);
-        if (f == 1.f && t.in[i] == t.out[i]) continue;
+        if (q == 1.0 && t.in[i] == t.out[i]) continue;
         const int64_t at = (int64_t)(c - t.chunk0[i]) * kChunk;
         const int len = (int)min((int64_t)kChunk, t.size[i] - at);
         if (t.type[i] == GAFIME_TYPE_FP32)
-            chunk_scale((const float*)t.in[i] + at, (float*)t.out[i] + at, len, f);
+            chunk_scale((const float*)t.in[i] + at, (float*)t.out[i] + at, len, f, f2);
         else if (t.type[i] == GAFIME_TYPE_FP16)
-            chunk_scale((const __half*)t.in[i] + at, (__half*)t.out[i] + at, len, f);
+            chunk_scale((const __half*)t.in[i] + at, (__half*)t.out[i] + at, len, f, f2);
         else
-            chunk_scale((const __nv_bfloat16*)t.in[i] + at, (__nv_bfloat16*)t.out[i] + at, len, f);
+            chunk_scale((const __nv_bfloat16*)t.in[i] + at, (__nv_bfloat16*)t.out[i] + at, len, f, f2);
     }
 }
 

@@ -501,9 +501,9 @@ int gafime_xent_workspace(int type, const void* d_x, int64_t x_row, int64_t x_co
  * NEW.  2-norm over all elements of n_tensors contiguous tensors together (device pointers,
  * element counts and GAFIME_TYPE_* in host arrays), summed in fp64 in a fixed order, to the
  * device float *d_norm.  With d_outs (host array of device pointers) the tensors are also
- * scaled to a norm of at most max_norm: out = g * min(1, max_norm / norm), rounded once;
+ * scaled to a norm of at most max_norm: out = g * min(1, max_norm / norm), factor and product in fp32;
  * d_outs[i] is d_tensors[i] (in place) or memory that overlaps none of the tensors and outs.
- * A norm that is not finite leaves the values as they are.  d_outs NULL: the norm only.
+ * A norm that is not finite in fp32 leaves the values as they are.  d_outs NULL: the norm only.
  * workspace: 256-byte aligned, gafime_grad_norm_workspace(n_tensors) bytes.
  */
 int gafime_grad_norm(const void* const* d_tensors, const int64_t* sizes, const int* types, int64_t n_tensors,
