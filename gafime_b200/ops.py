@@ -205,12 +205,12 @@ def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
     if set(map(_device, tensors)) != {index} or not all(map(_contiguous, tensors)):
         raise ValueError("the tensors must be contiguous and on one GPU")
     lib = _native.load()
-    outs = None
+    outs = written = None
     ptrs = array.array("q", map(_pointer, tensors))
     if out is tensors:
-        outs = ptrs
+        outs, written = ptrs, tensors
     elif out is not None:
-        out = list(out)
+        written = out = list(out)
         if len(out) != count:
             raise ValueError(f"{count} tensors, but {len(out)} outs")
         if (list(map(_dtype, out)) != dtypes or array.array("q", map(_numel, out)) != sizes
@@ -224,6 +224,9 @@ def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
     args = (_address(ptrs), _address(sizes), _address(types), count, None if outs is None else _address(outs), max_norm,
             norm.data_ptr(), ws.data_ptr(), size)
     _on_device(index, "gafime_grad_norm", lib.gafime_grad_norm, args)
+    if written:
+        # torch does not see the writes: a tensor that autograd saved before has to be noticed
+        torch.autograd.graph.increment_version(written)
     return norm
 
 
