@@ -16,6 +16,7 @@ import operator
 from typing import NamedTuple, Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -167,12 +168,17 @@ def softmax_xent(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
     x (n, d) and w (c, d): float32, float16 or bfloat16 alike, any strides (a bucket's columns
     as they are); labels (n,) int64 or int32; bias (c,) float32, -inf excludes a class.  A row
     with a negative label is left out: loss 0, no part in any gradient, whatever its features
-    hold.  A label >= c makes the row's loss, and the gradients it enters, NaN.
+    hold.  A label >= c makes the row's loss, and the gradients it enters, NaN.  Reverse mode and
+    first order only: tensors with forward-mode tangents are refused.
 
     To capture a backward pass into a CUDA graph, let go of eager graphs of the same leaves
     first (torch's autograd waits for the stream on which they were made), or capture
     softmax_xent_grad, which needs no autograd."""
     _check(x, w, labels, bias, None)
+    # (the level is -1 outside of forward mode)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, w, bias)):
+        raise RuntimeError("softmax_xent has no forward-mode derivative")
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)):
         return _SoftmaxXent.apply(x, w, labels, bias)
     return _call(x, w, labels, bias, x.shape[0], x.shape[1], w.shape[0], 0)[0]

@@ -51,3 +51,15 @@ def test_tensors_of_inference_mode(ops):
         assert abs(float(norm) - 20.0) < 1e-5 and abs(float(a[0]) - 0.5) < 1e-6
         x, w, labels, b = data()
         assert torch.isfinite(ops.softmax_xent(x, w, labels, b)).all()
+
+
+@pytest.mark.parametrize("which", [0, 1, 3])
+def test_forward_mode_is_refused(ops, which):
+    import torch.autograd.forward_ad as fw
+    args = list(data())
+    with fw.dual_level():
+        args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward"):
+            ops.softmax_xent(*args)
+        # without tangents nothing is lost
+        ops.softmax_xent(*data())
