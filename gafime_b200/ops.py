@@ -190,9 +190,33 @@ def softmax_xent_grad(x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, bi
     """Losses, and the gradients of ``sum_i scale * row_weight[i] * loss[i]``, in one call: the
     step of a fit whose row weights are known beforehand (1 / n for the mean).  With few classes
     and need_dx=False that is one pass over x.  The gradient of a bias that is None is None.
+    The losses are detached, like the gradients: for a loss to differentiate take softmax_xent.
     Arguments as softmax_xent; row_weight (n,) float32, None for ones."""
     n, d, c = _check(x, w, labels, bias, row_weight)
     return _gradients(x, w, labels, bias, n, d, c, row_weight, float(scale), need_dx, need_dw, bias is not None)
+
+
+def _whole(t: torch.Tensor) -> bool:
+    """The elements are, in some order of the dimensions, those of a whole storage: a transposed or
+    channels-last tensor (a slice of one is not)."""
+    if t.storage_offset() or t.untyped_storage().nbytes() != t.numel() * t.element_size():
+        return False
+    step = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size != 1:
+            if stride != step:
+                return False
+            step *= size
+    return True
+
+
+def _dense(tensors: list) -> bool:
+    return all(t.is_contiguous() or _whole(t) for t in tensors)
+
+
+def _alike(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Elements in the same order: both contiguous, or of the same shape and strides."""
+    return (a.is_contiguous() and b.is_contiguous()) or (a.shape == b.shape and a.stride() == b.stride())
 
 
 def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
@@ -208,8 +232,9 @@ def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
     dtypes = list(map(_dtype, tensors))
     if not set(dtypes) <= TYPES.keys():
         raise TypeError(f"tensors must be float32, float16 or bfloat16, got {set(dtypes) - TYPES.keys()}")
-    if set(map(_device, tensors)) != {index} or not all(map(_contiguous, tensors)):
-        raise ValueError("the tensors must be contiguous and on one GPU")
+    plain = all(map(_contiguous, tensors))
+    if set(map(_device, tensors)) != {index} or not (plain or _dense(tensors)):
+        raise ValueError("the tensors must be on one GPU, and contiguous or a whole storage in another order")
     lib = _native.load()
     outs = written = None
     ptrs = array.array("q", map(_pointer, tensors))
@@ -220,8 +245,9 @@ def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
         if len(out) != count:
             raise ValueError(f"{count} tensors, but {len(out)} outs")
         if (list(map(_dtype, out)) != dtypes or array.array("q", map(_numel, out)) != sizes
-                or set(map(_device, out)) != {index} or not all(map(_contiguous, out))):
-            raise ValueError("every out must have its tensor's size, type and device, and be contiguous")
+                or set(map(_device, out)) != {index}
+                or not (plain and all(map(_contiguous, out)) or _dense(out) and all(map(_alike, tensors, out)))):
+            raise ValueError("every out must have its tensor's size, type, device and order of elements")
         outs = array.array("q", map(_pointer, out))
     size = _norm_workspace(count)
     ws = torch.empty(size, dtype=torch.uint8, device=device)
@@ -246,8 +272,10 @@ def _norm_workspace(count: int) -> int:
 
 @torch.no_grad()
 def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
-    """2-norm over all elements of the tensors together, a float32 scalar on their GPU.  The
-    tensors are contiguous, float32, float16 or bfloat16 in any mix; squares are summed in fp64."""
+    """2-norm over all elements of the tensors together, a float32 scalar on their GPU, detached.
+    The tensors are contiguous, or hold a whole storage in another order of their dimensions (a
+    transposed dx, channels last); float32, float16 or bfloat16 in any mix.  Squares are summed in
+    fp64."""
     return _grad_norm(list(tensors), None, 0.0)
 
 
@@ -255,9 +283,10 @@ def grad_norm(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
 def clip_grad_norm(tensors: Sequence[torch.Tensor], max_norm: float,
                    out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scale the tensors by min(1, max_norm / norm) of their norm together, in place or into
-    ``out`` (one contiguous tensor each, alike in size and type, apart from one another and
-    from the tensors), and return the norm before it.  A norm that is not finite leaves the
-    values as they are: the caller sees it in the result and skips the step."""
+    ``out`` (one tensor each, alike in size, type and order of elements, apart from one another
+    and from the tensors), and return the norm before it, detached.  Tensors as grad_norm.  A norm
+    that is not finite leaves the values as they are: the caller sees it in the result and skips the
+    step."""
     max_norm = float(max_norm)
     if not 0.0 <= max_norm <= 3.4028234663852886e38:
         raise ValueError(f"max_norm must be a finite number >= 0, got {max_norm}")

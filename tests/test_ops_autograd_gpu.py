@@ -63,3 +63,44 @@ def test_forward_mode_is_refused(ops, which):
             ops.softmax_xent(*args)
         # without tangents nothing is lost
         ops.softmax_xent(*data())
+
+
+@pytest.mark.parametrize("c", [3, 40])
+def test_the_gradients_of_a_table_by_columns_are_clipped(ops, c):
+    """dx of features held column by column comes column by column, and can be clipped as it is."""
+    x, w, labels, b = data(c=c)
+    x = x.t().contiguous().t()
+    g = ops.softmax_xent_grad(x, w, labels, b)
+    assert not g.dx.is_contiguous()
+    want = (g.dx.double().square().sum() + g.dw.double().square().sum()).sqrt()
+    assert abs(float(ops.grad_norm([g.dx, g.dw])) / float(want) - 1) < 2.0 ** -22
+    dx, dw = g.dx.clone(), g.dw.clone()
+    limit = float(want) / 3
+    out = [torch.empty_like(g.dx), torch.empty_like(g.dw)]       # (empty_like keeps the order)
+    ops.clip_grad_norm([g.dx, g.dw], limit, out=out)
+    ops.clip_grad_norm([g.dx, g.dw], limit)
+    for got, o, before in ((g.dx, out[0], dx), (g.dw, out[1], dw)):
+        assert torch.equal(got, o)
+        assert ((got.double() - before.double() / 3).abs() <= 4 * 2.0 ** -24 * before.double().abs() + 1e-38).all()
+    # an out in another order would mix the elements up
+    with pytest.raises(ValueError):
+        ops.clip_grad_norm([g.dx], limit, out=[torch.empty(g.dx.shape, device="cuda")])
+
+
+def test_gradients_in_channels_last_order(ops):
+    t = torch.randn((4, 6, 5, 3), device="cuda").to(memory_format=torch.channels_last)
+    assert not t.is_contiguous()
+    before = t.clone()
+    want = float(t.double().square().sum().sqrt())
+    assert abs(float(ops.clip_grad_norm([t], want / 2)) / want - 1) < 2.0 ** -22
+    assert ((t.double() - before.double() / 2).abs() <= 4 * 2.0 ** -24 * before.double().abs() + 1e-38).all()
+
+
+def test_layouts_without_every_element_once_are_refused(ops):
+    base = torch.ones((6, 8), device="cuda")
+    for t in (base[:, ::2], base[:1].expand(6, 8), base.t()[1:], base.t()[:, 1:]):
+        with pytest.raises(ValueError):
+            ops.grad_norm([t])
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm([t], 1.0)
+    assert (base == 1.0).all()
