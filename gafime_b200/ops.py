@@ -80,6 +80,11 @@ def _check(x, w, labels, bias, row_weight):
     return n, d, c
 
 
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    """Memory that holds the values themselves (a conjugate's imaginary part holds the other sign)."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _on_device(index: int, name: str, fn, args) -> None:
     """fn(*args, stream) on torch's current stream of device `index`."""
     if torch.cuda.current_device() == index:
@@ -94,6 +99,8 @@ def _on_device(index: int, name: str, fn, args) -> None:
 def _call(x, w, labels, bias, n, d, c, want, row_weight=None, scale=1.0, loss=None, lse=None, dx=None, dw=None,
           dbias=None):
     """One library call on the current stream of x's device; loss and lse given: read, not written."""
+    x, w = _plain(x), _plain(w)
+    bias, row_weight = bias if bias is None else _plain(bias), row_weight if row_weight is None else _plain(row_weight)
     lib = _native.load()
     type_id, device, index = TYPES[x.dtype], x.device, x.get_device()
     xp, wp = x.data_ptr(), w.data_ptr()
@@ -248,6 +255,9 @@ def _grad_norm(tensors: list, out, max_norm: float) -> torch.Tensor:
                 or set(map(_device, out)) != {index}
                 or not (plain and all(map(_contiguous, out)) or _dense(out) and all(map(_alike, tensors, out)))):
             raise ValueError("every out must have its tensor's size, type, device and order of elements")
+        # (a dense view that negates has one element: imaginary parts lie two apart)
+        if 1 in sizes and any(t.is_neg() != o.is_neg() for t, o, m in zip(tensors, out, sizes) if m == 1):
+            raise ValueError("a view that negates can be clipped in place only")
         outs = array.array("q", map(_pointer, out))
     size = _norm_workspace(count)
     ws = torch.empty(size, dtype=torch.uint8, device=device)

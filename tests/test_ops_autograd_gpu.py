@@ -104,3 +104,39 @@ def test_layouts_without_every_element_once_are_refused(ops):
         with pytest.raises(ValueError):
             ops.clip_grad_norm([t], 1.0)
     assert (base == 1.0).all()
+
+
+@pytest.mark.parametrize("c", [3, 30])
+def test_views_that_negate(ops, c):
+    """The imaginary part of a conjugate is a view that holds the other sign in memory."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def view(*shape):
+        z = torch.randn(shape, generator=g, device="cuda", dtype=torch.complex64).conj().imag
+        assert z.is_neg()
+        return z
+
+    _, _, labels, _ = data(c=c)
+    x, w, b, r = view(50, 12), view(c, 12), view(c), view(50)
+    plain = [t.resolve_neg() for t in (x, w, b, r)]
+    want = ops.softmax_xent_grad(plain[0], plain[1], labels, plain[2], row_weight=plain[3])
+    got = ops.softmax_xent_grad(x, w, labels, b, row_weight=r)
+    for a, q in zip(want, got):
+        assert torch.allclose(a, q, rtol=1e-5, atol=1e-5)
+    assert torch.allclose(ops.softmax_xent(plain[0], plain[1], labels, plain[2]), ops.softmax_xent(x, w, labels, b),
+                          rtol=1e-5, atol=1e-5)
+
+
+def test_clipping_into_or_from_a_view_that_negates_is_refused(ops):
+    """A dense one holds one element (a conjugate's imaginary parts lie two apart)."""
+    z = torch.full((1,), 2.0 - 3.0j, device="cuda", dtype=torch.complex64).conj().imag
+    assert z.is_neg() and z.is_contiguous() and float(z) == 3.0
+    one = torch.ones(1, device="cuda")
+    assert float(ops.grad_norm([z])) == 3.0          # the sign does not matter to a norm
+    with pytest.raises(ValueError):
+        ops.clip_grad_norm([one], 0.5, out=[z])
+    with pytest.raises(ValueError):
+        ops.clip_grad_norm([z], 0.5, out=[one])
+    assert float(z) == 3.0 and float(one) == 1.0
+    ops.clip_grad_norm([z], 1.5)                     # in place both sides hold the same sign
+    assert float(z) == 1.5
