@@ -48,8 +48,9 @@ def _workspace_bytes(device: int, type_id: int, x_off: int, xr: int, xk: int, w_
     """Of sizes, strides and alignments alone (x_off, w_off: addresses modulo 16)."""
     out = ctypes.c_size_t(0)
     lib = _native.load(require_gpu=False)
-    _native.check("gafime_xent_workspace", lib.gafime_xent_workspace(
-        type_id, 256 + x_off, xr, xk, 256 + w_off, wr, wk, n, d, c, want, ctypes.byref(out)))
+    with torch.cuda.device(device):      # the plan follows from the device's SM count
+        _native.check("gafime_xent_workspace", lib.gafime_xent_workspace(
+            type_id, 256 + x_off, xr, xk, 256 + w_off, wr, wk, n, d, c, want, ctypes.byref(out)))
     return out.value
 
 
