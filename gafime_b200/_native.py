@@ -52,7 +52,7 @@ EXPORTED = (
     "gafime_allpairs_topk_device", "gafime_topk_merge_device", "gafime_contiguous_bucket_upload_columns",
     "gafime_contiguous_bucket_device_columns", "gafime_contiguous_bucket_mark_updated",
     "gafime_xent_forward", "gafime_xent_gradient", "gafime_xent_workspace", "gafime_grad_norm",
-    "gafime_grad_norm_workspace",
+    "gafime_grad_norm_workspace", "gafime_xent_fail_waits",
 )
 
 # kernel ids of the timing registry (GAFIME_KERNEL_* in the header)
@@ -136,6 +136,7 @@ def _bind(lib: ctypes.CDLL) -> None:
                                   _i, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp], _i),
         "gafime_xent_workspace": ([_i, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i,
                                    ctypes.POINTER(ctypes.c_size_t)], _i),
+        "gafime_xent_fail_waits": ([_i], _i),
         "gafime_grad_norm": ([_vp, _vp, _vp, _i64, _vp, _f, _vp, _vp, ctypes.c_size_t, _vp], _i),
         "gafime_grad_norm_workspace": ([_i64, ctypes.POINTER(ctypes.c_size_t)], _i),
     }

@@ -29,7 +29,7 @@
 // queues its CTA's TMA loads of 128 x 64 of A and BN / 2 x 64 of B into a ring; warp 1 of the
 // pair's first CTA issues the MMAs into one of two tensor-memory accumulators; warps 4-11 turn
 // the other accumulator's 128 rows of their CTA into sums, g, dx or dw.  Every mbarrier wait is
-// bounded; one that gives up records a code, and the call's losses and gradients of w become NaN.
+// bounded; one that gives up records a code, and everything that the call writes becomes NaN.
 //
 // What bounds it, measured on a B200 (1,645 TFLOP/s bf16 in a burst, 1,381 sustained under the
 // power cap):
@@ -1056,29 +1056,39 @@ __global__ void __launch_bounds__(256) xent_colsum_kernel(const float* __restric
     }
 }
 
-// dbias from its splits; and NaN in dw (BOTH: losses) where a kernel's wait gave up.
+// The end of a gradient call: dbias from its splits; and, where a kernel's wait gave up, NaN in
+// everything that the call writes (loss and lse null: given).
 template <typename T>
-__global__ void __launch_bounds__(256) xent_finish_kernel(int64_t c, int64_t d, int half_g, const Meta* __restrict__ meta,
-                                                          T* __restrict__ dw, const double* __restrict__ bias_part,
-                                                          int bias_splits, float* __restrict__ dbias, int64_t n,
-                                                          float* __restrict__ loss, float* __restrict__ lse) {
-    const bool failed = meta->err != 0;
+struct FinishArgs {
+    const Meta* meta;
+    int half_g, bias_splits;
+    int64_t n, d, c;
+    T *dx, *dw;
+    int64_t dxr, dxk;
+    const double* bias_part;
+    float *dbias, *loss, *lse;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) xent_finish_kernel(const FinishArgs<T> a) {
+    const bool failed = a.meta->err != 0;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)gridDim.x * 256;
-    if (dbias)
-        for (int64_t j = at / 32; j < c; j += all / 32) {   // a warp a class
+    if (a.dbias)
+        for (int64_t j = at / 32; j < a.c; j += all / 32) {   // a warp a class
             double v = 0.0;
-            for (int s = threadIdx.x & 31; s < bias_splits; s += 32) v += bias_part[s * c + j];
+            for (int s = threadIdx.x & 31; s < a.bias_splits; s += 32) v += a.bias_part[s * a.c + j];
             #pragma unroll
             for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if ((threadIdx.x & 31) == 0) dbias[j] = failed ? NAN : (float)ldexp(v, -g_exponent(meta, half_g));
+            if ((threadIdx.x & 31) == 0) a.dbias[j] = failed ? NAN : (float)ldexp(v, -g_exponent(a.meta, a.half_g));
         }
-    if (dw && failed)
-        for (int64_t i = at; i < c * d; i += all) dw[i] = from_float<T>(NAN);
-    if (loss && failed)
-        for (int64_t i = at; i < n; i += all) {
-            loss[i] = NAN;
-            if (lse) lse[i] = NAN;
-        }
+    if (!failed) return;
+    if (a.dw)
+        for (int64_t i = at; i < a.c * a.d; i += all) a.dw[i] = from_float<T>(NAN);
+    if (a.dx)
+        for (int64_t i = at; i < a.n * a.d; i += all) a.dx[i / a.d * a.dxr + i % a.d * a.dxk] = from_float<T>(NAN);
+    if (a.loss)
+        for (int64_t i = at; i < a.n; i += all) a.loss[i] = NAN;
+    if (a.lse)
+        for (int64_t i = at; i < a.n; i += all) a.lse[i] = NAN;
 }
 
 // dw or dx from several splits' sums: a block makes 32 rows x 8 features, a warp a feature.  Rows
@@ -1347,6 +1357,8 @@ cudaError_t planes(PlaneArgs s, int sms, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+std::atomic<int> fail_waits{0};   // gafime_xent_fail_waits
+
 template <typename T, typename E>
 cudaError_t run_tc(const XentCall& a, int sms) {
     const Plan p = make_plan(a, sms, a.ws);
@@ -1359,6 +1371,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         return cudaSuccess;
     }
     XENT_TRY(cudaMemsetAsync(p.meta, 0, sizeof(Meta), st));
+    if (fail_waits.load(std::memory_order_relaxed)) XENT_TRY(cudaMemsetAsync(&p.meta->err, 1, sizeof(int), st));
     // one tile of classes: the call's losses come with its g
     const bool both = p.products && !a.have_lse && p.c_tiles == 1;
     const bool forward = !a.have_lse && !both;
@@ -1552,10 +1565,16 @@ cudaError_t run_tc(const XentCall& a, int sms) {
             p.dw_part, p.dw_splits, p.dw_stride, (int)p.dw_d_tiles, p.bn_dw, a.c, (int)a.d, !kBf16, p.meta, nullptr, (T*)a.dw, a.d, 1);
         XENT_TRY(cudaGetLastError());
     }
-    if (a.dw || a.dbias || both) {
+    {
+        FinishArgs<T> f{};
+        f.meta = p.meta; f.half_g = !kBf16; f.bias_splits = p.bias_splits;
+        f.n = a.n; f.d = a.d; f.c = a.c;
+        f.dx = (T*)a.dx; f.dxr = a.dxr; f.dxk = a.dxk;
+        f.dw = (T*)a.dw;
+        f.bias_part = p.bias_part; f.dbias = a.dbias;
+        if (!a.have_lse) f.loss = a.loss, f.lse = a.lse;
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_finish_kernel<T><<<(unsigned)std::min<int64_t>(2 * sms, cdiv(a.c, 8)), 256, 0, st>>>(
-            a.c, a.d, !kBf16, p.meta, (T*)a.dw, p.bias_part, p.bias_splits, a.dbias, a.n, both ? a.loss : nullptr, a.lse);
+        xent_finish_kernel<T><<<(unsigned)std::min<int64_t>(2 * sms, cdiv(a.c, 8)), 256, 0, st>>>(f);
         XENT_TRY(cudaGetLastError());
     }
     return cudaSuccess;
@@ -1574,3 +1593,8 @@ cudaError_t xent_tc(const XentCall& a, int sms) {
 }
 
 }  // namespace gafime
+
+extern "C" int gafime_xent_fail_waits(int enable) {
+    gafime::fail_waits.store(enable != 0);
+    return GAFIME_SUCCESS;
+}

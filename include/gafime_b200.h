@@ -467,8 +467,8 @@ int gafime_contiguous_bucket_mark_updated(ContiguousBucket bucket);
  *   d_loss      n floats;  d_lse: n floats, or NULL (for a later gradient call).
  *   workspace   256-byte aligned, at least gafime_xent_workspace(... want = 0) bytes.
  *
- * Results are bit-identical from run to run.  A kernel whose bounded waits gave up (a fault)
- * leaves NaN in every loss.
+ * Results are bit-identical from run to run.  A call of whose kernels a bounded wait gave up (a
+ * fault) leaves NaN in everything it writes.
  */
 int gafime_xent_forward(int type, const void* d_x, int64_t x_row, int64_t x_col, const void* d_w, int64_t w_row,
                         int64_t w_col, const float* d_bias, const int64_t* d_labels, int64_t n, int64_t d, int64_t c,
@@ -482,14 +482,17 @@ int gafime_xent_forward(int type, const void* d_x, int64_t x_row, int64_t x_col,
  * have_lse = 0: computes d_loss and (unless NULL) d_lse as gafime_xent_forward does; with few
  * classes the loss, dw and dbias take one pass over x.  have_lse = 1: d_loss and d_lse are those
  * of a forward call on the same inputs and are only read.
- * The outputs may not overlap the inputs; dx of rows left out is zero.  A kernel whose bounded
- * waits gave up leaves NaN in every loss (have_lse = 0) and in dw.
+ * The outputs may not overlap the inputs; dx of rows left out is zero.
  */
 int gafime_xent_gradient(int type, const void* d_x, int64_t x_row, int64_t x_col, const void* d_w, int64_t w_row,
                          int64_t w_col, const float* d_bias, const int64_t* d_labels, int64_t n, int64_t d, int64_t c,
                          const float* d_row_weight, int64_t row_weight_stride, float scale, int have_lse, float* d_loss,
                          float* d_lse, void* d_dx, int64_t dx_row, int64_t dx_col, void* d_dw, float* d_dbias,
                          void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* NEW, for tests.  enable = 1: the calls queued from now on (many classes) end as if a kernel's
+ * bounded wait had given up, though none has; 0: as usual.  Host only. */
+int gafime_xent_fail_waits(int enable);
 
 /* NEW.  Workspace bytes of the call with these arguments (of the pointers only their alignment
  * matters).  want: 0 for gafime_xent_forward, else GAFIME_XENT_GRADIENT with the gradients
