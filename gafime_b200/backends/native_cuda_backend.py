@@ -216,7 +216,7 @@ class NativeCudaBackend(Backend):
             centers, scales = [], []
             for row, combo in zip(values, combos):
                 v = self._interaction(columns, combo)
-                mean = v.mean()
+                mean = self._mean(v)
                 sd = (v - mean).square().mean().sqrt()
                 sd = torch.where(sd > 0, sd, torch.ones_like(sd))   # a constant says nothing: zeros
                 row.copy_((v - mean) / sd)
@@ -245,6 +245,15 @@ class NativeCudaBackend(Backend):
                     "centers": torch.stack(centers).cpu().tolist(), "scales": torch.stack(scales).cpu().tolist(),
                     "log_loss": float(last.loss.double().mean()), "gradient_norm": float(norm), "steps": taken}
 
+    @staticmethod
+    def _mean(v):
+        """Mean of fp64 values; of a constant the value itself (its sum times 1 / n need not be), so
+        that what is left of it is zeros and not its rounding."""
+        import torch
+
+        low, high = torch.aminmax(v)
+        return torch.where(low == high, low, v.mean())
+
     def _interaction(self, columns, combo: Tuple[int, ...]):
         """A combo's values in fp64 from the resident fp32 columns, as the scores define them:
         the raw column, or a op b (of centred columns with center)."""
@@ -255,7 +264,7 @@ class NativeCudaBackend(Backend):
             return a
         c = columns[combo[1]].double()
         if self.center:
-            a, c = a - a.mean(), c - c.mean()
+            a, c = a - self._mean(a), c - self._mean(c)
         if self.operator == "multiply":
             return a * c
         if self.operator == "add":

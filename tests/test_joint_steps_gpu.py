@@ -1,4 +1,4 @@
-"""The joint fit's steps against the same descent in fp64 on the host."""
+"""The joint fit's steps against the same descent in fp64 on the host, and columns that are constant."""
 import numpy as np
 import pytest
 
@@ -57,3 +57,23 @@ def test_the_steps_are_those_of_the_descent(classes, steps, clip):
     assert np.abs(np.array(j.weights) - w).max() <= tol
     assert np.abs(np.array(j.biases) - b).max() <= tol
     assert np.abs(w).max() > 50 * tol            # (not a comparison of zeros)
+
+
+@pytest.mark.parametrize("center", [True, False])
+@pytest.mark.parametrize("n", [91, 93, 400, 1003])
+@pytest.mark.parametrize("value", [0.1, 1.5, -7.3, 1e-20, 3e30])
+def test_a_constant_column_is_zeros(value, n, center):
+    """Whether or not the fp64 mean of the column is its value again; with centering the pairs with it
+    are zeros too, not copies of the other feature."""
+    rng = np.random.default_rng(n)
+    X = rng.standard_normal((n, 4)).astype(np.float32)
+    X[:, 2] = value
+    y = (X[:, 0] > 0.2).astype(np.float64)
+    rep = engine(8, center=center).analyze(X, y)
+    j = rep.joint
+    at = [i for i, c in enumerate(j.combos) if tuple(c) == (2,) or (center and len(c) == 2 and 2 in c)]
+    assert at
+    for i in at:
+        assert j.scales[i] == 1.0
+        assert all(row[i] == 0.0 for row in j.weights)
+    assert np.isfinite(j.log_loss) and np.isfinite(j.weights).all()
