@@ -224,3 +224,26 @@ def test_a_weight_of_minus_infinity_excludes_its_class(ops, n, c):
     labels[1] = 4
     got = ops.softmax_xent(x, w, labels, b)
     assert math.isinf(float(got[1])) and float(got[1]) > 0
+
+
+@pytest.mark.parametrize("order", ["rows", "columns"])
+@pytest.mark.parametrize("n,d,c", [(300, 200, 100), (700, 520, 300), (260, 130, 60), (40, 700, 4000)])
+def test_infinite_weights_in_tables_of_several_blocks(ops, n, d, c, order):
+    """Every width of a class tile, several blocks of features, and the losses after the backward pass."""
+    x, w, labels, b, r = data(n, d, c, seed=10, order=order)
+    x[:, d - 3] = x[:, d - 3].abs() + 0.1
+    labels = torch.where(labels % 7 == 3, torch.zeros_like(labels), labels)
+    off = (torch.arange(c, device="cuda") % 7 == 3)
+    excluded = torch.where(off, float("-inf"), b)
+    finite = w.clone()
+    w[off, d - 3] = float("-inf")
+    want = ops.softmax_xent_grad(x, finite, labels, excluded, row_weight=r)
+    got = ops.softmax_xent_grad(x, w, labels, b, row_weight=r)
+    assert torch.equal(got.loss, want.loss) and torch.equal(got.dw, want.dw) and torch.equal(got.dbias, want.dbias)
+    rest = [k for k in range(d) if k != d - 3]
+    assert torch.equal(got.dx[:, rest], want.dx[:, rest]) and torch.isnan(got.dx[:, d - 3]).all()
+    leaf = w.clone().requires_grad_()
+    loss = ops.softmax_xent(x, leaf, labels, b)
+    assert torch.equal(loss, ops.softmax_xent(x, finite, labels, excluded))
+    loss.backward(r)
+    assert torch.isfinite(leaf.grad).all() and not leaf.grad[off].any()
