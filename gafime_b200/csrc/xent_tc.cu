@@ -97,6 +97,7 @@ static_assert(smem_of(256, 4096) <= 232448 && smem_of(128, 4096) <= 232448 && sm
 struct Meta {
     int err;                 // code of a wait that gave up
     uint32_t weight_bits;    // largest finite |row weight| as float bits
+    uint32_t far;            // a given lse is too coarse to normalise with
     uint32_t wild;           // fp32: some weight is infinite
     uint32_t poison;         // some left-out row of an x read in place holds a value that is not finite
 };
@@ -127,6 +128,7 @@ __device__ __forceinline__ int g_exponent(const Meta* m, int half_g) { return ha
 struct TcArgs {
     CUtensorMap a[3], b[4];   // planes: one, or h, m, l of fp32, w's infinities (b[1] also: see cleaned)
     CUtensorMap out[3];       // G: planes of g; DX, DW: dx, dw
+    int if_far;               // LSE: nothing to do unless meta->far is set
     int half_g;               // g in fp16 (scaled by 2^u), else bf16
     int units, m_tiles, n_tiles, splits;
     int per_split;            // LSE: class tiles of a split; DW: k blocks of a split
@@ -141,7 +143,7 @@ struct TcArgs {
     Meta* meta;
     const float* bias;        // -inf past the classes
     const int64_t* labels;
-    float *loss_out, *lse_out;   // BOTH: [n]; the second may be null
+    float *loss_out, *lse_out;   // BOTH: [n]; null: not wanted
     float2* part;             // LSE: [n][2 splits] maximum, sum
     float* zy;                // LSE: label's logit
     const float2* shift;      // G: [n] maximum and log of the sum
@@ -280,6 +282,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
     constexpr bool kAMn = MODE == DW, kBMn = MODE == DX || MODE == DW;
     constexpr bool kBf16 = sizeof(E) == 2 && !std::is_same<E, __half>::value;
     constexpr uint32_t kId = tc::idesc(BN, kBf16, kAMn, kBMn);
+    if (MODE == LSE && a.if_far && a.meta->far == 0) return;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (tc::smem_addr(raw) + 1023) & ~1023u;
     uint8_t* gbase = raw + (base - tc::smem_addr(raw));
@@ -569,7 +572,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) xent_tc
                     const float l = logf(sum * expf(top - shift) + o.y * expf(o.x - shift));
                     if (isnan(zy)) zy = o.z;
                     const float loss = y >= 0 ? (shift - zy) + l : 0.f;
-                    if (half == 0 && valid) {
+                    if (half == 0 && valid && a.loss_out) {
                         a.loss_out[a.row0 + row] = loss;
                         if (a.lse_out)
                             a.lse_out[a.row0 + row] = y >= 0 ? shift + l : 0.f;
@@ -824,10 +827,12 @@ __global__ void __launch_bounds__(256) xent_poison_kernel(const int64_t* __restr
     }
 }
 
-// lse and loss of a row from its partial maxima and sums
+// lse and loss of a row (null: given) from its partial maxima and sums, and the shift of its g
 __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part, int parts, int lanes,
                                                         const float* zy, const int64_t* labels, int64_t n,
-                                                        float* loss, float* lse, float2* shift, const Meta* meta) {
+                                                        float* loss, float* lse, float2* shift, int if_far,
+                                                        const Meta* meta) {
+    if (if_far && meta->far == 0) return;
     // `lanes` neighbouring threads to a row, 1 or 32
     const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, r = at / lanes;
     const int lane = (int)(at % lanes);
@@ -849,43 +854,25 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
     if (lane != 0) return;
     const float l = logf(s);
     if (shift) shift[r] = make_float2(sh, l);
+    if (!loss) return;
     const bool kept = labels[r] >= 0;
     const bool failed = meta->err != 0;
     loss[r] = failed ? NAN : kept ? (sh - zy[r]) + l : 0.f;
     if (lse) lse[r] = failed ? NAN : kept ? sh + l : 0.f;
 }
 
-// The shift that g subtracts where loss and lse are given: lse, which is rounded to its last bit.
-// Past kFarLse that bit (2^-19 and more) shows in every probability of the row, and where the
-// logits are the type's lowest value nothing is left beside it of the log of their sum; there the
-// shift is the label's logit, formed once more, and the loss, held in two floats.
-constexpr float kFarLse = 64.f;
-template <typename T>
-__global__ void __launch_bounds__(256) xent_shift_kernel(const T* __restrict__ x, int64_t xr, int64_t xk,
-                                                         const T* __restrict__ w, int64_t wr, int64_t wk,
-                                                         const float* __restrict__ bias, const int64_t* __restrict__ labels,
-                                                         int64_t n, int64_t d, int64_t c, const float* __restrict__ loss,
-                                                         const float* __restrict__ lse, float2* __restrict__ shift) {
+// The shift that g subtracts where loss and lse are given: lse, as it was rounded.  Past kFarLse its
+// last bit (2^-16 and more) shows in every probability of the row, and where a mask has left the
+// type's lowest value for all logits, nothing of the log of their sum is left in it.  A call with
+// such a row forms the maxima and sums again from the same products (meta->far).
+constexpr float kFarLse = 256.f;
+__global__ void __launch_bounds__(256) xent_shift_kernel(const int64_t* __restrict__ labels, int64_t n, const float* __restrict__ lse,
+                                                         float2* __restrict__ shift, Meta* meta) {
     const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int lane = threadIdx.x & 31;
-    const int64_t y = r < n ? labels[r] : -1;
-    float2 s = make_float2(r < n ? lse[r] : 0.f, 0.f);
-    uint32_t far = __ballot_sync(0xffffffffu, y >= 0 && y < c && fabsf(s.x) > kFarLse && fabsf(s.x) <= 3.402823466e38f);
-    while (far) {
-        const int l = __ffs(far) - 1;
-        far &= far - 1;
-        const int64_t row = r - lane + l, cls = __shfl_sync(0xffffffffu, y, l);
-        float v = 0.f;
-        for (int64_t k = lane; k < d; k += 32) v = fmaf(to_float(x[row * xr + k * xk]), to_float(w[cls * wr + k * wk]), v);
-        #pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == l) {
-            // the sum and, exactly, what it rounded off
-            const float z = v + bias[cls], q = loss[r], sum = z + q, part = sum - z;
-            if (isfinite(sum)) s = make_float2(sum, (z - (sum - part)) + (q - part));
-        }
-    }
-    if (r < n) shift[r] = s;
+    if (r >= n) return;
+    const float l = lse[r];
+    shift[r] = make_float2(l, 0.f);
+    if (labels[r] >= 0 && fabsf(l) > kFarLse) meta->far = 1;
 }
 
 // Rows read four features at a time: unit features, 16-byte aligned rows.
@@ -1372,15 +1359,15 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     }
     XENT_TRY(cudaMemsetAsync(p.meta, 0, sizeof(Meta), st));
     if (fail_waits.load(std::memory_order_relaxed)) XENT_TRY(cudaMemsetAsync(&p.meta->err, 1, sizeof(int), st));
-    // one tile of classes: the call's losses come with its g
-    const bool both = p.products && !a.have_lse && p.c_tiles == 1;
-    const bool forward = !a.have_lse && !both;
+    // one tile of classes: the call's losses come with its g, which its own sums normalise
+    const bool both = p.products && p.c_tiles == 1;
+    const bool forward = !a.have_lse && !both, again = a.have_lse && p.products && !both;
     {
         SetupArgs s{};
         s.labels = a.labels; s.n = a.n; s.weight = a.weight; s.weight_stride = a.weight_stride; s.scale = a.scale;
         s.want_weight = p.products && !kBf16;
         s.bias = a.bias; s.bias_pad = p.bias; s.c = a.c; s.c_pad = p.c_tiles * p.bn_c + 256;
-        s.zy = forward ? p.zy : nullptr;
+        s.zy = forward || again ? p.zy : nullptr;
         s.keep = p.x[0] || p.xc ? p.keep : nullptr;
         s.meta = p.meta;
         const int64_t threads = std::max<int64_t>(s.c_pad, a.n);
@@ -1425,8 +1412,14 @@ cudaError_t run_tc(const XentCall& a, int sms) {
     t.weight = a.weight; t.weight_stride = a.weight_stride; t.scale = a.scale;
     t.c_total = a.c;
     t.splits = p.splits;
-    if (forward) {
+    if (again) {
+        KernelTimer kt(st, GAFIME_KERNEL_XENT);
+        xent_shift_kernel<<<(unsigned)cdiv(a.n, 256), 256, 0, st>>>(a.labels, a.n, a.lse, p.shift, p.meta);
+        XENT_TRY(cudaGetLastError());
+    }
+    if (forward || again) {
         TcArgs l = t;
+        l.if_far = again;
         XENT_TRY(map(l.a, xs, a.d, a.n, ldx, kBM));
         XENT_TRY(map(l.b, ws, a.d, a.c, ldw, p.bn_c / 2));
         l.m_tiles = (int)p.m_tiles;
@@ -1440,17 +1433,12 @@ cudaError_t run_tc(const XentCall& a, int sms) {
         l.zy = p.zy;
         XENT_TRY((launch<LSE, E, kPlanes>(l, p.bn_c, sms, st)));
     }
-    if (forward) {
+    if (forward || again) {
         KernelTimer kt(st, GAFIME_KERNEL_XENT);
         const int lanes = p.splits >= 16 ? 32 : 1;
-        xent_join_kernel<<<(unsigned)cdiv(a.n * lanes, 256), 256, 0, st>>>(p.part, 2 * p.splits, lanes, p.zy, a.labels, a.n,
-                                                                           a.loss, a.lse, p.products ? p.shift : nullptr,
-                                                                           p.meta);
-        XENT_TRY(cudaGetLastError());
-    } else if (p.products && !both) {
-        KernelTimer kt(st, GAFIME_KERNEL_XENT);
-        xent_shift_kernel<T><<<(unsigned)cdiv(a.n, 256), 256, 0, st>>>((const T*)a.x, a.xr, a.xk, (const T*)a.w, a.wr, a.wk,
-                                                                      p.bias, a.labels, a.n, a.d, a.c, a.loss, a.lse, p.shift);
+        xent_join_kernel<<<(unsigned)cdiv(a.n * lanes, 256), 256, 0, st>>>(
+            p.part, 2 * p.splits, lanes, p.zy, a.labels, a.n, forward ? a.loss : nullptr, forward ? a.lse : nullptr,
+            p.products ? p.shift : nullptr, again, p.meta);
         XENT_TRY(cudaGetLastError());
     }
     if (!p.products) return cudaSuccess;
@@ -1481,7 +1469,7 @@ cudaError_t run_tc(const XentCall& a, int sms) {
                     return cudaErrorInvalidValue;
             g.ldg = p.ldg;
             g.bias_part = a.dbias ? p.bias_sums : nullptr;
-            g.loss_out = a.loss;
+            g.loss_out = a.have_lse ? nullptr : a.loss;
             g.lse_out = a.lse;
             if (both)
                 XENT_TRY((launch<BOTH, E, kPlanes>(g, p.bn_c, sms, st)));

@@ -97,3 +97,31 @@ def test_logits_far_from_zero(ops, n, c, offset):
     # sums of c probabilities of fp32, n rows of them, and each row's label
     assert abs(float(db.double().sum())) <= n * (c + 64) * 4 * U
     assert abs(float(g.dbias.double().sum())) <= n * (c + 64) * 4 * U
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,c", PATHS)
+@pytest.mark.parametrize("size", [1e2, 1e6, 1e12, 1e20])
+def test_logits_of_any_size_have_a_backward_pass(ops, size, n, c, dtype):
+    """One class takes nearly every row: its probability is 1 to the last bits, however the label's
+    logit was rounded, and the gradients are those of the one-call form."""
+    x, w, labels, b = data(n, c, dtype=dtype, seed=4)
+    x = (x.float() * size).to(dtype)
+    g = ops.softmax_xent_grad(x, w, labels, b)
+    loss, dx, dw, db = through_autograd(ops, x, w, labels, b)
+    for name, got, want in (("dx", dx, g.dx), ("dw", dw, g.dw), ("dbias", db, g.dbias)):
+        assert torch.isfinite(got).all(), name
+    # logits of 1e2 and more, rounded to 2^-24 of themselves, move a probability between two classes
+    # that lie close by as much; rows with a clear winner (all but a few) have none of that
+    z = x.double() @ w.double().t() + b.double()
+    top = z.topk(2, dim=1).values
+    clear = (top[:, 0] - top[:, 1]) > 2.0 ** -16 * z.abs().amax(1) + 40
+    assert clear.float().mean() > (0.5 if size > 1e3 else 0.2)
+    p = torch.zeros((n, c), dtype=torch.float64, device="cuda")
+    p.scatter_(1, z.argmax(1, keepdim=True), 1.0)
+    p.scatter_add_(1, labels[:, None], -torch.ones((n, 1), device="cuda", dtype=torch.float64))
+    half = torch.finfo(dtype).eps / 2 if dtype != F32 else 0.0
+    err = (dx.double() - p @ w.double()).abs()[clear]
+    # (up to 256 the shift is the lse as the loss call rounded it)
+    rounded = torch.logsumexp(z, 1).abs().clamp(max=256.0)[:, None]
+    assert (err <= ((half * 2 + (64 + rounded) * U) * (p.abs() @ w.double().abs()) + 2.0 ** -24)[clear]).all()
