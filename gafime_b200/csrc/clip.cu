@@ -7,7 +7,7 @@
 // parameters, so that no table is copied to the device and a graph holds the whole call.
 // Measured on a B200 (copy rate 6,551 GB/s): the norm of 2 GB of fp32 0.29 ms (6,900 GB/s); 401
 // tensors, 534 MB in 16 and 32 bits: norm 0.09 to 0.11 ms, scaling 0.19 ms (5,600 GB/s read and
-// written), with the host's lists of pointers 0.32 ms a call.
+// written), with the host's lists of pointers 0.34 ms a call.
 // Squares are summed in fp64 (a square of an fp32 or bf16 value can leave fp32's range): each
 // CTA writes one partial sum, and whoever needs the norm adds the partials in the same order.
 #include <cuda_bf16.h>

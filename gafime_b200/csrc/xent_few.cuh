@@ -40,7 +40,7 @@
 namespace gafime {
 
 // Most classes of this path.  With gradients 8: at 16 their sums leave no registers (200000 x 1024
-// fp32: 1.5 to 3.1 ms a step, the tensor cores' path 1.04 ms); without, 16 (0.34 ms against 1.04 ms).
+// fp32: 1.5 to 3.1 ms a step, the tensor cores' path 1.16 ms); without, 16 (0.31 ms against 0.72).
 constexpr int kFewMaxC = 16, kFewMaxGrad = 8;
 // Features of a warp's tile: 128 with gradients, 64 without and for narrow tables (up to 24 warps
 // an SM in place of 12 to 16: steps of 4e6 x 16 with 2 classes 217 -> 174 us, 500000 x 33 with 8

@@ -14,7 +14,8 @@
 // Types.  16-bit x and w are multiplied as they are (TMA reads them in place where their
 // strides allow, else from a copy); g is rounded once to their type (half a step, 2^-8 or 2^-11
 // relative, independent from element to element, which is what rounding the result costs too); in
-// fp16 it is scaled by a power of two first, from the largest row weight, and held to 2^-38 of that.
+// fp16 it is scaled by a power of two first, from the largest row weight, and held to 2^-38 of that:
+// fp16's own 40 bits, from the largest row's gradients down to steps that its outputs have as well.
 // An fp32 value is held as three bf16 planes, its bits eight by eight, x = h + m + l exactly
 // (below 2^-110, to 2^-134), and so is g in fp32.  bf16 has fp32's exponents, so there is nothing to
 // scale and no value changes another's bits: a row, a feature, a class or a row weight far above the
@@ -36,12 +37,14 @@
 //   16 bits, 8192 x 1024, 32768 classes (0.55 TFLOP a product): lse 0.41 ms, g 0.47, dx 0.45, dw
 //     0.45 = 1,150 to 1,340 TFLOP/s, 83 to 97 % of the sustained rate.  With the MMAs left out the
 //     loads alone take 0.29 ms; g adds its exponentials, packing, stores and column sums.
-//   fp32, 200000 x 256, 1000 classes (3 products of 0.10 TFLOP): lse 0.26 ms, g 0.45, dx 0.32, dw
-//     0.30 = 680 to 1,200 TFLOP/s of 16-bit products.  The drains of tensor memory every two blocks
-//     and the epilogues bound it: without its epilogue's arithmetic g takes 0.24 ms.
-// Pairs of CTAs against single ones of 128 x 256: lse 0.54 -> 0.41 ms together with even runs of
-// class tiles, dw 0.47 -> 0.45.  Pieces of 256 MB against 128: 0.62 -> 0.32 ms for dx in fp32,
-// together with tabled scales (one round of the pairs to a launch exposes its start and end).
+//   fp32, 200000 x 256, 1000 classes (6 products of 0.10 TFLOP): lse 0.45 ms, g 0.73, dx 0.50, dw
+//     0.51 = 1,370 TFLOP/s of 16-bit products in lse, 1,230 in dx and dw: the tensor cores; g 850,
+//     bound by its epilogue (exponentials, three planes, column sums).  Two scaled fp16 planes took
+//     0.26, 0.43, 0.31 and 0.30 ms, and lost rows beside a large value.
+// Pairs of CTAs against single ones of 128 x 256 (16 bits): lse 0.54 -> 0.41 ms together with even
+// runs of class tiles, dw 0.47 -> 0.45.  Pieces of half the size: dx nearly twice as long (one round
+// of the pairs to a launch exposes its start and end); of 256 MB in place of 384 with three planes,
+// the step of 8192 x 1024 with 8192 classes 1.71 -> 2.37 ms.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>

@@ -457,7 +457,9 @@ int gafime_contiguous_bucket_mark_updated(ContiguousBucket bucket);
  * NEW.  Softmax cross entropy of a linear head, without keeping the logits:
  *   z_ij = sum_k x_ik w_jk + bias_j,  lse_i = log sum_j exp z_ij,  loss_i = lse_i - z_i,label(i)
  *
- *   type        of x and w (GAFIME_TYPE_*).  Products are summed in fp32.
+ *   type        of x and w (GAFIME_TYPE_*).  Products are summed in fp32.  fp32 values count with all
+ *               their bits, whatever the others' sizes (on the products' path those below 2^-110 to
+ *               2^-134).
  *   d_x         n x d; row i, feature k at i * x_row + k * x_col elements.  A bucket's columns
  *               (gafime_contiguous_bucket_device_columns) are x_row = 1, x_col = ld.
  *   d_w         c x d, likewise.
@@ -482,7 +484,9 @@ int gafime_xent_forward(int type, const void* d_x, int64_t x_row, int64_t x_col,
  * have_lse = 0: computes d_loss and (unless NULL) d_lse as gafime_xent_forward does; with few
  * classes the loss, dw and dbias take one pass over x.  have_lse = 1: d_loss and d_lse are those
  * of a forward call on the same inputs and are only read.
- * The outputs may not overlap the inputs; dx of rows left out is zero.
+ * The outputs may not overlap the inputs; dx of rows left out is zero.  In 16 bits with many
+ * classes g is rounded once to the type before it is multiplied; in fp16 it is held to 2^-38 of the
+ * largest |r_i|.
  */
 int gafime_xent_gradient(int type, const void* d_x, int64_t x_row, int64_t x_col, const void* d_w, int64_t w_row,
                          int64_t w_col, const float* d_bias, const int64_t* d_labels, int64_t n, int64_t d, int64_t c,
