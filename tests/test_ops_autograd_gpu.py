@@ -140,3 +140,40 @@ def test_clipping_into_or_from_a_view_that_negates_is_refused(ops):
     assert float(z) == 3.0 and float(one) == 1.0
     ops.clip_grad_norm([z], 1.5)                     # in place both sides hold the same sign
     assert float(z) == 1.5
+
+
+@pytest.mark.parametrize("c", [3, 12, 40, 300])
+@pytest.mark.parametrize("n", [0, 5, 60])
+def test_any_subset_of_the_gradients(ops, n, c):
+    """Each leaf alone and every pair, through autograd and in one call, is what the full call gives."""
+    x, w, labels, b = data(n=n, c=c)
+    full = ops.softmax_xent_grad(x, w, labels, b)
+    tensors = {"dx": x, "dw": w, "dbias": b}
+    for wanted in (("dx",), ("dw",), ("dbias",), ("dx", "dw"), ("dx", "dbias"), ("dw", "dbias")):
+        leaves = {k: (t.clone().requires_grad_() if k in wanted else t) for k, t in tensors.items()}
+        loss = ops.softmax_xent(leaves["dx"], leaves["dw"], labels, leaves["dbias"])
+        grads = torch.autograd.grad(loss.sum(), [leaves[k] for k in wanted])
+        for k, g in zip(wanted, grads):
+            assert torch.allclose(g, getattr(full, k), rtol=1e-4, atol=1e-5), (wanted, k)
+    for need_dx in (False, True):
+        for need_dw in (False, True):
+            for bias in (None, b):
+                one = ops.softmax_xent_grad(x, w, labels, bias, need_dx=need_dx, need_dw=need_dw)
+                assert (one.dx is None) != need_dx and (one.dw is None) != need_dw
+                assert (one.dbias is None) == (bias is None)
+                assert torch.allclose(one.loss, ops.softmax_xent(x, w, labels, bias), rtol=1e-5, atol=1e-5)
+                if bias is not None:
+                    for k in ("dx", "dw", "dbias"):
+                        if getattr(one, k) is not None:
+                            assert torch.allclose(getattr(one, k), getattr(full, k), rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("c", [3, 40])
+def test_one_tensor_as_features_and_weights(ops, c):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    t = torch.randn((c, 12), generator=g, device="cuda") * 0.5
+    labels = torch.arange(c, device="cuda")
+    a, q = t.clone().requires_grad_(), t.double().requires_grad_()
+    ops.softmax_xent(a, a, labels).sum().backward()
+    torch.nn.functional.cross_entropy(q @ q.t(), labels, reduction="sum").backward()
+    assert torch.allclose(a.grad.double(), q.grad, rtol=1e-4, atol=1e-5)

@@ -125,3 +125,29 @@ def test_logits_of_any_size_have_a_backward_pass(ops, size, n, c, dtype):
     # (up to 256 the shift is the lse as the loss call rounded it)
     rounded = torch.logsumexp(z, 1).abs().clamp(max=256.0)[:, None]
     assert (err <= ((half * 2 + (64 + rounded) * U) * (p.abs() @ w.double().abs()) + 2.0 ** -24)[clear]).all()
+
+
+@pytest.mark.parametrize("n,c", PATHS)
+def test_a_captured_backward_pass_sees_each_replays_logits(ops, n, c):
+    """Whether the sums are formed again is decided on the device: a graph captured over ordinary
+    logits normalises when a replay's lie far from zero, and the other way round."""
+    x, w, labels, b = data(n, c, seed=5)
+    held = b.clone()
+    leaf = w.clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(ops.softmax_xent(x, leaf, labels, b).sum(), leaf)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (dw,) = torch.autograd.grad(ops.softmax_xent(x, leaf, labels, b).sum(), leaf)
+    for bias in (held, held * 100 + 1e8, torch.full_like(held, LOWEST), held):
+        b.copy_(bias)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = torch.autograd.grad(ops.softmax_xent(x, leaf, labels, bias).sum(), leaf)[0]
+        assert torch.equal(dw, eager)
+        # every row's g sums to zero over the classes, so dw does, up to its rounding
+        assert (dw.double().sum(0).abs() <= n * (c + 64) * 4 * U * x.abs().max()).all()
